@@ -10,12 +10,13 @@ import os
 import re
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-HEADERS = ("cactus_b200.h", "cactus_b200_engine.h", "cactus_ffi.h")
+HEADERS = ("cactus_b200.h", "cactus_b200_kv4.h", "cactus_b200_engine.h", "cactus_ffi.h")
 
 _SCALAR = {
     "int": C.c_int,
     "unsigned": C.c_uint,
     "uint32_t": C.c_uint32,
+    "int32_t": C.c_int32,
     "uint64_t": C.c_uint64,
     "size_t": C.c_size_t,
     "float": C.c_float,

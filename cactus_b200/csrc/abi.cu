@@ -44,6 +44,9 @@ std::map<std::tuple<int, uint32_t, int>, RopeTable> g_rope;  // (device, theta b
 }  // namespace
 
 namespace cb {
+int abi_fail(int code, const std::string& msg) { return fail(code, msg); }
+int abi_check_launch(const char* what) { return check_launch(what); }
+
 bool& pdl_flag() {
     static thread_local bool f = false;
     return f;

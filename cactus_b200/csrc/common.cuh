@@ -30,6 +30,7 @@ enum DevError : unsigned {
     kDevOk = 0,
     kDevTmaTimeout = 1,
     kDevFlagTimeout = 2,
+    kDevBadPage = 3,  // 4-bit KV cache: a page id, position or length outside what the call gave
 };
 #ifdef __CUDACC_RDC__
 extern __device__ unsigned g_dev_error;

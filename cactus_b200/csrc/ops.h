@@ -4,9 +4,15 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <string>
+
 #include "kv_paging.h"
 
 namespace cb {
+
+// ---- error reporting of the C ABI (abi.cu): the message for cactus_cuda_last_error(), and the code
+int abi_fail(int code, const std::string& msg);
+int abi_check_launch(const char* what);  // the last launch's error as CB_ERR_LAUNCH, or CB_OK
 
 // ---- grouped GEMV (gemv.cu)
 enum GemvPro { kProPreq = 0, kProQuant = 1, kProRmsNormQuant = 2 };

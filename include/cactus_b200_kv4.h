@@ -1,0 +1,105 @@
+/*
+ * cactus_b200_kv4.h — C ABI of the 4-bit paged KV cache: append, read, attention, page copies and
+ * compaction as kernel entry points, and a cache handle that keeps the pages of many sequences
+ * (grow, fork, truncate, compact, free).
+ *
+ * Conventions are those of cactus_b200.h: DEVICE pointers unless a comment says host, fp16 as
+ * uint16_t bits, asynchronous calls on `stream`, 0 or a negative code with a message in
+ * cactus_cuda_last_error(). The kernel entry points allocate nothing and can be captured in a
+ * CUDA graph. Lengths, offsets, tables and row lists are read on the device; what they name
+ * outside the pool (a page id that is not in [0, num_pages), a position past the end of a table
+ * row) is skipped and raises the device error word (cactus_cuda_device_error() == 3).
+ *
+ * Format. A pool holds pages of page_size rows (16, 32, 64, 128 or 256); page p's bytes for one
+ * layer start at pool + p * page_stride and are, for each kv head,
+ *
+ *   key codes [page_size][head_dim / 2] | key parameters [page_size][head_dim / group_size]
+ *   | value codes | value parameters
+ *
+ * Byte i of a row holds element 2i in its low and 2i + 1 in its high half. The parameters of a
+ * group of group_size consecutive elements are two fp16 numbers, (step, low); code c stands for
+ * fp16(c * step + low) with one rounding. The append takes low = the group's smallest element,
+ * step = (largest - smallest) / 15 rounded towards zero, c = round-half-even((x - low) / step) in
+ * 0..15. A constant group has step 0 and codes 0. A group that holds an infinity or a NaN reads
+ * as NaN throughout, so that it shows in every output that sees it.
+ *
+ * Row r of sequence b is row r % page_size of page block_table[b * table_stride + r / page_size].
+ * head_dim is 64, 128 or 256; group_size 32, 64 or 128 and a divisor of head_dim. Pool and strides
+ * are 16-byte aligned.
+ *
+ * Batches are ragged: sequence b has the token rows token_offsets[b] .. token_offsets[b + 1] - 1
+ * (token_offsets: [num_seqs + 1], rising from 0; token_offsets[num_seqs] <= num_tokens, and rows
+ * past it are ignored) and context_lens[b] rows in the cache, its new ones included. So token i of
+ * S has position context_lens[b] - S + i. Positions below 0 are ignored by the append, and such
+ * queries see nothing but what the rule of the attention below gives them.
+ */
+#ifndef CACTUS_B200_KV4_H
+#define CACTUS_B200_KV4_H
+
+#include "cactus_b200.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/* Bytes of one page of one layer (the least page_stride); 0 where the geometry is not supported. */
+CB_API size_t cactus_cuda_kv4_page_bytes(size_t page_size, size_t num_kv_heads, size_t head_dim, size_t group_size);
+
+/* Quantises keys and values [num_tokens][num_kv_heads][head_dim], whose rows are row_stride fp16
+ * elements apart (a multiple of 8; keys and values 16-byte aligned), into the pages. */
+CB_API int cactus_cuda_kv4_append(const uint16_t* keys, const uint16_t* values, size_t row_stride,
+                                  const int32_t* token_offsets, const int32_t* context_lens,
+                                  const int32_t* block_table, size_t table_stride, void* pool, size_t num_pages,
+                                  size_t page_stride, size_t num_seqs, size_t num_tokens, size_t page_size,
+                                  size_t num_kv_heads, size_t head_dim, size_t group_size, void* stream);
+
+/* Reads rows back as fp16: row j of sequence b's row_offsets[b + 1] - row_offsets[b] rows is its
+ * position first_rows[b] + j (first_rows NULL: 0 for all) and goes to row row_offsets[b] + j of
+ * keys and values [num_rows][num_kv_heads][head_dim] (16-byte aligned; either may be NULL). */
+CB_API int cactus_cuda_kv4_read(const void* pool, size_t num_pages, size_t page_stride, const int32_t* block_table,
+                                size_t table_stride, const int32_t* row_offsets, const int32_t* first_rows,
+                                uint16_t* keys, uint16_t* values, size_t num_seqs, size_t num_rows, size_t page_size,
+                                size_t num_kv_heads, size_t head_dim, size_t group_size, void* stream);
+
+/* Softmax attention of queries [num_tokens][num_q_heads][head_dim] (rows query_stride elements
+ * apart, a multiple of 8, 16-byte aligned) over the cached rows; q head h reads kv head
+ * h / (num_q_heads / num_kv_heads). The query at position p sees position k of its sequence's
+ * context_lens[b] rows where k <= p (if is_causal) and k > p - window_size (if window_size > 0).
+ * output [num_tokens][num_q_heads][head_dim] fp16 (16-byte aligned), lse
+ * [num_tokens][num_q_heads] fp32, natural log-sum-exp of the scaled scores (may be NULL). A query
+ * that sees no row gives zeros and -inf. Pages that hold no visible row are not read (their table
+ * entries may be anything), and neither are rows past context_lens[b].
+ * max_query_len bounds every sequence's token count; a longer one is cut there and raises the
+ * device error word. workspace: cactus_cuda_kv4_attention_workspace() bytes, 16-byte aligned, zeroed
+ * once before its first use; every call leaves it ready for the next, also of other shapes that
+ * need no more bytes. Calls that may overlap in time need a workspace each. */
+CB_API size_t cactus_cuda_kv4_attention_workspace(size_t num_seqs, size_t num_tokens, size_t num_q_heads,
+                                                  size_t num_kv_heads, size_t head_dim);
+CB_API int cactus_cuda_kv4_attention(const uint16_t* queries, size_t query_stride, const int32_t* token_offsets,
+                                     const int32_t* context_lens, const int32_t* block_table, size_t table_stride,
+                                     const void* pool, size_t num_pages, size_t page_stride, uint16_t* output,
+                                     float* lse, size_t num_seqs, size_t num_tokens, size_t max_query_len,
+                                     size_t num_q_heads, size_t page_size, size_t num_kv_heads, size_t head_dim,
+                                     size_t group_size, float scale, size_t window_size, int is_causal,
+                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* Copies page src_pages[i] to page dst_pages[i] in each of num_planes planes (layers) that lie
+ * plane_stride bytes apart: page_bytes bytes each, all sizes multiples of 16. Pages of any format.
+ * A page may be the source of many copies; a destination is neither a source nor named twice. */
+CB_API int cactus_cuda_kv_copy_pages(void* pool, size_t num_pages, size_t page_bytes, size_t page_stride,
+                                     size_t num_planes, size_t plane_stride, const int32_t* src_pages,
+                                     const int32_t* dst_pages, size_t num_copies, void* stream);
+
+/* Moves the rows that sequences keep into other pages: row j of dst_table's sequence b becomes row
+ * kept_rows[kept_offsets[b] + j] of src_table's (both [num_seqs][table_stride]), in every plane;
+ * kept_offsets [num_seqs + 1] rises from 0 to num_kept. Destination pages are not source pages. */
+CB_API int cactus_cuda_kv4_compact(void* pool, size_t num_pages, size_t page_stride, size_t num_planes,
+                                   size_t plane_stride, const int32_t* src_table, const int32_t* dst_table,
+                                   size_t table_stride, const int32_t* kept_rows, const int32_t* kept_offsets,
+                                   size_t num_seqs, size_t num_kept, size_t page_size, size_t num_kv_heads,
+                                   size_t head_dim, size_t group_size, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif
