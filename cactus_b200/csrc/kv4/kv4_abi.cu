@@ -36,6 +36,7 @@ const char* make_pages(const void* pool, size_t num_pages, size_t page_stride, c
     if (!pool || !table) return "null pool or block table";
     if (num_pages == 0 || num_pages > kIntMax) return "num_pages must be 1 to 2^31 - 1";
     if (table_stride == 0 || table_stride > kIntMax) return "table_stride must be 1 to 2^31 - 1";
+    if (table_stride * (size_t)ge.page() > kIntMax - 1024) return "a table row holds more than 2^31 - 1024 positions";
     if (!aligned(pool, 16) || page_stride % 16) return "pool and page_stride must be 16-byte aligned";
     if (page_stride < (size_t)ge.block_bytes() * (size_t)ge.hkv) return "page_stride is less than a page";
     if (page_stride > ((size_t)1 << 62) / num_pages) return "pool size overflows";

@@ -20,7 +20,6 @@ int launch_copy_pages(uint8_t* pool, long long num_pages, long long page_bytes, 
 int launch_compact(const Pages& src, const int* dst_table, int planes, long long plane_stride, const int* kept,
                    const int* offsets, int num_seqs, int num_kept, const Geom& ge, cudaStream_t st);
 
-// attention.cu
 struct AttnCall {
     const __half* q;
     long long q_stride;
@@ -33,6 +32,10 @@ struct AttnCall {
     int causal;
     uint8_t* ws;
 };
+// decode.cu
+size_t decode_workspace(int num_seqs, int num_tokens, int hq, int hkv);
+int launch_decode(const AttnCall& c, const Pages& pg, const Geom& ge, cudaStream_t st);
+// attention.cu
 size_t attention_workspace(int num_seqs, int num_tokens, int hq, int hkv, int d);
 int launch_attention(const AttnCall& c, const Pages& pg, const Geom& ge, cudaStream_t st);
 

@@ -24,7 +24,7 @@
  * as NaN throughout, so that it shows in every output that sees it.
  *
  * Row r of sequence b is row r % page_size of page block_table[b * table_stride + r / page_size].
- * head_dim is 64, 128 or 256; group_size 32, 64 or 128 and a divisor of head_dim. Pool and strides
+ * table_stride * page_size is below 2^31 - 1024. head_dim is 64, 128 or 256; group_size 32, 64 or 128 and a divisor of head_dim. Pool and strides
  * are 16-byte aligned.
  *
  * Batches are ragged: sequence b has the token rows token_offsets[b] .. token_offsets[b + 1] - 1
