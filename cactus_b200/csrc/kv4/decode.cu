@@ -2,17 +2,18 @@
 // bound by the cache's bytes.
 //
 // Work. A sequence's q rows of one kv head (its tokens times the heads that share it, in tiles of
-// 8 or 16 rows) over its visible keys is an item; items are cut into tiles of 64 keys, and the
+// 4, 8 or 16 rows) over its visible keys is an item; items are cut into tiles of 64 keys, and the
 // tiles of all items, in one list, are dealt in equal contiguous ranges to as many CTAs as the GPU
 // holds at once, whatever the sequences' lengths. Every CTA finds its range itself from the lengths
 // in device memory. An item inside one range is finished there; the parts of one that spans several
 // go to the workspace, and the CTA that brings the last part joins them in range order, so the
 // result does not depend on which one that is.
 //
-// CTA. Warp 4 streams tiles into a ring in shared memory with 1-D bulk copies: 16 keys of one head
-// are four contiguous pieces (codes and parameters of keys and values) of one page, whatever the
-// page size. Warps 0-3 take 16 keys each and keep their own softmax state, so the loop has no
-// barrier; the four states are joined at the item's end.
+// CTA. Four warps; each takes 16 or 32 keys of every tile through its own ring in shared memory and
+// keeps its own softmax state, so the loop has no barrier and no registers go to a producer. The ring
+// is filled by 16-byte asynchronous copies, whose addresses differ by constants within a page; page
+// ids are fetched a step ahead. (Bulk copies by lanes of the warp run one after another and took 60
+// instructions for 32 keys.) The four states are joined at the item's end, in the rings' memory.
 //
 // Tensor cores. S^T = K Q^T and O^T = V^T P^T, m16n8k16 with keys (and value dims) on the 16 side
 // and q rows on the 8 side: 8 rows waste nothing, and the operand that comes from the cache is the
@@ -21,12 +22,14 @@
 // quarter of the 16 keys for the values, where the codes of two keys are interleaved by bytes first
 // so that one mask gives the same dim of both. Key i of the fragment is row kappa(i) of the 16,
 // which spreads the lanes' shared-memory reads over the banks. The weights go into O as two fp16
-// numbers, p = hi + lo (22 bits): the matrix instructions for lo are idle otherwise, and the result
-// is then as good as fp32 weights'.
+// numbers, p = hi + lo (22 bits), which makes the result as good as with fp32 weights; up to 4 rows
+// have lo in the columns that they leave empty.
 //
 // Softmax. The running maximum is raised only when a score exceeds it by more than 2^kLazy; until
 // then weights grow past 1 (at most 2^kLazy, far inside fp16), which is exact up to rounding and
 // saves the reduction over the lanes for almost every tile.
+#include <atomic>
+
 #include "attention.cuh"
 #include "kv4.cuh"
 #include "kv4_ops.h"
@@ -36,9 +39,9 @@ namespace kv4 {
 
 namespace {
 
-constexpr int kConsumers = 4, kThreads = (kConsumers + 1) * 32, kTile = 16 * kConsumers;
+constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr float kLazy = 8.0f;  // base-2 exponent
-constexpr int kMaxCtas = kNumSMs * 4;
+constexpr int kMaxCtas = kNumSMs * 5;
 constexpr int kMaxPartFloats = 16 * (128 + 2);  // rows * (D + 2): 16 x 128 or 8 x 256 (2064) at most
 constexpr size_t kPartBytes = (size_t)kMaxCtas * 2 * kMaxPartFloats * 4;
 
@@ -62,16 +65,8 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ void consumer_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
-
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, unsigned parity, volatile int* abort) {
-    if (mbar_try_wait(bar, parity)) return true;
-    for (uint32_t i = 0; i < (1u << 24); ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 255) == 255 && *abort) return false;
-    }
-    *abort = 1;
-    return false;
+__device__ __forceinline__ void cp_async16_at(uint32_t smem, const void* gmem) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem), "l"(gmem) : "memory");
 }
 
 // What one sequence asks for, in tiles. Positions fit 31 bits (the entry point checks the table's
@@ -80,10 +75,10 @@ struct Seq {
     int tokens, row_tiles;  // queries, tiles of q rows per kv head
     int pos0;               // position of token 0
     int start, end;         // keys that any of its queries sees
-    int base, ntiles;       // tiles of 64 keys from base (1 for none: the item still has to write)
+    int base, ntiles;       // tiles of keys from base (1 for none: the item still has to write)
 };
 
-template <int ROWS>
+template <int ROWS, int TILE>
 __device__ __forceinline__ Seq seq_of(const AttnCall& c, const Pages& pg, const Geom& ge, int b, bool report) {
     Seq s;
     const int count = c.offsets[b + 1] - c.offsets[b], len = max(c.lens[b], 0);
@@ -96,36 +91,43 @@ __device__ __forceinline__ Seq seq_of(const AttnCall& c, const Pages& pg, const 
     s.end = c.causal ? min(n, s.pos0 + s.tokens) : n;
     s.start = c.window > 0 ? (int)max(0LL, s.pos0 - c.window + 1) : 0;
     if (s.start >= s.end) s.start = s.end = 0;
-    s.base = s.start & ~15;
-    s.ntiles = max(1, (s.end - s.base + kTile - 1) / kTile);
+    s.base = s.start & ~(TILE - 1);
+    s.ntiles = max(1, (s.end - s.base + TILE - 1) / TILE);
     return s;
 }
 
-template <int D, int NT>
+// ROWS q rows are a tile: 16 or 8, which fill the columns of one or two fragments, or 4, which leave
+// columns 4-7 of one to the low parts of the weights.
+template <int ROWS>
+constexpr int columns() { return ROWS < 8 ? 8 : ROWS; }
+// Blocks of 16 keys that a warp takes at a time, CTAs a multiprocessor holds (by registers: 168 a
+// thread, 128 for four), stages of a ring (what shared memory then holds)
+template <int D, int ROWS>
+constexpr int blocks() { return D == 64 || (D == 128 && ROWS <= 8) ? 2 : 1; }
+template <int D, int ROWS>
+constexpr int ctas_per_sm() { return D == 64 && ROWS <= 8 ? 4 : 3; }
+template <int D, int ROWS>
+constexpr int stages() { return D == 64 ? 4 : D == 128 && ROWS == 16 ? 5 : 3; }
+
+template <int D, int ROWS>
 struct Smem {
-    static constexpr int kRows = 8 * NT, kPad = D + 4;
-    float o[kConsumers][kRows][kPad];
-    float m[kConsumers][kRows], l[kConsumers][kRows];
+    static constexpr int kCols = columns<ROWS>();
+    uint4 q[kCols / 8][D / 32][32];
+    float m[kWarps][kCols], l[kWarps][kCols];
     long long scan[kThreads], scan_items[kThreads];
-    long long w0, w1, base, total;  // this CTA's tiles, the first one's sequence's first tile, all tiles
-    long long item0;                // that sequence's first item
-    int b0, n, last, nan, abort;
+    long long base, item0;  // of the sequence that this CTA starts with: its first tile, its first item
+    int b0, last, nan;
 };
 
-template <int D>
-constexpr int stage_bytes(int ng) { return kTile * (D + 8 * ng); }
-
-template <int D, int NT>
-__global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2)
-    kv4_decode_kernel(const __grid_constant__ AttnCall c, const __grid_constant__ Pages pg, const __grid_constant__ Geom ge,
-                      int stages) {
+template <int D, int ROWS>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
+    kv4_decode_kernel(const __grid_constant__ AttnCall c, const __grid_constant__ Pages pg, const __grid_constant__ Geom ge) {
     pdl_launch_dependents();
     pdl_wait();
-    constexpr int kRows = 8 * NT;
+    constexpr int kCols = columns<ROWS>(), NT = kCols / 8, KB = blocks<D, ROWS>(), kTile = 16 * KB * kWarps, kStages = stages<D, ROWS>(), kPad = D + 4;
+    constexpr bool kPaired = ROWS < 8;  // columns 4-7 repeat 0-3 and take the weights' low parts
     extern __shared__ __align__(128) uint8_t ring[];
-    __shared__ Smem<D, NT> sm;
-    __shared__ uint64_t full[8], empty[8];
-    __shared__ int s_ok[8 * kConsumers];
+    __shared__ Smem<D, ROWS> sm;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int share = c.hq / ge.hkv, ng = ge.ng();
 
@@ -133,19 +135,13 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2)
     const int per = (c.num_seqs + kThreads - 1) / kThreads, first_b = tid * per;
     long long mine = 0, items = 0;
     for (int b = first_b; b < min(first_b + per, c.num_seqs); ++b) {
-        const Seq s = seq_of<kRows>(c, pg, ge, b, blockIdx.x == 0);
+        const Seq s = seq_of<ROWS, kTile>(c, pg, ge, b, blockIdx.x == 0);
         mine += (long long)s.row_tiles * ge.hkv * s.ntiles;
         items += (long long)s.row_tiles * ge.hkv;
     }
     sm.scan[tid] = mine;
     sm.scan_items[tid] = items;
     if (tid == 0) {
-        for (int s = 0; s < stages; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&empty[s], kConsumers);
-        }
-        fence_mbar_init();
-        sm.abort = 0;
         sm.nan = 0;
     }
     __syncthreads();
@@ -163,7 +159,7 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2)
     if (w0 >= sm.scan[tid] - mine && w0 < sm.scan[tid]) {
         long long at = sm.scan[tid] - mine, it = sm.scan_items[tid] - items;
         for (int b = first_b;; ++b) {
-            const Seq s = seq_of<kRows>(c, pg, ge, b, false);
+            const Seq s = seq_of<ROWS, kTile>(c, pg, ge, b, false);
             const long long k = (long long)s.row_tiles * ge.hkv;
             if (w0 < at + k * s.ntiles) {
                 sm.b0 = b;
@@ -176,9 +172,6 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2)
         }
     }
     __syncthreads();
-    const int bytes_block = 16 * (D + 8 * ng), bytes_stage = kConsumers * bytes_block;
-    volatile int* const abort = &sm.abort;
-
     // walks the items of [w0, w1): item `it` of sequence b (kv head it / row_tiles), tiles t .. t + k - 1
     struct Walk {
         int b;
@@ -188,207 +181,240 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2)
     wk.b = sm.b0;
     wk.base = sm.base;
     wk.item0 = sm.item0;
-    wk.s = seq_of<kRows>(c, pg, ge, wk.b, false);
+    wk.s = seq_of<ROWS, kTile>(c, pg, ge, wk.b, false);
     auto next_seq = [&](long long w) {  // moves to the sequence that tile w belongs to
         while (w >= wk.base + (long long)wk.s.row_tiles * ge.hkv * wk.s.ntiles) {
             wk.base += (long long)wk.s.row_tiles * ge.hkv * wk.s.ntiles;
             wk.item0 += (long long)wk.s.row_tiles * ge.hkv;
             ++wk.b;
-            wk.s = seq_of<kRows>(c, pg, ge, wk.b, false);
+            wk.s = seq_of<ROWS, kTile>(c, pg, ge, wk.b, false);
         }
     };
 
-    if (warp == kConsumers) {
-        // ---------------------------------------------------------------- producer
-        int issued = 0;
-        const int blk = lane >> 2, part = lane & 3;  // lanes 0-15: a 16-key block's four pieces
-        const int cb = 16 * (D / 2), pb = 64 * ng;
-        const int in_block = (part & 2 ? ge.v_codes() : 0) + (part & 1 ? ge.k_params() : 0);
-        const int row_bytes = part & 1 ? 4 * ng : D / 2, piece = part & 1 ? pb : cb;
-        const int in_stage = blk * bytes_block + (part & 2 ? cb + pb : 0) + (part & 1 ? cb : 0);
-        bool ok = true;
-        for (long long w = w0; w < w1 && ok;) {
-            next_seq(w);
-            const int it = (int)((w - wk.base) / wk.s.ntiles), tile0 = (int)((w - wk.base) % wk.s.ntiles);
-            const int head = it / wk.s.row_tiles, ntile = (int)min((long long)(wk.s.ntiles - tile0), w1 - w);
-            for (int i = 0; i < ntile; ++i) {
-                const int k0 = wk.s.base + (tile0 + i) * kTile + blk * 16;
-                long long off = -1;
-                if (lane < 16 && k0 < wk.s.end) off = page_offset(pg, wk.b, k0, ge.page_shift);
-                const int slot = issued % stages;
-                if (issued >= stages && !wait_or_abort(&empty[slot], ((issued / stages) - 1) & 1, abort)) {
-                    ok = false;
-                    break;
-                }
-                const unsigned valid = __ballot_sync(0xffffffffu, off >= 0) & 0x1111u;
-                if (lane < 16 && part == 0) s_ok[slot * kConsumers + blk] = off >= 0;
-                __syncwarp();
-                if (lane == 0) {
-                    fence_proxy_async_shared();
-                    mbar_arrive_expect_tx(&full[slot], (unsigned)(__popc(valid) * bytes_block));
-                }
-                __syncwarp();
-                if (off >= 0) {
-                    const int row = k0 & (ge.page() - 1);
-                    const uint8_t* src = pg.pool + off + (long long)head * ge.block_bytes() + in_block + row * row_bytes;
-                    tma_load_1d(ring + slot * bytes_stage + in_stage, src, (unsigned)piece, &full[slot]);
-                }
-                ++issued;
-            }
-            w += ntile;
-        }
-        // no copy may land after the block leaves
-        if (*abort && lane == 0)
-            for (int i = issued > stages ? issued - stages : 0; i < issued; ++i)
-                mbar_wait_bounded(&full[i % stages], (i / stages) & 1);
-        __syncwarp();
-        if (lane == 0 && *abort) report_dev_error(kDevTmaTimeout);
-        return;
-    }
-
-    // ---------------------------------------------------------------- consumers
     const int g = lane >> 2, t = lane & 3;
-    const int kg = kappa(g);
     const float sc = c.scale * 1.4426950408889634f;
     float* const parts = reinterpret_cast<float*>(c.ws);
     unsigned* const counters = reinterpret_cast<unsigned*>(c.ws + kPartBytes);
-    int used = 0;
+    // A stage is the parts of one page (KB = 2 and a page of 16 rows: of two pages) one after the
+    // other, R rows each: codes | parameters | the values' codes | parameters
+    const int R = min(ge.page(), 16 * KB), row_p = 4 * ng, chunk_bytes = R * (D + 2 * row_p);
+    const int stage_bytes = 16 * KB * (D + 2 * row_p);
+    uint8_t* const mine_ring = ring + warp * kStages * stage_bytes;
+    float* const s_o = reinterpret_cast<float*>(ring);  // [warp][row][kPad], at an item's end
+    // byte offsets in a stage of this lane's parts of the first block: key kappa(g) (and 8 rows on), two
+    // groups of parameters at most; value rows kappa(2 t), kappa(2 t + 1) (and 8 on), one group; and
+    // how far the second block's are on
+    const int kg = kappa(g), vk0 = kappa(2 * t), vk1 = kappa(2 * t + 1);
+    const int p0 = R * (D / 2), v0 = p0 + R * row_p, q0 = v0 + R * (D / 2);
+    const int k_codes = kg * (D / 2) + t * (D / 8);
+    const int k_par0 = p0 + kg * row_p + t * (D / 4) / ge.g * 4;
+    const int k_par1 = p0 + kg * row_p + (t * (D / 4) + 32) / ge.g * 4;
+    const int v_codes0 = v0 + vk0 * (D / 2) + g * (D / 16), v_codes1 = v_codes0 + (vk1 - vk0) * (D / 2);
+    const int v_par0 = q0 + vk0 * row_p + g * (D / 8) / ge.g * 4, v_par1 = v_par0 + (vk1 - vk0) * row_p;
+    const int step_codes = R == 16 ? chunk_bytes : 8 * D, step_par = R == 16 ? chunk_bytes : 16 * row_p;
+    const uint32_t ring_at = smem_u32(mine_ring) + lane * 16;
+    const bool copies_par = lane < R * ng / 4;  // 16-byte pieces of R rows' parameters: at most 32
+
     for (long long w = w0; w < w1;) {
         next_seq(w);
         const Seq s = wk.s;
         const long long rel = w - wk.base;
         const int it = (int)(rel / s.ntiles), tile0 = (int)(rel % s.ntiles);
-        const int head = it / s.row_tiles, row0 = (it % s.row_tiles) * kRows;
+        const int head = it / s.row_tiles, row0 = (it % s.row_tiles) * ROWS;
         const int ntile = (int)min((long long)(s.ntiles - tile0), w1 - w);
-        const int tok0 = c.offsets[wk.b], rows = min(kRows, s.tokens * share - row0);
+        const int tok0 = c.offsets[wk.b], rows = min(ROWS, s.tokens * share - row0);
         const int qhead0 = head * share;
 
-        // ---- q fragments: column g of n-tile j is row row0 + 8 j + g
-        uint32_t q[NT][D / 16][2];
+        // ---- the ring: stage i of this warp is the keys first + i * kTile .. + 16 KB - 1
+        const int first = s.base + tile0 * kTile + warp * 16 * KB, stop = min(s.end, first + ntile * kTile);
+        const int* const table = pg.table + (long long)wk.b * pg.table_stride;
+        const uint8_t* const pool = pg.pool + (long long)head * ge.block_bytes() + lane * 16;
+        unsigned have = 0;  // bits KB * slot ..: the blocks of the slot that were loaded
+        auto page_of = [&](int k0) -> int {  // id of the page with the R keys from k0; -1: nothing to load
+            if (k0 >= stop || k0 + R <= s.start) return -1;
+            const int p = __ldg(table + (k0 >> ge.page_shift));
+            if ((unsigned)p < (unsigned)pg.num_pages) return p;
+            report_dev_error(kDevBadPage);
+            return -1;
+        };
+        auto copy = [&](int page, int k0, uint32_t dst) {  // R keys
+            const int r = k0 & (ge.page() - 1);
+            const uint8_t* src = pool + (long long)page * pg.page_stride;
+            const uint8_t* codes = src + r * (D / 2);
+            const uint8_t* par = src + ge.k_params() + r * row_p;
+            if (R == 16) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int r = row0 + 8 * j + g;
-            const bool on = 8 * j + g < rows;
-            const __half* src = c.q + (long long)(tok0 + (on ? r / share : 0)) * c.q_stride +
-                                (long long)(qhead0 + (on ? r % share : 0)) * D + t * (D / 4);
+                for (int x = 0; x < D / 64; ++x) cp_async16_at(dst + x * 512, codes + x * 512);
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                const uint4 v = on ? __ldg(reinterpret_cast<const uint4*>(src) + i) : uint4{0, 0, 0, 0};
-                q[j][2 * i][0] = __byte_perm(v.x, v.z, 0x5410);
-                q[j][2 * i][1] = __byte_perm(v.x, v.z, 0x7632);
-                q[j][2 * i + 1][0] = __byte_perm(v.y, v.w, 0x5410);
-                q[j][2 * i + 1][1] = __byte_perm(v.y, v.w, 0x7632);
+                for (int x = 0; x < D / 64; ++x) cp_async16_at(dst + v0 + x * 512, codes + ge.v_codes() + x * 512);
+            } else {
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x) cp_async16_at(dst + x * 512, codes + x * 512);
+#pragma unroll
+                for (int x = 0; x < D / 32; ++x) cp_async16_at(dst + v0 + x * 512, codes + ge.v_codes() + x * 512);
             }
+            if (copies_par) {
+                cp_async16_at(dst + p0, par);
+                cp_async16_at(dst + q0, par + ge.v_codes());
+            }
+        };
+        int page[KB];  // of the next stage; with R = 16 KB only the first counts
+        auto pages_of = [&](int k0) {
+            page[0] = page_of(k0);
+            if (KB > 1 && R == 16) page[KB - 1] = page_of(k0 + 16);
+        };
+        auto advance = [&](int i, int slot) {  // stage i into the slot, and the ids for the next one
+            const int k0 = first + i * kTile;
+            const uint32_t dst = ring_at + slot * stage_bytes;
+            unsigned got = 0;
+            if (page[0] >= 0) {
+                copy(page[0], k0, dst);
+                got = R == 16 ? 1 : (1u << KB) - 1;
+            }
+            if (KB > 1 && R == 16 && page[KB - 1] >= 0) {
+                copy(page[KB - 1], k0 + 16, dst + chunk_bytes);
+                got |= 2;
+            }
+            have = (have & ~(((1u << KB) - 1) << KB * slot)) | got << KB * slot;
+            cp_async_commit();
+            pages_of(k0 + kTile);
+        };
+        pages_of(first);
+#pragma unroll
+        for (int i = 0; i < kStages - 1; ++i) advance(i, i);
+
+        // ---- q fragments: column g of n-tile j is row row0 + 8 j + g (paired: row0 + g % 4)
+        for (int i = warp; i < NT * (D / 32); i += kWarps) {
+            const int j = i / (D / 32), x = i % (D / 32), col = kPaired ? g & 3 : 8 * j + g, r = row0 + col;
+            uint4 v = {0, 0, 0, 0};
+            if (col < rows)
+                v = __ldg(reinterpret_cast<const uint4*>(c.q + (long long)(tok0 + r / share) * c.q_stride +
+                                                         (long long)(qhead0 + r % share) * D + t * (D / 4)) + x);
+            sm.q[j][x][lane] = uint4{__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                                     __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632)};
         }
-        // keys that the two columns of this thread (rows 2 t, 2 t + 1 of each n-tile) see
-        int from[NT][2], to[NT][2];
-        bool edge_cols = c.window > 0 || (c.causal && s.tokens > 1) || rows < kRows;
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int r = row0 + 8 * j + 2 * t + e;
-                const int pos = s.pos0 + r / share;
-                from[j][e] = c.window > 0 ? (int)max(0LL, pos - c.window + 1) : 0;
-                to[j][e] = c.causal ? min(s.end, pos + 1) : s.end;
-                if (8 * j + 2 * t + e >= rows) to[j][e] = 0;
-            }
-        float o[NT][D / 16][4], m[NT][2], l[NT][2];  // m: base-2 exponent that the state is relative to
+        __syncthreads();
+        // keys that every row of the tile sees
+        const int tok_a = row0 / share, tok_b = min((row0 + ROWS - 1) / share, s.tokens - 1);
+        const int all_from = c.window > 0 ? (int)max((long long)s.start, s.pos0 + tok_b - c.window + 1) : s.start;
+        const int all_to = c.causal ? min(s.end, s.pos0 + tok_a + 1) : s.end;
+        float o[NT][D / 16][4], l[NT][2];
+        float base[NT][2], limit[NT][2];  // base-2 exponent that the state is relative to (0 at first); the
+                                          // largest score that keeps it (-inf at first)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
             for (int i = 0; i < D / 16; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[j][i][e] = 0.0f;
-            m[j][0] = m[j][1] = -INFINITY;
+            limit[j][0] = limit[j][1] = -INFINITY;
+            base[j][0] = base[j][1] = 0.0f;
             l[j][0] = l[j][1] = 0.0f;
         }
 
+        int slot = 0;
 #pragma unroll 1
-        for (int i = 0; i < ntile; ++i, ++used) {
-            const int slot = used % stages;
-            const bool got = wait_or_abort(&full[slot], (used / stages) & 1, abort);
-            const int k0 = s.base + (tile0 + i) * kTile + warp * 16;
-            if (got && s_ok[slot * kConsumers + warp]) {
-                const uint8_t* blk = ring + slot * bytes_stage + warp * bytes_block;
-                const uint8_t* kp = blk + 16 * (D / 2);
-                const uint8_t* vc = kp + 64 * ng;
-                const uint8_t* vp = vc + 16 * (D / 2);
-                const bool whole = k0 >= s.start && k0 + 16 <= s.end;
-                // ---- S^T
-                float acc[NT][4];
+        for (int i = 0; i < ntile; ++i) {
+            __syncwarp();  // every lane is done with the stage that is filled next
+            advance(i + kStages - 1, slot == 0 ? kStages - 1 : slot - 1);
+            cp_async_wait<kStages - 1>();
+            __syncwarp();
+            const uint8_t* const blk0 = mine_ring + slot * stage_bytes;
+            const unsigned got = have >> KB * slot & ((1u << KB) - 1);
+            slot = slot + 1 == kStages ? 0 : slot + 1;
+            if (!got) continue;
+            int k0[KB];  // first key of each block; a block that was not loaded counts as past the end
+            bool whole = true;
+#pragma unroll
+            for (int k = 0; k < KB; ++k) {
+                k0[k] = got >> k & 1 ? first + i * kTile + k * 16 : 0x40000000;
+                whole &= k0[k] >= all_from && k0[k] + 16 <= all_to;
+            }
+            // ---- S^T
+            float acc[KB][NT][4];
+            constexpr int kWords = D / 32;  // words of codes of one key in a lane's quarter
+#pragma unroll
+            for (int k = 0; k < KB; ++k) {
+            const uint8_t* const blk = blk0 + k * step_codes;
+            const uint8_t* const pars = blk0 + k * step_par;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[k][j][e] = 0.0f;
+            uint32_t wa[kWords], wb[kWords];
+            if constexpr (kWords >= 4) {
+#pragma unroll
+                for (int x = 0; x < kWords / 4; ++x) {
+                    *reinterpret_cast<uint4*>(wa + 4 * x) = *reinterpret_cast<const uint4*>(blk + k_codes + 16 * x);
+                    *reinterpret_cast<uint4*>(wb + 4 * x) = *reinterpret_cast<const uint4*>(blk + k_codes + 16 * x + 4 * D);
+                }
+            } else {
+                *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(blk + k_codes);
+                *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(blk + k_codes + 4 * D);
+            }
+            __half2 sa, la, sb, lb;
+#pragma unroll
+            for (int x = 0; x < kWords; ++x) {
+                if (x == 0 || (D == 256 && x == 4)) {  // at most two groups in a lane's quarter
+                    const int par = x == 0 ? k_par0 : k_par1;
+                    const __half2 pa = *reinterpret_cast<const __half2*>(pars + par);
+                    const __half2 pb = *reinterpret_cast<const __half2*>(pars + par + 8 * row_p);
+                    sa = __low2half2(pa);
+                    la = __high2half2(pa);
+                    sb = __low2half2(pb);
+                    lb = __high2half2(pb);
+                }
+                __half2 ha[4], hb[4];
+                codes_to_half(wa[x], ha);
+                codes_to_half(wb[x], hb);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    ha[e] = __hfma2(ha[e], sa, la);
+                    hb[e] = __hfma2(hb[e], sb, lb);
+                }
+                const uint32_t a0[4] = {h2u(ha[0]), h2u(hb[0]), h2u(ha[1]), h2u(hb[1])};
+                const uint32_t a1[4] = {h2u(ha[2]), h2u(hb[2]), h2u(ha[3]), h2u(hb[3])};
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const uint4 q = sm.q[j][x][lane];
+                    mma16816(acc[k][j], a0, q.x, q.y);
+                    mma16816(acc[k][j], a1, q.z, q.w);
+                }
+            }
+            }
+            // ---- weights
+            bool rise = false;
+#pragma unroll
+            for (int k = 0; k < KB; ++k)
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
-                constexpr int kWords = D / 32;  // words of codes of one key in a lane's quarter
-                const uint32_t* ka = reinterpret_cast<const uint32_t*>(blk + kg * (D / 2) + t * (D / 8));
-                const uint32_t* kb = reinterpret_cast<const uint32_t*>(blk + (kg + 8) * (D / 2) + t * (D / 8));
-                uint32_t wa[kWords], wb[kWords];
-                if constexpr (kWords >= 4) {
-#pragma unroll
-                    for (int x = 0; x < kWords / 4; ++x) {
-                        *reinterpret_cast<uint4*>(wa + 4 * x) = *reinterpret_cast<const uint4*>(ka + 4 * x);
-                        *reinterpret_cast<uint4*>(wb + 4 * x) = *reinterpret_cast<const uint4*>(kb + 4 * x);
-                    }
-                } else {
-                    *reinterpret_cast<uint2*>(wa) = *reinterpret_cast<const uint2*>(ka);
-                    *reinterpret_cast<uint2*>(wb) = *reinterpret_cast<const uint2*>(kb);
-                }
-                __half2 sa, la, sb, lb;
-#pragma unroll
-                for (int x = 0; x < kWords; ++x) {
-                    if (x == 0 || (D == 256 && x == 4)) {  // at most two groups in a lane's quarter
-                        const int grp = (t * (D / 4) + x * 8) / ge.g;
-                        const __half2 pa = *reinterpret_cast<const __half2*>(kp + (kg * ng + grp) * 4);
-                        const __half2 pb = *reinterpret_cast<const __half2*>(kp + ((kg + 8) * ng + grp) * 4);
-                        sa = __low2half2(pa);
-                        la = __high2half2(pa);
-                        sb = __low2half2(pb);
-                        lb = __high2half2(pb);
-                    }
-                    __half2 ha[4], hb[4];
-                    codes_to_half(wa[x], ha);
-                    codes_to_half(wb[x], hb);
-#pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        ha[e] = __hfma2(ha[e], sa, la);
-                        hb[e] = __hfma2(hb[e], sb, lb);
+                        float x = acc[k][j][e] * sc;
+                        if (!whole) {
+                            const int key = k0[k] + kg + (e & 2 ? 8 : 0), col = 8 * j + 2 * t + (e & 1);
+                            const int tok = (row0 + (kPaired ? col & 3 : col)) / share;
+                            const int pos = s.pos0 + tok;
+                            if (key >= s.end || (c.causal && key > pos) || (c.window > 0 && pos - key >= c.window))
+                                x = -INFINITY;
+                        }
+                        acc[k][j][e] = x;
+                        rise |= x > limit[j][e & 1];
                     }
-                    const uint32_t a0[4] = {h2u(ha[0]), h2u(hb[0]), h2u(ha[1]), h2u(hb[1])};
-                    const uint32_t a1[4] = {h2u(ha[2]), h2u(hb[2]), h2u(ha[3]), h2u(hb[3])};
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        mma16816(acc[j], a0, q[j][2 * x][0], q[j][2 * x][1]);
-                        mma16816(acc[j], a1, q[j][2 * x + 1][0], q[j][2 * x + 1][1]);
-                    }
-                }
-                // ---- weights
-                bool rise = false;
+            if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float x = acc[j][e] * sc;
-                        if (!whole || edge_cols) {
-                            const int k = k0 + kg + (e & 2 ? 8 : 0);
-                            if (k < from[j][e & 1] || k >= to[j][e & 1]) x = -INFINITY;
-                        }
-                        acc[j][e] = x;
-                        rise |= x > m[j][e & 1] + kLazy;
-                    }
-                }
-                if (__any_sync(0xffffffffu, rise)) {
+                    for (int e = 0; e < 2; ++e) {
+                        float top = fmaxf(acc[0][j][e], acc[0][j][e + 2]);
+                        if (KB > 1) top = fmaxf(top, fmaxf(acc[KB - 1][j][e], acc[KB - 1][j][e + 2]));
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            float top = fmaxf(acc[j][e], acc[j][e + 2]);
-#pragma unroll
-                            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                            const float now = fmaxf(m[j][e], top);
-                            const float fix = now > m[j][e] ? ex2(m[j][e] - now) : 1.0f;
-                            m[j][e] = now;
+                        for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        if (limit[j][e] != -INFINITY) top = fmaxf(top, base[j][e]);
+                        if (top != -INFINITY) {
+                            const float fix = limit[j][e] == -INFINITY ? 0.0f : ex2(base[j][e] - top);
+                            base[j][e] = top;
+                            limit[j][e] = top + kLazy;
                             l[j][e] *= fix;
 #pragma unroll
                             for (int x = 0; x < D / 16; ++x) {
@@ -398,69 +424,78 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2)
                         }
                     }
                 }
-                uint32_t hi[NT][2], lo[NT][2];
+            }
+            uint32_t hi[KB][NT][2], lo[KB][NT][2];
+#pragma unroll
+            for (int k = 0; k < KB; ++k)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const float m0 = m[j][0] == -INFINITY ? 0.0f : m[j][0], m1 = m[j][1] == -INFINITY ? 0.0f : m[j][1];
                     float p[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) p[e] = ex2(acc[j][e] - ((e & 1) ? m1 : m0));
+                    for (int e = 0; e < 4; ++e) p[e] = ex2(acc[k][j][e] - base[j][e & 1]);
                     l[j][0] += p[0] + p[2];
                     l[j][1] += p[1] + p[3];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const __half2 h = __floats2half2_rn(p[2 * e], p[2 * e + 1]);
                         const float2 f = __half22float2(h);
-                        hi[j][e] = movmatrix_t(h2u(h));
-                        lo[j][e] = movmatrix_t(h2u(__floats2half2_rn(p[2 * e] - f.x, p[2 * e + 1] - f.y)));
+                        const __half2 rest = __floats2half2_rn(p[2 * e] - f.x, p[2 * e + 1] - f.y);
+                        hi[k][j][e] = movmatrix_t(h2u(kPaired && t >= 2 ? rest : h));
+                        if (!kPaired) lo[k][j][e] = movmatrix_t(h2u(rest));
                     }
                 }
-                // ---- O^T
-                int vk[4];
+            // ---- O^T
 #pragma unroll
-                for (int e = 0; e < 4; ++e) vk[e] = kappa(2 * t + (e & 1) + (e & 2 ? 8 : 0));
-                uint32_t vw[4][D / 64], par[4];
-                const int grp = g * (D / 8) / ge.g;
+            for (int k = 0; k < KB; ++k) {
+            const uint8_t* const blk = blk0 + k * step_codes;
+            const uint8_t* const pars = blk0 + k * step_par;
+            uint32_t vw[4][D / 64], par[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint8_t* src = blk + (e & 1 ? v_codes1 : v_codes0) + (e & 2 ? 4 * D : 0);
+                if constexpr (D == 64) vw[e][0] = *reinterpret_cast<const uint32_t*>(src);
+                if constexpr (D == 128) *reinterpret_cast<uint2*>(vw[e]) = *reinterpret_cast<const uint2*>(src);
+                if constexpr (D == 256) *reinterpret_cast<uint4*>(vw[e]) = *reinterpret_cast<const uint4*>(src);
+                par[e] = *reinterpret_cast<const uint32_t*>(pars + (e & 1 ? v_par1 : v_par0) + (e & 2 ? 8 * row_p : 0));
+            }
+            if (!whole) {  // rows that nobody sees may hold anything: they count as zeros
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint8_t* src = vc + vk[e] * (D / 2) + g * (D / 16);
-                    if constexpr (D == 64) vw[e][0] = *reinterpret_cast<const uint32_t*>(src);
-                    if constexpr (D == 128) *reinterpret_cast<uint2*>(vw[e]) = *reinterpret_cast<const uint2*>(src);
-                    if constexpr (D == 256) *reinterpret_cast<uint4*>(vw[e]) = *reinterpret_cast<const uint4*>(src);
-                    par[e] = *reinterpret_cast<const uint32_t*>(vp + (vk[e] * ng + grp) * 4);
-                    // rows that nobody sees may hold anything: they count as zeros
-                    if (!whole && (k0 + vk[e] < s.start || k0 + vk[e] >= s.end)) par[e] = 0;
+                    const int key = k0[k] + (e & 1 ? vk1 : vk0) + (e & 2 ? 8 : 0);
+                    if (key < s.start || key >= s.end) par[e] = 0;
                 }
-                const __half2 s01 = u2h(__byte_perm(par[0], par[1], 0x5410)), l01 = u2h(__byte_perm(par[0], par[1], 0x7632));
-                const __half2 s23 = u2h(__byte_perm(par[2], par[3], 0x5410)), l23 = u2h(__byte_perm(par[2], par[3], 0x7632));
+            }
+            const __half2 s01 = u2h(__byte_perm(par[0], par[1], 0x5410)), l01 = u2h(__byte_perm(par[0], par[1], 0x7632));
+            const __half2 s23 = u2h(__byte_perm(par[2], par[3], 0x5410)), l23 = u2h(__byte_perm(par[2], par[3], 0x7632));
 #pragma unroll
-                for (int x = 0; x < D / 64; ++x) {
+            for (int x = 0; x < D / 64; ++x) {
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {  // dims 8 x + 4 y .. + 3 of the lane's D / 8
-                        const unsigned sel = y ? 0x7632 : 0x5410;
-                        __half2 a[4], b[4];
-                        codes_to_half(__byte_perm(vw[0][x], vw[1][x], sel), a);
-                        codes_to_half(__byte_perm(vw[2][x], vw[3][x], sel), b);
+                for (int y = 0; y < 2; ++y) {  // dims 8 x + 4 y .. + 3 of the lane's D / 8
+                    const unsigned sel = y ? 0x7632 : 0x5410;
+                    __half2 a[4], b[4];
+                    codes_to_half(__byte_perm(vw[0][x], vw[1][x], sel), a);
+                    codes_to_half(__byte_perm(vw[2][x], vw[3][x], sel), b);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            a[e] = __hfma2(a[e], s01, l01);
-                            b[e] = __hfma2(b[e], s23, l23);
-                        }
-                        const uint32_t f0[4] = {h2u(a[0]), h2u(a[1]), h2u(b[0]), h2u(b[1])};
-                        const uint32_t f1[4] = {h2u(a[2]), h2u(a[3]), h2u(b[2]), h2u(b[3])};
+                    for (int e = 0; e < 4; ++e) {
+                        a[e] = __hfma2(a[e], s01, l01);
+                        b[e] = __hfma2(b[e], s23, l23);
+                    }
+                    const uint32_t f0[4] = {h2u(a[0]), h2u(a[1]), h2u(b[0]), h2u(b[1])};
+                    const uint32_t f1[4] = {h2u(a[2]), h2u(a[3]), h2u(b[2]), h2u(b[3])};
 #pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            mma16816(o[j][4 * x + 2 * y], f0, hi[j][0], hi[j][1]);
-                            mma16816(o[j][4 * x + 2 * y + 1], f1, hi[j][0], hi[j][1]);
-                            mma16816(o[j][4 * x + 2 * y], f0, lo[j][0], lo[j][1]);
-                            mma16816(o[j][4 * x + 2 * y + 1], f1, lo[j][0], lo[j][1]);
-                        }
+                    for (int j = 0; j < NT; ++j) {
+                        mma16816(o[j][4 * x + 2 * y], f0, hi[k][j][0], hi[k][j][1]);
+                        mma16816(o[j][4 * x + 2 * y + 1], f1, hi[k][j][0], hi[k][j][1]);
+                        if (kPaired) continue;
+                        mma16816(o[j][4 * x + 2 * y], f0, lo[k][j][0], lo[k][j][1]);
+                        mma16816(o[j][4 * x + 2 * y + 1], f1, lo[k][j][0], lo[k][j][1]);
                     }
                 }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[slot]);
+            }
         }
+        cp_async_wait<0>();
+        __syncthreads();
 
         // ---- the four warps' states -> one; fragment row g of step x is dim 2 x (row g + 8: 2 x + 1)
         // of lane g's D / 8, kept at column dim * 8 + g
@@ -473,17 +508,17 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2)
                 for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
                 const int r = 8 * j + 2 * t + e;
                 if (g == 0) {
-                    sm.m[warp][r] = m[j][e];
+                    sm.m[warp][r] = limit[j][e] == -INFINITY ? -INFINITY : base[j][e];
                     sm.l[warp][r] = sum;
                 }
 #pragma unroll
                 for (int x = 0; x < D / 16; ++x) {
-                    sm.o[warp][r][(2 * x) * 8 + g] = o[j][x][e];
-                    sm.o[warp][r][(2 * x + 1) * 8 + g] = o[j][x][e + 2];
+                    s_o[(warp * kCols + r) * kPad + (2 * x) * 8 + g] = o[j][x][e];
+                    s_o[(warp * kCols + r) * kPad + (2 * x + 1) * 8 + g] = o[j][x][e + 2];
                 }
             }
-        consumer_sync();
-        constexpr int kPer = D / 8, kPasses = kRows * kPer / 128 ? kRows * kPer / 128 : 1;  // 8 dims a thread
+        __syncthreads();
+        constexpr int kPer = D / 8, kPasses = ROWS * kPer > 128 ? ROWS * kPer / 128 : 1;  // 8 dims a thread
         const long long item = wk.item0 + it, item_tile = wk.base + (long long)it * s.ntiles;
         const bool alone = ntile == s.ntiles;
         float* part = parts + ((size_t)blockIdx.x * 2 + (item_tile < w0 ? 0 : 1)) * kMaxPartFloats;
@@ -494,18 +529,19 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2)
             if (r >= rows) continue;
             mm[p] = -INFINITY;
 #pragma unroll
-            for (int x = 0; x < kConsumers; ++x) mm[p] = fmaxf(mm[p], sm.m[x][r]);
+            for (int x = 0; x < kWarps; ++x) mm[p] = fmaxf(mm[p], sm.m[x][r]);
             ll[p] = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[p][e] = 0.0f;
 #pragma unroll
-            for (int x = 0; x < kConsumers; ++x) {
+            for (int x = 0; x < kWarps; ++x) {
                 const float f = sm.m[x][r] == -INFINITY ? (sm.l[x][r] != sm.l[x][r] ? 1.0f : 0.0f) : ex2(sm.m[x][r] - mm[p]);
                 ll[p] = fmaf(sm.l[x][r], f, ll[p]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     const int d = d8 * 8 + e;
-                    v[p][e] = fmaf(sm.o[x][r][(d % (D / 8)) * 8 + d / (D / 8)], f, v[p][e]);
+                    const float* at = s_o + (x * kCols + r) * kPad + (d % (D / 8)) * 8 + d / (D / 8);
+                    v[p][e] = fmaf(kPaired ? at[0] + at[4 * kPad] : at[0], f, v[p][e]);
                 }
             }
             if (!alone) {
@@ -513,21 +549,21 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2)
                 dst[0] = make_float4(v[p][0], v[p][1], v[p][2], v[p][3]);
                 dst[1] = make_float4(v[p][4], v[p][5], v[p][6], v[p][7]);
                 if (d8 == 0) {
-                    part[kRows * D + r] = mm[p];
-                    part[kRows * D + kRows + r] = ll[p];
+                    part[ROWS * D + r] = mm[p];
+                    part[ROWS * D + ROWS + r] = ll[p];
                 }
             }
         }
         bool last = alone;
         if (!alone) {
             __threadfence();
-            consumer_sync();
+            __syncthreads();
             if (tid == 0) {
                 const unsigned before = atomicAdd(&counters[item], (unsigned)ntile);
                 sm.last = before + (unsigned)ntile == (unsigned)s.ntiles;
                 if (sm.last) counters[item] = 0;
             }
-            consumer_sync();
+            __syncthreads();
             last = sm.last != 0;
             if (last) {
                 __threadfence();
@@ -544,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2)
 #pragma unroll 4
                     for (int x = c0; x <= c1; ++x) {
                         const float* src = parts + ((size_t)x * 2 + (item_tile < total * x / n ? 0 : 1)) * kMaxPartFloats;
-                        const float pm = __ldcg(src + kRows * D + r), pl = __ldcg(src + kRows * D + kRows + r);
+                        const float pm = __ldcg(src + ROWS * D + r), pl = __ldcg(src + ROWS * D + ROWS + r);
                         const float4 a = __ldcg(reinterpret_cast<const float4*>(src + r * D + d8 * 8));
                         const float4 b = __ldcg(reinterpret_cast<const float4*>(src + r * D + d8 * 8) + 1);
                         const float now = fmaxf(mm[p], pm);
@@ -580,41 +616,43 @@ __global__ void __launch_bounds__(kThreads, D * NT <= 128 ? 4 : 2)
                 if (nan) atomicOr(&sm.nan, 1 << r);
             }
         }
-        consumer_sync();
+        __syncthreads();
         // A NaN among the values of a row that some of these queries see reaches all of them through
         // the products with weight zero: such rows are computed again one by one.
         const int nan = sm.nan;
         if (nan) {
-            for (int r = warp; r < rows; r += kConsumers)
+            for (int r = warp; r < rows; r += kWarps)
                 if (nan >> r & 1)
                     attention_row<D>(c, pg, ge, wk.b, tok0 + (row0 + r) / share, qhead0 + (row0 + r) % share, lane);
-            consumer_sync();
-            if (tid == 0) sm.nan = 0;
+            __syncthreads();
+            if (tid == 0) {
+        sm.nan = 0;
+    }
         }
         w += ntile;
     }
 }
 
-template <int D, int NT>
+template <int D, int ROWS>
 int launch(const AttnCall& c, const Pages& pg, const Geom& ge, cudaStream_t st) {
-    auto kernel = kv4_decode_kernel<D, NT>;
-    constexpr int kPerSm = D * NT <= 128 ? 4 : 2;
-    // as many stages as fit with the CTAs that the registers allow (1 KB of each is the system's)
-    const int room = 227 * 1024 / kPerSm - 1024 - (int)sizeof(Smem<D, NT>) - 512;
-    int stages = room / stage_bytes<D>(ge.ng());
-    stages = stages > 8 ? 8 : stages < 2 ? 2 : stages;
-    const int smem = stages * stage_bytes<D>(ge.ng());
-    static int most = 0;
-    if (smem > most) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return -1;
-        most = smem;
+    auto kernel = kv4_decode_kernel<D, ROWS>;
+    constexpr int kPerSm = ctas_per_sm<D, ROWS>(), kBlocks = kWarps * stages<D, ROWS>() * blocks<D, ROWS>() * 16, kMost = kBlocks * (D + 8 * (D / 32));
+    const int smem = kBlocks * (D + 8 * ge.ng());
+    if (kMost > 48 * 1024) {
+        static std::atomic<unsigned long long> set{0};  // a bit a device
+        int dev = 0;
+        cudaGetDevice(&dev);
+        if (!(set.load() >> (dev & 63) & 1)) {
+            if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost) != cudaSuccess) return -1;
+            set.fetch_or(1ull << (dev & 63));
+        }
     }
     // no more CTAs than the tables have room for tiles
     const int share = c.hq / ge.hkv;
-    const long long rows_most = (long long)c.max_q * share, tiles = (pg.table_stride * ge.page() + kTile - 1) / kTile + 1;
-    const double bound = (double)c.num_seqs * ge.hkv * ((rows_most + 8 * NT - 1) / (8 * NT)) * tiles;
+    const long long rows_most = (long long)c.max_q * share, tiles = pg.table_stride * ge.page() / (16 * blocks<D, ROWS>() * kWarps) + 2;
+    const double bound = (double)c.num_seqs * ge.hkv * ((rows_most + ROWS - 1) / ROWS) * tiles;
     const unsigned grid = (unsigned)(bound < kNumSMs * kPerSm ? bound : kNumSMs * kPerSm);
-    return launch_k(kernel, dim3(grid), dim3(kThreads), (size_t)smem, st, c, pg, ge, stages) == cudaSuccess ? 0 : -1;
+    return launch_k(kernel, dim3(grid), dim3(kThreads), (size_t)smem, st, c, pg, ge) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace
@@ -628,9 +666,9 @@ size_t decode_workspace(int num_seqs, int num_tokens, int hq, int hkv) {
 int launch_decode(const AttnCall& c, const Pages& pg, const Geom& ge, cudaStream_t st) {
     const int rows = c.max_q * (c.hq / ge.hkv);
     switch (ge.d) {
-        case 64: return rows <= 8 ? launch<64, 1>(c, pg, ge, st) : launch<64, 2>(c, pg, ge, st);
-        case 128: return rows <= 8 ? launch<128, 1>(c, pg, ge, st) : launch<128, 2>(c, pg, ge, st);
-        default: return launch<256, 1>(c, pg, ge, st);
+        case 64: return rows <= 4 ? launch<64, 4>(c, pg, ge, st) : rows <= 8 ? launch<64, 8>(c, pg, ge, st) : launch<64, 16>(c, pg, ge, st);
+        case 128: return rows <= 4 ? launch<128, 4>(c, pg, ge, st) : rows <= 8 ? launch<128, 8>(c, pg, ge, st) : launch<128, 16>(c, pg, ge, st);
+        default: return rows <= 4 ? launch<256, 4>(c, pg, ge, st) : launch<256, 8>(c, pg, ge, st);
     }
 }
 

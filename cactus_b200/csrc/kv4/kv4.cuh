@@ -58,19 +58,26 @@ __device__ __forceinline__ int find_seq(const int* offsets, int n, int t) {
     return lo;
 }
 
+__device__ __forceinline__ __half2 as_half2(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// (w & MASK) | 0x64006400 as one instruction (the compiler makes two of the expression)
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t mask_magic(uint32_t w) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(w), "n"(MASK), "r"(0x64006400u));
+    return r;
+}
+
 // Eight codes (element i in bits 4i..4i+3) as exact fp16 integers, in the order (0, 4), (1, 5),
-// (2, 6), (3, 7): 0x6400 | c is the fp16 number 1024 + c, and 0x6400 | (c << 4) is 1024 + 16 c.
+// (2, 6), (3, 7): 0x6400 | c is the fp16 number 1024 + c, and 0x6400 | (c << 4) is 1024 + 16 c. The
+// shift by 8 is a multiplication, which does not compete with the masks for the logic unit.
 __device__ __forceinline__ void codes_to_half(uint32_t w, __half2 (&h)[4]) {
-    const uint32_t k = 0x64006400u;
-    const __half2 m1024 = __floats2half2_rn(-1024.0f, -1024.0f);
-    const __half2 r16 = __floats2half2_rn(0.0625f, 0.0625f), m64 = __floats2half2_rn(-64.0f, -64.0f);
+    const uint32_t n1024 = 0xE400E400u, r16 = 0x2C002C00u, n64 = 0xD400D400u;  // -1024, 1/16, -64
     const uint32_t w8 = w >> 8;
-    uint32_t a0 = (w & 0x000F000Fu) | k, a1 = (w & 0x00F000F0u) | k;
-    uint32_t a2 = (w8 & 0x000F000Fu) | k, a3 = (w8 & 0x00F000F0u) | k;
-    h[0] = __hadd2(*reinterpret_cast<__half2*>(&a0), m1024);
-    h[1] = __hfma2(*reinterpret_cast<__half2*>(&a1), r16, m64);
-    h[2] = __hadd2(*reinterpret_cast<__half2*>(&a2), m1024);
-    h[3] = __hfma2(*reinterpret_cast<__half2*>(&a3), r16, m64);
+    h[0] = __hadd2(as_half2(mask_magic<0x000F000Fu>(w)), as_half2(n1024));
+    h[1] = __hfma2(as_half2(mask_magic<0x00F000F0u>(w)), as_half2(r16), as_half2(n64));
+    h[2] = __hadd2(as_half2(mask_magic<0x000F000Fu>(w8)), as_half2(n1024));
+    h[3] = __hfma2(as_half2(mask_magic<0x00F000F0u>(w8)), as_half2(r16), as_half2(n64));
 }
 
 }  // namespace kv4
