@@ -114,9 +114,9 @@ struct Smem {
     static constexpr int kCols = columns<ROWS>();
     uint4 q[kCols / 8][D / 32][32];
     float m[kWarps][kCols], l[kWarps][kCols];
-    long long scan[kThreads], scan_items[kThreads];
-    long long base, item0;  // of the sequence that this CTA starts with: its first tile, its first item
-    int b0, last, nan;
+    int scan[kWarps], scan_items[kWarps];
+    int base, item0, b0;  // the sequence that this CTA starts with: its first tile, its first item
+    int last, nan;
 };
 
 template <int D, int ROWS>
@@ -133,34 +133,51 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
 
     // ---- the list of tiles, and this CTA's part of it
     const int per = (c.num_seqs + kThreads - 1) / kThreads, first_b = tid * per;
-    long long mine = 0, items = 0;
+    int mine = 0, items = 0;
     for (int b = first_b; b < min(first_b + per, c.num_seqs); ++b) {
         const Seq s = seq_of<ROWS, kTile>(c, pg, ge, b, blockIdx.x == 0);
-        mine += (long long)s.row_tiles * ge.hkv * s.ntiles;
-        items += (long long)s.row_tiles * ge.hkv;
+        mine += s.row_tiles * ge.hkv * s.ntiles;
+        items += s.row_tiles * ge.hkv;
     }
-    sm.scan[tid] = mine;
-    sm.scan_items[tid] = items;
-    if (tid == 0) {
-        sm.nan = 0;
+    int upto = mine, items_upto = items;  // sums over this thread and those before it
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int a = __shfl_up_sync(0xffffffffu, upto, o), i = __shfl_up_sync(0xffffffffu, items_upto, o);
+        if (lane >= o) {
+            upto += a;
+            items_upto += i;
+        }
     }
+    if (lane == 31) {
+        sm.scan[warp] = upto;
+        sm.scan_items[warp] = items_upto;
+    }
+    if (tid == 0) sm.nan = 0;
     __syncthreads();
-    for (int o = 1; o < kThreads; o <<= 1) {
-        const long long a = tid >= o ? sm.scan[tid - o] : 0, i = tid >= o ? sm.scan_items[tid - o] : 0;
-        __syncthreads();
-        sm.scan[tid] += a;
-        sm.scan_items[tid] += i;
-        __syncthreads();
+    int total = 0;
+#pragma unroll
+    for (int x = 0; x < kWarps; ++x) {
+        if (x < warp) {
+            upto += sm.scan[x];
+            items_upto += sm.scan_items[x];
+        }
+        total += sm.scan[x];
     }
-    const long long total = sm.scan[kThreads - 1];
-    const int n = (int)min((long long)gridDim.x, total);
+    // CTA x of n has the tiles first_tile(x) .. first_tile(x + 1) - 1: as many as the others, or one more
+    const int n = min((int)gridDim.x, total);
     if ((int)blockIdx.x >= n) return;
-    const long long w0 = total * blockIdx.x / n, w1 = total * (blockIdx.x + 1) / n;
-    if (w0 >= sm.scan[tid] - mine && w0 < sm.scan[tid]) {
-        long long at = sm.scan[tid] - mine, it = sm.scan_items[tid] - items;
+    const int each = total / n, more = total - each * n;
+    auto first_tile = [&](int x) { return x * each + min(x, more); };
+    auto owner = [&](int tile) {
+        const int lead = more * (each + 1);
+        return tile < lead ? tile / (each + 1) : more + (tile - lead) / each;
+    };
+    const int w0 = first_tile(blockIdx.x), w1 = first_tile(blockIdx.x + 1);
+    if (w0 >= upto - mine && w0 < upto) {
+        int at = upto - mine, it = items_upto - items;
         for (int b = first_b;; ++b) {
             const Seq s = seq_of<ROWS, kTile>(c, pg, ge, b, false);
-            const long long k = (long long)s.row_tiles * ge.hkv;
+            const int k = s.row_tiles * ge.hkv;
             if (w0 < at + k * s.ntiles) {
                 sm.b0 = b;
                 sm.base = at;
@@ -174,18 +191,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
     __syncthreads();
     // walks the items of [w0, w1): item `it` of sequence b (kv head it / row_tiles), tiles t .. t + k - 1
     struct Walk {
-        int b;
-        long long base, item0;
+        int b, base, item0;
         Seq s;
     } wk;
     wk.b = sm.b0;
     wk.base = sm.base;
     wk.item0 = sm.item0;
     wk.s = seq_of<ROWS, kTile>(c, pg, ge, wk.b, false);
-    auto next_seq = [&](long long w) {  // moves to the sequence that tile w belongs to
-        while (w >= wk.base + (long long)wk.s.row_tiles * ge.hkv * wk.s.ntiles) {
-            wk.base += (long long)wk.s.row_tiles * ge.hkv * wk.s.ntiles;
-            wk.item0 += (long long)wk.s.row_tiles * ge.hkv;
+    auto next_seq = [&](int w) {  // moves to the sequence that tile w belongs to
+        while (w >= wk.base + wk.s.row_tiles * ge.hkv * wk.s.ntiles) {
+            wk.base += wk.s.row_tiles * ge.hkv * wk.s.ntiles;
+            wk.item0 += wk.s.row_tiles * ge.hkv;
             ++wk.b;
             wk.s = seq_of<ROWS, kTile>(c, pg, ge, wk.b, false);
         }
@@ -215,13 +231,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
     const uint32_t ring_at = smem_u32(mine_ring) + lane * 16;
     const bool copies_par = lane < R * ng / 4;  // 16-byte pieces of R rows' parameters: at most 32
 
-    for (long long w = w0; w < w1;) {
+    for (int w = w0; w < w1;) {
         next_seq(w);
         const Seq s = wk.s;
-        const long long rel = w - wk.base;
-        const int it = (int)(rel / s.ntiles), tile0 = (int)(rel % s.ntiles);
-        const int head = it / s.row_tiles, row0 = (it % s.row_tiles) * ROWS;
-        const int ntile = (int)min((long long)(s.ntiles - tile0), w1 - w);
+        const int it = (w - wk.base) / s.ntiles, tile0 = w - wk.base - it * s.ntiles;
+        const int head = s.row_tiles == 1 ? it : it / s.row_tiles, row0 = (it - head * s.row_tiles) * ROWS;
+        const int ntile = min(s.ntiles - tile0, w1 - w);
         const int tok0 = c.offsets[wk.b], rows = min(ROWS, s.tokens * share - row0);
         const int qhead0 = head * share;
 
@@ -519,14 +534,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
             }
         __syncthreads();
         constexpr int kPer = D / 8, kPasses = ROWS * kPer > 128 ? ROWS * kPer / 128 : 1;  // 8 dims a thread
-        const long long item = wk.item0 + it, item_tile = wk.base + (long long)it * s.ntiles;
+        const int item = wk.item0 + it, item_tile = wk.base + it * s.ntiles;
         const bool alone = ntile == s.ntiles;
         float* part = parts + ((size_t)blockIdx.x * 2 + (item_tile < w0 ? 0 : 1)) * kMaxPartFloats;
         float mm[kPasses], ll[kPasses], v[kPasses][8];
 #pragma unroll
         for (int p = 0; p < kPasses; ++p) {
-            const int r = tid / kPer + p * (128 / kPer), d8 = tid % kPer;
-            if (r >= rows) continue;
+            // threads past the last row repeat it (no divergence up to the barriers) and store nothing
+            const int mine_r = tid / kPer + p * (128 / kPer), r = min(mine_r, rows - 1), d8 = tid % kPer;
             mm[p] = -INFINITY;
 #pragma unroll
             for (int x = 0; x < kWarps; ++x) mm[p] = fmaxf(mm[p], sm.m[x][r]);
@@ -544,7 +559,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
                     v[p][e] = fmaf(kPaired ? at[0] + at[4 * kPad] : at[0], f, v[p][e]);
                 }
             }
-            if (!alone) {
+            if (!alone && mine_r == r) {
                 float4* dst = reinterpret_cast<float4*>(part + r * D + d8 * 8);
                 dst[0] = make_float4(v[p][0], v[p][1], v[p][2], v[p][3]);
                 dst[1] = make_float4(v[p][4], v[p][5], v[p][6], v[p][7]);
@@ -555,6 +570,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
             }
         }
         bool last = alone;
+        __syncwarp();
         if (!alone) {
             __threadfence();
             __syncthreads();
@@ -567,19 +583,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
             last = sm.last != 0;
             if (last) {
                 __threadfence();
-                const int c0 = (int)(((item_tile + 1) * n - 1) / total);
-                const int c1 = (int)(((item_tile + s.ntiles) * n - 1) / total);
+                const int c0 = owner(item_tile), c1 = owner(item_tile + s.ntiles - 1);
 #pragma unroll
                 for (int p = 0; p < kPasses; ++p) {
-                    const int r = tid / kPer + p * (128 / kPer), d8 = tid % kPer;
-                    if (r >= rows) continue;
+                    const int r = min(tid / kPer + p * (128 / kPer), rows - 1), d8 = tid % kPer;
                     mm[p] = -INFINITY;
                     ll[p] = 0.0f;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) v[p][e] = 0.0f;
-#pragma unroll 4
+#pragma unroll 8
                     for (int x = c0; x <= c1; ++x) {
-                        const float* src = parts + ((size_t)x * 2 + (item_tile < total * x / n ? 0 : 1)) * kMaxPartFloats;
+                        const float* src = parts + ((size_t)x * 2 + (item_tile < first_tile(x) ? 0 : 1)) * kMaxPartFloats;
                         const float pm = __ldcg(src + ROWS * D + r), pl = __ldcg(src + ROWS * D + ROWS + r);
                         const float4 a = __ldcg(reinterpret_cast<const float4*>(src + r * D + d8 * 8));
                         const float4 b = __ldcg(reinterpret_cast<const float4*>(src + r * D + d8 * 8) + 1);
@@ -598,8 +612,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
         if (last) {
 #pragma unroll
             for (int p = 0; p < kPasses; ++p) {
-                const int r = tid / kPer + p * (128 / kPer), d8 = tid % kPer;
-                if (r >= rows) continue;
+                const int mine_r = tid / kPer + p * (128 / kPer), r = min(mine_r, rows - 1), d8 = tid % kPer;
                 const int tok = tok0 + (row0 + r) / share, h = qhead0 + (row0 + r) % share;
                 const float inv = ll[p] > 0.0f ? 1.0f / ll[p] : 0.0f;
                 bool nan = ll[p] != ll[p];
@@ -611,11 +624,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
                     out[e] = __floats2half2_rn(a, b);
                 }
                 const long long at = (long long)tok * c.hq + h;
-                *reinterpret_cast<uint4*>(c.out + at * D + d8 * 8) = *reinterpret_cast<const uint4*>(out);
-                if (d8 == 0 && c.lse) c.lse[at] = ll[p] > 0.0f ? (mm[p] + log2f(ll[p])) * 0.6931471805599453f : -INFINITY;
+                if (mine_r == r) *reinterpret_cast<uint4*>(c.out + at * D + d8 * 8) = *reinterpret_cast<const uint4*>(out);
+                if (mine_r == r && d8 == 0 && c.lse)
+                    c.lse[at] = ll[p] > 0.0f ? (mm[p] + log2f(ll[p])) * 0.6931471805599453f : -INFINITY;
                 if (nan) atomicOr(&sm.nan, 1 << r);
             }
         }
+        __syncwarp();
         __syncthreads();
         // A NaN among the values of a row that some of these queries see reaches all of them through
         // the products with weight zero: such rows are computed again one by one.
@@ -625,9 +640,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
                 if (nan >> r & 1)
                     attention_row<D>(c, pg, ge, wk.b, tok0 + (row0 + r) / share, qhead0 + (row0 + r) % share, lane);
             __syncthreads();
-            if (tid == 0) {
-        sm.nan = 0;
-    }
+            if (tid == 0) sm.nan = 0;
         }
         w += ntile;
     }
@@ -651,6 +664,7 @@ int launch(const AttnCall& c, const Pages& pg, const Geom& ge, cudaStream_t st) 
     const int share = c.hq / ge.hkv;
     const long long rows_most = (long long)c.max_q * share, tiles = pg.table_stride * ge.page() / (16 * blocks<D, ROWS>() * kWarps) + 2;
     const double bound = (double)c.num_seqs * ge.hkv * ((rows_most + ROWS - 1) / ROWS) * tiles;
+    if (bound > 2147483647.0) return -2;  // tiles are counted in 31 bits
     const unsigned grid = (unsigned)(bound < kNumSMs * kPerSm ? bound : kNumSMs * kPerSm);
     return launch_k(kernel, dim3(grid), dim3(kThreads), (size_t)smem, st, c, pg, ge) == cudaSuccess ? 0 : -1;
 }

@@ -156,7 +156,8 @@ CB_API int cactus_cuda_kv4_attention(const uint16_t* queries, size_t query_strid
     c.window = window_size > kIntMax ? 0 : (long long)window_size;
     c.causal = is_causal != 0;
     c.ws = static_cast<uint8_t*>(workspace);
-    cb::kv4::launch_attention(c, pg, ge, S(stream));
+    if (cb::kv4::launch_attention(c, pg, ge, S(stream)) == -2)
+        return arg(name, "too many sequences of too wide a block table");
     return abi_check_launch(name);
 }
 
