@@ -24,7 +24,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libcactus_b200.so")
 ARCH = "-gencode=arch=compute_100a,code=sm_100a"
-WHOLE_PROGRAM = ("gemm_tc.cu",)
+WHOLE_PROGRAM = ("gemm_tc.cu", "prefill_tc.cu")
 
 
 def sources():

@@ -28,6 +28,7 @@
 // Softmax. The running maximum is raised only when a score exceeds it by more than 2^kLazy; until
 // then weights grow past 1 (at most 2^kLazy, far inside fp16), which is exact up to rounding and
 // saves the reduction over the lanes for almost every tile.
+#include <algorithm>
 #include <atomic>
 
 #include "attention.cuh"
@@ -41,10 +42,6 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr float kLazy = 8.0f;  // base-2 exponent
-constexpr int kMaxCtas = kNumSMs * 5;
-constexpr int kMaxPartFloats = 16 * (128 + 2);  // rows * (D + 2): 16 x 128 or 8 x 256 (2064) at most
-constexpr size_t kPartBytes = (size_t)kMaxCtas * 2 * kMaxPartFloats * 4;
-
 // row of the 16 that key i of the fragments is
 __device__ __forceinline__ int kappa(int i) { return (i & 8) + (((i & 7) >> 1) ^ ((i & 1) * 5)); }
 
@@ -79,13 +76,14 @@ struct Seq {
 };
 
 template <int ROWS, int TILE>
-__device__ __forceinline__ Seq seq_of(const AttnCall& c, const Pages& pg, const Geom& ge, int b, bool report) {
+__device__ __forceinline__ Seq seq_of(const AttnCall& c, const Pages& pg, const Geom& ge, int max_rows, int b, bool report) {
     Seq s;
     const int count = c.offsets[b + 1] - c.offsets[b], len = max(c.lens[b], 0);
     const int room = (int)(pg.table_stride << ge.page_shift);
     s.tokens = max(0, min(count, c.max_q));
     if (report && (count > c.max_q || (len > room && count > 0))) report_dev_error(kDevBadPage);
-    s.row_tiles = (s.tokens * (c.hq / ge.hkv) + ROWS - 1) / ROWS;
+    const int rows = s.tokens * (c.hq / ge.hkv);
+    s.row_tiles = rows > max_rows ? 0 : (rows + ROWS - 1) / ROWS;
     s.pos0 = len - count;
     const int n = min(len, room);
     s.end = c.causal ? min(n, s.pos0 + s.tokens) : n;
@@ -121,7 +119,8 @@ struct Smem {
 
 template <int D, int ROWS>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
-    kv4_decode_kernel(const __grid_constant__ AttnCall c, const __grid_constant__ Pages pg, const __grid_constant__ Geom ge) {
+    kv4_decode_kernel(const __grid_constant__ AttnCall c, const __grid_constant__ Pages pg, const __grid_constant__ Geom ge,
+                      int max_rows) {
     pdl_launch_dependents();
     pdl_wait();
     constexpr int kCols = columns<ROWS>(), NT = kCols / 8, KB = blocks<D, ROWS>(), kTile = 16 * KB * kWarps, kStages = stages<D, ROWS>(), kPad = D + 4;
@@ -135,7 +134,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
     const int per = (c.num_seqs + kThreads - 1) / kThreads, first_b = tid * per;
     int mine = 0, items = 0;
     for (int b = first_b; b < min(first_b + per, c.num_seqs); ++b) {
-        const Seq s = seq_of<ROWS, kTile>(c, pg, ge, b, blockIdx.x == 0);
+        const Seq s = seq_of<ROWS, kTile>(c, pg, ge, max_rows, b, blockIdx.x == 0);
         mine += s.row_tiles * ge.hkv * s.ntiles;
         items += s.row_tiles * ge.hkv;
     }
@@ -176,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
     if (w0 >= upto - mine && w0 < upto) {
         int at = upto - mine, it = items_upto - items;
         for (int b = first_b;; ++b) {
-            const Seq s = seq_of<ROWS, kTile>(c, pg, ge, b, false);
+            const Seq s = seq_of<ROWS, kTile>(c, pg, ge, max_rows, b, false);
             const int k = s.row_tiles * ge.hkv;
             if (w0 < at + k * s.ntiles) {
                 sm.b0 = b;
@@ -197,13 +196,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
     wk.b = sm.b0;
     wk.base = sm.base;
     wk.item0 = sm.item0;
-    wk.s = seq_of<ROWS, kTile>(c, pg, ge, wk.b, false);
+    wk.s = seq_of<ROWS, kTile>(c, pg, ge, max_rows, wk.b, false);
     auto next_seq = [&](int w) {  // moves to the sequence that tile w belongs to
         while (w >= wk.base + wk.s.row_tiles * ge.hkv * wk.s.ntiles) {
             wk.base += wk.s.row_tiles * ge.hkv * wk.s.ntiles;
             wk.item0 += wk.s.row_tiles * ge.hkv;
             ++wk.b;
-            wk.s = seq_of<ROWS, kTile>(c, pg, ge, wk.b, false);
+            wk.s = seq_of<ROWS, kTile>(c, pg, ge, max_rows, wk.b, false);
         }
     };
 
@@ -536,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
         constexpr int kPer = D / 8, kPasses = ROWS * kPer > 128 ? ROWS * kPer / 128 : 1;  // 8 dims a thread
         const int item = wk.item0 + it, item_tile = wk.base + it * s.ntiles;
         const bool alone = ntile == s.ntiles;
-        float* part = parts + ((size_t)blockIdx.x * 2 + (item_tile < w0 ? 0 : 1)) * kMaxPartFloats;
+        float* part = parts + ((size_t)blockIdx.x * 2 + (item_tile < w0 ? 0 : 1)) * kDecodePartFloats;
         float mm[kPasses], ll[kPasses], v[kPasses][8];
 #pragma unroll
         for (int p = 0; p < kPasses; ++p) {
@@ -593,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
                     for (int e = 0; e < 8; ++e) v[p][e] = 0.0f;
 #pragma unroll 8
                     for (int x = c0; x <= c1; ++x) {
-                        const float* src = parts + ((size_t)x * 2 + (item_tile < first_tile(x) ? 0 : 1)) * kMaxPartFloats;
+                        const float* src = parts + ((size_t)x * 2 + (item_tile < first_tile(x) ? 0 : 1)) * kDecodePartFloats;
                         const float pm = __ldcg(src + ROWS * D + r), pl = __ldcg(src + ROWS * D + ROWS + r);
                         const float4 a = __ldcg(reinterpret_cast<const float4*>(src + r * D + d8 * 8));
                         const float4 b = __ldcg(reinterpret_cast<const float4*>(src + r * D + d8 * 8) + 1);
@@ -647,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
 }
 
 template <int D, int ROWS>
-int launch(const AttnCall& c, const Pages& pg, const Geom& ge, cudaStream_t st) {
+int launch(const AttnCall& c, const Pages& pg, const Geom& ge, int max_rows, cudaStream_t st) {
     auto kernel = kv4_decode_kernel<D, ROWS>;
     constexpr int kPerSm = ctas_per_sm<D, ROWS>(), kBlocks = kWarps * stages<D, ROWS>() * blocks<D, ROWS>() * 16, kMost = kBlocks * (D + 8 * (D / 32));
     const int smem = kBlocks * (D + 8 * ge.ng());
@@ -662,27 +661,33 @@ int launch(const AttnCall& c, const Pages& pg, const Geom& ge, cudaStream_t st) 
     }
     // no more CTAs than the tables have room for tiles
     const int share = c.hq / ge.hkv;
-    const long long rows_most = (long long)c.max_q * share, tiles = pg.table_stride * ge.page() / (16 * blocks<D, ROWS>() * kWarps) + 2;
+    const long long rows_most = std::min<long long>((long long)c.max_q * share, max_rows), tiles = pg.table_stride * ge.page() / (16 * blocks<D, ROWS>() * kWarps) + 2;
     const double bound = (double)c.num_seqs * ge.hkv * ((rows_most + ROWS - 1) / ROWS) * tiles;
     if (bound > 2147483647.0) return -2;  // tiles are counted in 31 bits
     const unsigned grid = (unsigned)(bound < kNumSMs * kPerSm ? bound : kNumSMs * kPerSm);
-    return launch_k(kernel, dim3(grid), dim3(kThreads), (size_t)smem, st, c, pg, ge) == cudaSuccess ? 0 : -1;
+    return launch_k(kernel, dim3(grid), dim3(kThreads), (size_t)smem, st, c, pg, ge, max_rows) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace
 
-size_t decode_workspace(int num_seqs, int num_tokens, int hq, int hkv) {
-    // a counter an item: at most a row tile of 8 per 8 rows, and one more a sequence, per kv head
-    const size_t items = ((size_t)num_tokens * (size_t)(hq / (hkv ? hkv : 1)) / 8 + (size_t)num_seqs) * (size_t)hkv;
-    return kPartBytes + (items * 4 + 15) / 16 * 16;
+size_t decode_counters(int num_seqs, int num_tokens, int hq, int hkv) {
+    // one an item: at most a row tile of 8 per 8 rows, and one more a sequence, per kv head
+    return ((size_t)num_tokens * (size_t)(hq / hkv) / 8 + (size_t)num_seqs) * (size_t)hkv;
 }
 
-int launch_decode(const AttnCall& c, const Pages& pg, const Geom& ge, cudaStream_t st) {
-    const int rows = c.max_q * (c.hq / ge.hkv);
+int launch_decode(const AttnCall& c, const Pages& pg, const Geom& ge, int max_rows, cudaStream_t st) {
+    const long long most = (long long)c.max_q * (c.hq / ge.hkv);
+    const int rows = (int)(most < max_rows ? most : max_rows);
     switch (ge.d) {
-        case 64: return rows <= 4 ? launch<64, 4>(c, pg, ge, st) : rows <= 8 ? launch<64, 8>(c, pg, ge, st) : launch<64, 16>(c, pg, ge, st);
-        case 128: return rows <= 4 ? launch<128, 4>(c, pg, ge, st) : rows <= 8 ? launch<128, 8>(c, pg, ge, st) : launch<128, 16>(c, pg, ge, st);
-        default: return rows <= 4 ? launch<256, 4>(c, pg, ge, st) : launch<256, 8>(c, pg, ge, st);
+        case 64:
+            return rows <= 4   ? launch<64, 4>(c, pg, ge, max_rows, st)
+                   : rows <= 8 ? launch<64, 8>(c, pg, ge, max_rows, st)
+                               : launch<64, 16>(c, pg, ge, max_rows, st);
+        case 128:
+            return rows <= 4   ? launch<128, 4>(c, pg, ge, max_rows, st)
+                   : rows <= 8 ? launch<128, 8>(c, pg, ge, max_rows, st)
+                               : launch<128, 16>(c, pg, ge, max_rows, st);
+        default: return rows <= 4 ? launch<256, 4>(c, pg, ge, max_rows, st) : launch<256, 8>(c, pg, ge, max_rows, st);
     }
 }
 

@@ -109,7 +109,7 @@ CB_API int cactus_cuda_kv4_read(const void* pool, size_t num_pages, size_t page_
 CB_API size_t cactus_cuda_kv4_attention_workspace(size_t num_seqs, size_t num_tokens, size_t num_q_heads,
                                                   size_t num_kv_heads, size_t head_dim) {
     if (num_seqs > kIntMax - 1 || num_tokens > kIntMax - 64 || num_q_heads > 65536 || num_kv_heads > 1024 ||
-        head_dim > 256)
+        num_kv_heads == 0 || num_q_heads < num_kv_heads || head_dim > 256)
         return 0;
     return cb::kv4::attention_workspace((int)num_seqs, (int)num_tokens, (int)num_q_heads, (int)num_kv_heads,
                                         (int)head_dim);

@@ -32,9 +32,20 @@ struct AttnCall {
     int causal;
     uint8_t* ws;
 };
-// decode.cu
-size_t decode_workspace(int num_seqs, int num_tokens, int hq, int hkv);
-int launch_decode(const AttnCall& c, const Pages& pg, const Geom& ge, cudaStream_t st);
+
+// The workspace is two regions: the parts of results that several blocks share, at a fixed size, so
+// that the counters after it, which have to be zero before every call, are at the same place for
+// every shape.
+constexpr int kDecodeCtas = 148 * 4, kDecodePartFloats = 16 * (128 + 2);  // 2 parts a block, 16 rows of 128 at most
+constexpr int kPrefillParts = 2 * 148;                                    // of 256 rows of 128 (128 of 256) at most
+constexpr size_t kPartBytes = (size_t)kPrefillParts * 256 * (128 + 2) * 4;
+static_assert(kPartBytes >= (size_t)kDecodeCtas * 2 * kDecodePartFloats * 4, "workspace");
+
+// decode.cu: sequences with at most max_rows q rows (tokens times the heads that share a kv head)
+size_t decode_counters(int num_seqs, int num_tokens, int hq, int hkv);
+int launch_decode(const AttnCall& c, const Pages& pg, const Geom& ge, int max_rows, cudaStream_t st);
+// prefill_tc.cu: sequences with at least min_rows q rows
+int launch_prefill(const AttnCall& c, const Pages& pg, const Geom& ge, int min_rows, cudaStream_t st);
 // attention.cu
 size_t attention_workspace(int num_seqs, int num_tokens, int hq, int hkv, int d);
 int launch_attention(const AttnCall& c, const Pages& pg, const Geom& ge, cudaStream_t st);

@@ -1,0 +1,633 @@
+// Attention over the 4-bit paged KV cache for many queries a sequence (prompts, their chunks), on the
+// 5th-generation tensor cores.
+//
+// Work. A CTA takes 256 q rows of one sequence and kv head (two tiles of 128; 128 rows at
+// head_dim 256), row = token * heads that share the kv head + head, over a range of key tiles (128
+// keys, 64 at head_dim 256). Where there are too few such row tiles for the GPU, the keys are split
+// too; the parts go to the workspace, and the CTA that brings the last one joins them in order.
+//
+// Warps (14), handing over through mbarriers:
+//   producer  raw codes and parameters of K and V half tiles into a ring (1-D bulk copies);
+//   dequant   codes -> fp16 values in the swizzled operand layout, once for all 256 rows;
+//   mma       one thread: S = Q K^T (operands in shared memory), O += P V (P in TMEM);
+//   softmax   one thread a row: S from TMEM, weights as fp16 back over S, O rescaled in TMEM when the
+//             running maximum has risen by more than 2^8, the result at the end.
+// The two row tiles alternate on the tensor core, so one's products overlap the other's softmax.
+//
+// Layout. K, V and Q tiles are blocks of 64 elements (128 bytes) by rows with the 128-byte swizzle.
+// K and Q are read K-major; V with its rows as the contraction, MN-major, from the same layout. The
+// 8 elements of a 16-byte piece stand in the order 0 4 1 5 2 6 3 7 that the unpacking gives: Q is
+// permuted alike when it is loaded, and O when it is stored.
+// Weights are rounded to fp16 for the tensor core: 2^-11 of each, as much as the result's own rounding.
+//
+// This file is compiled as whole-program device code (build.py WHOLE_PROGRAM).
+#include <atomic>
+
+#include "attention.cuh"
+#include "kv4.cuh"
+#include "kv4_ops.h"
+
+namespace cb {
+namespace kv4 {
+
+namespace {
+
+constexpr int kWarps = 14, kThreads = kWarps * 32;
+constexpr float kLazy = 8.0f;
+
+template <int D>
+struct Cfg {
+    static constexpr int kKeys = D == 256 ? 64 : 128;   // of a tile
+    static constexpr int kTiles = D == 256 ? 1 : 2;     // row tiles
+    static constexpr int kRows = 128 * kTiles;
+    static constexpr int kBufBytes = kKeys * D * 2;     // a K or V tile in fp16
+    static constexpr int kBufs = D == 64 ? 4 : 3;
+    static constexpr int kRaw = 4;                      // raw half tiles
+    static constexpr int kSoftmax = 4 * kTiles, kDequant = kWarps - 2 - kSoftmax;
+    static constexpr int kQBytes = kRows * D * 2;
+    static constexpr int kO = 256;                      // TMEM column of O (S: kKeys columns a row tile from 0)
+    __host__ __device__ static constexpr int raw_bytes(int ng) { return kKeys * (D / 2 + 4 * ng); }
+    __host__ __device__ static constexpr int smem(int ng) { return kQBytes + kBufs * kBufBytes + kRaw * raw_bytes(ng) + 1024; }
+};
+
+struct Args {
+    AttnCall c;
+    Pages pg;
+    Geom ge;
+    unsigned* err;
+    float* parts;
+    unsigned* counters;
+    int min_rows;  // sequences with fewer rows a kv head are another kernel's
+    int splits;
+};
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// Shared-memory matrix descriptor with the 128-byte swizzle: 8-row groups 1024 bytes apart; LBO is
+// the distance of 64-element blocks for the MN-major operand (not used for K-major).
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
+    return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// kind::f16: D fp32, A and B fp16, M = 128; B MN-major where mn
+constexpr uint32_t idesc(int n, bool mn) {
+    return (1u << 4) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc));
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+          "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+        "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]),
+        "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]),
+        "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+            taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, unsigned parity, volatile int* abort) {
+    if (mbar_try_wait(bar, parity)) return true;
+    for (uint32_t i = 0; i < (1u << 24); ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 63) == 63 && *abort) return false;
+    }
+    *abort = 1;
+    return false;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_constant__ Args a) {
+    pdl_launch_dependents();
+    using C = Cfg<D>;
+    constexpr int KT = C::kKeys, MT = C::kTiles;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    uint8_t* const s_q = smem;                       // [row tile][D / 64][128 rows][128 bytes]
+    uint8_t* const s_buf = smem + C::kQBytes;        // ring of K, V tiles [D / 64][KT rows][128 bytes]
+    uint8_t* const s_raw = s_buf + C::kBufs * C::kBufBytes;
+    __shared__ uint64_t s_full[MT], p_full[MT], o_full[MT], buf_full[C::kBufs], buf_free[C::kBufs], raw_full[C::kRaw],
+        raw_free[C::kRaw], drain;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort, s_item[4], s_scan[kWarps], s_last;
+    __shared__ unsigned s_valid[8];  // a bit for each 16 keys of a tile that were loaded, tiles modulo 8
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const AttnCall& c = a.c;
+    const Pages& pg = a.pg;
+    const Geom& ge = a.ge;
+    const int share = c.hq / ge.hkv, ng = ge.ng();
+    pdl_wait();
+
+    // ---- which sequence, rows, kv head and part of the keys: row tiles of a sequence from its last,
+    // which sees the most
+    const int split = blockIdx.x % a.splits, item = blockIdx.x / a.splits;
+    const int pair = item / ge.hkv, head = item % ge.hkv;
+    const int per = (c.num_seqs + kThreads - 1) / kThreads;
+    auto row_tiles = [&](int b) {
+        const int rows = max(0, min(c.offsets[b + 1] - c.offsets[b], c.max_q)) * share;
+        return rows < a.min_rows ? 0 : (rows + C::kRows - 1) / C::kRows;
+    };
+    int mine = 0;
+    for (int b = tid * per; b < min((tid + 1) * per, c.num_seqs); ++b) mine += row_tiles(b);
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
+    }
+    if (lane == 31) s_scan[warp] = upto;
+    if (tid == 0) {
+        s_item[0] = -1;
+        s_abort = 0;
+    }
+    __syncthreads();
+    for (int x = 0; x < warp; ++x) upto += s_scan[x];
+    if (pair >= upto - mine && pair < upto) {
+        int at = upto - mine, b = tid * per;
+        for (;; ++b) {
+            const int k = row_tiles(b);
+            if (pair < at + k) {
+                s_item[0] = b;
+                s_item[1] = k - 1 - (pair - at);
+                break;
+            }
+            at += k;
+        }
+    }
+    __syncwarp();
+    __syncthreads();
+    const int b = s_item[0];
+    if (b < 0) return;
+    const int count = c.offsets[b + 1] - c.offsets[b], tok0 = c.offsets[b], tokens = min(count, c.max_q);
+    const int row0 = s_item[1] * C::kRows, rows = min(C::kRows, tokens * share - row0);
+    const int len = max(c.lens[b], 0), room = (int)(pg.table_stride << ge.page_shift), n = min(len, room);
+    const int pos0 = len - count;  // position of token 0
+    if (tid == 0 && (count > c.max_q || len > room)) atomicCAS(a.err, 0u, (unsigned)kDevBadPage);
+    // the keys that these rows see, and this part's tiles of them
+    const int first_tok = row0 / share, last_tok = (row0 + rows - 1) / share;
+    int end = c.causal ? min(n, pos0 + last_tok + 1) : n;
+    int start = c.window > 0 ? (int)max(0LL, pos0 + first_tok - c.window + 1) : 0;
+    if (start >= end) start = end = 0;
+    const int base = start & ~(KT - 1), all = (end - base + KT - 1) / KT;
+    const int t_from = (int)((long long)all * split / a.splits), t_to = (int)((long long)all * (split + 1) / a.splits);
+    const int tiles = t_to - t_from, key0 = base + t_from * KT;
+
+    // ---- set-up: barriers, TMEM, Q
+    if (warp == kWarps - 2) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        for (int i = 0; i < MT; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 128);
+            mbar_init(&o_full[i], 1);
+        }
+        for (int i = 0; i < C::kBufs; ++i) {
+            mbar_init(&buf_full[i], C::kDequant * 32);
+            mbar_init(&buf_free[i], 1);
+        }
+        for (int i = 0; i < C::kRaw; ++i) {
+            mbar_init(&raw_full[i], 1);
+            mbar_init(&raw_free[i], C::kDequant);
+        }
+        mbar_init(&drain, 1);
+        fence_mbar_init();
+    }
+    for (int i = tid; i < C::kRows * (D / 8); i += kThreads) {
+        const int r = i / (D / 8), ch = i % (D / 8);
+        uint4 v = {0, 0, 0, 0};
+        if (r < rows) {
+            const int row = row0 + r;
+            v = __ldg(reinterpret_cast<const uint4*>(c.q + (long long)(tok0 + row / share) * c.q_stride +
+                                                     (long long)(head * share + row % share) * D) + ch);
+        }
+        const uint4 p = {__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
+                         __byte_perm(v.y, v.w, 0x7632)};
+        const int rt = r & 127;
+        *reinterpret_cast<uint4*>(s_q + (r >> 7) * (128 * D * 2) + (ch >> 3) * (128 * 128) + rt * 128 +
+                                  (((ch & 7) ^ (rt & 7)) << 4)) = p;
+    }
+    fence_proxy_async_shared();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    volatile int* const abort = &s_abort;
+    const int halves = 2 * tiles;  // K and V of each tile in turn
+    const int R = min(ge.page(), KT), half_chunk = R * (D / 2 + 4 * ng), raw_bytes = C::raw_bytes(ng);
+
+    if (warp == kWarps - 1) {
+        // ------------------------------------------------------------ producer
+        // lane 2 i + p: chunk i of a half tile (the rows of one page), codes (0) or parameters (1); a
+        // chunk that is all of a page's rows is one piece
+        const int chunk = lane >> 1, part = lane & 1;
+        int issued = 0;
+        for (int h = 0; h < halves; ++h) {
+            const int slot = h % C::kRaw, tile = h >> 1, k0 = key0 + tile * KT + chunk * R;
+            long long off = -1;
+            if (chunk * R < KT && k0 < end && k0 + R > start) {
+                off = page_offset(pg, b, k0, ge.page_shift);
+                if (off < 0 && part == 0 && !(h & 1)) atomicCAS(a.err, 0u, (unsigned)kDevBadPage);
+            }
+            const int n_rows = min(R, (end - k0 + 15) & ~15);
+            const int bytes = __reduce_add_sync(0xffffffffu, off >= 0 && part == 0 ? (R == ge.page() ? R : n_rows) * (D / 2 + 4 * ng) : 0);
+            if (h >= C::kRaw && !wait_or_abort(&raw_free[slot], ((h / C::kRaw) - 1) & 1, abort)) break;
+            if (!(h & 1)) {
+                unsigned bits = 0;
+                if (off >= 0 && part == 0) bits = ((1u << (R / 16)) - 1) << (chunk * R / 16);
+                bits = __reduce_or_sync(0xffffffffu, bits);
+                if (lane == 0) s_valid[tile & 7] = bits;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive_expect_tx(&raw_full[slot], (unsigned)bytes);
+            __syncwarp();
+            if (off >= 0 && !(R == ge.page() && part)) {
+                const int row_bytes = part ? 4 * ng : D / 2, r = k0 & (ge.page() - 1);
+                const uint8_t* src = pg.pool + off + (long long)head * ge.block_bytes() + (h & 1 ? ge.v_codes() : 0) +
+                                     (part ? ge.k_params() : 0) + r * row_bytes;
+                tma_load_1d(s_raw + slot * raw_bytes + chunk * half_chunk + (part ? R * (D / 2) : 0), src,
+                            (unsigned)(R == ge.page() ? half_chunk : n_rows * row_bytes), &raw_full[slot]);
+            }
+            ++issued;
+        }
+        // no copy may land after the block leaves
+        if (*abort && lane == 0)
+            for (int h = max(0, issued - C::kRaw); h < issued; ++h) mbar_wait_bounded(&raw_full[h % C::kRaw], (h / C::kRaw) & 1);
+    } else if (warp == kWarps - 2) {
+        // ------------------------------------------------------------ tensor core
+        if (lane == 0) {
+            const uint32_t q = smem_u32(s_q), buf = smem_u32(s_buf);
+            bool ok = true;
+            auto need = [&](int h) {
+                ok = ok && wait_or_abort(&buf_full[h % C::kBufs], (h / C::kBufs) & 1, abort);
+                tc_fence_after();
+            };
+            auto qk = [&](int t, int j) {
+                const uint32_t kb = buf + (2 * j % C::kBufs) * C::kBufBytes, qa = q + t * (128 * D * 2);
+                for (int k = 0; k < D / 16; ++k)
+                    mma_ss(tmem + t * KT, desc(qa + (k >> 2) * (128 * 128) + (k & 3) * 32, 16),
+                           desc(kb + (k >> 2) * (KT * 128) + (k & 3) * 32, 16), idesc(KT, false), k > 0);
+                commit(&s_full[t]);
+            };
+            if (tiles > 0) {
+                need(0);
+                for (int t = 0; t < MT && ok; ++t) qk(t, 0);
+                if (ok) commit(&buf_free[0]);
+            }
+            for (int j = 0; j < tiles && ok; ++j) {
+                for (int t = 0; t < MT && ok; ++t) {
+                    if (t == 0) need(2 * j + 1);
+                    ok = ok && wait_or_abort(&p_full[t], j & 1, abort);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t vb = buf + ((2 * j + 1) % C::kBufs) * C::kBufBytes;
+                    for (int k = 0; k < KT / 16; ++k)
+                        mma_ts(tmem + C::kO + t * D, tmem + t * KT + k * 8, desc(vb + k * 2048, KT * 128), idesc(D, true),
+                               j > 0 || k > 0);
+                    if (t == MT - 1) commit(&buf_free[(2 * j + 1) % C::kBufs]);
+                    if (j + 1 < tiles) {
+                        if (t == 0) need(2 * j + 2);
+                        if (!ok) break;
+                        qk(t, j + 1);
+                        if (t == MT - 1) commit(&buf_free[(2 * j + 2) % C::kBufs]);
+                    } else {
+                        commit(&o_full[t]);
+                    }
+                }
+            }
+            commit(&drain);  // every product issued has completed before TMEM is released
+            mbar_wait_bounded(&drain, 0);
+        }
+        __syncwarp();
+    } else if (warp >= C::kSoftmax) {
+        // ------------------------------------------------------------ dequantisation
+        const int dt = tid - C::kSoftmax * 32;
+        constexpr int kTasks = KT * (D / 32);  // 32 elements of a row
+        for (int h = 0; h < halves; ++h) {
+            const int slot = h % C::kRaw, bslot = h % C::kBufs, k0 = key0 + (h >> 1) * KT;
+            if (!wait_or_abort(&raw_full[slot], (h / C::kRaw) & 1, abort)) break;
+            if (h >= C::kBufs && !wait_or_abort(&buf_free[bslot], ((h / C::kBufs) - 1) & 1, abort)) break;
+            const uint8_t* raw = s_raw + slot * raw_bytes;
+            uint8_t* out = s_buf + bslot * C::kBufBytes;
+            const unsigned valid = s_valid[(h >> 1) & 7];
+            const bool whole = valid == (1u << (KT / 16)) - 1 && k0 >= start && k0 + KT <= end;
+#pragma unroll 2
+            for (int i = dt; i < kTasks; i += C::kDequant * 32) {
+                // neighbouring lanes take 4 rows by 2 pieces: their stores then miss each other's banks
+                const int rest = i >> 3, q = (rest % (D / 64)) * 2 + (i & 1), r = rest / (D / 64) * 4 + ((i >> 1) & 3);
+                const uint8_t* src = raw + r / R * half_chunk;
+                const int rr = r % R;
+                const uint4 w = *reinterpret_cast<const uint4*>(src + rr * (D / 2) + q * 16);
+                uint32_t par = *reinterpret_cast<const uint32_t*>(src + R * (D / 2) + (rr * ng + q * 32 / ge.g) * 4);
+                // rows that nobody sees may hold anything: they count as zeros
+                if (!whole && !((valid >> (r >> 4) & 1) && k0 + r >= start && k0 + r < end)) par = 0;
+                const __half2 step = __low2half2(as_half2(par)), low = __high2half2(as_half2(par));
+                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
+                uint8_t* dst = out + (q >> 1) * (KT * 128) + r * 128;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    __half2 f[4];
+                    codes_to_half(ww[x], f);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) f[e] = __hfma2(f[e], step, low);
+                    *reinterpret_cast<uint4*>(dst + ((((q & 1) * 4 + x) ^ (r & 7)) << 4)) = *reinterpret_cast<const uint4*>(f);
+                }
+            }
+            fence_proxy_async_shared();
+            mbar_arrive(&buf_full[bslot]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&raw_free[slot]);
+        }
+    } else {
+        // ------------------------------------------------------------ softmax: a thread a row
+        const int t = warp >> 2, r = t * 128 + (warp & 3) * 32 + lane, row = row0 + r;
+        const bool on = r < rows;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lanes + t * KT, o_at = tmem + lanes + C::kO + t * D;
+        const int tok = tok0 + (on ? row / share : 0), qh = head * share + row % share;
+        const int pos = pos0 + (on ? row / share : 0);
+        // the row sees keys [lo, hi); rows past the last one see all, and nobody reads them
+        const int lo = on && c.window > 0 ? (int)max(0LL, pos - c.window + 1) : 0;
+        const int hi = !on ? INT_MAX : c.causal ? min(n, pos + 1) : n;
+        const float sc = c.scale * 1.4426950408889634f;
+        float m = 0.0f, limit = -INFINITY, l = 0.0f;  // as in the kernel for few queries
+        bool ok = true;
+        for (int j = 0; j < tiles; ++j) {
+            if (!(ok = wait_or_abort(&s_full[t], j & 1, abort))) break;
+            tc_fence_after();
+            const int k0 = key0 + j * KT;
+            const unsigned valid = s_valid[j & 7];
+            const bool whole = lo <= k0 && hi >= k0 + KT && valid == (1u << (KT / 16)) - 1;
+            const bool masked = __any_sync(0xffffffffu, !whole);
+            const int c_lo = max(lo - k0, 0), c_hi = min(max(hi, k0) - k0, KT);
+            auto mask = [&](float (&v)[32], int c0) {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int col = c0 + i;
+                    if (col < c_lo || col >= c_hi || !(valid >> (col >> 4) & 1)) v[i] = -INFINITY;
+                }
+            };
+            float top = -INFINITY;
+#pragma unroll
+            for (int c0 = 0; c0 < KT; c0 += 32) {
+                float v[32];
+                tmem_ld32(s_at + c0, v);
+                if (masked) mask(v, c0);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) top = fmaxf(top, v[i]);
+            }
+            top *= sc;
+            if (__any_sync(0xffffffffu, top > limit)) {
+                float fix = 1.0f;
+                if (top > limit) {
+                    fix = limit == -INFINITY ? 0.0f : ex2(m - top);
+                    m = top;
+                    limit = top + kLazy;
+                    l *= fix;
+                }
+                if (j > 0) {
+#pragma unroll
+                    for (int d = 0; d < D; d += 32) {
+                        float v[32];
+                        tmem_ld32(o_at + d, v);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] *= fix;
+                        tmem_st32(o_at + d, v);
+                    }
+                }
+            }
+#pragma unroll
+            for (int c0 = 0; c0 < KT; c0 += 32) {
+                float v[32];
+                tmem_ld32(s_at + c0, v);
+                if (masked) mask(v, c0);
+                uint32_t p[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float x = ex2(fmaf(v[2 * i], sc, -m)), y = ex2(fmaf(v[2 * i + 1], sc, -m));
+                    l += x + y;
+                    const __half2 h = __floats2half2_rn(x, y);
+                    p[i] = *reinterpret_cast<const uint32_t*>(&h);
+                }
+                tmem_st16(s_at + c0 / 2, p);  // over columns that this thread has read
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(&p_full[t]);
+        }
+        if (tiles > 0 && ok) ok = wait_or_abort(&o_full[t], 0, abort);
+        tc_fence_after();
+        // ---- the result, or this part of it
+        const float m_out = limit == -INFINITY ? -INFINITY : m;
+        bool last = a.splits == 1;
+        const int slot0 = item * a.splits;
+        constexpr int kSlot = C::kRows * (D + 2);  // floats: [D / 4][row][4], then m and l of the rows
+        if (!last) {
+            float* part = a.parts + (size_t)(slot0 + split) * kSlot;
+            if (ok && tiles > 0) {
+#pragma unroll
+                for (int d = 0; d < D; d += 32) {
+                    float v[32];
+                    tmem_ld32(o_at + d, v);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4)
+                        *reinterpret_cast<float4*>(part + ((size_t)((d + i) / 4) * C::kRows + r) * 4) =
+                            make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                }
+            }
+            part[(size_t)C::kRows * D + r] = m_out;
+            part[(size_t)C::kRows * D + C::kRows + r] = l;
+            __threadfence();
+            asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftmax * 32) : "memory");
+            if (tid == 0) {
+                const unsigned before = atomicAdd(&a.counters[item], 1u);
+                s_last = before + 1 == (unsigned)a.splits;
+                if (s_last) a.counters[item] = 0;
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftmax * 32) : "memory");
+            last = s_last != 0;
+            __threadfence();
+        }
+        if (last) {
+            float mm = m_out, ll = l;
+            if (a.splits > 1) {
+                mm = -INFINITY;
+                for (int x = 0; x < a.splits; ++x)
+                    mm = fmaxf(mm, __ldcg(a.parts + (size_t)(slot0 + x) * kSlot + (size_t)C::kRows * D + r));
+                ll = 0.0f;
+                for (int x = 0; x < a.splits; ++x) {
+                    const float* p = a.parts + (size_t)(slot0 + x) * kSlot + (size_t)C::kRows * D + r;
+                    const float pl = __ldcg(p + C::kRows), pm = __ldcg(p);
+                    ll += pl * (pm == -INFINITY ? (pl != pl ? 1.0f : 0.0f) : ex2(pm - mm));
+                }
+            }
+            const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
+            bool nan = ll != ll;
+            const long long at = (long long)tok * c.hq + qh;
+#pragma unroll
+            for (int d = 0; d < D; d += 32) {
+                float v[32];
+                if (a.splits == 1) {
+                    if (tiles > 0) {
+                        tmem_ld32(o_at + d, v);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+                    for (int x = 0; x < a.splits; ++x) {
+                        const float* p = a.parts + (size_t)(slot0 + x) * kSlot;
+                        const float pm = __ldcg(p + (size_t)C::kRows * D + r), pl = __ldcg(p + (size_t)C::kRows * D + C::kRows + r);
+                        const float f = pm == -INFINITY ? (pl != pl ? 1.0f : 0.0f) : ex2(pm - mm);
+                        if (f == 0.0f) continue;  // a part that saw nothing has no values
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4) {
+                            const float4 u = __ldcg(reinterpret_cast<const float4*>(p + ((size_t)((d + i) / 4) * C::kRows + r) * 4));
+                            v[i] = fmaf(u.x, f, v[i]);
+                            v[i + 1] = fmaf(u.y, f, v[i + 1]);
+                            v[i + 2] = fmaf(u.z, f, v[i + 2]);
+                            v[i + 3] = fmaf(u.w, f, v[i + 3]);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {  // column e + i is dim e + {0, 4, 1, 5, 2, 6, 3, 7}[i]
+                    float f[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        f[(i >> 1) + (i & 1) * 4] = v[e + i] * inv;
+                        nan |= v[e + i] != v[e + i];
+                    }
+                    const __half2 h[4] = {__floats2half2_rn(f[0], f[1]), __floats2half2_rn(f[2], f[3]),
+                                          __floats2half2_rn(f[4], f[5]), __floats2half2_rn(f[6], f[7])};
+                    if (on) *reinterpret_cast<uint4*>(c.out + at * D + d + e) = *reinterpret_cast<const uint4*>(h);
+                }
+            }
+            if (on && c.lse) c.lse[at] = ll > 0.0f ? (mm + log2f(ll)) * 0.6931471805599453f : -INFINITY;
+            // rows whose result is not a number are computed again one by one: a NaN among the values
+            // reaches rows that do not see it through weights of zero
+            unsigned again = __ballot_sync(0xffffffffu, on && nan && !*abort);
+            while (again) {
+                const int x = __ffs(again) - 1;
+                again &= again - 1;
+                attention_row<D>(c, pg, ge, b, __shfl_sync(0xffffffffu, tok, x), __shfl_sync(0xffffffffu, qh, x), lane);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncwarp();
+    __syncthreads();
+    if (tid == 0 && *abort) atomicCAS(a.err, 0u, (unsigned)kDevTmaTimeout);
+    if (warp == kWarps - 2) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+// How many parts the keys of a row tile are split into: the number (up to 16, and up to kPrefillParts
+// CTAs in all) with which the rounds over the GPU, each as long as 1 / parts of a row tile's keys
+// and a fixed start and end, take the least.
+int splits_of(long long items, long long key_tiles) {
+    int best = 1;
+    double least = 1e30;
+    for (int p = 1; p <= 16 && (p == 1 || items * p <= kPrefillParts) && p <= key_tiles; ++p) {
+        const double rounds = (double)((items * p + kNumSMs - 1) / kNumSMs);
+        const double time = rounds * ((double)key_tiles / p + 3.0 + (p > 1 ? 2.0 + 0.25 * p : 0.0));
+        if (time < least * 0.97) {
+            least = time;
+            best = p;
+        }
+    }
+    return best;
+}
+
+template <int D>
+int launch(const AttnCall& c, const Pages& pg, const Geom& ge, int min_rows, cudaStream_t st) {
+    using C = Cfg<D>;
+    auto kernel = kv4_prefill_kernel<D>;
+    static std::atomic<unsigned long long> set{0};  // a bit a device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!(set.load() >> (dev & 63) & 1)) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(D / 32)) != cudaSuccess)
+            return -1;
+        set.fetch_or(1ull << (dev & 63));
+    }
+    Args a = {};
+    a.c = c;
+    a.pg = pg;
+    a.ge = ge;
+    a.err = dev_error_ptr();
+    if (!a.err) return -1;
+    a.parts = reinterpret_cast<float*>(c.ws);
+    a.counters = reinterpret_cast<unsigned*>(c.ws + kPartBytes);
+    a.min_rows = min_rows;
+    // row tiles: no more than the tokens fill, and one a sequence that they fill in part
+    const int share = c.hq / ge.hkv;
+    const long long rows = (long long)c.num_tokens * share, most = (long long)c.max_q * share;
+    const long long tiles_most = c.num_seqs * ((most + C::kRows - 1) / C::kRows);
+    const long long pairs = rows / C::kRows + c.num_seqs < tiles_most ? rows / C::kRows + c.num_seqs : tiles_most;
+    const long long items = pairs * ge.hkv;
+    long long keys = pg.table_stride << ge.page_shift;
+    if (c.window > 0 && c.window + C::kRows / share + 1 < keys) keys = c.window + C::kRows / share + 1;
+    a.splits = splits_of(items, (keys + C::kKeys - 1) / C::kKeys);
+    if (items * a.splits > 0x7fffffffLL) return -2;
+    return launch_k(kernel, dim3((unsigned)(items * a.splits)), dim3(kThreads), (size_t)C::smem(ge.ng()), st, a) == cudaSuccess
+               ? 0
+               : -1;
+}
+
+}  // namespace
+
+int launch_prefill(const AttnCall& c, const Pages& pg, const Geom& ge, int min_rows, cudaStream_t st) {
+    switch (ge.d) {
+        case 64: return launch<64>(c, pg, ge, min_rows, st);
+        case 128: return launch<128>(c, pg, ge, min_rows, st);
+        default: return launch<256>(c, pg, ge, min_rows, st);
+    }
+}
+
+}  // namespace kv4
+}  // namespace cb
