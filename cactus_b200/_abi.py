@@ -25,6 +25,7 @@ _SCALAR = {
     "void": None,
     "cactus_model_t": C.c_void_p,
     "cactus_engine_t": C.c_void_p,
+    "cactus_kv4_t": C.c_void_p,
     "cactus_token_callback": C.c_void_p,
 }
 

@@ -99,6 +99,52 @@ CB_API int cactus_cuda_kv4_compact(void* pool, size_t num_pages, size_t page_str
                                    size_t num_seqs, size_t num_kept, size_t page_size, size_t num_kv_heads,
                                    size_t head_dim, size_t group_size, void* stream);
 
+/* ---- The cache as a handle: one pool for all layers of a model, and the pages of many sequences,
+ * shared between forked ones until they are written. Lists of sequences, row counts and kept rows
+ * are HOST arrays; keys, values, queries and results are device pointers. Sequences are numbered 0
+ * to max_seqs - 1 and empty at first. The calls of one cache are made in order, on one stream or on
+ * streams that the caller orders (a page that is freed is given out again); not from two threads at
+ * once. A call that fails for its arguments or for lack of pages changes nothing. */
+typedef void* cactus_kv4_t;
+
+/* num_pages pages of page_size rows for every layer, block tables for max_context rows, batches of up
+ * to max_tokens new rows. NULL on failure. */
+CB_API cactus_kv4_t cactus_kv4_create(size_t num_layers, size_t num_q_heads, size_t num_kv_heads, size_t head_dim,
+                                      size_t group_size, size_t page_size, size_t num_pages, size_t max_seqs,
+                                      size_t max_context, size_t max_tokens, int device);
+/* Waits for nothing: no work of the cache may be in flight. */
+CB_API void cactus_kv4_destroy(cactus_kv4_t cache);
+/* Makes room for new_rows[i] rows at the end of sequence seqs[i] (none of them twice; a shared page
+ * that these rows would be written into is copied first, in every layer) and makes these sequences the
+ * batch that the next appends, for each layer, and attention calls are about: token rows of seqs[0],
+ * seqs[1], ... one after another. The rows count as cached from here on. */
+CB_API int cactus_kv4_begin(cactus_kv4_t cache, const int32_t* seqs, const int32_t* new_rows, size_t num_seqs,
+                            void* stream);
+/* cactus_cuda_kv4_append / _attention for the batch. */
+CB_API int cactus_kv4_append(cactus_kv4_t cache, size_t layer, const uint16_t* keys, const uint16_t* values,
+                             size_t row_stride, void* stream);
+CB_API int cactus_kv4_attention(cactus_kv4_t cache, size_t layer, const uint16_t* queries, size_t query_stride,
+                                uint16_t* output, float* lse, float scale, size_t window_size, int is_causal,
+                                void* stream);
+/* Rows first .. first + count - 1 of a sequence as fp16 [count][num_kv_heads][head_dim]. */
+CB_API int cactus_kv4_read(cactus_kv4_t cache, size_t layer, int32_t seq, size_t first, size_t count, uint16_t* keys,
+                           uint16_t* values, void* stream);
+/* Sequence dst[i] becomes a copy of what src[i] was before the call (its pages are shared, nothing is
+ * moved); what dst[i] held is freed. Beams are reordered in one call. Ends the batch, as do the next
+ * three. */
+CB_API int cactus_kv4_fork(cactus_kv4_t cache, const int32_t* src, const int32_t* dst, size_t n);
+/* Keeps a sequence's first `length` rows (drafted tokens that were refused, for instance). */
+CB_API int cactus_kv4_truncate(cactus_kv4_t cache, int32_t seq, size_t length);
+CB_API int cactus_kv4_free(cactus_kv4_t cache, const int32_t* seqs, size_t n);
+/* Keeps the rows kept_rows[kept_offsets[i]] .. of sequence seqs[i], in that order, in new pages; there
+ * have to be enough free ones for them before the old ones are freed. */
+CB_API int cactus_kv4_compact(cactus_kv4_t cache, const int32_t* seqs, const int32_t* kept_rows,
+                              const int32_t* kept_offsets, size_t num_seqs, void* stream);
+/* Rows of a sequence, or a negative error code. */
+CB_API int cactus_kv4_length(cactus_kv4_t cache, int32_t seq);
+/* out4 (host): pages, free pages, bytes of a page in one layer, bytes of the pool. */
+CB_API int cactus_kv4_info(cactus_kv4_t cache, size_t* out4);
+
 #ifdef __cplusplus
 }
 #endif

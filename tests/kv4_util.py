@@ -30,7 +30,7 @@ def quantise(x, g):
     codes = np.clip(np.rint(q), 0, 15).astype(np.uint8)
     step = np.where(bad, np.float16(np.nan), step).astype(np.float16)
     low = np.where(bad, np.float16(np.nan), lo.astype(np.float16)).astype(np.float16)
-    return codes.reshape(*x.shape[:-2], -1), step, low
+    return codes.reshape(*x.shape[:-2], x.shape[-2] * g), step, low
 
 
 def values(codes, step, low, g):

@@ -113,3 +113,34 @@ def test_plain_quantisation_error_is_half_a_step():
     # half a step, what the step's rounding leaves at the top (15 steps of 2^-10), and fp16's rounding
     bound = np.repeat(step.astype(np.float64), 32, axis=-1) * (0.5 + 15 * 2.0 ** -10) + 2.0 ** -11 * np.abs(v)
     assert np.all(np.abs(v - x.astype(np.float64)) <= bound)
+
+
+def test_page_map(tmp_path):
+    """The handle's bookkeeping (csrc/kv4/page_map.h) against a plain model, with random programs."""
+    import os
+    import subprocess
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe = str(tmp_path / "page_map_test")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-fsanitize=address,undefined",
+                    "-I", os.path.join(root, "cactus_b200", "csrc"),
+                    os.path.join(root, "tests", "native", "kv4_page_map_test.cpp"), "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout == "ok\n", r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("change", [dict(layers=0), dict(hq=6), dict(hq=0), dict(d=96), dict(page=24), dict(pages=0),
+                                    dict(seqs=0), dict(context=0), dict(tokens=0)])
+def test_cache_refuses_what_it_cannot_hold(change):
+    a = dict(layers=2, hq=8, hkv=4, d=64, g=32, page=16, pages=10, seqs=2, context=100, tokens=8)
+    a.update(change)
+    L = cb.lib()
+    assert not L.cactus_kv4_create(a["layers"], a["hq"], a["hkv"], a["d"], a["g"], a["page"], a["pages"], a["seqs"],
+                                   a["context"], a["tokens"], 0)
+    assert b"kv4_create" in L.cactus_cuda_last_error()
+
+
+def test_calls_on_no_cache_are_refused():
+    L = cb.lib()
+    assert L.cactus_kv4_length(None, 0) == -1 and L.cactus_kv4_truncate(None, 0, 0) == -1
+    assert L.cactus_kv4_fork(None, None, None, 0) == -1 and b"null cache" in L.cactus_cuda_last_error()
+    L.cactus_kv4_destroy(None)

@@ -496,3 +496,128 @@ def test_compact_skips_rows_that_the_tables_lack_and_reports_them():
             part[2, :, 0], part[2, :, 4] = part[0, :, 3].copy(), part[0, :, 5].copy()
     assert np.array_equal(host(d[0], np.uint8), pool.bytes)
     assert _err() == 3
+
+
+# ------------------------------------------------------------------------------------ the handle
+def _rows_of(cache, ge, layer, seq):
+    n = cache.length(seq)
+    got = [empty((n, ge.hkv, ge.d), np.float16) for _ in range(2)]
+    cache.read(layer, seq, 0, n, *(ptr(g) for g in got))
+    return [host(g, np.float16) for g in got]
+
+
+def _quantised(x, g):
+    return U.values(*U.quantise(x, g), g)
+
+
+@pytest.mark.parametrize("geom", [(16, 2, 64, 32), (32, 1, 128, 64)])
+def test_cache_keeps_what_sequences_hold(geom):
+    """Random growth, forks, cuts and compactions of a cache of three layers against lists of rows."""
+    from cactus_b200.kv4 import KVCache4
+    ge, layers, seqs, hq = U.Geom(*geom), 3, 5, 4
+    rng = np.random.default_rng(ge.d)
+    cache = KVCache4(layers, hq, ge.hkv, ge.d, num_pages=60, max_seqs=seqs, max_context=300, max_tokens=200,
+                     group_size=ge.g, page_size=ge.page)
+    width = ge.hkv * ge.d
+    rows = [[[np.zeros((0, ge.hkv, ge.d), np.float16)] * 2 for _ in range(layers)] for _ in range(seqs)]
+    for step in range(40):
+        kind = rng.integers(6)
+        if kind <= 2:
+            ids = rng.permutation(seqs)[:rng.integers(1, seqs + 1)].tolist()
+            counts = [int(rng.integers(0, 4)) if rng.random() < 0.7 else int(rng.integers(0, 40)) for _ in ids]
+            if sum(counts) == 0 or any(rows[s][0][0].shape[0] + c > 300 for s, c in zip(ids, counts)):
+                continue
+            free = cache.info()["free_pages"]
+            try:
+                cache.begin(ids, counts)
+            except cb.CactusError as e:
+                assert "out of pages" in str(e) and cache.info()["free_pages"] == free
+                cache.free(range(seqs))
+                rows = [[[np.zeros((0, ge.hkv, ge.d), np.float16)] * 2 for _ in range(layers)] for _ in range(seqs)]
+                continue
+            t, off = sum(counts), _offsets(counts)
+            for l in range(layers):
+                kv = rng.standard_normal((2, t, width)).astype(np.float16)
+                q = rng.standard_normal((t, hq, ge.d)).astype(np.float16)
+                d = [dev(kv[0]), dev(kv[1]), dev(q)]
+                out, lse = empty((t, hq, ge.d), np.float16), empty((t, hq), np.float32)
+                cache.append(l, ptr(d[0]), ptr(d[1]))
+                cache.attention(l, ptr(d[2]), ptr(out), 0.1, lse=ptr(lse))
+                out = host(out, np.float16).astype(np.float64)
+                for i, s in enumerate(ids):
+                    at = slice(off[i], off[i + 1])
+                    rows[s][l] = [np.concatenate([rows[s][l][w], _quantised(kv[w, at].reshape(-1, ge.hkv, ge.d), ge.g)])
+                                  for w in (0, 1)]
+                    if counts[i]:
+                        ref, _, tol, _ = U.attention(q[at], *rows[s][l], 0.1, True, 0)
+                        assert np.all(np.abs(out[at] - ref) <= tol)
+        elif kind == 3:
+            src = [int(s) for s in rng.integers(0, seqs, seqs)]
+            cache.fork(src, list(range(seqs)))
+            rows = [[list(rows[s][l]) for l in range(layers)] for s in src]
+        elif kind == 4:
+            s = int(rng.integers(seqs))
+            n = int(rng.integers(0, rows[s][0][0].shape[0] + 1))
+            cache.truncate(s, n)
+            rows[s] = [[x[:n] for x in kv] for kv in rows[s]]
+        else:
+            ids = rng.permutation(seqs)[:2].tolist()
+            kept = [np.flatnonzero(rng.random(rows[s][0][0].shape[0]) < 0.7) for s in ids]
+            try:
+                cache.compact(ids, kept)
+            except cb.CactusError as e:
+                assert "out of pages" in str(e)
+                continue
+            for s, k in zip(ids, kept):
+                rows[s] = [[x[k] for x in kv] for kv in rows[s]]
+        for s in range(seqs):
+            assert cache.length(s) == rows[s][0][0].shape[0]
+            for l in range(layers):
+                if cache.length(s):
+                    got = _rows_of(cache, ge, l, s)
+                    assert all(np.array_equal(g, r) for g, r in zip(got, rows[s][l])), (step, s, l)
+    cache.free(range(seqs))
+    assert cache.info()["free_pages"] == 60
+    cache.close()
+    assert _err() == 0
+
+
+def test_cache_slide_and_refusals():
+    from cactus_b200.kv4 import KVCache4
+    ge = U.Geom(16, 1, 64, 32)
+    cache = KVCache4(1, 2, 1, 64, num_pages=12, max_seqs=2, max_context=128, max_tokens=128, page_size=16)
+    x = np.random.default_rng(1).standard_normal((100, 64)).astype(np.float16)
+    d = dev(x)
+    with pytest.raises(cb.CactusError, match="no batch"):
+        cache.append(0, ptr(d), ptr(d))
+    cache.begin([1], [100])
+    cache.append(0, ptr(d), ptr(d))
+    cache.slide([1], sink=4, window=20)
+    kept = list(range(4)) + list(range(84, 100))
+    assert np.array_equal(_rows_of(cache, ge, 0, 1)[0].reshape(-1, 64), _quantised(x, 32)[kept])
+    assert cache.info()["free_pages"] == 10
+    for call, why in ((lambda: cache.begin([0], [129]), "max_tokens"), (lambda: cache.begin([1], [120]), "longest context"),
+                      (lambda: cache.begin([2], [1]), "no sequence"), (lambda: cache.begin([0, 0], [1, 1]), "twice"),
+                      (lambda: cache.append(0, ptr(d), ptr(d)), "no batch"), (lambda: cache.truncate(1, 21), "length"),
+                      (lambda: cache.compact([1], [[20]]), "kept row"), (lambda: cache.compact([1], [[-1]]), "kept row"),
+                      (lambda: cache.read(0, 1, 15, 6, ptr(d), ptr(d)), "rows"), (lambda: cache.fork([0], [5]), "no sequence"),
+                      (lambda: cache.read(1, 1, 0, 1, ptr(d), ptr(d)), "layer"), (lambda: cache.free([0, 7]), "no sequence")):
+        with pytest.raises(cb.CactusError, match=why):
+            call()
+    assert cache.length(1) == 20 and cache.length(0) == 0
+    cache.close()
+    assert _err() == 0
+
+
+def test_example_runs(capsys):
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "kv4_sampling.py")
+    spec = importlib.util.spec_from_file_location("kv4_sampling", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    # 4 bits a value: a step is a fifteenth of a group's range (about 4 deviations of 32 normal values), so
+    # its rounding is 0.27 / sqrt(12) = 8 % of a deviation, in the values and, through the scores, again
+    assert example.main(["--prompt", "300", "--samples", "4", "--steps", "20"]) < 0.25
+    assert "samples" in capsys.readouterr().out
+    assert _err() == 0
