@@ -16,13 +16,38 @@ namespace {
 // element by shuffles, and each lane stores its 8 codes as one word.
 constexpr int kAppendTokens = 32, kAppendThreads = 256;
 
-// (x - low) / step rounded half to even, held in 0..15. Below 16 the product with the reciprocal is
-// within 4e-6 of the quotient (two roundings of 2^-24 each), so only a result that near a half,
-// where the rounding could differ, takes the true division.
-__device__ __forceinline__ uint32_t quant_code(float x, float step, float inv) {
-    float q = __fmul_rn(x, inv);
-    if (fabsf(__fsub_rn(fabsf(__fsub_rn(q, rintf(q))), 0.5f)) < 1e-5f) q = __fdiv_rn(x, step);
-    return (uint32_t)fminf(rintf(q), 15.0f);
+// (largest - smallest) / 15 rounded towards zero to fp16: the product with 1/15 is a unit in the last
+// place off at most, and fifteen times an fp16 number is exact in fp32.
+__device__ __forceinline__ __half step_of(float range) {
+    const unsigned short s = __half_as_ushort(__float2half_rz(__fmul_rn(range, 1.0f / 15.0f)));
+    const float at = __fmul_rn(__half2float(__ushort_as_half(s)), 15.0f);
+    const float above = __fmul_rn(__half2float(__ushort_as_half((unsigned short)(s + 1))), 15.0f);
+    return __ushort_as_half((unsigned short)(s + (above <= range ? 1 : 0) - (at > range ? 1 : 0)));
+}
+
+// The codes of 8 elements x - low of a group as a word: each quotient rounded half to even, at most 15.
+// The product with the reciprocal is within 5e-6 of a quotient below 16 (2^-23 for the reciprocal, 2^-24
+// for the product), so where every product is further than that from a half its rounding is the
+// quotient's; else (rare) the 8 are divided, as they are where the step is so small (a few of fp16's
+// smallest units) that a quotient can pass 15.5. Adding 1.5 * 2^23 rounds to an integer and leaves it
+// in the low bits.
+__device__ __forceinline__ uint32_t quant_codes(const float (&x)[8], float step) {
+    const float magic = 12582912.0f;
+    float inv, far = 0.0f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));
+    uint32_t w = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float t = fmaf(x[j], inv, magic);
+        far = fmaxf(far, fabsf(fmaf(x[j], inv, -__fsub_rn(t, magic))));
+        w += __float_as_uint(t) << (4 * j);  // 0x4B400000 + code: the sum of the constants is taken off below
+    }
+    if (far > 0.49999f || step < 0x1p-18f) {
+        w = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w += __float_as_uint(__fadd_rn(fminf(__fdiv_rn(x[j], step), 15.0f), magic)) << (4 * j);
+    }
+    return w - 0x4B400000u * 0x11111111u;
 }
 
 template <int D>
@@ -36,6 +61,18 @@ __global__ void __launch_bounds__(kAppendThreads)
     __shared__ int s_row[kAppendTokens];
     constexpr int kLanes = D / 8, kRows = kAppendThreads / kLanes;
     const int t0 = blockIdx.x * kAppendTokens, head = blockIdx.y;
+    const int lane = threadIdx.x % kLanes, per_group = ge.g / 8;
+    const unsigned full = 0xffffffffu;
+    constexpr int kPasses = kAppendTokens / kRows;
+    static_assert(kAppendTokens % kRows == 0, "whole passes");
+    uint4 x[2 * kPasses];
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {  // in flight while the rows' pages are looked up
+        const int t = min(t0 + threadIdx.x / kLanes + i * kRows, num_tokens - 1);
+        const long long at = (long long)t * row_stride + head * D + lane * 8;
+        x[2 * i] = __ldg(reinterpret_cast<const uint4*>(keys + at));
+        x[2 * i + 1] = __ldg(reinterpret_cast<const uint4*>(values + at));
+    }
     if (threadIdx.x < kAppendTokens) {
         const int t = t0 + threadIdx.x;
         const int b = t < num_tokens ? find_seq(offsets, num_seqs, t) : -1;
@@ -50,57 +87,39 @@ __global__ void __launch_bounds__(kAppendThreads)
         s_row[threadIdx.x] = row;
     }
     __syncthreads();
-    const int lane = threadIdx.x % kLanes, per_group = ge.g / 8;
-    const unsigned full = 0xffffffffu;
-    constexpr int kPasses = (kAppendTokens + kRows - 1) / kRows;
-    uint4 x[2 * kPasses];
-#pragma unroll
-    for (int i = 0; i < kPasses; ++i) {
-        const int r = threadIdx.x / kLanes + i * kRows;
-        const bool on = s_page[r] >= 0;
-        const long long at = (long long)(t0 + r) * row_stride + head * D + lane * 8;
-        x[2 * i] = on ? __ldg(reinterpret_cast<const uint4*>(keys + at)) : uint4{0, 0, 0, 0};
-        x[2 * i + 1] = on ? __ldg(reinterpret_cast<const uint4*>(values + at)) : uint4{0, 0, 0, 0};
-    }
 #pragma unroll
     for (int i = 0; i < 2 * kPasses; ++i) {
         const int r = threadIdx.x / kLanes + (i / 2) * kRows;
-        float f[8];
         const __half2* h = reinterpret_cast<const __half2*>(&x[i]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 p = __half22float2(h[j]);
-            f[2 * j] = p.x;
-            f[2 * j + 1] = p.y;
-        }
-        float lo = f[0], hi = f[0];
-        bool bad = false;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            lo = fminf(lo, f[j]);
-            hi = fmaxf(hi, f[j]);
-            bad |= !(fabsf(f[j]) <= 65504.0f);  // an infinity or a NaN
-        }
-        for (int o = 1; o < per_group; o <<= 1) {
-            lo = fminf(lo, __shfl_xor_sync(full, lo, o));
-            hi = fmaxf(hi, __shfl_xor_sync(full, hi, o));
-            bad |= __shfl_xor_sync(full, (int)bad, o) != 0;
-        }
-        const __half step = __float2half_rz(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
-        const float fs = __half2float(step), inv = fs > 0.0f ? __frcp_rn(fs) : 0.0f;
+        // (largest, -smallest): exact in fp16, and a NaN stays one
+        const __half2 hi2 = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
+        const __half2 lo2 = __hmin2_nan(__hmin2_nan(h[0], h[1]), __hmin2_nan(h[2], h[3]));
+        __half2 ends = __hmax2_nan(__lows2half2(hi2, __hneg2(lo2)), __highs2half2(hi2, __hneg2(lo2)));
+        for (int o = 1; o < per_group; o <<= 1) ends = __hmax2_nan(ends, __shfl_xor_sync(full, ends, o));
+        const float hi = __low2float(ends), lo = -__high2float(ends);
+        const __half step = step_of(__fsub_rn(hi, lo));
+        const float fs = __half2float(step);
+        const bool bad = !(__fsub_rn(hi, lo) < INFINITY);  // an infinity or a NaN in the group
         uint32_t w = 0;
         if (!bad && fs > 0.0f) {
+            float f[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w |= quant_code(__fsub_rn(f[j], lo), fs, inv) << (4 * j);
+            for (int j = 0; j < 4; ++j) {
+                const float2 p = __half22float2(h[j]);
+                f[2 * j] = __fsub_rn(p.x, lo);
+                f[2 * j + 1] = __fsub_rn(p.y, lo);
+            }
+            w = quant_codes(f, fs);
         }
-        if (s_page[r] < 0) continue;
-        uint8_t* block = pg.pool + s_page[r] + (long long)head * ge.block_bytes() + ((i & 1) ? ge.v_codes() : 0);
-        const int row = s_row[r];
-        *reinterpret_cast<uint32_t*>(block + row * (D / 2) + lane * 4) = w;
-        if (lane % per_group == 0) {
-            const __half nan = __ushort_as_half(0x7FFF);
-            *reinterpret_cast<__half2*>(block + ge.k_params() + (row * ge.ng() + lane / per_group) * 4) =
-                bad ? __halves2half2(nan, nan) : __halves2half2(step, __float2half_rn(lo));
+        if (s_page[r] >= 0) {
+            uint8_t* block = pg.pool + s_page[r] + (long long)head * ge.block_bytes() + ((i & 1) ? ge.v_codes() : 0);
+            const int row = s_row[r];
+            *reinterpret_cast<uint32_t*>(block + row * (D / 2) + lane * 4) = w;
+            if (lane % per_group == 0) {
+                const __half nan = __ushort_as_half(0x7FFF);
+                *reinterpret_cast<__half2*>(block + ge.k_params() + (row * ge.ng() + lane / per_group) * 4) =
+                    bad ? __halves2half2(nan, nan) : __halves2half2(step, __float2half_rn(lo));
+            }
         }
     }
 }
@@ -132,28 +151,31 @@ __global__ void __launch_bounds__(kAppendThreads)
     }
     __syncthreads();
     const int lane = threadIdx.x % kLanes, group = lane * 8 / ge.g;
-    for (int r = threadIdx.x / kLanes; r < kAppendTokens; r += kRows) {
-        if (s_page[r] < 0) continue;
-        const uint8_t* block = pg.pool + s_page[r] + (long long)head * ge.block_bytes();
-        const int row = s_row[r];
-        const long long at = ((long long)(t0 + r) * ge.hkv + head) * D + lane * 8;
+    constexpr int kPasses = kAppendTokens / kRows;
+    uint32_t w[2 * kPasses];
+    __half2 par[2 * kPasses];
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            __half* out = which ? values : keys;
-            if (!out) continue;
-            const uint8_t* part = block + (which ? ge.v_codes() : 0);
-            const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(part + row * (D / 2) + lane * 4));
-            const __half2 par =
-                __ldg(reinterpret_cast<const __half2*>(part + ge.k_params() + (row * ge.ng() + group) * 4));
-            const __half2 step = __low2half2(par), low = __high2half2(par);
-            __half2 c[4];
-            codes_to_half(w, c);
+    for (int i = 0; i < 2 * kPasses; ++i) {
+        const int r = threadIdx.x / kLanes + (i / 2) * kRows;
+        if (s_page[r] < 0 || !((i & 1) ? values : keys)) continue;
+        const uint8_t* part = pg.pool + s_page[r] + (long long)head * ge.block_bytes() + ((i & 1) ? ge.v_codes() : 0);
+        w[i] = __ldg(reinterpret_cast<const uint32_t*>(part + s_row[r] * (D / 2) + lane * 4));
+        par[i] = __ldg(reinterpret_cast<const __half2*>(part + ge.k_params() + (s_row[r] * ge.ng() + group) * 4));
+    }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) c[j] = __hfma2(c[j], step, low);
-            __half2 o[4] = {__lows2half2(c[0], c[1]), __lows2half2(c[2], c[3]), __highs2half2(c[0], c[1]),
-                            __highs2half2(c[2], c[3])};
-            *reinterpret_cast<uint4*>(out + at) = *reinterpret_cast<const uint4*>(o);
-        }
+    for (int i = 0; i < 2 * kPasses; ++i) {
+        const int r = threadIdx.x / kLanes + (i / 2) * kRows;
+        __half* out = (i & 1) ? values : keys;
+        if (s_page[r] < 0 || !out) continue;
+        const __half2 step = __low2half2(par[i]), low = __high2half2(par[i]);
+        __half2 c[4];
+        codes_to_half(w[i], c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c[j] = __hfma2(c[j], step, low);
+        const __half2 o[4] = {__lows2half2(c[0], c[1]), __lows2half2(c[2], c[3]), __highs2half2(c[0], c[1]),
+                              __highs2half2(c[2], c[3])};
+        *reinterpret_cast<uint4*>(out + ((long long)(t0 + r) * ge.hkv + head) * D + lane * 8) =
+            *reinterpret_cast<const uint4*>(o);
     }
 }
 
@@ -217,24 +239,50 @@ __global__ void __launch_bounds__(kMoveThreads)
     }
     __syncthreads();
     uint8_t* plane = src.pool + blockIdx.y * plane_stride;
-    const int cw = ge.code_bytes() / 16, block = ge.block_bytes();  // 16-byte pieces of a row's codes: 2, 4 or 8
-    const int per_head = 2 * kMoveRows * cw;
-    for (int i = threadIdx.x; i < per_head * ge.hkv; i += kMoveThreads) {
-        const int head = i / per_head, k = i % per_head, piece = k % cw, r = (k / cw) % kMoveRows;
+    const int block = ge.block_bytes();
+    // codes: a thread keeps one 16-byte piece of one row and goes through the heads, four at a time
+    const int cw = ge.code_bytes() / 16, units = 2 * kMoveRows * cw;  // pieces of a row: 2, 4 or 8
+    const int lanes = min(units, kMoveThreads), heads = kMoveThreads / lanes;
+    for (int u = threadIdx.x % lanes; u < units; u += lanes) {
+        const int piece = u % cw, r = u / cw % kMoveRows;
         if (s_from[r] < 0) continue;
-        const long long at = (long long)head * block + (k >= kMoveRows * cw ? ge.v_codes() : 0) + piece * 16;
-        *reinterpret_cast<uint4*>(plane + s_to[r] + at + s_trow[r] * ge.code_bytes()) =
-            *reinterpret_cast<const uint4*>(plane + s_from[r] + at + s_frow[r] * ge.code_bytes());
+        const long long at = (u >= kMoveRows * cw ? ge.v_codes() : 0) + piece * 16;
+        const uint8_t* from = plane + s_from[r] + at + s_frow[r] * ge.code_bytes();
+        uint8_t* to = plane + s_to[r] + at + s_trow[r] * ge.code_bytes();
+        for (int h = threadIdx.x / lanes; h < ge.hkv; h += 4 * heads) {
+            uint4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (h + i * heads < ge.hkv) v[i] = *reinterpret_cast<const uint4*>(from + (long long)(h + i * heads) * block);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (h + i * heads < ge.hkv) *reinterpret_cast<uint4*>(to + (long long)(h + i * heads) * block) = v[i];
+        }
     }
-    const int ng = ge.ng(), words = 2 * kMoveRows * ng;
-    for (int i = threadIdx.x; i < words * ge.hkv; i += kMoveThreads) {
-        const int head = i / words, k = i % words, piece = k % ng, r = (k / ng) % kMoveRows;
-        if (s_from[r] < 0) continue;
-        const long long at =
-            (long long)head * block + (k >= kMoveRows * ng ? ge.v_params() : ge.k_params()) + piece * 4;
-        *reinterpret_cast<uint32_t*>(plane + s_to[r] + at + s_trow[r] * ge.param_bytes()) =
-            *reinterpret_cast<const uint32_t*>(plane + s_from[r] + at + s_frow[r] * ge.param_bytes());
-    }
+    // parameters: a thread keeps those of one row, keys or values, and goes through every fourth head
+    const int r = threadIdx.x % kMoveRows, ng = ge.ng();
+    if (s_from[r] < 0) return;
+    const long long at = (threadIdx.x & kMoveRows) ? ge.v_params() : ge.k_params();
+    const uint8_t* from = plane + s_from[r] + at + s_frow[r] * ge.param_bytes();
+    uint8_t* to = plane + s_to[r] + at + s_trow[r] * ge.param_bytes();
+    constexpr int kStep = kMoveThreads / (2 * kMoveRows);
+    auto move = [&](auto word) {
+        using T = decltype(word);
+        for (int h = threadIdx.x / (2 * kMoveRows); h < ge.hkv; h += 2 * kStep) {
+            const bool two = h + kStep < ge.hkv;
+            const long long x = (long long)h * block, y = x + (long long)kStep * block;
+            const T a = *reinterpret_cast<const T*>(from + x), b = *reinterpret_cast<const T*>(from + (two ? y : x));
+            *reinterpret_cast<T*>(to + x) = a;
+            if (two) *reinterpret_cast<T*>(to + y) = b;
+        }
+    };
+    struct alignas(16) Eight {
+        uint4 a, b;
+    };
+    if (ng == 1) move(uint32_t{});
+    else if (ng == 2) move(uint2{});
+    else if (ng == 4) move(uint4{});
+    else move(Eight{});
 }
 
 }  // namespace
