@@ -100,6 +100,45 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
         : "r"(taddr)
         : "memory");
 }
+// The same without the wait: the registers hold the values after tmem_wait_ld on them.
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, float (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+          "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+          "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+          "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        : "r"(taddr)
+        : "memory");
+}
+// Waits for every load of the thread; the operands keep uses of the registers behind it.
+__device__ __forceinline__ void tmem_wait_ld(float (&v)[32]) {
+    asm volatile(
+        "tcgen05.wait::ld.sync.aligned;"
+        : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]),
+          "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]), "+f"(v[16]),
+          "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]), "+f"(v[23]), "+f"(v[24]),
+          "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]), "+f"(v[30]), "+f"(v[31])
+        :
+        : "memory");
+}
+// Two fp32 operations in one instruction, each rounded as its own
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)),
+          "l"(reinterpret_cast<unsigned long long&>(c)));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("add.rn.f32x2 %0, %1, %2;"
+        : "=l"(reinterpret_cast<unsigned long long&>(d))
+        : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
+    return d;
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
@@ -407,15 +446,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     if (col < c_lo || col >= c_hi || !(valid >> (col >> 4) & 1)) v[i] = -INFINITY;
                 }
             };
-            float top = -INFINITY;
+            // two buffers of 32 columns: one is loaded while the other is used
+            float v[2][32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            tmem_ld32_start(s_at, v[0]);
 #pragma unroll
-            for (int c0 = 0; c0 < KT; c0 += 32) {
-                float v[32];
-                tmem_ld32(s_at + c0, v);
-                if (masked) mask(v, c0);
+            for (int i = 0; i < KT / 32; ++i) {
+                tmem_wait_ld(v[i & 1]);
+                tmem_ld32_start(s_at + (i + 1) % (KT / 32) * 32, v[(i + 1) & 1]);  // at last the first ones again
+                if (masked) mask(v[i & 1], i * 32);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) top = fmaxf(top, v[i]);
+                for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tops[k] = fmaxf(tops[k], fmaxf(v[i & 1][e + 2 * k], v[i & 1][e + 2 * k + 1]));
             }
+            float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             top *= sc;
             if (__any_sync(0xffffffffu, top > limit)) {
                 float fix = 1.0f;
@@ -426,31 +470,36 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     l *= fix;
                 }
                 if (j > 0) {
+                    tmem_wait_ld(v[0]);
 #pragma unroll
                     for (int d = 0; d < D; d += 32) {
-                        float v[32];
-                        tmem_ld32(o_at + d, v);
+                        tmem_ld32(o_at + d, v[1]);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] *= fix;
-                        tmem_st32(o_at + d, v);
+                        for (int i = 0; i < 32; ++i) v[1][i] *= fix;
+                        tmem_st32(o_at + d, v[1]);
                     }
                 }
             }
+            const float2 scale2 = make_float2(sc, sc), shift2 = make_float2(-m, -m);
+            float2 sums[2] = {};
 #pragma unroll
-            for (int c0 = 0; c0 < KT; c0 += 32) {
-                float v[32];
-                tmem_ld32(s_at + c0, v);
-                if (masked) mask(v, c0);
+            for (int i = 0; i < KT / 32; ++i) {
+                float (&x)[32] = v[i & 1];
+                tmem_wait_ld(x);
+                if (i + 1 < KT / 32) tmem_ld32_start(s_at + (i + 1) * 32, v[(i + 1) & 1]);
+                if (masked) mask(x, i * 32);
                 uint32_t p[16];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float x = ex2(fmaf(v[2 * i], sc, -m)), y = ex2(fmaf(v[2 * i + 1], sc, -m));
-                    l += x + y;
-                    const __half2 h = __floats2half2_rn(x, y);
-                    p[i] = *reinterpret_cast<const uint32_t*>(&h);
+                for (int e = 0; e < 16; ++e) {
+                    float2 w = fma2(make_float2(x[2 * e], x[2 * e + 1]), scale2, shift2);
+                    w = make_float2(ex2(w.x), ex2(w.y));
+                    sums[e & 1] = add2(sums[e & 1], w);
+                    const __half2 h = __floats2half2_rn(w.x, w.y);
+                    p[e] = *reinterpret_cast<const uint32_t*>(&h);
                 }
-                tmem_st16(s_at + c0 / 2, p);  // over columns that this thread has read
+                tmem_st16(s_at + i * 16, p);  // over columns that this thread has read
             }
+            l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
             tmem_wait_st();
             tc_fence_before();
             mbar_arrive(&p_full[t]);
