@@ -380,29 +380,32 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         __syncwarp();
     } else if (warp >= C::kSoftmax) {
         // ------------------------------------------------------------ dequantisation
-        const int dt = tid - C::kSoftmax * 32;
-        constexpr int kTasks = KT * (D / 32);  // 32 elements of a row
+        // A task is 32 elements of a row: piece q of row r. Neighbouring lanes take 4 rows by 2 pieces, so
+        // that their stores miss each other's banks; a thread keeps its piece and goes down the rows.
+        constexpr int kTasks = KT * (D / 32), kStep = C::kDequant * 32 / (D / 32);  // rows from task to task
+        static_assert(C::kDequant * 32 % (2 * D / 8) == 0, "a thread keeps its piece");
+        const int dt = tid - C::kSoftmax * 32, q = ((dt >> 3) % (D / 64)) * 2 + (dt & 1);
+        const int r0 = (dt >> 3) / (D / 64) * 4 + ((dt >> 1) & 3);
+        const int shift = 31 - __clz(R), par_at = R * (D / 2) + (q * 32 / ge.g) * 4, row_p = 4 * ng;
         for (int h = 0; h < halves; ++h) {
             const int slot = h % C::kRaw, bslot = h % C::kBufs, k0 = key0 + (h >> 1) * KT;
             if (!wait_or_abort(&raw_full[slot], (h / C::kRaw) & 1, abort)) break;
             if (h >= C::kBufs && !wait_or_abort(&buf_free[bslot], ((h / C::kBufs) - 1) & 1, abort)) break;
             const uint8_t* raw = s_raw + slot * raw_bytes;
-            uint8_t* out = s_buf + bslot * C::kBufBytes;
+            uint8_t* out = s_buf + bslot * C::kBufBytes + (q >> 1) * (KT * 128);
             const unsigned valid = s_valid[(h >> 1) & 7];
             const bool whole = valid == (1u << (KT / 16)) - 1 && k0 >= start && k0 + KT <= end;
 #pragma unroll 2
-            for (int i = dt; i < kTasks; i += C::kDequant * 32) {
-                // neighbouring lanes take 4 rows by 2 pieces: their stores then miss each other's banks
-                const int rest = i >> 3, q = (rest % (D / 64)) * 2 + (i & 1), r = rest / (D / 64) * 4 + ((i >> 1) & 3);
-                const uint8_t* src = raw + r / R * half_chunk;
-                const int rr = r % R;
+            for (int i = 0; i < kTasks / (C::kDequant * 32); ++i) {
+                const int r = r0 + i * kStep, rr = r & (R - 1);
+                const uint8_t* src = raw + (r >> shift) * half_chunk;
                 const uint4 w = *reinterpret_cast<const uint4*>(src + rr * (D / 2) + q * 16);
-                uint32_t par = *reinterpret_cast<const uint32_t*>(src + R * (D / 2) + (rr * ng + q * 32 / ge.g) * 4);
+                uint32_t par = *reinterpret_cast<const uint32_t*>(src + rr * row_p + par_at);
                 // rows that nobody sees may hold anything: they count as zeros
                 if (!whole && !((valid >> (r >> 4) & 1) && k0 + r >= start && k0 + r < end)) par = 0;
                 const __half2 step = __low2half2(as_half2(par)), low = __high2half2(as_half2(par));
                 const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-                uint8_t* dst = out + (q >> 1) * (KT * 128) + r * 128;
+                uint8_t* dst = out + r * 128;
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     __half2 f[4];
@@ -438,27 +441,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             const unsigned valid = s_valid[j & 7];
             const bool whole = lo <= k0 && hi >= k0 + KT && valid == (1u << (KT / 16)) - 1;
             const bool masked = __any_sync(0xffffffffu, !whole);
-            const int c_lo = max(lo - k0, 0), c_hi = min(max(hi, k0) - k0, KT);
-            auto mask = [&](float (&v)[32], int c0) {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const int col = c0 + i;
-                    if (col < c_lo || col >= c_hi || !(valid >> (col >> 4) & 1)) v[i] = -INFINITY;
-                }
-            };
             // two buffers of 32 columns: one is loaded while the other is used
-            float v[2][32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            tmem_ld32_start(s_at, v[0]);
+            float v0[32], v1[32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto take_max = [&](float (&v)[32], int c0) {
+                if (masked) {  // what the row does not see is written back as -inf
+                    const int c_lo = min(max(lo - k0 - c0, 0), 32), c_hi = min(max(max(hi, k0) - k0 - c0, 0), 32);
+                    unsigned bits = (c_hi == 32 ? ~0u : (1u << c_hi) - 1) & (c_lo == 32 ? 0u : ~0u << c_lo);
+                    bits &= ((valid >> (c0 / 16) & 1) ? 0xFFFFu : 0u) | ((valid >> (c0 / 16) & 2) ? 0xFFFF0000u : 0u);
 #pragma unroll
-            for (int i = 0; i < KT / 32; ++i) {
-                tmem_wait_ld(v[i & 1]);
-                tmem_ld32_start(s_at + (i + 1) % (KT / 32) * 32, v[(i + 1) & 1]);  // at last the first ones again
-                if (masked) mask(v[i & 1], i * 32);
+                    for (int i = 0; i < 32; ++i) v[i] = bits >> i & 1 ? v[i] : -INFINITY;
+                    tmem_st32(s_at + c0, v);
+                    tmem_wait_st();
+                }
 #pragma unroll
                 for (int e = 0; e < 32; e += 8)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tops[k] = fmaxf(tops[k], fmaxf(v[i & 1][e + 2 * k], v[i & 1][e + 2 * k + 1]));
+                    for (int k = 0; k < 4; ++k) tops[k] = fmaxf(tops[k], fmaxf(v[e + 2 * k], v[e + 2 * k + 1]));
+            };
+            tmem_ld32_start(s_at, v0);
+#pragma unroll 1
+            for (int c0 = 0; c0 < KT; c0 += 64) {
+                tmem_wait_ld(v0);
+                tmem_ld32_start(s_at + c0 + 32, v1);
+                take_max(v0, c0);
+                tmem_wait_ld(v1);
+                if (c0 + 64 < KT) tmem_ld32_start(s_at + c0 + 64, v0);
+                take_max(v1, c0 + 32);
             }
+            tmem_ld32_start(s_at, v0);
             float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             top *= sc;
             if (__any_sync(0xffffffffu, top > limit)) {
@@ -470,24 +480,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     l *= fix;
                 }
                 if (j > 0) {
-                    tmem_wait_ld(v[0]);
-#pragma unroll
+                    tmem_wait_ld(v0);
+#pragma unroll 1
                     for (int d = 0; d < D; d += 32) {
-                        tmem_ld32(o_at + d, v[1]);
+                        tmem_ld32(o_at + d, v1);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[1][i] *= fix;
-                        tmem_st32(o_at + d, v[1]);
+                        for (int i = 0; i < 32; ++i) v1[i] *= fix;
+                        tmem_st32(o_at + d, v1);
                     }
                 }
             }
             const float2 scale2 = make_float2(sc, sc), shift2 = make_float2(-m, -m);
             float2 sums[2] = {};
-#pragma unroll
-            for (int i = 0; i < KT / 32; ++i) {
-                float (&x)[32] = v[i & 1];
-                tmem_wait_ld(x);
-                if (i + 1 < KT / 32) tmem_ld32_start(s_at + (i + 1) * 32, v[(i + 1) & 1]);
-                if (masked) mask(x, i * 32);
+            auto weights = [&](const float (&x)[32], int c0) {  // over columns that this thread has read
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
@@ -497,7 +502,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     const __half2 h = __floats2half2_rn(w.x, w.y);
                     p[e] = *reinterpret_cast<const uint32_t*>(&h);
                 }
-                tmem_st16(s_at + i * 16, p);  // over columns that this thread has read
+                tmem_st16(s_at + c0 / 2, p);
+            };
+#pragma unroll 1
+            for (int c0 = 0; c0 < KT; c0 += 64) {
+                tmem_wait_ld(v0);
+                tmem_ld32_start(s_at + c0 + 32, v1);
+                weights(v0, c0);
+                tmem_wait_ld(v1);
+                if (c0 + 64 < KT) tmem_ld32_start(s_at + c0 + 64, v0);
+                weights(v1, c0 + 32);
             }
             l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
             tmem_wait_st();
