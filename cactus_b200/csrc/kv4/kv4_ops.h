@@ -37,7 +37,7 @@ struct AttnCall {
 // that the counters after it, which have to be zero before every call, are at the same place for
 // every shape.
 constexpr int kDecodeCtas = 148 * 4, kDecodePartFloats = 16 * (128 + 2);  // 2 parts a block, 16 rows of 128 at most
-constexpr int kPrefillParts = 2 * 148;                                    // of 256 rows of 128 (128 of 256) at most
+constexpr int kPrefillParts = 148;                                        // of 256 rows of 128 (128 of 256) at most
 constexpr size_t kPartBytes = (size_t)kPrefillParts * 256 * (128 + 2) * 4;
 static_assert(kPartBytes >= (size_t)kDecodeCtas * 2 * kDecodePartFloats * 4, "workspace");
 

@@ -3,8 +3,9 @@
 //
 // Work. A CTA takes 256 q rows of one sequence and kv head (two tiles of 128; 128 rows at
 // head_dim 256), row = token * heads that share the kv head + head, over a range of key tiles (128
-// keys, 64 at head_dim 256). Where there are too few such row tiles for the GPU, the keys are split
-// too; the parts go to the workspace, and the CTA that brings the last one joins them in order.
+// keys, 64 at head_dim 256). The row tiles that do not fill a round of the GPU (all, if they are few)
+// have their keys split over several CTAs; the parts go to the workspace, and the CTA that brings the
+// last one joins them in order.
 //
 // Warps (14), handing over through mbarriers:
 //   producer  raw codes and parameters of K and V half tiles into a ring (1-D bulk copies);
@@ -57,8 +58,8 @@ struct Args {
     unsigned* err;
     float* parts;
     unsigned* counters;
-    int min_rows;  // sequences with fewer rows a kv head are another kernel's
-    int splits;
+    int min_rows;    // sequences with fewer rows a kv head are another kernel's
+    int most_parts;  // of a row tile's keys
 };
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -183,7 +184,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     uint8_t* const s_q = smem;                       // [row tile][D / 64][128 rows][128 bytes]
     uint8_t* const s_buf = smem + C::kQBytes;        // ring of K, V tiles [D / 64][KT rows][128 bytes]
     uint8_t* const s_raw = s_buf + C::kBufs * C::kBufBytes;
-    __shared__ uint64_t s_full[MT], p_full[MT], o_full[MT], buf_full[C::kBufs], buf_free[C::kBufs], raw_full[C::kRaw],
+    __shared__ uint64_t s_full[MT], p_full[MT][2], o_full[MT], buf_full[C::kBufs], buf_free[C::kBufs], raw_full[C::kRaw],
         raw_free[C::kRaw], drain;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_item[4], s_scan[kWarps], s_last;
@@ -197,8 +198,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
 
     // ---- which sequence, rows, kv head and part of the keys: row tiles of a sequence from its last,
     // which sees the most
-    const int split = blockIdx.x % a.splits, item = blockIdx.x / a.splits;
-    const int pair = item / ge.hkv, head = item % ge.hkv;
     const int per = (c.num_seqs + kThreads - 1) / kThreads;
     auto row_tiles = [&](int b) {
         const int rows = max(0, min(c.offsets[b + 1] - c.offsets[b], c.max_q)) * share;
@@ -218,7 +217,18 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         s_abort = 0;
     }
     __syncthreads();
-    for (int x = 0; x < warp; ++x) upto += s_scan[x];
+    int items = 0;
+    for (int x = 0; x < kWarps; ++x) {
+        if (x < warp) upto += s_scan[x];
+        items += s_scan[x] * ge.hkv;
+    }
+    // whole rounds of the GPU first; the rest in as many parts as a round has room for
+    const int whole_items = items / kNumSMs * kNumSMs, rest = items - whole_items;
+    const int parts = rest ? min(kNumSMs / rest, a.most_parts) : 1, unit = (int)blockIdx.x - whole_items;
+    if (unit >= rest * parts) return;
+    const int splits = unit < 0 ? 1 : parts, split = unit < 0 ? 0 : unit % parts;
+    const int item = unit < 0 ? (int)blockIdx.x : whole_items + unit / parts;
+    const int pair = item / ge.hkv, head = item % ge.hkv;
     if (pair >= upto - mine && pair < upto) {
         int at = upto - mine, b = tid * per;
         for (;; ++b) {
@@ -246,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     int start = c.window > 0 ? (int)max(0LL, pos0 + first_tok - c.window + 1) : 0;
     if (start >= end) start = end = 0;
     const int base = start & ~(KT - 1), all = (end - base + KT - 1) / KT;
-    const int t_from = (int)((long long)all * split / a.splits), t_to = (int)((long long)all * (split + 1) / a.splits);
+    const int t_from = (int)((long long)all * split / splits), t_to = (int)((long long)all * (split + 1) / splits);
     const int tiles = t_to - t_from, key0 = base + t_from * KT;
 
     // ---- set-up: barriers, TMEM, Q
@@ -258,7 +268,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     if (tid == 0) {
         for (int i = 0; i < MT; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 128);
+            mbar_init(&p_full[i][0], 128);
+            mbar_init(&p_full[i][1], 128);
             mbar_init(&o_full[i], 1);
         }
         for (int i = 0; i < C::kBufs; ++i) {
@@ -356,13 +367,16 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             for (int j = 0; j < tiles && ok; ++j) {
                 for (int t = 0; t < MT && ok; ++t) {
                     if (t == 0) need(2 * j + 1);
-                    ok = ok && wait_or_abort(&p_full[t], j & 1, abort);
-                    if (!ok) break;
-                    tc_fence_after();
                     const uint32_t vb = buf + ((2 * j + 1) % C::kBufs) * C::kBufBytes;
-                    for (int k = 0; k < KT / 16; ++k)
-                        mma_ts(tmem + C::kO + t * D, tmem + t * KT + k * 8, desc(vb + k * 2048, KT * 128), idesc(D, true),
-                               j > 0 || k > 0);
+                    for (int half = 0; half < 2 && ok; ++half) {  // the weights come in two halves
+                        ok = wait_or_abort(&p_full[t][half], j & 1, abort);
+                        if (!ok) break;
+                        tc_fence_after();
+                        for (int k = half * (KT / 32); k < (half + 1) * (KT / 32); ++k)
+                            mma_ts(tmem + C::kO + t * D, tmem + t * KT + k * 8, desc(vb + k * 2048, KT * 128),
+                                   idesc(D, true), j > 0 || k > 0);
+                    }
+                    if (!ok) break;
                     if (t == MT - 1) commit(&buf_free[(2 * j + 1) % C::kBufs]);
                     if (j + 1 < tiles) {
                         if (t == 0) need(2 * j + 2);
@@ -492,6 +506,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             }
             const float2 scale2 = make_float2(sc, sc), shift2 = make_float2(-m, -m);
             float2 sums[2] = {};
+            auto hand_over = [&](int half) {
+                tmem_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_full[t][half]);
+            };
             auto weights = [&](const float (&x)[32], int c0) {  // over columns that this thread has read
                 uint32_t p[16];
 #pragma unroll
@@ -509,21 +528,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 tmem_wait_ld(v0);
                 tmem_ld32_start(s_at + c0 + 32, v1);
                 weights(v0, c0);
+                if (KT == 64) hand_over(0);
                 tmem_wait_ld(v1);
                 if (c0 + 64 < KT) tmem_ld32_start(s_at + c0 + 64, v0);
                 weights(v1, c0 + 32);
+                hand_over(KT == 64 ? 1 : c0 / 64);
             }
             l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
-            tmem_wait_st();
-            tc_fence_before();
-            mbar_arrive(&p_full[t]);
         }
         if (tiles > 0 && ok) ok = wait_or_abort(&o_full[t], 0, abort);
         tc_fence_after();
         // ---- the result, or this part of it
         const float m_out = limit == -INFINITY ? -INFINITY : m;
-        bool last = a.splits == 1;
-        const int slot0 = item * a.splits;
+        bool last = splits == 1;
+        const int slot0 = unit - split;  // where there are parts
         constexpr int kSlot = C::kRows * (D + 2);  // floats: [D / 4][row][4], then m and l of the rows
         if (!last) {
             float* part = a.parts + (size_t)(slot0 + split) * kSlot;
@@ -543,9 +561,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             __threadfence();
             asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftmax * 32) : "memory");
             if (tid == 0) {
-                const unsigned before = atomicAdd(&a.counters[item], 1u);
-                s_last = before + 1 == (unsigned)a.splits;
-                if (s_last) a.counters[item] = 0;
+                const unsigned before = atomicAdd(&a.counters[item - whole_items], 1u);
+                s_last = before + 1 == (unsigned)splits;
+                if (s_last) a.counters[item - whole_items] = 0;
             }
             asm volatile("bar.sync 1, %0;" ::"n"(C::kSoftmax * 32) : "memory");
             last = s_last != 0;
@@ -553,12 +571,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         }
         if (last) {
             float mm = m_out, ll = l;
-            if (a.splits > 1) {
+            if (splits > 1) {
                 mm = -INFINITY;
-                for (int x = 0; x < a.splits; ++x)
+                for (int x = 0; x < splits; ++x)
                     mm = fmaxf(mm, __ldcg(a.parts + (size_t)(slot0 + x) * kSlot + (size_t)C::kRows * D + r));
                 ll = 0.0f;
-                for (int x = 0; x < a.splits; ++x) {
+                for (int x = 0; x < splits; ++x) {
                     const float* p = a.parts + (size_t)(slot0 + x) * kSlot + (size_t)C::kRows * D + r;
                     const float pl = __ldcg(p + C::kRows), pm = __ldcg(p);
                     ll += pl * (pm == -INFINITY ? (pl != pl ? 1.0f : 0.0f) : ex2(pm - mm));
@@ -570,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
 #pragma unroll
             for (int d = 0; d < D; d += 32) {
                 float v[32];
-                if (a.splits == 1) {
+                if (splits == 1) {
                     if (tiles > 0) {
                         tmem_ld32(o_at + d, v);
                     } else {
@@ -580,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = 0.0f;
-                    for (int x = 0; x < a.splits; ++x) {
+                    for (int x = 0; x < splits; ++x) {
                         const float* p = a.parts + (size_t)(slot0 + x) * kSlot;
                         const float pm = __ldcg(p + (size_t)C::kRows * D + r), pl = __ldcg(p + (size_t)C::kRows * D + C::kRows + r);
                         const float f = pm == -INFINITY ? (pl != pl ? 1.0f : 0.0f) : ex2(pm - mm);
@@ -629,23 +647,6 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     }
 }
 
-// How many parts the keys of a row tile are split into: the number (up to 16, and up to kPrefillParts
-// CTAs in all) with which the rounds over the GPU, each as long as 1 / parts of a row tile's keys
-// and a fixed start and end, take the least.
-int splits_of(long long items, long long key_tiles) {
-    int best = 1;
-    double least = 1e30;
-    for (int p = 1; p <= 16 && (p == 1 || items * p <= kPrefillParts) && p <= key_tiles; ++p) {
-        const double rounds = (double)((items * p + kNumSMs - 1) / kNumSMs);
-        const double time = rounds * ((double)key_tiles / p + 3.0 + (p > 1 ? 2.0 + 0.25 * p : 0.0));
-        if (time < least * 0.97) {
-            least = time;
-            best = p;
-        }
-    }
-    return best;
-}
-
 template <int D>
 int launch(const AttnCall& c, const Pages& pg, const Geom& ge, int min_rows, cudaStream_t st) {
     using C = Cfg<D>;
@@ -675,11 +676,12 @@ int launch(const AttnCall& c, const Pages& pg, const Geom& ge, int min_rows, cud
     const long long items = pairs * ge.hkv;
     long long keys = pg.table_stride << ge.page_shift;
     if (c.window > 0 && c.window + C::kRows / share + 1 < keys) keys = c.window + C::kRows / share + 1;
-    a.splits = splits_of(items, (keys + C::kKeys - 1) / C::kKeys);
-    if (items * a.splits > 0x7fffffffLL) return -2;
-    return launch_k(kernel, dim3((unsigned)(items * a.splits)), dim3(kThreads), (size_t)C::smem(ge.ng()), st, a) == cudaSuccess
-               ? 0
-               : -1;
+    // four tiles of keys a part at least: joining costs about as much
+    const long long parts = (keys + C::kKeys - 1) / C::kKeys / 4;
+    a.most_parts = parts < 1 ? 1 : parts > 32 ? 32 : (int)parts;
+    const long long grid = (items / kNumSMs + 1) * kNumSMs;
+    if (grid > 0x7fffffffLL) return -2;
+    return launch_k(kernel, dim3((unsigned)grid), dim3(kThreads), (size_t)C::smem(ge.ng()), st, a) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace
