@@ -346,43 +346,58 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     } else if (warp == kWarps - 2) {
         // ------------------------------------------------------------ tensor core
         if (lane == 0) {
-            const uint32_t q = smem_u32(s_q), buf = smem_u32(s_buf);
+            // descriptors differ from these by constants: a product must take less time to issue than to run
+            const uint64_t q_desc = desc(smem_u32(s_q), 16), k_desc = desc(smem_u32(s_buf), 16),
+                           v_desc = desc(smem_u32(s_buf), KT * 128);
             bool ok = true;
-            auto need = [&](int h) {
-                ok = ok && wait_or_abort(&buf_full[h % C::kBufs], (h / C::kBufs) & 1, abort);
+            int slot = 0;        // ring slot of half h, the next to be waited for, and its parity
+            unsigned phase = 0;
+            auto need = [&]() -> int {
+                const int s = slot;
+                ok = ok && wait_or_abort(&buf_full[s], phase, abort);
                 tc_fence_after();
+                if (++slot == C::kBufs) {
+                    slot = 0;
+                    phase ^= 1;
+                }
+                return s;
             };
-            auto qk = [&](int t, int j) {
-                const uint32_t kb = buf + (2 * j % C::kBufs) * C::kBufBytes, qa = q + t * (128 * D * 2);
+            auto qk = [&](int t, int s) {
+                const uint64_t qa = q_desc + (uint64_t)(t * (128 * D * 2 / 16)), kb = k_desc + (uint64_t)(s * (C::kBufBytes / 16));
+#pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_ss(tmem + t * KT, desc(qa + (k >> 2) * (128 * 128) + (k & 3) * 32, 16),
-                           desc(kb + (k >> 2) * (KT * 128) + (k & 3) * 32, 16), idesc(KT, false), k > 0);
+                    mma_ss(tmem + t * KT, qa + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16,
+                           kb + ((k >> 2) * (KT * 128) + (k & 3) * 32) / 16, idesc(KT, false), k > 0);
                 commit(&s_full[t]);
             };
+            int ks = 0, vs = 0;
             if (tiles > 0) {
-                need(0);
-                for (int t = 0; t < MT && ok; ++t) qk(t, 0);
-                if (ok) commit(&buf_free[0]);
+                ks = need();
+                for (int t = 0; t < MT && ok; ++t) qk(t, ks);
+                if (ok) commit(&buf_free[ks]);
             }
             for (int j = 0; j < tiles && ok; ++j) {
-                for (int t = 0; t < MT && ok; ++t) {
-                    if (t == 0) need(2 * j + 1);
-                    const uint32_t vb = buf + ((2 * j + 1) % C::kBufs) * C::kBufBytes;
-                    for (int half = 0; half < 2 && ok; ++half) {  // the weights come in two halves
-                        ok = wait_or_abort(&p_full[t][half], j & 1, abort);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    if (t == 0) vs = need();
+                    const uint64_t vb = v_desc + (uint64_t)(vs * (C::kBufBytes / 16));
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {  // the weights come in two halves
+                        ok = ok && wait_or_abort(&p_full[t][half], j & 1, abort);
                         if (!ok) break;
                         tc_fence_after();
+#pragma unroll
                         for (int k = half * (KT / 32); k < (half + 1) * (KT / 32); ++k)
-                            mma_ts(tmem + C::kO + t * D, tmem + t * KT + k * 8, desc(vb + k * 2048, KT * 128),
-                                   idesc(D, true), j > 0 || k > 0);
+                            mma_ts(tmem + C::kO + t * D, tmem + t * KT + k * 8, vb + k * (2048 / 16), idesc(D, true),
+                                   j > 0 || k > 0);
                     }
                     if (!ok) break;
-                    if (t == MT - 1) commit(&buf_free[(2 * j + 1) % C::kBufs]);
+                    if (t == MT - 1) commit(&buf_free[vs]);
                     if (j + 1 < tiles) {
-                        if (t == 0) need(2 * j + 2);
+                        if (t == 0) ks = need();
                         if (!ok) break;
-                        qk(t, j + 1);
-                        if (t == MT - 1) commit(&buf_free[(2 * j + 2) % C::kBufs]);
+                        qk(t, ks);
+                        if (t == MT - 1) commit(&buf_free[ks]);
                     } else {
                         commit(&o_full[t]);
                     }
