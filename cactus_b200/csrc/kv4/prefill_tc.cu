@@ -7,7 +7,7 @@
 // have their keys split over several CTAs; the parts go to the workspace, and the CTA that brings the
 // last one joins them in order.
 //
-// Warps (14), handing over through mbarriers:
+// Warps (16, whose registers are dealt out by their need), handing over through mbarriers:
 //   producer  raw codes and parameters of K and V half tiles into a ring (1-D bulk copies);
 //   dequant   codes -> fp16 values in the swizzled operand layout, once for all 256 rows;
 //   mma       one thread: S = Q K^T (operands in shared memory), O += P V (P in TMEM);
@@ -33,7 +33,7 @@ namespace kv4 {
 
 namespace {
 
-constexpr int kWarps = 14, kThreads = kWarps * 32;
+constexpr int kWarps = 16, kThreads = kWarps * 32, kMma = 12, kProducer = 13;  // warps 14 and 15 have no work
 constexpr float kLazy = 8.0f;
 
 template <int D>
@@ -42,9 +42,12 @@ struct Cfg {
     static constexpr int kTiles = D == 256 ? 1 : 2;     // row tiles
     static constexpr int kRows = 128 * kTiles;
     static constexpr int kBufBytes = kKeys * D * 2;     // a K or V tile in fp16
-    static constexpr int kBufs = D == 64 ? 4 : 3;
-    static constexpr int kRaw = 4;                      // raw half tiles
-    static constexpr int kSoftmax = 4 * kTiles, kDequant = kWarps - 2 - kSoftmax;
+    static constexpr int kBufs = D == 64 ? 6 : 4;
+    static constexpr int kRaw = D == 64 ? 6 : 3;         // raw half tiles
+    static constexpr int kSoftmax = 4 * kTiles, kDequant = kMma - kSoftmax;  // warps
+    // registers a thread: the block is launched with 128 each
+    static constexpr int kSoftmaxRegs = 192, kDequantRegs = kTiles == 2 ? 88 : 96, kOtherRegs = 40;
+    static constexpr int kRegs = 32 * (kSoftmax * kSoftmaxRegs + kDequant * kDequantRegs + 4 * kOtherRegs);
     static constexpr int kQBytes = kRows * D * 2;
     static constexpr int kO = 256;                      // TMEM column of O (S: kKeys columns a row tile from 0)
     __host__ __device__ static constexpr int raw_bytes(int ng) { return kKeys * (D / 2 + 4 * ng); }
@@ -75,19 +78,31 @@ __device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo) {
 constexpr uint32_t idesc(int n, bool mn) {
     return (1u << 4) | ((mn ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc));
+// The issuing warp runs converged, one elected lane's predicate on the instructions themselves: their
+// operands then stay in uniform registers (in a branch of one lane each product took 120 cycles to issue).
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc));
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc),
+        "r"(leader));
 }
-__device__ __forceinline__ void commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc),
+        "r"(leader));
+}
+__device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(smem_u32(bar)),
+        "r"(leader)
+        : "memory");
 }
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
     asm volatile(
@@ -140,14 +155,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
         : "l"(reinterpret_cast<unsigned long long&>(a)), "l"(reinterpret_cast<unsigned long long&>(b)));
     return d;
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-        "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
-        "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]),
-        "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]),
-        "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+          "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
         : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
@@ -260,7 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     const int tiles = t_to - t_from, key0 = base + t_from * KT;
 
     // ---- set-up: barriers, TMEM, Q
-    if (warp == kWarps - 2) {
+    if (warp == kMma) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -306,7 +320,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     const int halves = 2 * tiles;  // K and V of each tile in turn
     const int R = min(ge.page(), KT), half_chunk = R * (D / 2 + 4 * ng), raw_bytes = C::raw_bytes(ng);
 
-    if (warp == kWarps - 1) {
+    // each role starts with its share of the registers (a warpgroup asks for one number)
+    if (warp >= kMma) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kOtherRegs));
+    if (warp == kProducer) {
         // ------------------------------------------------------------ producer
         // lane 2 i + p: chunk i of a half tile (the rows of one page), codes (0) or parameters (1); a
         // chunk that is all of a page's rows is one piece
@@ -343,9 +360,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         // no copy may land after the block leaves
         if (*abort && lane == 0)
             for (int h = max(0, issued - C::kRaw); h < issued; ++h) mbar_wait_bounded(&raw_full[h % C::kRaw], (h / C::kRaw) & 1);
-    } else if (warp == kWarps - 2) {
+    } else if (warp == kMma) {
         // ------------------------------------------------------------ tensor core
-        if (lane == 0) {
+        {
+            const uint32_t leader = elect_one();
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const int n_tiles = __shfl_sync(0xffffffffu, tiles, 0);
             // descriptors differ from these by constants: a product must take less time to issue than to run
             const uint64_t q_desc = desc(smem_u32(s_q), 16), k_desc = desc(smem_u32(s_buf), 16),
                            v_desc = desc(smem_u32(s_buf), KT * 128);
@@ -354,7 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             unsigned phase = 0;
             auto need = [&]() -> int {
                 const int s = slot;
-                ok = ok && wait_or_abort(&buf_full[s], phase, abort);
+                ok = ok && __all_sync(0xffffffffu, wait_or_abort(&buf_full[s], phase, abort));
                 tc_fence_after();
                 if (++slot == C::kBufs) {
                     slot = 0;
@@ -366,49 +386,51 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 const uint64_t qa = q_desc + (uint64_t)(t * (128 * D * 2 / 16)), kb = k_desc + (uint64_t)(s * (C::kBufBytes / 16));
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_ss(tmem + t * KT, qa + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16,
+                    mma_ss(leader, tm + t * KT, qa + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16,
                            kb + ((k >> 2) * (KT * 128) + (k & 3) * 32) / 16, idesc(KT, false), k > 0);
-                commit(&s_full[t]);
+                commit(leader, &s_full[t]);
             };
             int ks = 0, vs = 0;
-            if (tiles > 0) {
+            if (n_tiles > 0) {
                 ks = need();
                 for (int t = 0; t < MT && ok; ++t) qk(t, ks);
-                if (ok) commit(&buf_free[ks]);
+                if (ok) commit(leader, &buf_free[ks]);
             }
-            for (int j = 0; j < tiles && ok; ++j) {
+            for (int j = 0; j < n_tiles && ok; ++j) {
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
                     if (t == 0) vs = need();
                     const uint64_t vb = v_desc + (uint64_t)(vs * (C::kBufBytes / 16));
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {  // the weights come in two halves
-                        ok = ok && wait_or_abort(&p_full[t][half], j & 1, abort);
+                        ok = ok && __all_sync(0xffffffffu, wait_or_abort(&p_full[t][half], j & 1, abort));
                         if (!ok) break;
                         tc_fence_after();
 #pragma unroll
                         for (int k = half * (KT / 32); k < (half + 1) * (KT / 32); ++k)
-                            mma_ts(tmem + C::kO + t * D, tmem + t * KT + k * 8, vb + k * (2048 / 16), idesc(D, true),
+                            mma_ts(leader, tm + C::kO + t * D, tm + t * KT + k * 8, vb + k * (2048 / 16), idesc(D, true),
                                    j > 0 || k > 0);
                     }
                     if (!ok) break;
-                    if (t == MT - 1) commit(&buf_free[vs]);
-                    if (j + 1 < tiles) {
+                    if (t == MT - 1) commit(leader, &buf_free[vs]);
+                    if (j + 1 < n_tiles) {
                         if (t == 0) ks = need();
                         if (!ok) break;
                         qk(t, ks);
-                        if (t == MT - 1) commit(&buf_free[ks]);
+                        if (t == MT - 1) commit(leader, &buf_free[ks]);
                     } else {
-                        commit(&o_full[t]);
+                        commit(leader, &o_full[t]);
                     }
                 }
             }
-            commit(&drain);  // every product issued has completed before TMEM is released
+            commit(leader, &drain);  // every product issued has completed before TMEM is released
             mbar_wait_bounded(&drain, 0);
         }
         __syncwarp();
+    }
     } else if (warp >= C::kSoftmax) {
         // ------------------------------------------------------------ dequantisation
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kDequantRegs));
         // A task is 32 elements of a row: piece q of row r. Neighbouring lanes take 4 rows by 2 pieces, so
         // that their stores miss each other's banks; a thread keeps its piece and goes down the rows.
         constexpr int kTasks = KT * (D / 32), kStep = C::kDequant * 32 / (D / 32);  // rows from task to task
@@ -451,6 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         }
     } else {
         // ------------------------------------------------------------ softmax: a thread a row
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
         const int t = warp >> 2, r = t * 128 + (warp & 3) * 32 + lane, row = row0 + r;
         const bool on = r < rows;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -470,34 +493,28 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             const unsigned valid = s_valid[j & 7];
             const bool whole = lo <= k0 && hi >= k0 + KT && valid == (1u << (KT / 16)) - 1;
             const bool masked = __any_sync(0xffffffffu, !whole);
-            // two buffers of 32 columns: one is loaded while the other is used
-            float v0[32], v1[32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            auto take_max = [&](float (&v)[32], int c0) {
-                if (masked) {  // what the row does not see is written back as -inf
+            float x[KT / 32][32], tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < KT / 32; ++i) tmem_ld32_start(s_at + i * 32, x[i]);
+#pragma unroll
+            for (int i = 0; i < KT / 32; ++i) tmem_wait_ld(x[i]);
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < KT / 32; ++i) {
+                    const int c0 = i * 32;
                     const int c_lo = min(max(lo - k0 - c0, 0), 32), c_hi = min(max(max(hi, k0) - k0 - c0, 0), 32);
                     unsigned bits = (c_hi == 32 ? ~0u : (1u << c_hi) - 1) & (c_lo == 32 ? 0u : ~0u << c_lo);
                     bits &= ((valid >> (c0 / 16) & 1) ? 0xFFFFu : 0u) | ((valid >> (c0 / 16) & 2) ? 0xFFFF0000u : 0u);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) v[i] = bits >> i & 1 ? v[i] : -INFINITY;
-                    tmem_st32(s_at + c0, v);
-                    tmem_wait_st();
+                    for (int e = 0; e < 32; ++e) x[i][e] = bits >> e & 1 ? x[i][e] : -INFINITY;
                 }
+            }
+#pragma unroll
+            for (int i = 0; i < KT / 32; ++i)
 #pragma unroll
                 for (int e = 0; e < 32; e += 8)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tops[k] = fmaxf(tops[k], fmaxf(v[e + 2 * k], v[e + 2 * k + 1]));
-            };
-            tmem_ld32_start(s_at, v0);
-#pragma unroll 1
-            for (int c0 = 0; c0 < KT; c0 += 64) {
-                tmem_wait_ld(v0);
-                tmem_ld32_start(s_at + c0 + 32, v1);
-                take_max(v0, c0);
-                tmem_wait_ld(v1);
-                if (c0 + 64 < KT) tmem_ld32_start(s_at + c0 + 64, v0);
-                take_max(v1, c0 + 32);
-            }
-            tmem_ld32_start(s_at, v0);
+                    for (int k = 0; k < 4; ++k) tops[k] = fmaxf(tops[k], fmaxf(x[i][e + 2 * k], x[i][e + 2 * k + 1]));
             float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             top *= sc;
             if (__any_sync(0xffffffffu, top > limit)) {
@@ -509,13 +526,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     l *= fix;
                 }
                 if (j > 0) {
-                    tmem_wait_ld(v0);
 #pragma unroll 1
-                    for (int d = 0; d < D; d += 32) {
-                        tmem_ld32(o_at + d, v1);
+                    for (int d = 0; d < D; d += 16) {
+                        uint32_t v[16];
+                        tmem_ld16(o_at + d, v);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v1[i] *= fix;
-                        tmem_st32(o_at + d, v1);
+                        for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * fix);
+                        tmem_st16(o_at + d, v);
                     }
                 }
             }
@@ -526,28 +543,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 tc_fence_before();
                 mbar_arrive(&p_full[t][half]);
             };
-            auto weights = [&](const float (&x)[32], int c0) {  // over columns that this thread has read
+#pragma unroll
+            for (int i = 0; i < KT / 32; ++i) {
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    float2 w = fma2(make_float2(x[2 * e], x[2 * e + 1]), scale2, shift2);
+                    float2 w = fma2(make_float2(x[i][2 * e], x[i][2 * e + 1]), scale2, shift2);
                     w = make_float2(ex2(w.x), ex2(w.y));
                     sums[e & 1] = add2(sums[e & 1], w);
                     const __half2 h = __floats2half2_rn(w.x, w.y);
                     p[e] = *reinterpret_cast<const uint32_t*>(&h);
                 }
-                tmem_st16(s_at + c0 / 2, p);
-            };
-#pragma unroll 1
-            for (int c0 = 0; c0 < KT; c0 += 64) {
-                tmem_wait_ld(v0);
-                tmem_ld32_start(s_at + c0 + 32, v1);
-                weights(v0, c0);
-                if (KT == 64) hand_over(0);
-                tmem_wait_ld(v1);
-                if (c0 + 64 < KT) tmem_ld32_start(s_at + c0 + 64, v0);
-                weights(v1, c0 + 32);
-                hand_over(KT == 64 ? 1 : c0 / 64);
+                tmem_st16(s_at + i * 16, p);  // over S, which this thread has read
+                if ((i + 1) % (KT / 64) == 0) hand_over(i / (KT / 64));
             }
             l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
         }
@@ -656,7 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     __syncwarp();
     __syncthreads();
     if (tid == 0 && *abort) atomicCAS(a.err, 0u, (unsigned)kDevTmaTimeout);
-    if (warp == kWarps - 2) {
+    if (warp == kMma) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
@@ -670,6 +678,9 @@ int launch(const AttnCall& c, const Pages& pg, const Geom& ge, int min_rows, cud
     int dev = 0;
     cudaGetDevice(&dev);
     if (!(set.load() >> (dev & 63) & 1)) {
+        // the registers that the warps deal out among themselves have to be there
+        cudaFuncAttributes attr;
+        if (cudaFuncGetAttributes(&attr, kernel) != cudaSuccess || attr.numRegs * kThreads < C::kRegs) return -1;
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(D / 32)) != cudaSuccess)
             return -1;
         set.fetch_or(1ull << (dev & 63));
