@@ -46,7 +46,7 @@ struct Cfg {
     static constexpr int kRaw = D == 64 ? 6 : 3;         // raw half tiles
     static constexpr int kSoftmax = 4 * kTiles, kDequant = kMma - kSoftmax;  // warps
     // registers a thread: the block is launched with 128 each
-    static constexpr int kSoftmaxRegs = 192, kDequantRegs = kTiles == 2 ? 88 : 96, kOtherRegs = 40;
+    static constexpr int kSoftmaxRegs = 184, kDequantRegs = kTiles == 2 ? 88 : 96, kOtherRegs = 56;
     static constexpr int kRegs = 32 * (kSoftmax * kSoftmaxRegs + kDequant * kDequantRegs + 4 * kOtherRegs);
     static constexpr int kQBytes = kRows * D * 2;
     static constexpr int kO = 256;                      // TMEM column of O (S: kKeys columns a row tile from 0)
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     uint8_t* const s_buf = smem + C::kQBytes;        // ring of K, V tiles [D / 64][KT rows][128 bytes]
     uint8_t* const s_raw = s_buf + C::kBufs * C::kBufBytes;
     __shared__ uint64_t s_full[MT], p_full[MT][2], o_full[MT], buf_full[C::kBufs], buf_free[C::kBufs], raw_full[C::kRaw],
-        raw_free[C::kRaw], drain;
+        raw_free[C::kRaw], q_full, drain;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_item[4], s_scan[kWarps], s_last;
     __shared__ unsigned s_valid[8];  // a bit for each 16 keys of a tile that were loaded, tiles modulo 8
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     const int t_from = (int)((long long)all * split / splits), t_to = (int)((long long)all * (split + 1) / splits);
     const int tiles = t_to - t_from, key0 = base + t_from * KT;
 
-    // ---- set-up: barriers, TMEM, Q
+    // ---- set-up: barriers, TMEM
     if (warp == kMma) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(512)
                      : "memory");
@@ -294,24 +294,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             mbar_init(&raw_full[i], 1);
             mbar_init(&raw_free[i], C::kDequant);
         }
+        mbar_init(&q_full, kMma * 32);
         mbar_init(&drain, 1);
         fence_mbar_init();
     }
-    for (int i = tid; i < C::kRows * (D / 8); i += kThreads) {
-        const int r = i / (D / 8), ch = i % (D / 8);
-        uint4 v = {0, 0, 0, 0};
-        if (r < rows) {
-            const int row = row0 + r;
-            v = __ldg(reinterpret_cast<const uint4*>(c.q + (long long)(tok0 + row / share) * c.q_stride +
-                                                     (long long)(head * share + row % share) * D) + ch);
-        }
-        const uint4 p = {__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                         __byte_perm(v.y, v.w, 0x7632)};
-        const int rt = r & 127;
-        *reinterpret_cast<uint4*>(s_q + (r >> 7) * (128 * D * 2) + (ch >> 3) * (128 * 128) + rt * 128 +
-                                  (((ch & 7) ^ (rt & 7)) << 4)) = p;
-    }
-    fence_proxy_async_shared();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -319,6 +305,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     volatile int* const abort = &s_abort;
     const int halves = 2 * tiles;  // K and V of each tile in turn
     const int R = min(ge.page(), KT), half_chunk = R * (D / 2 + 4 * ng), raw_bytes = C::raw_bytes(ng);
+
+    auto load_q = [&] {  // by the softmax and dequantisation warps, while the first keys are on their way
+        constexpr int kAll = C::kRows * (D / 8), kStep = kMma * 32, kBatch = 6;
+#pragma unroll 1
+        for (int i0 = tid; i0 < kAll; i0 += kBatch * kStep) {
+            uint4 v[kBatch];
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int i = i0 + u * kStep, r = i / (D / 8), row = row0 + r, token = row / share;
+                v[u] = uint4{0, 0, 0, 0};
+                if (i < kAll && r < rows)
+                    v[u] = __ldg(reinterpret_cast<const uint4*>(c.q + (long long)(tok0 + token) * c.q_stride +
+                                                                (long long)(head * share + row - token * share) * D) +
+                                 i % (D / 8));
+            }
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int i = i0 + u * kStep, r = i / (D / 8), ch = i % (D / 8), rt = r & 127;
+                if (i < kAll)
+                    *reinterpret_cast<uint4*>(s_q + (r >> 7) * (128 * D * 2) + (ch >> 3) * (128 * 128) + rt * 128 +
+                                              (((ch & 7) ^ (rt & 7)) << 4)) =
+                        uint4{__byte_perm(v[u].x, v[u].z, 0x5410), __byte_perm(v[u].x, v[u].z, 0x7632),
+                              __byte_perm(v[u].y, v[u].w, 0x5410), __byte_perm(v[u].y, v[u].w, 0x7632)};
+            }
+        }
+        fence_proxy_async_shared();
+        mbar_arrive(&q_full);
+    };
 
     // each role starts with its share of the registers (a warpgroup asks for one number)
     if (warp >= kMma) {
@@ -392,6 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             };
             int ks = 0, vs = 0;
             if (n_tiles > 0) {
+                ok = __all_sync(0xffffffffu, wait_or_abort(&q_full, 0, abort));
                 ks = need();
                 for (int t = 0; t < MT && ok; ++t) qk(t, ks);
                 if (ok) commit(leader, &buf_free[ks]);
@@ -431,10 +446,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     } else if (warp >= C::kSoftmax) {
         // ------------------------------------------------------------ dequantisation
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kDequantRegs));
+        load_q();
         // A task is 32 elements of a row: piece q of row r. Neighbouring lanes take 4 rows by 2 pieces, so
         // that their stores miss each other's banks; a thread keeps its piece and goes down the rows.
         constexpr int kTasks = KT * (D / 32), kStep = C::kDequant * 32 / (D / 32);  // rows from task to task
-        static_assert(C::kDequant * 32 % (2 * D / 8) == 0, "a thread keeps its piece");
+        static_assert(C::kDequant * 32 % (2 * D / 8) == 0 && kTasks % (2 * C::kDequant * 32) == 0, "a thread keeps its piece");
         const int dt = tid - C::kSoftmax * 32, q = ((dt >> 3) % (D / 64)) * 2 + (dt & 1);
         const int r0 = (dt >> 3) / (D / 64) * 4 + ((dt >> 1) & 3);
         const int shift = 31 - __clz(R), par_at = R * (D / 2) + (q * 32 / ge.g) * 4, row_p = 4 * ng;
@@ -446,24 +462,34 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             uint8_t* out = s_buf + bslot * C::kBufBytes + (q >> 1) * (KT * 128);
             const unsigned valid = s_valid[(h >> 1) & 7];
             const bool whole = valid == (1u << (KT / 16)) - 1 && k0 >= start && k0 + KT <= end;
-#pragma unroll 2
-            for (int i = 0; i < kTasks / (C::kDequant * 32); ++i) {
-                const int r = r0 + i * kStep, rr = r & (R - 1);
-                const uint8_t* src = raw + (r >> shift) * half_chunk;
-                const uint4 w = *reinterpret_cast<const uint4*>(src + rr * (D / 2) + q * 16);
-                uint32_t par = *reinterpret_cast<const uint32_t*>(src + rr * row_p + par_at);
-                // rows that nobody sees may hold anything: they count as zeros
-                if (!whole && !((valid >> (r >> 4) & 1) && k0 + r >= start && k0 + r < end)) par = 0;
-                const __half2 step = __low2half2(as_half2(par)), low = __high2half2(as_half2(par));
-                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-                uint8_t* dst = out + r * 128;
+            constexpr int kMine = kTasks / (C::kDequant * 32);
+#pragma unroll 1
+            for (int i0 = 0; i0 < kMine; i0 += 2) {  // two tasks' loads first
+                uint4 w[2];
+                uint32_t par[2];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    __half2 f[4];
-                    codes_to_half(ww[x], f);
+                for (int u = 0; u < 2; ++u) {
+                    const int r = r0 + (i0 + u) * kStep, rr = r & (R - 1);
+                    const uint8_t* src = raw + (r >> shift) * half_chunk;
+                    w[u] = *reinterpret_cast<const uint4*>(src + rr * (D / 2) + q * 16);
+                    par[u] = *reinterpret_cast<const uint32_t*>(src + rr * row_p + par_at);
+                    // rows that nobody sees may hold anything: they count as zeros
+                    if (!whole && !((valid >> (r >> 4) & 1) && k0 + r >= start && k0 + r < end)) par[u] = 0;
+                }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) f[e] = __hfma2(f[e], step, low);
-                    *reinterpret_cast<uint4*>(dst + ((((q & 1) * 4 + x) ^ (r & 7)) << 4)) = *reinterpret_cast<const uint4*>(f);
+                for (int u = 0; u < 2; ++u) {
+                    const __half2 step = __low2half2(as_half2(par[u])), low = __high2half2(as_half2(par[u]));
+                    const uint32_t ww[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
+                    uint8_t* dst = out + (r0 + (i0 + u) * kStep) * 128;
+                    const int x7 = (r0 + (i0 + u) * kStep) & 7;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        __half2 f[4];
+                        codes_to_half(ww[x], f);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f[e] = __hfma2(f[e], step, low);
+                        *reinterpret_cast<uint4*>(dst + ((((q & 1) * 4 + x) ^ x7) << 4)) = *reinterpret_cast<const uint4*>(f);
+                    }
                 }
             }
             fence_proxy_async_shared();
@@ -474,6 +500,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     } else {
         // ------------------------------------------------------------ softmax: a thread a row
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kSoftmaxRegs));
+        load_q();
         const int t = warp >> 2, r = t * 128 + (warp & 3) * 32 + lane, row = row0 + r;
         const bool on = r < rows;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
@@ -608,6 +635,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
             bool nan = ll != ll;
             const long long at = (long long)tok * c.hq + qh;
+            // this row tile's part of Q's memory, which no product reads any more
+            uint8_t* const s_row = s_q + t * (128 * D * 2) + (warp & 3) * (32 * D * 2);
 #pragma unroll
             for (int d = 0; d < D; d += 32) {
                 float v[32];
@@ -646,9 +675,21 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     }
                     const __half2 h[4] = {__floats2half2_rn(f[0], f[1]), __floats2half2_rn(f[2], f[3]),
                                           __floats2half2_rn(f[4], f[5]), __floats2half2_rn(f[6], f[7])};
-                    if (on) *reinterpret_cast<uint4*>(c.out + at * D + d + e) = *reinterpret_cast<const uint4*>(h);
+                    *reinterpret_cast<uint4*>(s_row + lane * (D * 2) + ((((d + e) / 8) ^ (lane & 7)) << 4)) =
+                        *reinterpret_cast<const uint4*>(h);
                 }
             }
+            // the warp's rows to memory, neighbouring lanes along a row
+            __syncwarp();
+#pragma unroll 4
+            for (int i = lane; i < 32 * (D / 8); i += 32) {
+                const int rr = i / (D / 8), ch = i % (D / 8);
+                const long long to = __shfl_sync(0xffffffffu, on ? at : -1, rr);
+                if (to >= 0)
+                    *reinterpret_cast<uint4*>(c.out + to * D + ch * 8) =
+                        *reinterpret_cast<const uint4*>(s_row + rr * (D * 2) + ((ch ^ (rr & 7)) << 4));
+            }
+            __syncwarp();
             if (on && c.lse) c.lse[at] = ll > 0.0f ? (mm + log2f(ll)) * 0.6931471805599453f : -INFINITY;
             // rows whose result is not a number are computed again one by one: a NaN among the values
             // reaches rows that do not see it through weights of zero
