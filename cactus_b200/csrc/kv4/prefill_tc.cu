@@ -13,7 +13,9 @@
 //   mma       one thread: S = Q K^T (operands in shared memory), O += P V (P in TMEM);
 //   softmax   one thread a row: S from TMEM, weights as fp16 back over S, O rescaled in TMEM when the
 //             running maximum has risen by more than 2^8, the result at the end.
-// The two row tiles alternate on the tensor core, so one's products overlap the other's softmax.
+// The two row tiles alternate on the tensor core, so one's products overlap the other's softmax; the
+// one row tile of head_dim 256 has two buffers for S instead, and S of the next keys is computed
+// during the softmax.
 //
 // Layout. K, V and Q tiles are blocks of 64 elements (128 bytes) by rows with the 128-byte swizzle.
 // K and Q are read K-major; V with its rows as the contraction, MN-major, from the same layout. The
@@ -198,7 +200,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     uint8_t* const s_q = smem;                       // [row tile][D / 64][128 rows][128 bytes]
     uint8_t* const s_buf = smem + C::kQBytes;        // ring of K, V tiles [D / 64][KT rows][128 bytes]
     uint8_t* const s_raw = s_buf + C::kBufs * C::kBufBytes;
-    __shared__ uint64_t s_full[MT], p_full[MT][2], o_full[MT], buf_full[C::kBufs], buf_free[C::kBufs], raw_full[C::kRaw],
+    __shared__ uint64_t s_full[2], p_full[2][2], o_full[2], pv_done, buf_full[C::kBufs], buf_free[C::kBufs], raw_full[C::kRaw],
         raw_free[C::kRaw], q_full, drain;
     __shared__ uint32_t s_tmem;
     __shared__ int s_abort, s_item[4], s_scan[kWarps], s_last;
@@ -280,7 +282,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     if (tid == 0) {
-        for (int i = 0; i < MT; ++i) {
+        mbar_init(&pv_done, 1);
+        for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i][0], 128);
             mbar_init(&p_full[i][1], 128);
@@ -307,9 +310,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     const int R = min(ge.page(), KT), half_chunk = R * (D / 2 + 4 * ng), raw_bytes = C::raw_bytes(ng);
 
     auto load_q = [&] {  // by the softmax and dequantisation warps, while the first keys are on their way
-        constexpr int kAll = C::kRows * (D / 8), kStep = kMma * 32, kBatch = 6;
-#pragma unroll 1
-        for (int i0 = tid; i0 < kAll; i0 += kBatch * kStep) {
+        constexpr int kAll = C::kRows * (D / 8), kStep = kMma * 32,
+                      kBatch = (kAll + kStep - 1) / kStep;  // all loads in flight at once
+        const int i0 = tid;
+        {
             uint4 v[kBatch];
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
@@ -384,57 +388,70 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             const uint64_t q_desc = desc(smem_u32(s_q), 16), k_desc = desc(smem_u32(s_buf), 16),
                            v_desc = desc(smem_u32(s_buf), KT * 128);
             bool ok = true;
-            int slot = 0;        // ring slot of half h, the next to be waited for, and its parity
-            unsigned phase = 0;
-            auto need = [&]() -> int {
-                const int s = slot;
-                ok = ok && __all_sync(0xffffffffu, wait_or_abort(&buf_full[s], phase, abort));
+            auto need = [&](int h) -> int {  // waits for half tile h (K of tile h / 2, or its V) and returns its slot
+                const int s = h % C::kBufs;
+                ok = ok && __all_sync(0xffffffffu, wait_or_abort(&buf_full[s], (h / C::kBufs) & 1, abort));
                 tc_fence_after();
-                if (++slot == C::kBufs) {
-                    slot = 0;
-                    phase ^= 1;
-                }
                 return s;
             };
-            auto qk = [&](int t, int s) {
+            auto qk = [&](int t, int buf, int s) {
                 const uint64_t qa = q_desc + (uint64_t)(t * (128 * D * 2 / 16)), kb = k_desc + (uint64_t)(s * (C::kBufBytes / 16));
 #pragma unroll
                 for (int k = 0; k < D / 16; ++k)
-                    mma_ss(leader, tm + t * KT, qa + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16,
+                    mma_ss(leader, tm + buf * KT, qa + ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16,
                            kb + ((k >> 2) * (KT * 128) + (k & 3) * 32) / 16, idesc(KT, false), k > 0);
-                commit(leader, &s_full[t]);
+                commit(leader, &s_full[buf]);
             };
-            int ks = 0, vs = 0;
+            auto pv = [&](int t, int buf, int s, int parity, bool first) {
+                const uint64_t vb = v_desc + (uint64_t)(s * (C::kBufBytes / 16));
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {  // the weights come in two halves
+                    ok = ok && __all_sync(0xffffffffu, wait_or_abort(&p_full[buf][half], parity, abort));
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = half * (KT / 32); k < (half + 1) * (KT / 32); ++k)
+                        mma_ts(leader, tm + C::kO + t * D, tm + buf * KT + k * 8, vb + k * (2048 / 16), idesc(D, true),
+                               !first || k > 0);
+                }
+            };
             if (n_tiles > 0) {
                 ok = __all_sync(0xffffffffu, wait_or_abort(&q_full, 0, abort));
-                ks = need();
-                for (int t = 0; t < MT && ok; ++t) qk(t, ks);
-                if (ok) commit(leader, &buf_free[ks]);
+                const int s = need(0);
+                for (int t = 0; t < MT && ok; ++t) qk(t, t, s);
+                if (ok) commit(leader, &buf_free[s]);
             }
             for (int j = 0; j < n_tiles && ok; ++j) {
-#pragma unroll
-                for (int t = 0; t < MT; ++t) {
-                    if (t == 0) vs = need();
-                    const uint64_t vb = v_desc + (uint64_t)(vs * (C::kBufBytes / 16));
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {  // the weights come in two halves
-                        ok = ok && __all_sync(0xffffffffu, wait_or_abort(&p_full[t][half], j & 1, abort));
+                const bool more = j + 1 < n_tiles;
+                if (MT == 1) {  // S of the next tile into the other buffer, then this tile's values
+                    if (more) {
+                        const int s = need(2 * j + 2);
                         if (!ok) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (int k = half * (KT / 32); k < (half + 1) * (KT / 32); ++k)
-                            mma_ts(leader, tm + C::kO + t * D, tm + t * KT + k * 8, vb + k * (2048 / 16), idesc(D, true),
-                                   j > 0 || k > 0);
+                        qk(0, (j + 1) & 1, s);
+                        commit(leader, &buf_free[s]);
                     }
+                    const int s = need(2 * j + 1);
+                    pv(0, j & 1, s, (j >> 1) & 1, j == 0);
                     if (!ok) break;
-                    if (t == MT - 1) commit(leader, &buf_free[vs]);
-                    if (j + 1 < n_tiles) {
-                        if (t == 0) ks = need();
+                    commit(leader, &buf_free[s]);
+                    commit(leader, &pv_done);
+                    if (!more) commit(leader, &o_full[0]);
+                } else {
+                    int vs = 0, ks = 0;
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        if (t == 0) vs = need(2 * j + 1);
+                        pv(t, t, vs, j & 1, j == 0);
                         if (!ok) break;
-                        qk(t, ks);
-                        if (t == MT - 1) commit(leader, &buf_free[ks]);
-                    } else {
-                        commit(leader, &o_full[t]);
+                        if (t == MT - 1) commit(leader, &buf_free[vs]);
+                        if (more) {
+                            if (t == 0) ks = need(2 * j + 2);
+                            if (!ok) break;
+                            qk(t, t, ks);
+                            if (t == MT - 1) commit(leader, &buf_free[ks]);
+                        } else {
+                            commit(leader, &o_full[t]);
+                        }
                     }
                 }
             }
@@ -504,7 +521,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         const int t = warp >> 2, r = t * 128 + (warp & 3) * 32 + lane, row = row0 + r;
         const bool on = r < rows;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + t * KT, o_at = tmem + lanes + C::kO + t * D;
+        const uint32_t o_at = tmem + lanes + C::kO + t * D;
         const int tok = tok0 + (on ? row / share : 0), qh = head * share + row % share;
         const int pos = pos0 + (on ? row / share : 0);
         // the row sees keys [lo, hi); rows past the last one see all, and nobody reads them
@@ -514,7 +531,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         float m = 0.0f, limit = -INFINITY, l = 0.0f;  // as in the kernel for few queries
         bool ok = true;
         for (int j = 0; j < tiles; ++j) {
-            if (!(ok = wait_or_abort(&s_full[t], j & 1, abort))) break;
+            // its S buffer: its row tile's, or with one row tile the two in turn
+            const int buf = MT == 1 ? j & 1 : t;
+            const uint32_t s_at = tmem + lanes + buf * KT;
+            if (!(ok = wait_or_abort(&s_full[buf], (MT == 1 ? j >> 1 : j) & 1, abort))) break;
             tc_fence_after();
             const int k0 = key0 + j * KT;
             const unsigned valid = s_valid[j & 7];
@@ -552,7 +572,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     limit = top + kLazy;
                     l *= fix;
                 }
-                if (j > 0) {
+                if (j > 0) {  // with a row tile's own buffer its S was computed after the products before
+                    if (MT == 1) ok = wait_or_abort(&pv_done, (j - 1) & 1, abort);
+                    tc_fence_after();
 #pragma unroll 1
                     for (int d = 0; d < D; d += 16) {
                         uint32_t v[16];
@@ -568,7 +590,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             auto hand_over = [&](int half) {
                 tmem_wait_st();
                 tc_fence_before();
-                mbar_arrive(&p_full[t][half]);
+                mbar_arrive(&p_full[buf][half]);
             };
 #pragma unroll
             for (int i = 0; i < KT / 32; ++i) {
@@ -633,7 +655,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 }
             }
             const float inv = ll > 0.0f ? 1.0f / ll : 0.0f;
-            bool nan = ll != ll;
+            const float2 inv2 = make_float2(inv, inv), zero2 = {};
+            float2 test = {};
             const long long at = (long long)tok * c.hq + qh;
             // this row tile's part of Q's memory, which no product reads any more
             uint8_t* const s_row = s_q + t * (128 * D * 2) + (warp & 3) * (32 * D * 2);
@@ -667,14 +690,14 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {  // column e + i is dim e + {0, 4, 1, 5, 2, 6, 3, 7}[i]
-                    float f[8];
+                    float2 f[4];  // dims k and k + 4
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        f[(i >> 1) + (i & 1) * 4] = v[e + i] * inv;
-                        nan |= v[e + i] != v[e + i];
+                    for (int k = 0; k < 4; ++k) {
+                        f[k] = fma2(make_float2(v[e + 2 * k], v[e + 2 * k + 1]), inv2, zero2);
+                        test = fma2(f[k], zero2, test);  // not a number from here on if this is none
                     }
-                    const __half2 h[4] = {__floats2half2_rn(f[0], f[1]), __floats2half2_rn(f[2], f[3]),
-                                          __floats2half2_rn(f[4], f[5]), __floats2half2_rn(f[6], f[7])};
+                    const __half2 h[4] = {__floats2half2_rn(f[0].x, f[1].x), __floats2half2_rn(f[2].x, f[3].x),
+                                          __floats2half2_rn(f[0].y, f[1].y), __floats2half2_rn(f[2].y, f[3].y)};
                     *reinterpret_cast<uint4*>(s_row + lane * (D * 2) + ((((d + e) / 8) ^ (lane & 7)) << 4)) =
                         *reinterpret_cast<const uint4*>(h);
                 }
@@ -693,7 +716,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             if (on && c.lse) c.lse[at] = ll > 0.0f ? (mm + log2f(ll)) * 0.6931471805599453f : -INFINITY;
             // rows whose result is not a number are computed again one by one: a NaN among the values
             // reaches rows that do not see it through weights of zero
-            unsigned again = __ballot_sync(0xffffffffu, on && nan && !*abort);
+            unsigned again = __ballot_sync(0xffffffffu, on && !(ll == ll && test.x + test.y == 0.0f) && !*abort);
             while (again) {
                 const int x = __ffs(again) - 1;
                 again &= again - 1;
