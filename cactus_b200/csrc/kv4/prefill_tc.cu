@@ -617,15 +617,15 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         constexpr int kSlot = C::kRows * (D + 2);  // floats: [D / 4][row][4], then m and l of the rows
         if (!last) {
             float* part = a.parts + (size_t)(slot0 + split) * kSlot;
-            if (ok && tiles > 0) {
+            if (__any_sync(0xffffffffu, on)) {
 #pragma unroll
                 for (int d = 0; d < D; d += 32) {
                     float v[32];
                     tmem_ld32(o_at + d, v);
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4)
+                    for (int i = 0; i < 32; i += 4)  // a part that saw nothing has zeros
                         *reinterpret_cast<float4*>(part + ((size_t)((d + i) / 4) * C::kRows + r) * 4) =
-                            make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                            tiles > 0 ? make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 }
             }
             part[(size_t)C::kRows * D + r] = m_out;
@@ -673,18 +673,20 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 } else {
 #pragma unroll
                     for (int i = 0; i < 32; ++i) v[i] = 0.0f;
-                    for (int x = 0; x < splits; ++x) {
-                        const float* p = a.parts + (size_t)(slot0 + x) * kSlot;
-                        const float pm = __ldcg(p + (size_t)C::kRows * D + r), pl = __ldcg(p + (size_t)C::kRows * D + C::kRows + r);
-                        const float f = pm == -INFINITY ? (pl != pl ? 1.0f : 0.0f) : ex2(pm - mm);
-                        if (f == 0.0f) continue;  // a part that saw nothing has no values
+                    if (on) {
+#pragma unroll 4
+                        for (int x = 0; x < splits; ++x) {  // the parts' loads overlap
+                            const float* p = a.parts + (size_t)(slot0 + x) * kSlot;
+                            const float pm = __ldcg(p + (size_t)C::kRows * D + r), pl = __ldcg(p + (size_t)C::kRows * D + C::kRows + r);
+                            const float f = pm == -INFINITY ? (pl != pl ? 1.0f : 0.0f) : ex2(pm - mm);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
-                            const float4 u = __ldcg(reinterpret_cast<const float4*>(p + ((size_t)((d + i) / 4) * C::kRows + r) * 4));
-                            v[i] = fmaf(u.x, f, v[i]);
-                            v[i + 1] = fmaf(u.y, f, v[i + 1]);
-                            v[i + 2] = fmaf(u.z, f, v[i + 2]);
-                            v[i + 3] = fmaf(u.w, f, v[i + 3]);
+                            for (int i = 0; i < 32; i += 4) {
+                                const float4 u = __ldcg(reinterpret_cast<const float4*>(p + ((size_t)((d + i) / 4) * C::kRows + r) * 4));
+                                v[i] = fmaf(u.x, f, v[i]);
+                                v[i + 1] = fmaf(u.y, f, v[i + 1]);
+                                v[i + 2] = fmaf(u.z, f, v[i + 2]);
+                                v[i + 3] = fmaf(u.w, f, v[i + 3]);
+                            }
                         }
                     }
                 }
