@@ -13,9 +13,9 @@ namespace cb {
 namespace kv4 {
 
 struct Geom {
-    int page_shift, hkv, d, g;
+    int page_shift, hkv, d, g, groups;  // groups: of a row
     __host__ __device__ int page() const { return 1 << page_shift; }
-    __host__ __device__ int ng() const { return d / g; }
+    __host__ __device__ int ng() const { return groups; }
     __host__ __device__ int code_bytes() const { return d / 2; }      // of one row
     __host__ __device__ int param_bytes() const { return 4 * ng(); }  // of one row
     // byte offsets inside a block

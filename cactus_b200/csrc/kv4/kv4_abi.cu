@@ -27,7 +27,7 @@ const char* make_geom(size_t page_size, size_t hkv, size_t d, size_t g, Geom* ge
     if (hkv == 0 || hkv > 1024) return "num_kv_heads must be 1 to 1024";
     if (d != 64 && d != 128 && d != 256) return "head_dim must be 64, 128 or 256";
     if ((g != 32 && g != 64 && g != 128) || d % g) return "group_size must be 32, 64 or 128 and divide head_dim";
-    *ge = Geom{shift, (int)hkv, (int)d, (int)g};
+    *ge = Geom{shift, (int)hkv, (int)d, (int)g, (int)(d / g)};
     return nullptr;
 }
 

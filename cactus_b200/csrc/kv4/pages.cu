@@ -26,7 +26,7 @@ __device__ __forceinline__ __half step_of(float range) {
 }
 
 // The codes of 8 elements x - low of a group as a word: each quotient rounded half to even, at most 15.
-// The product with the reciprocal is within 5e-6 of a quotient below 16 (2^-23 for the reciprocal, 2^-24
+// The product with the reciprocal is within 4e-6 of a quotient below 16 (2^-23 for the reciprocal, 2^-24
 // for the product), so where every product is further than that from a half its rounding is the
 // quotient's; else (rare) the 8 are divided, as they are where the step is so small (a few of fp16's
 // smallest units) that a quotient can pass 15.5. Adding 1.5 * 2^23 rounds to an integer and leaves it
@@ -42,7 +42,7 @@ __device__ __forceinline__ uint32_t quant_codes(const float (&x)[8], float step)
         far = fmaxf(far, fabsf(fmaf(x[j], inv, -__fsub_rn(t, magic))));
         w += __float_as_uint(t) << (4 * j);  // 0x4B400000 + code: the sum of the constants is taken off below
     }
-    if (far > 0.49999f || step < 0x1p-18f) {
+    if (far > 0.499992f || step < 0x1p-18f) {
         w = 0;
 #pragma unroll
         for (int j = 0; j < 8; ++j) w += __float_as_uint(__fadd_rn(fminf(__fdiv_rn(x[j], step), 15.0f), magic)) << (4 * j);
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(kAppendThreads)
     __shared__ int s_row[kAppendTokens];
     constexpr int kLanes = D / 8, kRows = kAppendThreads / kLanes;
     const int t0 = blockIdx.x * kAppendTokens, head = blockIdx.y;
-    const int lane = threadIdx.x % kLanes, per_group = ge.g / 8;
+    const int lane = threadIdx.x % kLanes, per_group = ge.g >> 3, group = lane >> (__ffs(per_group) - 1);
     const unsigned full = 0xffffffffu;
     constexpr int kPasses = kAppendTokens / kRows;
     static_assert(kAppendTokens % kRows == 0, "whole passes");
@@ -115,9 +115,9 @@ __global__ void __launch_bounds__(kAppendThreads)
             uint8_t* block = pg.pool + s_page[r] + (long long)head * ge.block_bytes() + ((i & 1) ? ge.v_codes() : 0);
             const int row = s_row[r];
             *reinterpret_cast<uint32_t*>(block + row * (D / 2) + lane * 4) = w;
-            if (lane % per_group == 0) {
+            if ((lane & (per_group - 1)) == 0) {
                 const __half nan = __ushort_as_half(0x7FFF);
-                *reinterpret_cast<__half2*>(block + ge.k_params() + (row * ge.ng() + lane / per_group) * 4) =
+                *reinterpret_cast<__half2*>(block + ge.k_params() + (row * ge.ng() + group) * 4) =
                     bad ? __halves2half2(nan, nan) : __halves2half2(step, __float2half_rn(lo));
             }
         }
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kAppendThreads)
         s_row[threadIdx.x] = row;
     }
     __syncthreads();
-    const int lane = threadIdx.x % kLanes, group = lane * 8 / ge.g;
+    const int lane = threadIdx.x % kLanes, group = lane * 8 >> (__ffs(ge.g) - 1);
     constexpr int kPasses = kAppendTokens / kRows;
     uint32_t w[2 * kPasses];
     __half2 par[2 * kPasses];
