@@ -239,6 +239,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
         const int tok0 = c.offsets[wk.b], rows = min(ROWS, s.tokens * share - row0);
         const int qhead0 = head * share;
 
+        // ---- q, in flight beside the page ids: column g of n-tile j is row row0 + 8 j + g (paired: row0 + g % 4)
+        constexpr int kQ = (NT * (D / 32) + kWarps - 1) / kWarps;
+        uint4 qv[kQ];
+#pragma unroll
+        for (int u = 0; u < kQ; ++u) {
+            const int i = warp + u * kWarps, j = i / (D / 32), x = i % (D / 32);
+            const int col = kPaired ? g & 3 : 8 * j + g, r = row0 + col;
+            qv[u] = uint4{0, 0, 0, 0};
+            if (i < NT * (D / 32) && col < rows)
+                qv[u] = __ldg(reinterpret_cast<const uint4*>(c.q + (long long)(tok0 + r / share) * c.q_stride +
+                                                             (long long)(qhead0 + r % share) * D + t * (D / 4)) + x);
+        }
+
         // ---- the ring: stage i of this warp is the keys first + i * kTile .. + 16 KB - 1
         const int first = s.base + tile0 * kTile + warp * 16 * KB, stop = min(s.end, first + ntile * kTile);
         const int* const table = pg.table + (long long)wk.b * pg.table_stride;
@@ -297,15 +310,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
 #pragma unroll
         for (int i = 0; i < kStages - 1; ++i) advance(i, i);
 
-        // ---- q fragments: column g of n-tile j is row row0 + 8 j + g (paired: row0 + g % 4)
-        for (int i = warp; i < NT * (D / 32); i += kWarps) {
-            const int j = i / (D / 32), x = i % (D / 32), col = kPaired ? g & 3 : 8 * j + g, r = row0 + col;
-            uint4 v = {0, 0, 0, 0};
-            if (col < rows)
-                v = __ldg(reinterpret_cast<const uint4*>(c.q + (long long)(tok0 + r / share) * c.q_stride +
-                                                         (long long)(qhead0 + r % share) * D + t * (D / 4)) + x);
-            sm.q[j][x][lane] = uint4{__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632),
-                                     __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632)};
+        // q fragments for all warps
+#pragma unroll
+        for (int u = 0; u < kQ; ++u) {
+            const int i = warp + u * kWarps;
+            if (i < NT * (D / 32))
+                sm.q[i / (D / 32)][i % (D / 32)][lane] =
+                    uint4{__byte_perm(qv[u].x, qv[u].z, 0x5410), __byte_perm(qv[u].x, qv[u].z, 0x7632),
+                          __byte_perm(qv[u].y, qv[u].w, 0x5410), __byte_perm(qv[u].y, qv[u].w, 0x7632)};
         }
         __syncthreads();
         // keys that every row of the tile sees
