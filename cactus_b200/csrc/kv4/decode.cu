@@ -78,10 +78,12 @@ struct Seq {
 template <int ROWS, int TILE>
 __device__ __forceinline__ Seq seq_of(const AttnCall& c, const Pages& pg, const Geom& ge, int max_rows, int b, bool report) {
     Seq s;
-    const int count = c.offsets[b + 1] - c.offsets[b], len = max(c.lens[b], 0);
+    const int from = c.offsets[b], to = c.offsets[b + 1], len = max(c.lens[b], 0);
+    const bool good = from >= 0 && from <= to && to <= c.num_tokens;  // else the sequence is left out
+    const int count = good ? to - from : 0;
     const int room = (int)(pg.table_stride << ge.page_shift);
     s.tokens = max(0, min(count, c.max_q));
-    if (report && (count > c.max_q || (len > room && count > 0))) report_dev_error(kDevBadPage);
+    if (report && (!good || count > c.max_q || (len > room && count > 0))) report_dev_error(kDevBadPage);
     const int rows = s.tokens * (c.hq / ge.hkv);
     s.row_tiles = rows > max_rows ? 0 : (rows + ROWS - 1) / ROWS;
     s.pos0 = len - count;
@@ -120,7 +122,7 @@ struct Smem {
 template <int D, int ROWS>
 __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
     kv4_decode_kernel(const __grid_constant__ AttnCall c, const __grid_constant__ Pages pg, const __grid_constant__ Geom ge,
-                      int max_rows) {
+                      int max_rows, int max_items) {
     pdl_launch_dependents();
     pdl_wait();
     constexpr int kCols = columns<ROWS>(), NT = kCols / 8, KB = blocks<D, ROWS>(), kTile = 16 * KB * kWarps, kStages = stages<D, ROWS>(), kPad = D + 4;
@@ -153,9 +155,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
     }
     if (tid == 0) sm.nan = 0;
     __syncthreads();
-    int total = 0;
+    int total = 0, all_items = 0;
 #pragma unroll
     for (int x = 0; x < kWarps; ++x) {
+        all_items += sm.scan_items[x];
         if (x < warp) {
             upto += sm.scan[x];
             items_upto += sm.scan_items[x];
@@ -165,6 +168,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
     // CTA x of n has the tiles first_tile(x) .. first_tile(x + 1) - 1: as many as the others, or one more
     const int n = min((int)gridDim.x, total);
     if ((int)blockIdx.x >= n) return;
+    if (all_items > max_items) {  // token rows named by several sequences: there are not so many counters
+        if (tid == 0) report_dev_error(kDevBadPage);
+        return;
+    }
     const int each = total / n, more = total - each * n;
     auto first_tile = [&](int x) { return x * each + min(x, more); };
     auto owner = [&](int tile) {
@@ -677,7 +684,8 @@ int launch(const AttnCall& c, const Pages& pg, const Geom& ge, int max_rows, cud
     const double bound = (double)c.num_seqs * ge.hkv * ((rows_most + ROWS - 1) / ROWS) * tiles;
     if (bound > 2147483647.0) return -2;  // tiles are counted in 31 bits
     const unsigned grid = (unsigned)(bound < kNumSMs * kPerSm ? bound : kNumSMs * kPerSm);
-    return launch_k(kernel, dim3(grid), dim3(kThreads), (size_t)smem, st, c, pg, ge, max_rows) == cudaSuccess ? 0 : -1;
+    return launch_k(kernel, dim3(grid), dim3(kThreads), (size_t)smem, st, c, pg, ge, max_rows,
+                    (int)std::min<size_t>(decode_counters(c.num_seqs, c.num_tokens, c.hq, ge.hkv), 0x7fffffff)) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace

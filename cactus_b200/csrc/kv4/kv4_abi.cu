@@ -133,6 +133,8 @@ CB_API int cactus_cuda_kv4_attention(const uint16_t* queries, size_t query_strid
         return arg(name, why);
     if (!queries || !token_offsets || !context_lens || !output || !workspace) return arg(name, "null argument");
     if (num_seqs > kIntMax - 1 || num_tokens > kIntMax - 64) return arg(name, "size too large");
+    if ((max_query_len < num_tokens ? max_query_len : num_tokens) * (num_q_heads / num_kv_heads) > kIntMax / 2)
+        return arg(name, "too many query rows for one kv head");
     if (query_stride % 8 || !aligned(queries, 16) || !aligned(output, 16) || !aligned(workspace, 16))
         return arg(name, "queries, query_stride, output and workspace must be 16-byte aligned");
     if (query_stride < num_q_heads * head_dim || query_stride > ((size_t)1 << 40)) return arg(name, "bad query_stride");

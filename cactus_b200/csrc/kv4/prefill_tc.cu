@@ -216,7 +216,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     // which sees the most
     const int per = (c.num_seqs + kThreads - 1) / kThreads;
     auto row_tiles = [&](int b) {
-        const int rows = max(0, min(c.offsets[b + 1] - c.offsets[b], c.max_q)) * share;
+        const int from = c.offsets[b], to = c.offsets[b + 1];
+        if (from < 0 || from > to || to > c.num_tokens) {  // the sequence is left out
+            atomicCAS(a.err, 0u, (unsigned)kDevBadPage);
+            return 0;
+        }
+        const int rows = min(to - from, c.max_q) * share;
         return rows < a.min_rows ? 0 : (rows + C::kRows - 1) / C::kRows;
     };
     int mine = 0;

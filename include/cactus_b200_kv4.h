@@ -6,9 +6,11 @@
  * Conventions are those of cactus_b200.h: DEVICE pointers unless a comment says host, fp16 as
  * uint16_t bits, asynchronous calls on `stream`, 0 or a negative code with a message in
  * cactus_cuda_last_error(). The kernel entry points allocate nothing and can be captured in a
- * CUDA graph. Lengths, offsets, tables and row lists are read on the device; what they name
- * outside the pool (a page id that is not in [0, num_pages), a position past the end of a table
- * row) is skipped and raises the device error word (cactus_cuda_device_error() == 3).
+ * CUDA graph (after a first call of the same kind outside of it, which sets kernel attributes).
+ * Lengths, offsets, tables and row lists are read on the device; what they name outside the
+ * arguments (a page id that is not in [0, num_pages), a position past the end of a table row,
+ * token rows past num_tokens) is skipped and raises the device error word
+ * (cactus_cuda_device_error() == 3).
  *
  * Format. A pool holds pages of page_size rows (16, 32, 64, 128 or 256); page p's bytes for one
  * layer start at pool + p * page_stride and are, for each kv head,

@@ -68,7 +68,8 @@ REFUSED = (
     + [(_attention, k) for k in (dict(q=None), dict(out=None), dict(ws=None), dict(off=None), dict(lens=None),
                                  dict(table=None), dict(hq=0), dict(hq=12), dict(qs=2040), dict(qs=2052), dict(q=A + 8),
                                  dict(out=A + 8), dict(lse=A + 2), dict(ws=A + 4), dict(wsb=0), dict(scale=0.0),
-                                 dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(t=1 << 31))]
+                                 dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(t=1 << 31),
+                                 dict(t=1 << 30, mq=1 << 30, hq=64, qs=8192))]
     + [(_copy, k) for k in (dict(pool=None), dict(src=None), dict(dst=None), dict(np=0), dict(pool=A + 4), dict(pb=1000),
                             dict(ps=1016), dict(pb=2048), dict(pls=100), dict(planes=1 << 17), dict(n=1 << 32))]
     + [(_compact, k) for k in (dict(src=None), dict(dst=None), dict(kept=None), dict(off=None), dict(pls=8),

@@ -621,3 +621,34 @@ def test_example_runs(capsys):
     assert example.main(["--prompt", "300", "--samples", "4", "--steps", "20"]) < 0.25
     assert "samples" in capsys.readouterr().out
     assert _err() == 0
+
+
+@pytest.mark.parametrize("count", [2, 80])
+@pytest.mark.parametrize("wrong", ["past", "falling", "negative", "again"])
+def test_attention_leaves_out_token_rows_that_are_not_there(count, wrong):
+    """Offsets past num_tokens, falling, negative, or naming rows twice: reported, and nothing else is written."""
+    t = torch()
+    L, ge = cb.lib(), U.Geom(16, 1, 64, 32)
+    rng = np.random.default_rng(21)
+    lens = [100, 100, 100]
+    pool, table = _filled(ge, lens, rng)
+    n = 3 * count
+    q = rng.standard_normal((n, 2, 64)).astype(np.float16)
+    off = {"past": [0, count, 2 * count, n + 1], "falling": [0, count, 0, n], "negative": [-1, count, 2 * count, n],
+           "again": [0, n, 0, n]}[wrong]
+    d = [dev(a) for a in (q, np.array(off, np.int32), np.array(lens, np.int32), table, pool.bytes)]
+    out = t.full((n + 64, 2, 64), 7.0, dtype=t.float16, device="cuda")
+    ws = empty((L.cactus_cuda_kv4_attention_workspace(3, n, 2, 1, 64),), np.uint8)
+    for _ in range(2):
+        cb.check(L.cactus_cuda_kv4_attention(ptr(d[0]), 128, ptr(d[1]), ptr(d[2]), ptr(d[3]), table.shape[1], ptr(d[4]),
+                                             pool.pages, pool.stride, out.data_ptr(), None, 3, n, n, 2, *ge.args(), 0.125,
+                                             0, 1, ptr(ws), ws.numel(), None))
+        assert _err() == 3
+    assert bool((out[n:] == 7.0).all())
+    got = out.cpu().numpy()
+    if wrong in ("past", "negative"):  # the sequences whose rows are there
+        b = 0 if wrong == "past" else 1
+        at = slice(b * count, (b + 1) * count)
+        k, v = (pool.rows(w, table[b], 100) for w in (0, 1))
+        ref, _, tol, _ = U.attention(q[at], k, v, 0.125, True, 0)
+        assert np.all(np.abs(got[at].astype(np.float64) - ref) <= tol)
