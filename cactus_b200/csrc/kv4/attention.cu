@@ -7,7 +7,9 @@ namespace kv4 {
 
 namespace {
 // Sequences with up to so many q rows a kv head (tokens times the heads that share it) go to the
-// kernel for few queries, the others to the one for many.
+// kernel for few queries, which reads the keys once for 16 rows, the others to the one for many, which
+// does for 256. Over 8000 rows, 16 / 8 heads of 128: 32 q rows of 12 sequences 123 us there and 139
+// here, 48 rows 172 and 140; one sequence alone 32 rows 32 and 47, 64 rows 40 and 43.
 constexpr int kFewRows = 32;
 }  // namespace
 

@@ -1,8 +1,13 @@
-// Attention over the 4-bit paged KV cache for few queries a sequence (decode, drafted tokens):
-// bound by the cache's bytes.
+// Attention over the 4-bit paged KV cache for few queries a sequence (decode, drafted tokens). Its
+// floor is the cache's bytes, read once; what bounds it is the instructions that turn codes into
+// operands: of about 380 a warp for 16 keys of 128, 208 unpack and scale 1024 elements (13 for 8), and
+// groups of 128 (0.53 bytes an element) take as long as groups of 32 (0.63). On B200: 64 sequences of
+// 16 to 32 thousand rows, 8 kv heads of 128, 520 us, 3.9 TB/s of the cache (floor 313 us); 256 short
+// conversations in pages of 16, heads of 64, 76 us (floor 14 us: the starts and ends of 2048 items
+// and the 16-key overheads at half the elements weigh most there).
 //
 // Work. A sequence's q rows of one kv head (its tokens times the heads that share it, in tiles of
-// 4, 8 or 16 rows) over its visible keys is an item; items are cut into tiles of 64 keys, and the
+// 4, 8 or 16 rows) over its visible keys is an item; items are cut into tiles of 64 or 128 keys, and the
 // tiles of all items, in one list, are dealt in equal contiguous ranges to as many CTAs as the GPU
 // holds at once, whatever the sequences' lengths. Every CTA finds its range itself from the lengths
 // in device memory. An item inside one range is finished there; the parts of one that spans several
@@ -42,6 +47,7 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr float kLazy = 8.0f;  // base-2 exponent
+
 // row of the 16 that key i of the fragments is
 __device__ __forceinline__ int kappa(int i) { return (i & 8) + (((i & 7) >> 1) ^ ((i & 1) * 5)); }
 
@@ -100,8 +106,11 @@ __device__ __forceinline__ Seq seq_of(const AttnCall& c, const Pages& pg, const 
 // columns 4-7 of one to the low parts of the weights.
 template <int ROWS>
 constexpr int columns() { return ROWS < 8 ? 8 : ROWS; }
-// Blocks of 16 keys that a warp takes at a time, CTAs a multiprocessor holds (by registers: 168 a
-// thread, 128 for four), stages of a ring (what shared memory then holds)
+// Blocks of 16 keys that a warp takes at a time: two where the registers hold them (64 sequences of 4
+// to 8 thousand rows at head_dim 128: 137 us with two, 152 with one; 256 short conversations at 64: 79
+// and 73, 64 of 8000 rows: 100 and 114), one at 16 rows of 128, where both take 62 us. CTAs a
+// multiprocessor holds: by the registers, 168 a thread (three) or 128 (four, at 64); four at 128 take
+// 137 us too. Stages of a ring: what shared memory then holds.
 template <int D, int ROWS>
 constexpr int blocks() { return D == 64 || (D == 128 && ROWS <= 8) ? 2 : 1; }
 template <int D, int ROWS>
