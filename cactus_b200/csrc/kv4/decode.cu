@@ -28,7 +28,8 @@
 // so that one mask gives the same dim of both. Key i of the fragment is row kappa(i) of the 16,
 // which spreads the lanes' shared-memory reads over the banks. The weights go into O as two fp16
 // numbers, p = hi + lo (22 bits), which makes the result as good as with fp32 weights; up to 4 rows
-// have lo in the columns that they leave empty.
+// have lo in the columns that they leave empty, and 16 rows leave it out (as the kernel for many
+// queries does: the weights' rounding is then as large as the result's own).
 //
 // Softmax. The running maximum is raised only when a score exceeds it by more than 2^kLazy; until
 // then weights grow past 1 (at most 2^kLazy, far inside fp16), which is exact up to rounding and
@@ -136,6 +137,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
     pdl_wait();
     constexpr int kCols = columns<ROWS>(), NT = kCols / 8, KB = blocks<D, ROWS>(), kTile = 16 * KB * kWarps, kStages = stages<D, ROWS>(), kPad = D + 4;
     constexpr bool kPaired = ROWS < 8;  // columns 4-7 repeat 0-3 and take the weights' low parts
+    constexpr bool kTwice = ROWS == 8;  // the low parts have products of their own
+    constexpr int kNoKeys = 0x7fffff00; // past every position
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ Smem<D, ROWS> sm;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
             bool whole = true;
 #pragma unroll
             for (int k = 0; k < KB; ++k) {
-                k0[k] = got >> k & 1 ? first + i * kTile + k * 16 : 0x40000000;
+                k0[k] = got >> k & 1 ? first + i * kTile + k * 16 : kNoKeys;
                 whole &= k0[k] >= all_from && k0[k] + 16 <= all_to;
             }
             // ---- S^T
@@ -467,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
                     }
                 }
             }
-            uint32_t hi[KB][NT][2], lo[KB][NT][2];
+            uint32_t hi[KB][NT][2], lo[KB][NT][2] = {};
 #pragma unroll
             for (int k = 0; k < KB; ++k)
 #pragma unroll
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
                         const float2 f = __half22float2(h);
                         const __half2 rest = __floats2half2_rn(p[2 * e] - f.x, p[2 * e + 1] - f.y);
                         hi[k][j][e] = movmatrix_t(h2u(kPaired && t >= 2 ? rest : h));
-                        if (!kPaired) lo[k][j][e] = movmatrix_t(h2u(rest));
+                        if (kTwice) lo[k][j][e] = movmatrix_t(h2u(rest));
                     }
                 }
             // ---- O^T
@@ -528,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
                     for (int j = 0; j < NT; ++j) {
                         mma16816(o[j][4 * x + 2 * y], f0, hi[k][j][0], hi[k][j][1]);
                         mma16816(o[j][4 * x + 2 * y + 1], f1, hi[k][j][0], hi[k][j][1]);
-                        if (kPaired) continue;
+                        if (!kTwice) continue;
                         mma16816(o[j][4 * x + 2 * y], f0, lo[k][j][0], lo[k][j][1]);
                         mma16816(o[j][4 * x + 2 * y + 1], f1, lo[k][j][0], lo[k][j][1]);
                     }

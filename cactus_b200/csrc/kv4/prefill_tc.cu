@@ -13,8 +13,8 @@
 //   mma       one thread: S = Q K^T (operands in shared memory), O += P V (P in TMEM);
 //   softmax   one thread a row: S from TMEM, weights as fp16 back over S, O rescaled in TMEM when the
 //             running maximum has risen by more than 2^8, the result at the end.
-// The two row tiles alternate on the tensor core, so one's products overlap the other's softmax; the
-// one row tile of head_dim 256 has two buffers for S instead, and S of the next keys is computed
+// The two row tiles alternate on the tensor core, so one's products overlap the other's softmax; where
+// there is one (always at head_dim 256) it has both buffers for S, and S of the next keys is computed
 // during the softmax.
 //
 // Layout. K, V and Q tiles are blocks of 64 elements (128 bytes) by rows with the 128-byte swizzle.
@@ -287,6 +287,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
     const int base = start & ~(KT - 1), all = (end - base + KT - 1) / KT;
     const int t_from = (int)((long long)all * split / splits), t_to = (int)((long long)all * (split + 1) / splits);
     const int tiles = t_to - t_from, key0 = base + t_from * KT;
+    const bool one = MT == 1 || rows <= 128;  // one row tile: it has both S buffers
 
     // ---- set-up: barriers, TMEM
     if (warp == kMma) {
@@ -396,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         {
             const uint32_t leader = elect_one();
             const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-            const int n_tiles = __shfl_sync(0xffffffffu, tiles, 0);
+            const int n_tiles = __shfl_sync(0xffffffffu, tiles, 0), alone = __shfl_sync(0xffffffffu, (int)one, 0);
             // descriptors differ from these by constants: a product must take less time to issue than to run
             const uint64_t q_desc = desc(smem_u32(s_q), 16), k_desc = desc(smem_u32(s_buf), 16),
                            v_desc = desc(smem_u32(s_buf), KT * 128);
@@ -431,12 +432,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             if (n_tiles > 0) {
                 ok = __all_sync(0xffffffffu, wait_or_abort(&q_full, 0, abort));
                 const int s = need(0);
-                for (int t = 0; t < MT && ok; ++t) qk(t, t, s);
+                for (int t = 0; t < (alone ? 1 : MT) && ok; ++t) qk(t, t, s);
                 if (ok) commit(leader, &buf_free[s]);
             }
             for (int j = 0; j < n_tiles && ok; ++j) {
                 const bool more = j + 1 < n_tiles;
-                if (MT == 1) {  // S of the next tile into the other buffer, then this tile's values
+                if (alone) {  // S of the next tile into the other buffer, then this tile's values
                     if (more) {
                         const int s = need(2 * j + 2);
                         if (!ok) break;
@@ -543,11 +544,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
         const float sc = c.scale * 1.4426950408889634f;
         float m = 0.0f, limit = -INFINITY, l = 0.0f;  // as in the kernel for few queries
         bool ok = true;
-        for (int j = 0; j < tiles; ++j) {
-            // its S buffer: its row tile's, or with one row tile the two in turn
-            const int buf = MT == 1 ? j & 1 : t;
+        const int my_tiles = t == 0 || !one ? tiles : 0;
+        for (int j = 0; j < my_tiles; ++j) {
+            // its S buffer: its row tile's, or where there is one row tile the two in turn
+            const int buf = one ? j & 1 : t;
             const uint32_t s_at = tmem + lanes + buf * KT;
-            if (!(ok = wait_or_abort(&s_full[buf], (MT == 1 ? j >> 1 : j) & 1, abort))) break;
+            if (!(ok = wait_or_abort(&s_full[buf], (one ? j >> 1 : j) & 1, abort))) break;
             tc_fence_after();
             const int k0 = key0 + j * KT;
             const unsigned valid = s_valid[j & 7];
@@ -586,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     l *= fix;
                 }
                 if (j > 0) {  // with a row tile's own buffer its S was computed after the products before
-                    if (MT == 1) ok = wait_or_abort(&pv_done, (j - 1) & 1, abort);
+                    if (one) ok = wait_or_abort(&pv_done, (j - 1) & 1, abort);
                     tc_fence_after();
 #pragma unroll 1
                     for (int d = 0; d < D; d += 16) {
@@ -621,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             }
             l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
         }
-        if (tiles > 0 && ok) ok = wait_or_abort(&o_full[t], 0, abort);
+        if (my_tiles > 0 && ok) ok = wait_or_abort(&o_full[t], 0, abort);
         tc_fence_after();
         // ---- the result, or this part of it
         const float m_out = limit == -INFINITY ? -INFINITY : m;
