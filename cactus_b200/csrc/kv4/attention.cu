@@ -7,10 +7,17 @@ namespace kv4 {
 
 namespace {
 // Sequences with up to so many q rows a kv head (tokens times the heads that share it) go to the
-// kernel for few queries, which reads the keys once for 16 rows, the others to the one for many, which
-// does for 256. Over 8000 rows, 16 / 8 heads of 128: 32 q rows of 12 sequences 123 us there and 139
-// here, 48 rows 172 and 140; one sequence alone 32 rows 32 and 47, 64 rows 40 and 43.
-constexpr int kFewRows = 32;
+// kernel for few queries, which unpacks the keys once for 16 rows (8 at head_dim 256), the others to the
+// one for many, which does once for 256 (128). Measured over 8000 rows, times in us of the one for few
+// and the one for many. 12 sequences, heads of 128, 8 kv heads: 32 rows 106 and 106, 48 rows 147 and
+// 106 (one sequence 32 rows 31 and 40, 64 rows 41 and 40). Heads of 64, 8 kv heads: 32 rows 67 and 93, 48
+// rows 91 and 93. Heads of 256, 4 kv heads: 32 rows 148 and 88; but where there are few sequences and kv
+// heads, which the one for many does not split so far: 1 kv head 24 rows 44 and 61, 32 rows 52 and 51.
+int few_rows(const AttnCall& c, const Geom& ge) {
+    if (ge.d == 64) return 48;
+    if (ge.d == 128) return 32;
+    return (long long)c.num_seqs * ge.hkv >= 32 ? 16 : 32;
+}
 }  // namespace
 
 size_t attention_workspace(int num_seqs, int num_tokens, int hq, int hkv, int) {
@@ -19,13 +26,14 @@ size_t attention_workspace(int num_seqs, int num_tokens, int hq, int hkv, int) {
 }
 
 int launch_attention(const AttnCall& c, const Pages& pg, const Geom& ge, cudaStream_t st) {
-    if ((long long)c.max_q * (c.hq / ge.hkv) <= kFewRows) return launch_decode(c, pg, ge, kFewRows, st);
+    const int few = few_rows(c, ge);
+    if ((long long)c.max_q * (c.hq / ge.hkv) <= few) return launch_decode(c, pg, ge, few, st);
     // sequences of both kinds may be there unless all are as long as the longest
     if ((long long)c.num_seqs * c.max_q > c.num_tokens) {
-        const int rc = launch_decode(c, pg, ge, kFewRows, st);
+        const int rc = launch_decode(c, pg, ge, few, st);
         if (rc) return rc;
     }
-    return launch_prefill(c, pg, ge, kFewRows + 1, st);
+    return launch_prefill(c, pg, ge, few + 1, st);
 }
 
 }  // namespace kv4

@@ -1,5 +1,6 @@
 // The 4-bit paged KV cache as a handle: a pool for all layers, the sequences' pages (page_map.h) and
 // the current batch's metadata in device memory. The device work is the kernel entry points'.
+#include <algorithm>
 #include <cstring>
 #include <memory>
 #include <new>
@@ -77,10 +78,10 @@ struct Cache {
     uint8_t* pool = nullptr;  // [layer][page][page_bytes]
     uint8_t* ws = nullptr;
     size_t ws_bytes = 0;
-    int* meta = nullptr;      // the batch: offsets [max_seqs + 1] | lengths [max_seqs] | table [max_seqs][max_pages]
+    int* meta = nullptr;      // the batch: offsets [max_seqs + 1] | lengths [max_seqs] | table [sequences][batch_pages]
     int* lists = nullptr;     // copies, or a compaction's tables and rows
     size_t list_ints = 0;
-    size_t batch = 0, batch_tokens = 0, batch_longest = 0;
+    size_t batch = 0, batch_tokens = 0, batch_longest = 0, batch_pages = 0;  // pages: of the longest, the table's width
 
     ~Cache() {
         int prev = -1;
@@ -197,18 +198,21 @@ CB_API int cactus_kv4_begin(cactus_kv4_t cache, const int32_t* seqs, const int32
                                                      copies.size(), stream);
             if (rc) return rc;
         }
-        std::vector<int> v(2 * c.max_seqs + 1 + num_seqs * c.max_pages, 0);
+        size_t width = 1;
+        for (int id : ids) width = std::max(width, c.map->pages(id).size());
+        std::vector<int> v(2 * c.max_seqs + 1 + num_seqs * width, -1);
+        v[0] = 0;
         for (size_t i = 0; i < num_seqs; ++i) {
             v[i + 1] = v[i] + counts[i];
             v[c.max_seqs + 1 + i] = c.map->length(ids[i]);
-            int* row = v.data() + 2 * c.max_seqs + 1 + i * c.max_pages;
             const std::vector<int>& pages = c.map->pages(ids[i]);
-            for (size_t k = 0; k < c.max_pages; ++k) row[k] = k < pages.size() ? pages[k] : -1;
+            std::copy(pages.begin(), pages.end(), v.begin() + 2 * c.max_seqs + 1 + i * width);
         }
         c.staging.send(v, c.meta, st);
         c.batch = num_seqs;
         c.batch_tokens = total;
         c.batch_longest = longest;
+        c.batch_pages = width;
         return (int)CB_OK;
     });
 }
@@ -217,7 +221,7 @@ CB_API int cactus_kv4_append(cactus_kv4_t cache, size_t layer, const uint16_t* k
                              size_t row_stride, void* stream) {
     return guarded(cache, "kv4_append", [&](Cache& c) {
         require(layer < c.layers && c.batch, "no such layer, or no batch begun");
-        return cactus_cuda_kv4_append(keys, values, row_stride, c.offsets(), c.lens(), c.table(), c.max_pages,
+        return cactus_cuda_kv4_append(keys, values, row_stride, c.offsets(), c.lens(), c.table(), c.batch_pages,
                                       c.layer_pool(layer), c.num_pages, c.page_bytes, c.batch, c.batch_tokens, c.page,
                                       c.hkv, c.d, c.g, stream);
     });
@@ -228,7 +232,7 @@ CB_API int cactus_kv4_attention(cactus_kv4_t cache, size_t layer, const uint16_t
                                 void* stream) {
     return guarded(cache, "kv4_attention", [&](Cache& c) {
         require(layer < c.layers && c.batch, "no such layer, or no batch begun");
-        return cactus_cuda_kv4_attention(queries, query_stride, c.offsets(), c.lens(), c.table(), c.max_pages,
+        return cactus_cuda_kv4_attention(queries, query_stride, c.offsets(), c.lens(), c.table(), c.batch_pages,
                                          c.layer_pool(layer), c.num_pages, c.page_bytes, output, lse, c.batch,
                                          c.batch_tokens, c.batch_longest, c.hq, c.page, c.hkv, c.d, c.g, scale,
                                          window_size, is_causal, c.ws, c.ws_bytes, stream);
