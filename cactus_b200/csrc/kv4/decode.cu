@@ -2,8 +2,8 @@
 // floor is the cache's bytes, read once; what bounds it is the instructions that turn codes into
 // operands: of about 380 a warp for 16 keys of 128, 208 unpack and scale 1024 elements (13 for 8), and
 // groups of 128 (0.53 bytes an element) take as long as groups of 32 (0.63). On B200: 64 sequences of
-// 16 to 32 thousand rows, 8 kv heads of 128, 520 us, 3.9 TB/s of the cache (floor 313 us); 256 short
-// conversations in pages of 16, heads of 64, 76 us (floor 14 us: the starts and ends of 2048 items
+// 16 to 32 thousand rows, 8 kv heads of 128, 516 us, 3.9 TB/s of the cache (floor 313 us); 256 short
+// conversations in pages of 16, heads of 64, 78 us (floor 14 us: the starts and ends of 2048 items
 // and the 16-key overheads at half the elements weigh most there).
 //
 // Work. A sequence's q rows of one kv head (its tokens times the heads that share it, in tiles of
@@ -109,7 +109,8 @@ template <int ROWS>
 constexpr int columns() { return ROWS < 8 ? 8 : ROWS; }
 // Blocks of 16 keys that a warp takes at a time: two where the registers hold them (64 sequences of 4
 // to 8 thousand rows at head_dim 128: 137 us with two, 152 with one; 256 short conversations at 64: 79
-// and 73, 64 of 8000 rows: 100 and 114), one at 16 rows of 128, where both take 62 us. CTAs a
+// and 73, 64 of 8000 rows: 100 and 114), one at 16 rows of 128 (12 sequences of 5 tokens over 8000 rows: 63 us with one, 62 with two,
+// before the weights' low parts were left out there, 58 now). CTAs a
 // multiprocessor holds: by the registers, 168 a thread (three) or 128 (four, at 64); four at 128 take
 // 137 us too. Stages of a ring: what shared memory then holds.
 template <int D, int ROWS>

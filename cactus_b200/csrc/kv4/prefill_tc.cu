@@ -27,7 +27,7 @@
 // those of S at the shared-memory bandwidth), the exponentials of two row tiles 2048, the unpacking
 // of K and V 2700 on its four warps beside them; a row's chain from S to the next S takes 3500 to
 // 4000, of which the other row tile hides about half. On B200: 2048 queries after up to 6144 rows,
-// 4 sequences, 16 / 8 heads of 128: 491 us, 898 TFLOP/s (448 us back to back on one input; floor
+// 4 sequences, 16 / 8 heads of 128: 493 us, 895 TFLOP/s (450 us back to back on one input; floor
 // 266 us at the measured peak). 256 queries with a window of 512, 4 heads of 256 on one, 16 sequences:
 // 28.7 us, of which the start takes 6, the results 4 and 9 key tiles the rest.
 //
