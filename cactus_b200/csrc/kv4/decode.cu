@@ -708,9 +708,11 @@ size_t decode_counters(int num_seqs, int num_tokens, int hq, int hkv) {
     return ((size_t)num_tokens * (size_t)(hq / hkv) / 8 + (size_t)num_seqs) * (size_t)hkv;
 }
 
-int launch_decode(const AttnCall& c, const Pages& pg, const Geom& ge, int max_rows, cudaStream_t st) {
-    const long long most = (long long)c.max_q * (c.hq / ge.hkv);
-    const int rows = (int)(most < max_rows ? most : max_rows);
+int launch_decode(const AttnCall& c, const Pages& pg, const Geom& ge, int max_rows, int usual_rows, cudaStream_t st) {
+    // every kernel takes any number of rows, in tiles; the counters allow for tiles of 8 and more, and of 4
+    // where no sequence has more rows
+    const long long most = std::min<long long>((long long)c.max_q * (c.hq / ge.hkv), max_rows);
+    const int rows = most <= 4 ? (int)most : (int)std::min<long long>(most, std::max(usual_rows, 8));
     switch (ge.d) {
         case 64:
             return rows <= 4   ? launch<64, 4>(c, pg, ge, max_rows, st)

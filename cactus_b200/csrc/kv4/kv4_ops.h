@@ -41,9 +41,10 @@ constexpr int kPrefillParts = 148;                                        // of 
 constexpr size_t kPartBytes = (size_t)kPrefillParts * 256 * (128 + 2) * 4;
 static_assert(kPartBytes >= (size_t)kDecodeCtas * 2 * kDecodePartFloats * 4, "workspace");
 
-// decode.cu: sequences with at most max_rows q rows (tokens times the heads that share a kv head)
+// decode.cu: sequences with at most max_rows q rows (tokens times the heads that share a kv head), of
+// which most have at most usual_rows
 size_t decode_counters(int num_seqs, int num_tokens, int hq, int hkv);
-int launch_decode(const AttnCall& c, const Pages& pg, const Geom& ge, int max_rows, cudaStream_t st);
+int launch_decode(const AttnCall& c, const Pages& pg, const Geom& ge, int max_rows, int usual_rows, cudaStream_t st);
 // prefill_tc.cu: sequences with at least min_rows q rows
 int launch_prefill(const AttnCall& c, const Pages& pg, const Geom& ge, int min_rows, cudaStream_t st);
 // attention.cu

@@ -238,6 +238,30 @@ def test_attention(counts, lens, geom, hq, causal, window, extra):
     assert _err() == 0
 
 
+MIXED = [
+    # counts, (page, hkv, d, g), hq, window: a prompt's chunk among sequences of a token, and one or two of some
+    ([1] * 20 + [130] + [1] * 9, (32, 2, 128, 32), 4, 0),
+    ([1] * 30 + [16, 100] + [1] * 30 + [12], (16, 1, 128, 64), 2, 0),
+    ([1] * 40 + [90, 24], (16, 2, 64, 32), 4, 33),
+    ([1] * 24 + [48] + [1] * 8 + [7, 0], (16, 2, 256, 64), 4, 0),
+    ([17, 16, 15, 40, 16], (32, 1, 128, 32), 2, 0),
+]
+
+
+@pytest.mark.parametrize("counts,geom,hq,window", MIXED)
+def test_attention_of_a_chunk_among_single_tokens(counts, geom, hq, window):
+    ge = U.Geom(*geom)
+    rng = np.random.default_rng(sum(counts) + hq)
+    lens = [int(c + rng.integers(0, 400)) for c in counts]
+    pool, table = _filled(ge, lens, rng)
+    q = rng.standard_normal((sum(counts), hq, ge.d)).astype(np.float16)
+    out, lse, ws = _attend(pool, table, q, counts, lens, hq, True, window)
+    _check(pool, table, q, counts, lens, hq, True, window, out, lse)
+    again, _, _ = _attend(pool, table, q, counts, lens, hq, True, window, ws=ws)
+    assert np.array_equal(again.view(np.uint16), out.view(np.uint16))
+    assert _err() == 0
+
+
 @pytest.mark.parametrize("count", [1, 4, 90])
 def test_attention_with_scores_far_apart(count):
     """Scores of hundreds: one key's weight is 1 and the others vanish; the maximum comes late, early or between."""
