@@ -28,8 +28,7 @@
 // so that one mask gives the same dim of both. Key i of the fragment is row kappa(i) of the 16,
 // which spreads the lanes' shared-memory reads over the banks. The weights go into O as two fp16
 // numbers, p = hi + lo (22 bits), which makes the result as good as with fp32 weights; up to 4 rows
-// have lo in the columns that they leave empty, and 16 rows leave it out (as the kernel for many
-// queries does: the weights' rounding is then as large as the result's own).
+// have lo in the columns that they leave empty.
 //
 // Softmax. The running maximum is raised only when a score exceeds it by more than 2^kLazy; until
 // then weights grow past 1 (at most 2^kLazy, far inside fp16), which is exact up to rounding and
@@ -109,8 +108,7 @@ template <int ROWS>
 constexpr int columns() { return ROWS < 8 ? 8 : ROWS; }
 // Blocks of 16 keys that a warp takes at a time: two where the registers hold them (64 sequences of 4
 // to 8 thousand rows at head_dim 128: 137 us with two, 152 with one; 256 short conversations at 64: 79
-// and 73, 64 of 8000 rows: 100 and 114), one at 16 rows of 128 (12 sequences of 5 tokens over 8000 rows: 63 us with one, 62 with two,
-// before the weights' low parts were left out there, 58 now). CTAs a
+// and 73, 64 of 8000 rows: 100 and 114), one at 16 rows of 128 (12 sequences of 5 tokens over 8000 rows: 63 us with one, 62 with two). CTAs a
 // multiprocessor holds: by the registers, 168 a thread (three) or 128 (four, at 64); four at 128 take
 // 137 us too. Stages of a ring: what shared memory then holds.
 template <int D, int ROWS>
@@ -138,7 +136,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
     pdl_wait();
     constexpr int kCols = columns<ROWS>(), NT = kCols / 8, KB = blocks<D, ROWS>(), kTile = 16 * KB * kWarps, kStages = stages<D, ROWS>(), kPad = D + 4;
     constexpr bool kPaired = ROWS < 8;  // columns 4-7 repeat 0-3 and take the weights' low parts
-    constexpr bool kTwice = ROWS == 8;  // the low parts have products of their own
     constexpr int kNoKeys = 0x7fffff00; // past every position
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ Smem<D, ROWS> sm;
@@ -471,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
                     }
                 }
             }
-            uint32_t hi[KB][NT][2], lo[KB][NT][2] = {};
+            uint32_t hi[KB][NT][2], lo[KB][NT][2];
 #pragma unroll
             for (int k = 0; k < KB; ++k)
 #pragma unroll
@@ -487,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
                         const float2 f = __half22float2(h);
                         const __half2 rest = __floats2half2_rn(p[2 * e] - f.x, p[2 * e + 1] - f.y);
                         hi[k][j][e] = movmatrix_t(h2u(kPaired && t >= 2 ? rest : h));
-                        if (kTwice) lo[k][j][e] = movmatrix_t(h2u(rest));
+                        if (!kPaired) lo[k][j][e] = movmatrix_t(h2u(rest));
                     }
                 }
             // ---- O^T
@@ -532,7 +529,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
                     for (int j = 0; j < NT; ++j) {
                         mma16816(o[j][4 * x + 2 * y], f0, hi[k][j][0], hi[k][j][1]);
                         mma16816(o[j][4 * x + 2 * y + 1], f1, hi[k][j][0], hi[k][j][1]);
-                        if (!kTwice) continue;
+                        if (kPaired) continue;
                         mma16816(o[j][4 * x + 2 * y], f0, lo[k][j][0], lo[k][j][1]);
                         mma16816(o[j][4 * x + 2 * y + 1], f1, lo[k][j][0], lo[k][j][1]);
                     }
