@@ -11,7 +11,7 @@
 //   producer  raw codes and parameters of K and V half tiles into a ring (1-D bulk copies);
 //   dequant   codes -> fp16 values in the swizzled operand layout, once for all 256 rows;
 //   mma       one thread: S = Q K^T (operands in shared memory), O += P V (P in TMEM);
-//   softmax   one thread a row: S from TMEM, weights as fp16 back over S, O rescaled in TMEM when the
+//   softmax   one thread a row: S from TMEM, weights as two fp16 parts back over S, O rescaled in TMEM when the
 //             running maximum has risen by more than 2^8, the result at the end.
 // The two row tiles alternate on the tensor core, so one's products overlap the other's softmax; where
 // there is one (always at head_dim 256) it has both buffers for S, and S of the next keys is computed
@@ -21,15 +21,17 @@
 // K and Q are read K-major; V with its rows as the contraction, MN-major, from the same layout. The
 // 8 elements of a 16-byte piece stand in the order 0 4 1 5 2 6 3 7 that the unpacking gives: Q is
 // permuted alike when it is loaded, and O when it is stored.
-// Weights are rounded to fp16 for the tensor core: 2^-11 of each, as much as the result's own rounding.
+// Weights go to the tensor core as two fp16 numbers, p = hi + lo (22 bits), in the columns of the S that
+// they come from: hi in its first half, lo in the other, each with a product of its own.
 //
-// What bounds it: per key tile of 128 and 256 rows the products take 1900 cycles (32 of 128 x 128 x 16,
-// those of S at the shared-memory bandwidth), the exponentials of two row tiles 2048, the unpacking
-// of K and V 2700 on its four warps beside them; a row's chain from S to the next S takes 3500 to
-// 4000, of which the other row tile hides about half. On B200: 2048 queries after up to 6144 rows,
-// 4 sequences, 16 / 8 heads of 128: 493 us, 895 TFLOP/s (450 us back to back on one input; floor
-// 266 us at the measured peak). 256 queries with a window of 512, 4 heads of 256 on one, 16 sequences:
-// 28.7 us, of which the start takes 6, the results 4 and 9 key tiles the rest.
+// What bounds it: a row's chain from S to the next S, of which the other row tile hides about half; it
+// has all of the weights' work (the exponentials of two row tiles take 2048 cycles a key tile of 128)
+// and both of their products. The unpacking of K and V takes 2700 cycles on its four warps beside
+// them. On B200: 2048 queries after up to 6144 rows, 4 sequences, 16 / 8 heads of 128: 605 us, 730
+// TFLOP/s of the 4 D operations a pair of query and key (with weights of one fp16 number 493 us, but
+// then their rounding is as large as the result's; floor 266 us at the measured peak). 256 queries with
+// a window of 512, 4 heads of 256 on one, 16 sequences: 31 us, of which the start takes 6, the results 4
+// and 9 key tiles the rest.
 //
 // This file is compiled as whole-program device code (build.py WHOLE_PROGRAM).
 #include <atomic>
@@ -158,6 +160,12 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
           "l"(reinterpret_cast<unsigned long long&>(c)));
     return d;
 }
+// w - h in one instruction; with h converted to fp32 first the prompts above take 682 us
+__device__ __forceinline__ float rest_of(__half h, float w) {
+    float d;
+    asm("fma.rn.f32.f16 %0, %1, %2, %3;" : "=f"(d) : "h"(__half_as_ushort(h)), "h"((unsigned short)0xBC00), "f"(w));
+    return d;
+}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 d;
     asm("add.rn.f32x2 %0, %1, %2;"
@@ -181,6 +189,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
@@ -424,9 +437,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
-                    for (int k = half * (KT / 32); k < (half + 1) * (KT / 32); ++k)
-                        mma_ts(leader, tm + C::kO + t * D, tm + buf * KT + k * 8, vb + k * (2048 / 16), idesc(D, true),
-                               !first || k > 0);
+                    for (int k = half * (KT / 32); k < (half + 1) * (KT / 32); ++k) {
+                        const uint32_t p = tm + buf * KT + k * 8;  // high parts, low parts
+                        mma_ts(leader, tm + C::kO + t * D, p, vb + k * (2048 / 16), idesc(D, true), !first || k > 0);
+                        mma_ts(leader, tm + C::kO + t * D, p + KT / 2, vb + k * (2048 / 16), idesc(D, true), 1);
+                    }
                 }
             };
             if (n_tiles > 0) {
@@ -608,18 +623,22 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                 mbar_arrive(&p_full[buf][half]);
             };
 #pragma unroll
-            for (int i = 0; i < KT / 32; ++i) {
-                uint32_t p[16];
+            for (int i = 0; i < KT / 16; ++i) {
+                uint32_t p[8], rest[8];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    float2 w = fma2(make_float2(x[i][2 * e], x[i][2 * e + 1]), scale2, shift2);
+                for (int e = 0; e < 8; ++e) {
+                    const float* const s2 = &x[i / 2][(i & 1) * 16 + 2 * e];
+                    float2 w = fma2(make_float2(s2[0], s2[1]), scale2, shift2);
                     w = make_float2(ex2(w.x), ex2(w.y));
                     sums[e & 1] = add2(sums[e & 1], w);
                     const __half2 h = __floats2half2_rn(w.x, w.y);
+                    const __half2 lo = __floats2half2_rn(rest_of(__low2half(h), w.x), rest_of(__high2half(h), w.y));
                     p[e] = *reinterpret_cast<const uint32_t*>(&h);
+                    rest[e] = *reinterpret_cast<const uint32_t*>(&lo);
                 }
-                tmem_st16(s_at + i * 16, p);  // over S, which this thread has read
-                if ((i + 1) % (KT / 64) == 0) hand_over(i / (KT / 64));
+                tmem_st8(s_at + i * 8, p);  // over S, which this thread has read
+                tmem_st8(s_at + KT / 2 + i * 8, rest);
+                if ((i + 1) % (KT / 32) == 0) hand_over(i / (KT / 32));
             }
             l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
         }

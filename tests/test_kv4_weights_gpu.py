@@ -12,8 +12,10 @@ from tests.test_kv4_gpu import _attend, _err
 
 pytestmark = pytest.mark.gpu
 
-# tokens (2 heads share a kv head), head_dim: tiles of 4, 8 and 16 rows
-FORMS = [(1, 64), (2, 128), (1, 256), (4, 64), (4, 128), (4, 256), (7, 64), (8, 128), (13, 128), (24, 64), (16, 256)]
+# tokens (2 heads share a kv head), head_dim: tiles of 4, 8 and 16 rows, and the kernel for many queries with
+# one row tile and two
+FORMS = [(1, 64), (2, 128), (1, 256), (4, 64), (4, 128), (4, 256), (7, 64), (8, 128), (13, 128), (24, 64), (16, 256),
+         (40, 64), (40, 128), (40, 256), (150, 64), (150, 128), (150, 256)]
 
 
 def _pool(ge, k, v, rng):
