@@ -643,6 +643,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             l += (sums[0].x + sums[0].y) + (sums[1].x + sums[1].y);
         }
         if (my_tiles > 0 && ok) ok = wait_or_abort(&o_full[t], 0, abort);
+        // the result goes through Q's memory, which every warp has to be done filling: without key tiles no
+        // product has waited for that
+        if (ok) ok = wait_or_abort(&q_full, 0, abort);
         tc_fence_after();
         // ---- the result, or this part of it
         const float m_out = limit == -INFINITY ? -INFINITY : m;
