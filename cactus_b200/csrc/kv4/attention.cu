@@ -28,16 +28,17 @@ size_t attention_workspace(int num_seqs, int num_tokens, int hq, int hkv, int) {
 int launch_attention(const AttnCall& c, const Pages& pg, const Geom& ge, cudaStream_t st) {
     const int few = few_rows(c, ge);
     if ((long long)c.max_q * (c.hq / ge.hkv) <= few) return launch_decode(c, pg, ge, few, few, st);
-    // sequences of both kinds may be there unless all are as long as the longest; a prompt's chunk among
-    // single tokens is the usual case, so the others' mean says how large a tile of rows they need. 256
-    // tokens among 63 single ones over 4096 rows, 2 heads of 128 to each of 8 kv heads: 146 us, 178 with the
-    // tile of 16 rows; among 127 over 1024 rows, 4 heads of 64 to each: 72 and 85
-    if ((long long)c.num_seqs * c.max_q > c.num_tokens) {
-        const long long others = (long long)(c.num_tokens - c.max_q) * (c.hq / ge.hkv);
-        const int rc = launch_decode(c, pg, ge, few, c.num_seqs > 1 && others <= 8LL * (c.num_seqs - 1) ? 8 : few, st);
-        if (rc) return rc;
-    }
-    return launch_prefill(c, pg, ge, few + 1, st);
+    // The counts are on the device, and there may be fewer tokens than the call has room for. Where all
+    // sequences may be as long as the longest, the kernel for many takes every one, also those that turn out
+    // short, and a batch of equal prompts needs no launch that finds nothing to do.
+    if ((long long)c.num_seqs * c.max_q <= c.num_tokens) return launch_prefill(c, pg, ge, 1, st);
+    // sequences of both kinds may be there; a prompt's chunk among single tokens is the usual case, so the
+    // others' mean says how large a tile of rows they need. 256 tokens among 63 single ones over 4096 rows, 2
+    // heads of 128 to each of 8 kv heads: 146 us, 178 with the tile of 16 rows; among 127 over 1024 rows, 4
+    // heads of 64 to each: 72 and 85
+    const long long others = (long long)(c.num_tokens - c.max_q) * (c.hq / ge.hkv);
+    const int rc = launch_decode(c, pg, ge, few, c.num_seqs > 1 && others <= 8LL * (c.num_seqs - 1) ? 8 : few, st);
+    return rc ? rc : launch_prefill(c, pg, ge, few + 1, st);
 }
 
 }  // namespace kv4

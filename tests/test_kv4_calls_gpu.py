@@ -83,3 +83,64 @@ def test_parts_of_the_keys_that_are_empty(d):
         call.run()
         assert np.array_equal(call.got()[0].view(np.uint16), first.view(np.uint16))
     assert _err() == 0
+
+
+PADDED = [
+    # counts, rows of the call, max_query_len, lens, (page, hkv, d, g), hq, window
+    ([10], 256, 256, [300], (16, 2, 64, 32), 4, 0),
+    ([5], 256, 256, [5], (32, 1, 128, 32), 2, 0),
+    ([100, 1], 200, 100, [900, 77], (16, 2, 128, 64), 4, 0),
+    ([256, 1], 512, 256, [256, 1000], (16, 1, 64, 64), 2, 0),
+    ([1, 90, 3], 300, 100, [400, 90, 12], (32, 1, 256, 32), 4, 50),
+    ([1, 0, 2], 384, 128, [33, 0, 2], (16, 2, 128, 128), 2, 0),
+    # room for fewer than all at their longest: both kernels
+    ([100, 1], 150, 100, [100, 500], (16, 1, 128, 32), 2, 0),
+    ([1, 3, 40], 64, 64, [9, 300, 41], (16, 1, 64, 32), 4, 0),
+    # few queries, padded
+    ([1, 2], 16, 4, [200, 2], (16, 2, 64, 32), 4, 0),
+]
+
+
+@pytest.mark.parametrize("counts,rows,max_q,lens,geom,hq,window", PADDED)
+def test_padded_token_rows(counts, rows, max_q, lens, geom, hq, window):
+    """Fewer tokens than the call has rows: every sequence is answered, and the rows past the last are left alone."""
+    ge = U.Geom(*geom)
+    rng = np.random.default_rng(rows + sum(lens))
+    pool, table = _filled(ge, lens, rng)
+    q = rng.standard_normal((rows, hq, ge.d)).astype(np.float16)
+    call = Call(pool, table, q, counts, lens, hq, max_q=max_q, window=window)
+    call.clear()
+    call.run()
+    n = sum(counts)
+    out, lse = call.got()
+    _check(pool, table, q[:n], counts, lens, hq, True, window, out[:n], lse[:n])
+    assert (out[n:] == 123.0).all() and (lse[n:] == 123.0).all()
+    assert _err() == 0
+
+
+@pytest.mark.parametrize("rows,max_q", [(160, 80), (120, 80), (80, 80)])
+def test_captured_call_follows_offsets_on_the_device(rows, max_q):
+    """A captured call whose sequences cross, from replay to replay, from many queries to few and back."""
+    t = torch()
+    ge, hq = U.Geom(32, 2, 128, 32), 4
+    rng = np.random.default_rng(rows)
+    lens = [400, 150]
+    pool, table = _filled(ge, lens, rng)
+    q = rng.standard_normal((rows, hq, ge.d)).astype(np.float16)
+    call = Call(pool, table, q, [rows // 2, rows // 2], lens, hq, max_q=max_q)
+    call.run()  # sets the kernels' attributes
+    t.cuda.synchronize()
+    graph = t.cuda.CUDAGraph()
+    with t.cuda.graph(graph):
+        call.run(t.cuda.current_stream().cuda_stream)
+    for counts, now in (([rows // 2, rows // 2], lens), ([1, 1], [399, 64]), ([rows // 2, 1], [120, 150]), ([2, 60 % rows], [17, 100]),
+                        ([0, 5], [0, 5]), ([min(max_q, rows - 1), 1], lens)):
+        call.clear()
+        call.off.copy_(dev(_offsets(counts)))
+        call.lens.copy_(dev(np.array(now, np.int32)))
+        graph.replay()
+        out, lse = call.got()
+        n = sum(counts)
+        _check(pool, table, q[:n], counts, now, hq, True, 0, out[:n], lse[:n])
+        assert (out[n:] == 123.0).all() and (lse[n:] == 123.0).all()
+    assert _err() == 0
