@@ -30,9 +30,10 @@
 // numbers, p = hi + lo (22 bits), which makes the result as good as with fp32 weights; up to 4 rows
 // have lo in the columns that they leave empty.
 //
-// Softmax. The running maximum is raised only when a score exceeds it by more than 2^kLazy; until
-// then weights grow past 1 (at most 2^kLazy, far inside fp16), which is exact up to rounding and
-// saves the reduction over the lanes for almost every tile.
+// Softmax. Weights are relative to 2^-kHead of the running maximum, which is raised only when a score
+// exceeds it by more than 2^kLazy: until then they grow past 2^kHead (at most 2^15, inside fp16), which
+// is exact up to rounding and saves the reduction over the lanes for almost every tile. At the other end
+// fp16's last bit is 2^-24: small weights keep what is above 2^-31 of the largest.
 #include <algorithm>
 #include <atomic>
 
@@ -46,7 +47,7 @@ namespace kv4 {
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr float kLazy = 8.0f;  // base-2 exponent
+constexpr float kLazy = 8.0f, kHead = 7.0f;  // base-2 exponents
 
 // row of the 16 that key i of the fragments is
 __device__ __forceinline__ int kappa(int i) { return (i & 8) + (((i & 7) >> 1) ^ ((i & 1) * 5)); }
@@ -453,11 +454,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
                         if (KB > 1) top = fmaxf(top, fmaxf(acc[KB - 1][j][e], acc[KB - 1][j][e + 2]));
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        top -= kHead;
                         if (limit[j][e] != -INFINITY) top = fmaxf(top, base[j][e]);
                         if (top != -INFINITY) {
                             const float fix = limit[j][e] == -INFINITY ? 0.0f : ex2(base[j][e] - top);
                             base[j][e] = top;
-                            limit[j][e] = top + kLazy;
+                            limit[j][e] = __fadd_rd(top, kHead + kLazy);
                             l[j][e] *= fix;
 #pragma unroll
                             for (int x = 0; x < D / 16; ++x) {
@@ -654,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm<D, ROWS>())
                 const long long at = (long long)tok * c.hq + h;
                 if (mine_r == r) *reinterpret_cast<uint4*>(c.out + at * D + d8 * 8) = *reinterpret_cast<const uint4*>(out);
                 if (mine_r == r && d8 == 0 && c.lse)
-                    c.lse[at] = ll[p] > 0.0f ? (mm[p] + log2f(ll[p])) * 0.6931471805599453f : -INFINITY;
+                    c.lse[at] = ll[p] > 0.0f ? (mm[p] + kHead + log2f(ll[p] * exp2f(-kHead))) * 0.6931471805599453f : -INFINITY;
                 if (nan) atomicOr(&sm.nan, 1 << r);
             }
         }

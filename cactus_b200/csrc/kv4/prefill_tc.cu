@@ -12,7 +12,7 @@
 //   dequant   codes -> fp16 values in the swizzled operand layout, once for all 256 rows;
 //   mma       one thread: S = Q K^T (operands in shared memory), O += P V (P in TMEM);
 //   softmax   one thread a row: S from TMEM, weights as two fp16 parts back over S, O rescaled in TMEM when the
-//             running maximum has risen by more than 2^8, the result at the end.
+//             running maximum has risen by more than 2^kLazy, the result at the end.
 // The two row tiles alternate on the tensor core, so one's products overlap the other's softmax; where
 // there is one (always at head_dim 256) it has both buffers for S, and S of the next keys is computed
 // during the softmax.
@@ -22,7 +22,8 @@
 // 8 elements of a 16-byte piece stand in the order 0 4 1 5 2 6 3 7 that the unpacking gives: Q is
 // permuted alike when it is loaded, and O when it is stored.
 // Weights go to the tensor core as two fp16 numbers, p = hi + lo (22 bits), in the columns of the S that
-// they come from: hi in its first half, lo in the other, each with a product of its own.
+// they come from: hi in its first half, lo in the other, each with a product of its own. They are
+// relative to 2^-kHead of the running maximum, as in the kernel for few queries.
 //
 // What bounds it: a row's chain from S to the next S, of which the other row tile hides about half; it
 // has all of the weights' work (the exponentials of two row tiles take 2048 cycles a key tile of 128)
@@ -46,7 +47,7 @@ namespace kv4 {
 namespace {
 
 constexpr int kWarps = 16, kThreads = kWarps * 32, kMma = 12, kProducer = 13;  // warps 14 and 15 have no work
-constexpr float kLazy = 8.0f;
+constexpr float kLazy = 8.0f, kHead = 7.0f;  // base-2 exponents
 
 template <int D>
 struct Cfg {
@@ -597,9 +598,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
             if (__any_sync(0xffffffffu, top > limit)) {
                 float fix = 1.0f;
                 if (top > limit) {
-                    fix = limit == -INFINITY ? 0.0f : ex2(m - top);
-                    m = top;
-                    limit = top + kLazy;
+                    const float now = top - kHead;
+                    fix = limit == -INFINITY ? 0.0f : ex2(m - now);
+                    m = now;
+                    limit = __fadd_rd(now, kHead + kLazy);
                     l *= fix;
                 }
                 if (j > 0) {  // with a row tile's own buffer its S was computed after the products before
@@ -752,7 +754,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv4_prefill_kernel(const __grid_c
                         *reinterpret_cast<const uint4*>(s_row + rr * (D * 2) + ((ch ^ (rr & 7)) << 4));
             }
             __syncwarp();
-            if (on && c.lse) c.lse[at] = ll > 0.0f ? (mm + log2f(ll)) * 0.6931471805599453f : -INFINITY;
+            if (on && c.lse) c.lse[at] = ll > 0.0f ? (mm + kHead + log2f(ll * exp2f(-kHead))) * 0.6931471805599453f : -INFINITY;
             // rows whose result is not a number are computed again one by one: a NaN among the values
             // reaches rows that do not see it through weights of zero
             unsigned again = __ballot_sync(0xffffffffu, on && !(ll == ll && test.x + test.y == 0.0f) && !*abort);
