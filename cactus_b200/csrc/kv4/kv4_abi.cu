@@ -48,6 +48,12 @@ const char* make_pages(const void* pool, size_t num_pages, size_t page_stride, c
 
 int arg(const char* name, const char* why) { return abi_fail(CB_ERR_ARG, std::string(name) + ": " + why); }
 
+// what a launcher's result means: a failure without an error of the runtime is one all the same
+int launched(const char* name, int rc) {
+    if (const int e = abi_check_launch(name)) return e;
+    return rc ? abi_fail(CB_ERR_LAUNCH, std::string(name) + ": launch failed") : CB_OK;
+}
+
 // the planes of a pool of pages: [plane][page], or each page with all its planes
 const char* planes_check(size_t num_planes, size_t plane_stride) {
     if (num_planes > 65535) return "num_planes must be at most 65535";
@@ -83,9 +89,8 @@ CB_API int cactus_cuda_kv4_append(const uint16_t* keys, const uint16_t* values, 
     if (row_stride % 8 || !aligned(keys, 16) || !aligned(values, 16))
         return arg(name, "keys, values and row_stride must be 16-byte aligned");
     if (row_stride < num_kv_heads * head_dim || row_stride > ((size_t)1 << 40)) return arg(name, "bad row_stride");
-    cb::kv4::launch_append(H(keys), H(values), (long long)row_stride, token_offsets, context_lens, pg, (int)num_seqs,
-                           (int)num_tokens, ge, S(stream));
-    return abi_check_launch(name);
+    return launched(name, cb::kv4::launch_append(H(keys), H(values), (long long)row_stride, token_offsets, context_lens,
+                                                 pg, (int)num_seqs, (int)num_tokens, ge, S(stream)));
 }
 
 CB_API int cactus_cuda_kv4_read(const void* pool, size_t num_pages, size_t page_stride, const int32_t* block_table,
@@ -102,8 +107,8 @@ CB_API int cactus_cuda_kv4_read(const void* pool, size_t num_pages, size_t page_
     if (!row_offsets || (!keys && !values)) return arg(name, "null argument");
     if (num_seqs > kIntMax - 1 || num_rows > kIntMax - 64) return arg(name, "size too large");
     if (!aligned(keys, 16) || !aligned(values, 16)) return arg(name, "keys and values must be 16-byte aligned");
-    cb::kv4::launch_read(pg, row_offsets, first_rows, H(keys), H(values), (int)num_seqs, (int)num_rows, ge, S(stream));
-    return abi_check_launch(name);
+    return launched(name, cb::kv4::launch_read(pg, row_offsets, first_rows, H(keys), H(values), (int)num_seqs,
+                                               (int)num_rows, ge, S(stream)));
 }
 
 CB_API size_t cactus_cuda_kv4_attention_workspace(size_t num_seqs, size_t num_tokens, size_t num_q_heads,
@@ -158,9 +163,9 @@ CB_API int cactus_cuda_kv4_attention(const uint16_t* queries, size_t query_strid
     c.window = window_size > kIntMax ? 0 : (long long)window_size;
     c.causal = is_causal != 0;
     c.ws = static_cast<uint8_t*>(workspace);
-    if (cb::kv4::launch_attention(c, pg, ge, S(stream)) == -2)
-        return arg(name, "too many sequences of too wide a block table");
-    return abi_check_launch(name);
+    const int rc = cb::kv4::launch_attention(c, pg, ge, S(stream));
+    if (rc == -2) return arg(name, "too many sequences of too wide a block table");
+    return launched(name, rc);
 }
 
 CB_API int cactus_cuda_kv_copy_pages(void* pool, size_t num_pages, size_t page_bytes, size_t page_stride,
@@ -175,10 +180,10 @@ CB_API int cactus_cuda_kv_copy_pages(void* pool, size_t num_pages, size_t page_b
     if (page_bytes > page_stride || page_bytes > ((size_t)1 << 28)) return arg(name, "bad page_bytes");
     if (page_stride > ((size_t)1 << 62) / num_pages) return arg(name, "pool size overflows");
     if (const char* why = planes_check(num_planes, plane_stride)) return arg(name, why);
-    cb::kv4::launch_copy_pages(static_cast<uint8_t*>(pool), (long long)num_pages, (long long)page_bytes,
-                               (long long)page_stride, (int)num_planes, (long long)plane_stride, src_pages, dst_pages,
-                               (int)num_copies, S(stream));
-    return abi_check_launch(name);
+    return launched(name, cb::kv4::launch_copy_pages(static_cast<uint8_t*>(pool), (long long)num_pages,
+                                                     (long long)page_bytes, (long long)page_stride, (int)num_planes,
+                                                     (long long)plane_stride, src_pages, dst_pages, (int)num_copies,
+                                                     S(stream)));
 }
 
 CB_API int cactus_cuda_kv4_compact(void* pool, size_t num_pages, size_t page_stride, size_t num_planes,
@@ -196,9 +201,8 @@ CB_API int cactus_cuda_kv4_compact(void* pool, size_t num_pages, size_t page_str
     if (!dst_table || !kept_rows || !kept_offsets) return arg(name, "null argument");
     if (num_seqs > kIntMax - 1 || num_kept > kIntMax - 64) return arg(name, "size too large");
     if (const char* why = planes_check(num_planes, plane_stride)) return arg(name, why);
-    cb::kv4::launch_compact(pg, dst_table, (int)num_planes, (long long)plane_stride, kept_rows, kept_offsets,
-                            (int)num_seqs, (int)num_kept, ge, S(stream));
-    return abi_check_launch(name);
+    return launched(name, cb::kv4::launch_compact(pg, dst_table, (int)num_planes, (long long)plane_stride, kept_rows,
+                                                  kept_offsets, (int)num_seqs, (int)num_kept, ge, S(stream)));
 }
 
 }  // extern "C"
