@@ -295,27 +295,37 @@ CB_API int cactus_kv4_compact(cactus_kv4_t cache, const int32_t* seqs, const int
         }
         const size_t kept = (size_t)offs.back();
         require(kept_rows || kept == 0, "null kept_rows");
-        for (size_t i = 0; i < num_seqs; ++i)
+        for (size_t i = 0; i < num_seqs; ++i) {
+            const int len = c.map->length(ids[i]);
             for (int j = offs[i]; j < offs[i + 1]; ++j)
-                require(kept_rows[j] >= 0 && kept_rows[j] < c.map->length(ids[i]), "a kept row that the sequence does not have");
-        require(2 * num_seqs * c.max_pages + num_seqs + 1 + kept <= c.list_ints, "too many rows kept in one call");
+                require(kept_rows[j] >= 0 && kept_rows[j] < len, "a kept row that the sequence does not have");
+        }
         const auto old = c.map->renew(ids, counts);
         c.batch = 0;
-        if (kept == 0) return (int)CB_OK;
+        // as many sequences at a time as the lists have room for, at least one (no sequence keeps more rows than
+        // its pages can hold); all new pages are taken by now, so none of them is read later
         const size_t w = c.max_pages;
-        std::vector<int> v(2 * num_seqs * w, -1);
-        for (size_t i = 0; i < num_seqs; ++i) {
-            const std::vector<int>& now = c.map->pages(ids[i]);
-            std::copy(old[i].begin(), old[i].end(), v.begin() + i * w);
-            std::copy(now.begin(), now.end(), v.begin() + (num_seqs + i) * w);
+        for (size_t from = 0, to; from < num_seqs; from = to) {
+            auto ints_of = [&](size_t end) { return 2 * (end - from) * w + (end - from) + 1 + (size_t)(offs[end] - offs[from]); };
+            for (to = from + 1; to < num_seqs && ints_of(to + 1) <= c.list_ints;) ++to;
+            const size_t n = to - from, rows = (size_t)(offs[to] - offs[from]);
+            if (rows == 0) continue;
+            std::vector<int> v(2 * n * w, -1);
+            for (size_t i = 0; i < n; ++i) {
+                const std::vector<int>& now = c.map->pages(ids[from + i]);
+                std::copy(old[from + i].begin(), old[from + i].end(), v.begin() + i * w);
+                std::copy(now.begin(), now.end(), v.begin() + (n + i) * w);
+            }
+            for (size_t i = from; i <= to; ++i) v.push_back(offs[i] - offs[from]);
+            v.insert(v.end(), kept_rows + offs[from], kept_rows + offs[to]);
+            c.staging.send(v, c.lists, static_cast<cudaStream_t>(stream));
+            const int* at = c.lists + 2 * n * w;
+            const int rc = cactus_cuda_kv4_compact(c.pool, c.num_pages, c.page_bytes, c.layers, c.num_pages * c.page_bytes,
+                                                   c.lists, c.lists + n * w, w, at + n + 1, at, n, rows, c.page, c.hkv, c.d,
+                                                   c.g, stream);
+            if (rc) return rc;
         }
-        v.insert(v.end(), offs.begin(), offs.end());
-        v.insert(v.end(), kept_rows, kept_rows + kept);
-        c.staging.send(v, c.lists, static_cast<cudaStream_t>(stream));
-        const int* at = c.lists + 2 * num_seqs * w;
-        return cactus_cuda_kv4_compact(c.pool, c.num_pages, c.page_bytes, c.layers, c.num_pages * c.page_bytes, c.lists,
-                                       c.lists + num_seqs * w, w, at + num_seqs + 1, at, num_seqs, kept, c.page, c.hkv,
-                                       c.d, c.g, stream);
+        return (int)CB_OK;
     });
 }
 

@@ -144,3 +144,52 @@ def test_captured_call_follows_offsets_on_the_device(rows, max_q):
         _check(pool, table, q[:n], counts, now, hq, True, 0, out[:n], lse[:n])
         assert (out[n:] == 123.0).all() and (lse[n:] == 123.0).all()
     assert _err() == 0
+
+
+def _batch_cache(ge, layers, lens, max_context, num_pages):
+    """A cache whose sequences hold lens rows each, and the rows [layer][seq][keys, values] as the format stands for them."""
+    from cactus_b200.kv4 import KVCache4
+    rng = np.random.default_rng(sum(lens))
+    cache = KVCache4(layers, 2 * ge.hkv, ge.hkv, ge.d, num_pages=num_pages, max_seqs=len(lens), max_context=max_context,
+                     max_tokens=sum(lens), group_size=ge.g, page_size=ge.page)
+    cache.begin(range(len(lens)), lens)
+    off, rows = _offsets(lens), []
+    for layer in range(layers):
+        kv = rng.standard_normal((2, sum(lens), ge.hkv, ge.d)).astype(np.float16)
+        d = [dev(x) for x in kv]
+        cache.append(layer, ptr(d[0]), ptr(d[1]))
+        want = [U.values(*U.quantise(x, ge.g), ge.g) for x in kv]
+        rows.append([[x[off[s]:off[s + 1]] for x in want] for s in range(len(lens))])
+    return cache, rows
+
+
+def _holds(cache, ge, layer, seq, want):
+    n = cache.length(seq)
+    assert n == want[0].shape[0]
+    got = [empty((n, ge.hkv, ge.d), np.float16) for _ in range(2)]
+    cache.read(layer, seq, 0, n, *(ptr(g) for g in got))
+    return all(np.array_equal(host(g, np.float16), w) for g, w in zip(got, want))
+
+
+def test_a_whole_batch_is_compacted_in_one_call():
+    """All sequences keep more rows together than one context holds, one of them all of its rows, one none."""
+    ge, layers = U.Geom(16, 2, 64, 32), 2
+    lens = [512, 400, 512, 17, 333, 512, 1, 480, 512, 256, 512, 90]
+    cache, rows = _batch_cache(ge, layers, lens, 512, 600)
+    rng = np.random.default_rng(4)
+    kept = [np.sort(rng.choice(n, n // 2 + 1 if n > 1 else 1, replace=False)) for n in lens]
+    kept[5], kept[7] = np.arange(512), np.arange(0)
+    cache.compact(range(len(lens)), kept)
+    for layer in range(layers):
+        for s in range(len(lens)):
+            rows[layer][s] = [x[kept[s]] for x in rows[layer][s]]
+            assert _holds(cache, ge, layer, s, rows[layer][s])
+    cache.slide(range(len(lens)), sink=3, window=200)
+    for layer in range(layers):
+        for s in range(len(lens)):
+            n = len(kept[s])
+            at = np.concatenate([np.arange(min(3, n)), np.arange(max(min(3, n), n - 197), n)])
+            assert _holds(cache, ge, layer, s, [x[at] for x in rows[layer][s]])
+    assert cache.info()["free_pages"] == 600 - sum(-(-cache.length(s) // 16) for s in range(len(lens)))
+    cache.close()
+    assert _err() == 0
