@@ -143,6 +143,7 @@ CB_API cactus_kv4_t cactus_kv4_create(size_t num_layers, size_t num_q_heads, siz
         require(num_q_heads >= 1 && num_q_heads % num_kv_heads == 0 && num_q_heads <= 65536,
                 "num_q_heads must be a multiple of num_kv_heads");
         require(num_pages >= 1 && num_pages < (size_t(1) << 30), "num_pages must be 1 to 2^30");
+        require(num_layers <= (size_t(1) << 62) / c->page_bytes / num_pages, "the pool would have 2^62 bytes or more");
         require(max_seqs >= 1 && max_seqs <= (size_t(1) << 20), "max_seqs must be 1 to 2^20");
         require(max_context >= 1 && max_context <= (size_t(1) << 30), "max_context must be 1 to 2^30");
         require(max_tokens >= 1 && max_tokens <= (size_t(1) << 30), "max_tokens must be 1 to 2^30");

@@ -19,3 +19,12 @@ def test_a_failed_launch_is_an_error(tmp_path):
                     os.path.join(ROOT, "tests", "native", "kv4_abi_launch_test.cpp"), "-o", exe], check=True)
     r = subprocess.run([exe], capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout == "ok\n", r.stdout + r.stderr
+
+
+@pytest.mark.parametrize("change", [dict(layers=1 << 14, pages=1 << 26), dict(layers=65535, pages=(1 << 30) - 1)])
+def test_a_pool_of_more_bytes_than_addresses_is_refused(change):
+    """2^14 layers of 2^26 pages of 5 * 2^24 bytes are 2^64 bytes five times: none, where the product wraps."""
+    L = cb.lib()
+    assert L.cactus_cuda_kv4_page_bytes(256, 1024, 256, 32) == 5 << 24
+    assert not L.cactus_kv4_create(change["layers"], 1024, 1024, 256, 32, 256, change["pages"], 1, 256, 1, 0)
+    assert b"kv4_create: the pool" in L.cactus_cuda_last_error()
