@@ -117,6 +117,14 @@ int guarded(cactus_kv4_t h, const char* name, F f) {
 void require(bool ok, const char* why) {
     if (!ok) throw std::invalid_argument(why);
 }
+// The stream of a call. A captured one would be wrong when it is replayed after the next begin: the batch's
+// counts and the table's width are arguments of the launches, and page lists pass through host memory.
+cudaStream_t stream_of(void* stream) {
+    cudaStreamCaptureStatus status;
+    cu(cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &status), "cudaStreamIsCapturing");
+    require(status == cudaStreamCaptureStatusNone, "a cache's calls cannot be captured (its kernel entry points can)");
+    return static_cast<cudaStream_t>(stream);
+}
 
 }  // namespace
 
@@ -143,7 +151,7 @@ CB_API cactus_kv4_t cactus_kv4_create(size_t num_layers, size_t num_q_heads, siz
         require(num_q_heads >= 1 && num_q_heads % num_kv_heads == 0 && num_q_heads <= 65536,
                 "num_q_heads must be a multiple of num_kv_heads");
         require(num_pages >= 1 && num_pages < (size_t(1) << 30), "num_pages must be 1 to 2^30");
-        require(num_layers <= (size_t(1) << 62) / c->page_bytes / num_pages, "the pool would have 2^62 bytes or more");
+        require(num_layers <= (size_t(1) << 62) / c->page_bytes / num_pages, "the pool would have more than 2^62 bytes");
         require(max_seqs >= 1 && max_seqs <= (size_t(1) << 20), "max_seqs must be 1 to 2^20");
         require(max_context >= 1 && max_context <= (size_t(1) << 30), "max_context must be 1 to 2^30");
         require(max_tokens >= 1 && max_tokens <= (size_t(1) << 30), "max_tokens must be 1 to 2^30");
@@ -186,7 +194,7 @@ CB_API int cactus_kv4_begin(cactus_kv4_t cache, const int32_t* seqs, const int32
             longest = longest > (size_t)n ? longest : (size_t)n;
         }
         require(total <= c.max_tokens, "more rows than max_tokens");
-        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        const cudaStream_t st = stream_of(stream);
         const auto copies = c.map->grow(ids, counts);
         c.batch = 0;  // no batch if anything fails from here
         if (!copies.empty()) {
@@ -222,6 +230,7 @@ CB_API int cactus_kv4_append(cactus_kv4_t cache, size_t layer, const uint16_t* k
                              size_t row_stride, void* stream) {
     return guarded(cache, "kv4_append", [&](Cache& c) {
         require(layer < c.layers && c.batch, "no such layer, or no batch begun");
+        stream_of(stream);
         return cactus_cuda_kv4_append(keys, values, row_stride, c.offsets(), c.lens(), c.table(), c.batch_pages,
                                       c.layer_pool(layer), c.num_pages, c.page_bytes, c.batch, c.batch_tokens, c.page,
                                       c.hkv, c.d, c.g, stream);
@@ -233,6 +242,7 @@ CB_API int cactus_kv4_attention(cactus_kv4_t cache, size_t layer, const uint16_t
                                 void* stream) {
     return guarded(cache, "kv4_attention", [&](Cache& c) {
         require(layer < c.layers && c.batch, "no such layer, or no batch begun");
+        stream_of(stream);
         return cactus_cuda_kv4_attention(queries, query_stride, c.offsets(), c.lens(), c.table(), c.batch_pages,
                                          c.layer_pool(layer), c.num_pages, c.page_bytes, output, lse, c.batch,
                                          c.batch_tokens, c.batch_longest, c.hq, c.page, c.hkv, c.d, c.g, scale,
@@ -246,10 +256,11 @@ CB_API int cactus_kv4_read(cactus_kv4_t cache, size_t layer, int32_t seq, size_t
         require(layer < c.layers, "no such layer");
         require(first + count >= first && first + count <= (size_t)c.map->length(seq), "rows that the sequence does not have");
         if (count == 0) return (int)CB_OK;
+        const cudaStream_t st = stream_of(stream);
         std::vector<int> v = {0, (int)count, (int)first};
         const std::vector<int>& pages = c.map->pages(seq);
         v.insert(v.end(), pages.begin(), pages.end());
-        c.staging.send(v, c.lists, static_cast<cudaStream_t>(stream));
+        c.staging.send(v, c.lists, st);
         return cactus_cuda_kv4_read(c.layer_pool(layer), c.num_pages, c.page_bytes, c.lists + 3, pages.size(), c.lists,
                                     c.lists + 2, keys, values, 1, count, c.page, c.hkv, c.d, c.g, stream);
     });
@@ -301,6 +312,7 @@ CB_API int cactus_kv4_compact(cactus_kv4_t cache, const int32_t* seqs, const int
             for (int j = offs[i]; j < offs[i + 1]; ++j)
                 require(kept_rows[j] >= 0 && kept_rows[j] < len, "a kept row that the sequence does not have");
         }
+        const cudaStream_t st = stream_of(stream);
         const auto old = c.map->renew(ids, counts);
         c.batch = 0;
         // as many sequences at a time as the lists have room for, at least one (no sequence keeps more rows than
@@ -319,7 +331,7 @@ CB_API int cactus_kv4_compact(cactus_kv4_t cache, const int32_t* seqs, const int
             }
             for (size_t i = from; i <= to; ++i) v.push_back(offs[i] - offs[from]);
             v.insert(v.end(), kept_rows + offs[from], kept_rows + offs[to]);
-            c.staging.send(v, c.lists, static_cast<cudaStream_t>(stream));
+            c.staging.send(v, c.lists, st);
             const int* at = c.lists + 2 * n * w;
             const int rc = cactus_cuda_kv4_compact(c.pool, c.num_pages, c.page_bytes, c.layers, c.num_pages * c.page_bytes,
                                                    c.lists, c.lists + n * w, w, at + n + 1, at, n, rows, c.page, c.hkv, c.d,

@@ -106,7 +106,9 @@ CB_API int cactus_cuda_kv4_compact(void* pool, size_t num_pages, size_t page_str
  * are HOST arrays; keys, values, queries and results are device pointers. Sequences are numbered 0
  * to max_seqs - 1 and empty at first. The calls of one cache are made in order, on one stream or on
  * streams that the caller orders (a page that is freed is given out again); not from two threads at
- * once. A call that fails for its arguments or for lack of pages changes nothing. */
+ * once. They cannot be captured in a CUDA graph (a batch's counts are the host's; a call on a capturing
+ * stream fails), the kernel entry points above can. A call that fails for its arguments or for lack of
+ * pages changes nothing. */
 typedef void* cactus_kv4_t;
 
 /* num_pages pages of page_size rows for every layer, block tables for max_context rows, batches of up

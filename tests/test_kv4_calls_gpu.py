@@ -193,3 +193,29 @@ def test_a_whole_batch_is_compacted_in_one_call():
     assert cache.info()["free_pages"] == 600 - sum(-(-cache.length(s) // 16) for s in range(len(lens)))
     cache.close()
     assert _err() == 0
+
+
+def test_the_handle_refuses_to_be_captured():
+    """The shapes of a batch's launches are the host's at the time of the call: a replay after the next begin would be wrong."""
+    t = torch()
+    ge = U.Geom(16, 1, 64, 32)
+    cache, rows = _batch_cache(ge, 1, [20, 3], 64, 12)
+    cache.begin([0, 1], [1, 1])
+    x = dev(np.ones((2, 2, 64), np.float16))
+    out = empty((2, 2, 64), np.float16)
+    t.cuda.synchronize()
+    graph = t.cuda.CUDAGraph()
+    with t.cuda.graph(graph):
+        t.zeros(1, device="cuda")
+        s = t.cuda.current_stream().cuda_stream
+        for call in (lambda: cache.append(0, ptr(x), ptr(x), stream=s),
+                     lambda: cache.attention(0, ptr(x), ptr(out), 0.125, stream=s),
+                     lambda: cache.read(0, 0, 0, 1, ptr(out), ptr(out), stream=s),
+                     lambda: cache.begin([0], [1], stream=s), lambda: cache.compact([0], [[0, 1]], stream=s)):
+            with pytest.raises(cb.CactusError, match="captured"):
+                call()
+    assert cache.length(0) == 21
+    cache.append(0, ptr(x), ptr(x))  # the batch is still there, outside of a capture
+    assert _holds(cache, ge, 0, 0, [np.concatenate([w, np.ones((1, 1, 64), np.float16)]) for w in rows[0][0]])
+    cache.close()
+    assert _err() == 0
