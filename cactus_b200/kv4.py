@@ -18,8 +18,17 @@ def _addr(x):
 
 
 def _host(v):
-    a = np.ascontiguousarray(v, np.int32).reshape(-1)
+    """A list of sequences, counts or rows as int32 values, none of them changed on the way."""
+    a = np.asarray(v).reshape(-1)
+    if a.size and (a.dtype.kind not in "iu" or int(a.min()) < -2 ** 31 or int(a.max()) >= 2 ** 31):
+        raise CactusError(f"lists hold whole numbers of 32 bits: got {a.dtype} {a[:4]}")
+    a = np.ascontiguousarray(a, np.int32)
     return a, a.ctypes.data_as(C.c_void_p)
+
+
+def _seq(v):
+    """One sequence number: ctypes would take the low 32 bits of a larger one."""
+    return int(_host([v])[0][0])
 
 
 class KVCache4:
@@ -61,7 +70,8 @@ class KVCache4:
                                            scale, window, int(causal), stream), "kv4_attention")
 
     def read(self, layer: int, seq: int, first: int, count: int, keys, values, stream: int = 0):
-        check(self._L.cactus_kv4_read(self.h, layer, seq, first, count, _addr(keys), _addr(values), stream), "kv4_read")
+        check(self._L.cactus_kv4_read(self.h, layer, _seq(seq), first, count, _addr(keys), _addr(values), stream),
+              "kv4_read")
 
     def fork(self, src, dst):
         """Sequences dst become copies of src (pages shared until they are written)."""
@@ -71,7 +81,7 @@ class KVCache4:
         check(self._L.cactus_kv4_fork(self.h, sp, dp, s.size), "kv4_fork")
 
     def truncate(self, seq: int, length: int):
-        check(self._L.cactus_kv4_truncate(self.h, seq, length), "kv4_truncate")
+        check(self._L.cactus_kv4_truncate(self.h, _seq(seq), length), "kv4_truncate")
 
     def free(self, seqs):
         s, sp = _host(seqs)
@@ -82,8 +92,9 @@ class KVCache4:
         s, sp = _host(seqs)
         if s.size != len(kept):
             raise CactusError("compact: a list of rows for each sequence is needed")
-        rows, rp = _host(np.concatenate([np.asarray(k, np.int32).reshape(-1) for k in kept]) if len(kept) else [])
-        offs, op = _host(np.concatenate([[0], np.cumsum([len(k) for k in kept])]))
+        kept = [_host(k)[0] for k in kept]
+        rows, rp = _host(np.concatenate(kept) if kept else [])
+        offs, op = _host(np.concatenate([[0], np.cumsum([len(k) for k in kept], dtype=np.int64)]))
         check(self._L.cactus_kv4_compact(self.h, sp, rp, op, s.size, stream), "kv4_compact")
 
     def slide(self, seqs, sink: int, window: int, stream: int = 0):
@@ -96,7 +107,7 @@ class KVCache4:
         self.compact(seqs, kept, stream)
 
     def length(self, seq: int) -> int:
-        n = self._L.cactus_kv4_length(self.h, seq)
+        n = self._L.cactus_kv4_length(self.h, _seq(seq))
         if n < 0:
             check(n, "kv4_length")
         return n
