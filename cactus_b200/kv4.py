@@ -99,6 +99,8 @@ class KVCache4:
 
     def slide(self, seqs, sink: int, window: int, stream: int = 0):
         """Sequences keep their first `sink` rows and their last ones, `window` in all."""
+        if sink < 0 or window < 0:
+            raise CactusError("slide: sink and window must not be negative")
         kept = []
         for s in seqs:
             n = self.length(s)

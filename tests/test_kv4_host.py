@@ -1,5 +1,6 @@
 """Host side of the 4-bit paged KV cache without a GPU: launch failures, sizes and lists that cannot be."""
 import ctypes as C
+import ctypes as C
 import os
 import subprocess
 
@@ -54,3 +55,32 @@ def test_a_sequence_number_is_not_cut_to_32_bits():
         for call in (lambda: cache.length(seq), lambda: cache.truncate(seq, 0), lambda: cache.read(0, seq, 0, 1, 0, 0)):
             with pytest.raises(cb.CactusError, match=why):
                 call()
+
+
+class _Recorded:
+    """Stands for the library: keeps what compact is called with, sequences hold 10 rows."""
+    rows = None
+
+    def cactus_kv4_length(self, h, seq):
+        return 10
+
+    def cactus_kv4_compact(self, h, seqs, rows, offsets, n, stream):
+        off = np.ctypeslib.as_array((C.c_int32 * (n + 1)).from_address(offsets.value)).tolist()
+        self.rows = [np.ctypeslib.as_array((C.c_int32 * max(1, off[-1])).from_address(rows.value)).tolist()[a:b]
+                     for a, b in zip(off, off[1:])]
+        return 0
+
+    def cactus_kv4_destroy(self, h):
+        pass
+
+
+def test_slide_keeps_first_and_last_rows_and_refuses_negative_sizes():
+    cache = kv4.KVCache4.__new__(kv4.KVCache4)
+    cache._L, cache.h = _Recorded(), 1
+    for sink, window, kept in ((2, 5, [0, 1, 7, 8, 9]), (0, 3, [7, 8, 9]), (4, 4, [0, 1, 2, 3]), (6, 4, [0, 1, 2, 3]),
+                               (3, 50, list(range(10))), (20, 30, list(range(10))), (0, 0, [])):
+        cache.slide([0, 1], sink, window)
+        assert cache._L.rows == [kept, kept], (sink, window)
+    for sink, window in ((0, -1), (-1, 4), (-2, -3)):
+        with pytest.raises(cb.CactusError, match="negative"):
+            cache.slide([0], sink, window)
