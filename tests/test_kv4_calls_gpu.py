@@ -219,3 +219,31 @@ def test_the_handle_refuses_to_be_captured():
     assert _holds(cache, ge, 0, 0, [np.concatenate([w, np.ones((1, 1, 64), np.float16)]) for w in rows[0][0]])
     cache.close()
     assert _err() == 0
+
+
+@pytest.mark.parametrize("d,g", [(64, 32), (64, 64), (128, 128), (256, 32)])
+def test_append_rounds_the_differences_as_they_are(d, g):
+    """Groups whose range and elements differ from fifteen steps and from halves by less than fp32 resolves beside
+    them: the format's step and codes are those of the exact differences."""
+    L, ge = cb.lib(), U.Geom(16, 1, d, g)
+    rng = np.random.default_rng(d + g)
+    n = 160
+    x = np.empty((n, d // g, g), np.float16)
+    for i in range(n):
+        for j in range(d // g):
+            s = 2.0 ** rng.integers(-3, 4)
+            row = s * (rng.integers(0, 15, g) + 0.5)     # halves of a step
+            row[rng.integers(0, g, g // 4)] = s * 7.0
+            row[0], row[1] = 15 * s, rng.choice([-1, 1, 1, 3]) * 2.0 ** -24 * 2.0 ** rng.integers(0, 6)
+            x[i, j] = rng.permutation(row) * rng.choice([-1, 1])
+    x = x.reshape(n, d)
+    pool = U.Pool(ge, n // 16, rng)
+    dpool, dx = dev(pool.bytes), dev(x)
+    meta = [dev(np.array(a, np.int32)) for a in ([0, n], [n], [list(range(n // 16))])]
+    cb.check(L.cactus_cuda_kv4_append(ptr(dx), ptr(dx), d, ptr(meta[0]), ptr(meta[1]), ptr(meta[2]), n // 16, ptr(dpool),
+                                      n // 16, pool.stride, 1, n, *ge.args(), None))
+    for i in range(n):
+        for which in (0, 1):
+            pool.write(which, i // 16, i % 16, x[i].reshape(1, d))
+    assert np.array_equal(host(dpool, np.uint8), pool.bytes)
+    assert _err() == 0
