@@ -1,10 +1,12 @@
 // Attention over the 4-bit paged KV cache for few queries a sequence (decode, drafted tokens). Its
 // floor is the cache's bytes, read once; what bounds it is the instructions that turn codes into
-// operands: of about 380 a warp for 16 keys of 128, 208 unpack and scale 1024 elements (13 for 8), and
-// groups of 128 (0.53 bytes an element) take as long as groups of 32 (0.63). On B200: 64 sequences of
-// 16 to 32 thousand rows, 8 kv heads of 128, 516 us, 3.9 TB/s of the cache (floor 313 us); 256 short
+// operands, and that they wait for one another: of about 419 a warp for 16 keys of 128, 208 unpack and
+// scale 1024 elements (13 for 8), groups of 128 (0.53 bytes an element) take as long as groups of 32
+// (0.63), and with under three warps a scheduler 59 % of the issue slots are used. On B200: 64 sequences
+// of 16 to 32 thousand rows, 8 kv heads of 128, 518 us, 3.9 TB/s of the cache (floor 314 us); 256 short
 // conversations in pages of 16, heads of 64, 78 us (floor 14 us: the starts and ends of 2048 items
-// and the 16-key overheads at half the elements weigh most there).
+// and the 16-key overheads at half the elements weigh most there); 12 sequences of 5 drafted tokens over 8
+// thousand rows, 62 us (floor 14 us: 10 q rows take two column tiles of 8, each with two products a weight).
 //
 // Work. A sequence's q rows of one kv head (its tokens times the heads that share it, in tiles of
 // 4, 8 or 16 rows) over its visible keys is an item; items are cut into tiles of 64 or 128 keys, and the
@@ -27,8 +29,9 @@
 // quarter of the 16 keys for the values, where the codes of two keys are interleaved by bytes first
 // so that one mask gives the same dim of both. Key i of the fragment is row kappa(i) of the 16,
 // which spreads the lanes' shared-memory reads over the banks. The weights go into O as two fp16
-// numbers, p = hi + lo (22 bits), which makes the result as good as with fp32 weights; up to 4 rows
-// have lo in the columns that they leave empty.
+// numbers, p = hi + lo (22 bits, what is below 2^-31 of the largest weight left out); up to 4 rows have lo
+// in the columns that they leave empty. The tensor core cuts its fp32 sums instead of rounding them, so a
+// result is low by what 16 keys at a time lose: 8e-6 of it over 32768 rows, 4e-7 over 2000.
 //
 // Softmax. Weights are relative to 2^-kHead of the running maximum, which is raised only when a score
 // exceeds it by more than 2^kLazy: until then they grow past 2^kHead (at most 2^15, inside fp16), which

@@ -69,8 +69,7 @@ __device__ __forceinline__ uint32_t mask_magic(uint32_t w) {
 }
 
 // Eight codes (element i in bits 4i..4i+3) as exact fp16 integers, in the order (0, 4), (1, 5),
-// (2, 6), (3, 7): 0x6400 | c is the fp16 number 1024 + c, and 0x6400 | (c << 4) is 1024 + 16 c. The
-// shift by 8 is a multiplication, which does not compete with the masks for the logic unit.
+// (2, 6), (3, 7): 0x6400 | c is the fp16 number 1024 + c, and 0x6400 | (c << 4) is 1024 + 16 c.
 __device__ __forceinline__ void codes_to_half(uint32_t w, __half2 (&h)[4]) {
     const uint32_t n1024 = 0xE400E400u, r16 = 0x2C002C00u, n64 = 0xD400D400u;  // -1024, 1/16, -64
     const uint32_t w8 = w >> 8;

@@ -2,9 +2,9 @@
 // rows), copy of whole pages, compaction (rows into other pages). Each input byte is read once and each
 // output byte written once, in 16-byte pieces where the row is long enough.
 //
-// On B200: append of 32 prompts (69 thousand rows, 8 heads of 128) about 125 us, bound by the
-// instructions of the quantisation (about 190 a warp for 256 elements; its bytes take 57 us); their
-// read-back 69 us (floor 57); copy of 640 pages in 16 layers 116 us, 7.2 TB/s (a quarter of the copies
+// On B200: append of 32 prompts (69 thousand rows, 8 heads of 128) about 129 us, bound by the
+// instructions of the quantisation (196 a warp for 256 elements; its bytes take 57 us); their
+// read-back 66 us (floor 57); copy of 640 pages in 16 layers 116 us, 7.2 TB/s (a quarter of the copies
 // read one page); compaction of 2045 scattered rows of 16 sequences in 16 layers 251 us, 4.8 TB/s
 // (floor 188 us; rows of 64 and 8 bytes do not fill the 64-byte units that DRAM reads).
 #include "kv4.cuh"

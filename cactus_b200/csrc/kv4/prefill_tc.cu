@@ -23,16 +23,18 @@
 // permuted alike when it is loaded, and O when it is stored.
 // Weights go to the tensor core as two fp16 numbers, p = hi + lo (22 bits), in the columns of the S that
 // they come from: hi in its first half, lo in the other, each with a product of its own. They are
-// relative to 2^-kHead of the running maximum, as in the kernel for few queries.
+// relative to 2^-kHead of the running maximum, as in the kernel for few queries. The tensor core cuts its
+// fp32 sums instead of rounding them, twice for 16 keys: a result is low by 4e-6 of it over 2300 rows, 1.9e-5
+// over 8192, in proportion to the rows.
 //
 // What bounds it: a row's chain from S to the next S, of which the other row tile hides about half; it
 // has all of the weights' work (the exponentials of two row tiles take 2048 cycles a key tile of 128)
-// and both of their products. The unpacking of K and V takes 2700 cycles on its four warps beside
-// them. On B200: 2048 queries after up to 6144 rows, 4 sequences, 16 / 8 heads of 128: 605 us, 730
-// TFLOP/s of the 4 D operations a pair of query and key (with weights of one fp16 number 493 us, but
-// then their rounding is as large as the result's; floor 266 us at the measured peak). 256 queries with
-// a window of 512, 4 heads of 256 on one, 16 sequences: 31 us, of which the start takes 6, the results 4
-// and 9 key tiles the rest.
+// and both of their products, with which the tensor pipe is busy 67 % of the time. The unpacking of K
+// and V takes 2700 cycles on its four warps beside them. On B200: 2048 queries after up to 6144 rows,
+// 4 sequences, 16 / 8 heads of 128: 608 us, 726 TFLOP/s of the 4 D operations a pair of query and key
+// (with weights of one fp16 number 493 us, but then their rounding is as large as the result's; floor
+// 266 us at the measured peak). 256 queries with a window of 512, 4 heads of 256 on one, 16 sequences:
+// 31 us, of which the start takes 6, the results 4 and 9 key tiles the rest.
 //
 // This file is compiled as whole-program device code (build.py WHOLE_PROGRAM).
 #include <atomic>

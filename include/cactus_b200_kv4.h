@@ -22,12 +22,12 @@
  * group of group_size consecutive elements are two fp16 numbers, (step, low); code c stands for
  * fp16(c * step + low) with one rounding. The append takes low = the group's smallest element,
  * step = (largest - smallest) / 15 rounded towards zero, c = round-half-even((x - low) / step) in
- * 0..15. A constant group has step 0 and codes 0. A group that holds an infinity or a NaN reads
- * as NaN throughout, so that it shows in every output that sees it.
+ * 0..15, all of the exact differences. A constant group has step 0 and codes 0. A group that holds
+ * an infinity or a NaN reads as NaN throughout, so that it shows in every output that sees it.
  *
  * Row r of sequence b is row r % page_size of page block_table[b * table_stride + r / page_size].
- * table_stride * page_size is below 2^31 - 1024. head_dim is 64, 128 or 256; group_size 32, 64 or 128 and a divisor of head_dim. Pool and strides
- * are 16-byte aligned.
+ * table_stride * page_size is below 2^31 - 1024. head_dim is 64, 128 or 256; group_size 32, 64 or
+ * 128 and a divisor of head_dim. Pool and strides are 16-byte aligned.
  *
  * Batches are ragged: sequence b has the token rows token_offsets[b] .. token_offsets[b + 1] - 1
  * (token_offsets: [num_seqs + 1], rising from 0; token_offsets[num_seqs] <= num_tokens, and rows
@@ -70,7 +70,9 @@ CB_API int cactus_cuda_kv4_read(const void* pool, size_t num_pages, size_t page_
  * output [num_tokens][num_q_heads][head_dim] fp16 (16-byte aligned), lse
  * [num_tokens][num_q_heads] fp32, natural log-sum-exp of the scaled scores (may be NULL). A query
  * that sees no row gives zeros and -inf. Pages that hold no visible row are not read (their table
- * entries may be anything), and neither are rows past context_lens[b].
+ * entries may be anything); rows past context_lens[b] on a page that holds one may be loaded, and
+ * whatever they hold does not reach a result. Scores, weights, their sums and the sums of weighted
+ * values are fp32 (weights enter the products as two fp16 numbers, 22 bits); results are rounded once.
  * max_query_len bounds every sequence's token count; a longer one is cut there and raises the
  * device error word. workspace: cactus_cuda_kv4_attention_workspace() bytes, 16-byte aligned, zeroed
  * once before its first use; every call leaves it ready for the next, also of other shapes that
