@@ -10,7 +10,7 @@ import os
 import re
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-HEADERS = ("cactus_b200.h", "cactus_b200_kv4.h", "cactus_b200_engine.h", "cactus_ffi.h")
+HEADERS = ("cactus_b200.h", "cactus_b200_kv4.h", "cactus_b200_batch.h", "cactus_b200_engine.h", "cactus_ffi.h")
 
 _SCALAR = {
     "int": C.c_int,

@@ -31,6 +31,7 @@ enum DevError : unsigned {
     kDevTmaTimeout = 1,
     kDevFlagTimeout = 2,
     kDevBadPage = 3,  // 4-bit KV cache: a page id, position or length outside what the call gave
+    kDevBadList = 4,  // a ragged batch's lists: an offset, id or length outside what the call gave
 };
 #ifdef __CUDACC_RDC__
 extern __device__ unsigned g_dev_error;

@@ -237,6 +237,21 @@ CB_API int cactus_kv4_append(cactus_kv4_t cache, size_t layer, const uint16_t* k
     });
 }
 
+CB_API int cactus_kv4_rope_append(cactus_kv4_t cache, size_t layer, const uint16_t* queries, size_t query_stride,
+                                  uint16_t* rotated, size_t rotated_stride, const uint16_t* keys,
+                                  const uint16_t* values, size_t row_stride, const float* rope_table,
+                                  size_t num_positions, size_t rotary_dim, const uint16_t* q_weight,
+                                  const uint16_t* k_weight, float eps, void* stream) {
+    return guarded(cache, "kv4_rope_append", [&](Cache& c) {
+        require(layer < c.layers && c.batch, "no such layer, or no batch begun");
+        stream_of(stream);
+        return cactus_cuda_kv4_rope_append(queries, query_stride, rotated, rotated_stride, keys, values, row_stride,
+                                           rope_table, num_positions, rotary_dim, q_weight, k_weight, eps, c.offsets(),
+                                           c.lens(), c.table(), c.batch_pages, c.layer_pool(layer), c.num_pages,
+                                           c.page_bytes, c.batch, c.batch_tokens, c.hq, c.page, c.hkv, c.d, c.g, stream);
+    });
+}
+
 CB_API int cactus_kv4_attention(cactus_kv4_t cache, size_t layer, const uint16_t* queries, size_t query_stride,
                                 uint16_t* output, float* lse, float scale, size_t window_size, int is_causal,
                                 void* stream) {

@@ -20,6 +20,22 @@ int launch_copy_pages(uint8_t* pool, long long num_pages, long long page_bytes, 
 int launch_compact(const Pages& src, const int* dst_table, int planes, long long plane_stride, const int* kept,
                    const int* offsets, int num_seqs, int num_kept, const Geom& ge, cudaStream_t st);
 
+// rope.cu
+struct RopeCall {
+    const __half *q, *k, *v;  // q may be null where hq is 0
+    long long q_stride, out_stride, row_stride;
+    __half* out;
+    const float2* turns;  // [num_positions][rotary / 2]
+    long long num_positions;
+    int rotary;
+    const __half *q_weight, *k_weight;  // may be null
+    float eps;
+    const int *offsets, *lens;
+    int num_seqs, num_tokens, hq;
+};
+int launch_rope_table(float theta, int half, long long positions, float* table, cudaStream_t st);
+int launch_rope_append(const RopeCall& c, const Pages& pg, const Geom& ge, cudaStream_t st);
+
 struct AttnCall {
     const __half* q;
     long long q_stride;

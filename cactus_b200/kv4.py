@@ -31,6 +31,11 @@ def _seq(v):
     return int(_host([v])[0][0])
 
 
+def rope_table(theta: float, rotary_dim: int, positions: int, table, stream: int = 0):
+    """Fills table [positions][rotary_dim / 2][2] (fp32, device) with the turns that rope_append takes."""
+    check(lib().cactus_cuda_rope_table(theta, rotary_dim, positions, _addr(table), stream), "rope_table")
+
+
 class KVCache4:
     def __init__(self, layers: int, q_heads: int, kv_heads: int, head_dim: int, num_pages: int, max_seqs: int,
                  max_context: int, max_tokens: int, group_size: int = 32, page_size: int = 64, device: int = 0):
@@ -62,6 +67,17 @@ class KVCache4:
     def append(self, layer: int, keys, values, row_stride: int | None = None, stream: int = 0):
         check(self._L.cactus_kv4_append(self.h, layer, _addr(keys), _addr(values),
                                         row_stride or self.kv_heads * self.head_dim, stream), "kv4_append")
+
+    def rope_append(self, layer: int, keys, values, table, positions: int, rotary_dim: int, queries=None, rotated=None,
+                    q_weight=None, k_weight=None, eps: float = 1e-6, row_stride: int | None = None,
+                    query_stride: int | None = None, rotated_stride: int | None = None, stream: int = 0):
+        """Normalises and turns keys and queries at their positions, appends keys and values."""
+        wide = self.q_heads * self.head_dim
+        check(self._L.cactus_kv4_rope_append(self.h, layer, _addr(queries), query_stride or wide, _addr(rotated),
+                                             rotated_stride or wide, _addr(keys), _addr(values),
+                                             row_stride or self.kv_heads * self.head_dim, _addr(table), positions,
+                                             rotary_dim, _addr(q_weight), _addr(k_weight), eps, stream),
+              "kv4_rope_append")
 
     def attention(self, layer: int, queries, output, scale: float, lse=None, query_stride: int | None = None,
                   window: int = 0, causal: bool = True, stream: int = 0):

@@ -55,6 +55,31 @@ CB_API int cactus_cuda_kv4_append(const uint16_t* keys, const uint16_t* values, 
                                   size_t page_stride, size_t num_seqs, size_t num_tokens, size_t page_size,
                                   size_t num_kv_heads, size_t head_dim, size_t group_size, void* stream);
 
+/* Turns for the append below: table[p][i] = (cos, sin) of p * theta^(-2 i / rotary_dim), [num_positions]
+ * [rotary_dim / 2] pairs of fp32 (16-byte aligned). Any other table of that shape will do as well (scaled
+ * frequencies, for instance). */
+CB_API int cactus_cuda_rope_table(float theta, size_t rotary_dim, size_t num_positions, float* table, void* stream);
+
+/* cactus_cuda_kv4_append of keys that are normalised and rotated first, and the same for queries
+ * [num_tokens][num_q_heads][head_dim] (rows query_stride elements apart), which go to `rotated` (rows
+ * rotated_stride apart; it may be queries, with the same stride). For each head's row x of a token at position p:
+ * x / sqrt(mean(x^2) + eps) * weight, with q_weight or k_weight [head_dim] (NULL: x as it is); then elements i and
+ * i + rotary_dim / 2 of the first rotary_dim (a multiple of 16, at most head_dim; 0: none) become
+ * (a cos - b sin, b cos + a sin) with row p of rope_table [num_positions][rotary_dim / 2]; then one rounding to
+ * fp16, which for keys is what is quantised. Values are quantised as they are. All of it is fp32. queries NULL:
+ * the append alone. A token at a position below 0, or past rope_table's end (which raises the device error word),
+ * is not appended and its rotated queries are zeros; token rows of no sequence stay as they are. Pointers are
+ * 16-byte aligned and strides multiples of 8. */
+CB_API int cactus_cuda_kv4_rope_append(const uint16_t* queries, size_t query_stride, uint16_t* rotated,
+                                       size_t rotated_stride, const uint16_t* keys, const uint16_t* values,
+                                       size_t row_stride, const float* rope_table, size_t num_positions,
+                                       size_t rotary_dim, const uint16_t* q_weight, const uint16_t* k_weight,
+                                       float eps, const int32_t* token_offsets, const int32_t* context_lens,
+                                       const int32_t* block_table, size_t table_stride, void* pool, size_t num_pages,
+                                       size_t page_stride, size_t num_seqs, size_t num_tokens, size_t num_q_heads,
+                                       size_t page_size, size_t num_kv_heads, size_t head_dim, size_t group_size,
+                                       void* stream);
+
 /* Reads rows back as fp16: row j of sequence b's row_offsets[b + 1] - row_offsets[b] rows is its
  * position first_rows[b] + j (first_rows NULL: 0 for all) and goes to row row_offsets[b] + j of
  * keys and values [num_rows][num_kv_heads][head_dim] (16-byte aligned; either may be NULL). */
@@ -126,9 +151,14 @@ CB_API void cactus_kv4_destroy(cactus_kv4_t cache);
  * seqs[1], ... one after another. The rows count as cached from here on. */
 CB_API int cactus_kv4_begin(cactus_kv4_t cache, const int32_t* seqs, const int32_t* new_rows, size_t num_seqs,
                             void* stream);
-/* cactus_cuda_kv4_append / _attention for the batch. */
+/* cactus_cuda_kv4_append, _rope_append (queries NULL: the append alone) and _attention for the batch. */
 CB_API int cactus_kv4_append(cactus_kv4_t cache, size_t layer, const uint16_t* keys, const uint16_t* values,
                              size_t row_stride, void* stream);
+CB_API int cactus_kv4_rope_append(cactus_kv4_t cache, size_t layer, const uint16_t* queries, size_t query_stride,
+                                  uint16_t* rotated, size_t rotated_stride, const uint16_t* keys,
+                                  const uint16_t* values, size_t row_stride, const float* rope_table,
+                                  size_t num_positions, size_t rotary_dim, const uint16_t* q_weight,
+                                  const uint16_t* k_weight, float eps, void* stream);
 CB_API int cactus_kv4_attention(cactus_kv4_t cache, size_t layer, const uint16_t* queries, size_t query_stride,
                                 uint16_t* output, float* lse, float scale, size_t window_size, int is_causal,
                                 void* stream);

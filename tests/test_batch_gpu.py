@@ -1,0 +1,550 @@
+"""A ragged batch's operators (include/cactus_b200_batch.h) against the 64-bit statements of tests/batch_util.py."""
+import numpy as np
+import pytest
+
+import cactus_b200 as cb
+from cactus_b200 import batch
+from tests import batch_util as U
+from tests.gpu_util import dev, empty, host, torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _err():
+    return cb.lib().cactus_cuda_device_error(None)
+
+
+def _padded(a, stride, rng, offset=0):
+    """Rows of `a` on the device, `stride` elements apart behind `offset` elements of something else."""
+    flat = (rng.integers(0, 1 << 16, offset + a.shape[0] * stride + 64, dtype=np.uint64).astype(np.uint16)).view(a.dtype)
+    rows = flat[offset:offset + a.shape[0] * stride].reshape(a.shape[0], stride)
+    rows[:, :a.shape[1]] = a
+    t = dev(flat)
+    return t, t.data_ptr() + offset * a.itemsize
+
+
+# ---------------------------------------------------------------------------------------- residual, RMSNorm, 8 bits
+def _check_norm(x, r, w, eps, got_sum, codes, scales, normed):
+    s = U.add16(x, r) if r is not None else x
+    if got_sum is not None:
+        assert np.array_equal(got_sum.view(np.uint16)[~np.isnan(s)], s.view(np.uint16)[~np.isnan(s)])
+        assert np.isnan(got_sum[np.isnan(s)]).all()
+    y, tol = U.norm(s, w, eps)
+    if normed is not None:
+        U.within(normed, np.where(np.abs(y) > 65519, np.copysign(np.inf, y), y), tol + U.fp16_step(y))
+    if codes is not None:
+        with np.errstate(invalid="ignore"):
+            top = np.abs(y).max(-1)
+            bad = ~(top < 3.4e38)
+        assert np.isnan(scales[bad]).all() and (codes[bad] == 0).all()
+        unit = np.maximum(top / 127, float(np.float32(1e-10)))[~bad]
+        assert (np.abs(scales[~bad] - unit) <= 5 * U.U32 * unit).all()
+        # a code is off its quotient by a half, and by what the quotient's steps leave: 8 of 2^-24 of 127
+        q = y[~bad] / unit[:, None]
+        assert (np.abs(codes[~bad] - q) <= 0.5 + 127 * 8 * U.U32).all()
+
+
+def _norm(x, w, r=None, xs=None, rs=None, eps=1e-6, want="sqn", inplace=None, rng=None, offset=0):
+    rows, dims = x.shape
+    rng = rng or np.random.default_rng(0)
+    tx, px = _padded(x, xs or dims, rng, offset)
+    tr, pr = _padded(r, rs or dims, rng, offset) if r is not None else (None, None)
+    tw = dev(w)
+    total = empty((rows, dims), np.float16) if "s" in want else None
+    codes, scales = (empty((rows, dims), np.int8), empty((rows,), np.float32)) if "q" in want else (None, None)
+    normed = empty((rows, dims), np.float16) if "n" in want else None
+    before = host(tx, np.uint16).copy()
+    ps, ss = (None, None) if total is None else (total.data_ptr(), dims)
+    if inplace:
+        ps, ss = (px, xs or dims) if inplace == "x" else (pr, rs or dims)
+    batch.add_rms_norm_q8(px, tw, rows, dims, codes, scales, normed, pr, ps, eps, xs or dims, rs or dims, ss)
+    if inplace:
+        flat = host(tx if inplace == "x" else tr, np.float16)
+        got = flat[offset:offset + rows * ss].reshape(rows, ss)[:, :dims].copy()
+    else:
+        got = None if total is None else host(total, np.float16)
+        assert np.array_equal(host(tx, np.uint16), before)
+    got = got, None if codes is None else host(codes, np.int8), None if codes is None else host(scales, np.float32), \
+        None if normed is None else host(normed, np.float16)
+    _check_norm(x, r, w, eps, *got)
+    assert _err() == 0
+    return got
+
+
+def _rows(rng, rows, dims, scale=1.0):
+    return (rng.standard_normal((rows, dims)) * scale).astype(np.float16)
+
+
+@pytest.mark.parametrize("dims", [1, 2, 7, 8, 31, 64, 100, 256, 1000, 1024, 1032, 2048, 2056, 4096, 5000, 8192, 8200, 12288, 16384,
+                                  20001, 32760, 32768])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_norm_dims(rows, dims):
+    rng = np.random.default_rng(dims)
+    _norm(_rows(rng, rows, dims, 2.0), _rows(rng, 1, dims)[0], _rows(rng, rows, dims))
+
+
+@pytest.mark.parametrize("want", ["s", "q", "n", "sq", "qn", "sqn", "sn"])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_outputs(want, residual):
+    if "q" not in want and "n" not in want:
+        want += "n"
+    rng = np.random.default_rng(3)
+    for dims in (264, 1030):
+        _norm(_rows(rng, 6, dims), _rows(rng, 1, dims)[0], _rows(rng, 6, dims) if residual else None, want=want)
+
+
+@pytest.mark.parametrize("dims,xs,rs,offset", [(512, 1024, 520, 0), (512, 515, 600, 0), (512, 512, 512, 1), (512, 520, 512, 8),
+                                               (77, 80, 77, 3), (4096, 12288, 4096, 0), (16384, 16385, 16400, 5)])
+@pytest.mark.parametrize("inplace", [None, "x", "r"])
+def test_norm_strides_alignment_and_in_place(dims, xs, rs, offset, inplace):
+    rng = np.random.default_rng(dims + offset)
+    _norm(_rows(rng, 7, dims), _rows(rng, 1, dims)[0], _rows(rng, 7, dims), xs, rs, inplace=inplace, rng=rng, offset=offset)
+
+
+def test_norm_many_rows_and_extreme_values():
+    rng = np.random.default_rng(9)
+    x, r = _rows(rng, 1500, 192), _rows(rng, 1500, 192)
+    x[0], r[0] = 0, 0                       # eps alone
+    x[1] *= np.float16(2.0 ** -10)          # near fp16's smallest
+    x[2], r[2] = 6e-8, 0
+    x[3], r[3] = 60000, 0
+    x[4, 5], r[4, 5] = 60000, 60000         # the sum is infinite: a row that shows it
+    x[5, 0] = np.nan
+    x[6, 191], r[6, 191] = np.inf, -np.inf
+    x[7], r[7, :] = 0, 0
+    x[7, 3] = 1.0                           # one element has all of the norm
+    w = _rows(rng, 1, 192)[0]
+    w[10], w[11] = 0, -w[11]
+    for eps in (1e-6, 1e-5, 0.1):
+        _norm(x, w, r, eps=eps)
+    _norm(x[1:], w, r[1:], eps=0.0)
+    w[20] = np.inf
+    _norm(x[8:12], w, r[8:12])
+
+
+def test_norm_codes_feed_the_projection():
+    """matmul_int8 of the codes: the product of what they stand for, to its own two roundings."""
+    rng = np.random.default_rng(12)
+    rows, k, n, g = 20, 256, 96, 32
+    x, w = _rows(rng, rows, k), _rows(rng, 1, k)[0]
+    q, s = empty((rows, k), np.int8), empty((rows,), np.float32)
+    tx, tw = dev(x), dev(w)
+    batch.add_rms_norm_q8(tx, tw, rows, k, q, s)
+    b = rng.integers(-127, 128, (n, k)).astype(np.int8)
+    bs = (rng.random((n, k // g)) * 0.01 + 0.001).astype(np.float16)
+    tb, tbs, c = dev(b), dev(bs), empty((rows, n), np.float16)
+    cb.check(cb.lib().cactus_cuda_matmul_int8(q.data_ptr(), s.data_ptr(), tb.data_ptr(), tbs.data_ptr(), c.data_ptr(), rows, k,
+                                              n, g, None))
+    a = host(q, np.int8).astype(np.float64) * host(s, np.float32).astype(np.float64)[:, None]
+    full = b.astype(np.float64) * np.repeat(bs.astype(np.float64), g, 1)
+    ref, size = a @ full.T, np.abs(a) @ np.abs(full).T
+    U.within(host(c, np.float16), ref, U.fp16_step(ref) + (k // g + 4) * U.U32 * size)
+
+
+# ---------------------------------------------------------------------------------------- adapters
+class Lora:
+    """Arguments of a lora call on the device; rows and columns past an adapter's rank hold NaN."""
+
+    def __init__(self, counts, ids, ranks, k, n, rng, top=None, pad=0, extra=0, tokens=None, integers=False, scales=True,
+                 spread=1.0):
+        self.ids, self.ranks, self.k, self.n, self.ad = list(ids), list(ranks), k, n, len(ranks)
+        self.top = top or max(8, -(-max(list(ranks) + [1]) // 8) * 8)
+        ends = np.cumsum(counts).tolist()
+        self.seqs = list(zip([0] + ends[:-1], ends))
+        self.t = tokens or ends[-1] + extra
+        make = (lambda *s: rng.integers(-3, 4, s).astype(np.float16)) if integers else \
+            (lambda *s: rng.standard_normal(s).astype(np.float16))
+        self.x, self.base = make(self.t, k), make(self.t, n)
+        ad = max(self.ad, 1)
+        self.a, self.b = make(ad, self.top, k), make(ad, n, self.top)
+        if not integers:
+            self.a = (self.a * (k ** -0.5 * spread)).astype(np.float16)
+        for i, r in enumerate(self.ranks):
+            self.a[i, r:], self.b[i, :, r:] = np.nan, np.nan
+        self.scales = (rng.random(ad) + 0.5).astype(np.float32) if scales else np.ones(ad, np.float32)
+        self.dx, self.px = _padded(self.x, k + pad, rng)
+        self.dbase, self.pbase = _padded(self.base, n + pad, rng)
+        self.pad = pad
+        self.da, self.db = dev(self.a), dev(self.b)
+        self.dr, self.ds = dev(np.array(self.ranks + [0], np.int32)), dev(self.scales) if scales else None
+        self.off = dev(np.array([0] + ends, np.int32))
+        self.did = dev(np.array(self.ids, np.int32))
+        s = len(self.ids)
+        self.pb = batch.lora_plan_bytes(s, self.t, self.ad)
+        self.wb = batch.lora_workspace(self.t, self.top)
+        self.dplan, self.ws = dev(rng.integers(0, 256, self.pb).astype(np.uint8)), dev(np.full(self.wb, 0xFF, np.uint8))
+        self.out = empty((self.t, n + pad), np.float16)
+        self.out.fill_(np.float16(123.0).view(np.int16).item())
+
+    def plan(self, stream=0):
+        batch.lora_plan(self.off, self.did, len(self.ids), self.t, self.ad, self.dplan, self.pb, stream)
+
+    def run(self, base=True, out=None, ranks=True, stream=0):
+        batch.lora(self.px, self.da, self.db, self.out if out is None else out, self.dplan, self.pb, len(self.ids), self.t,
+                   self.ad, self.top, self.k, self.n, self.ws, self.wb, self.pbase if base else None,
+                   self.dr if ranks else None, self.ds, self.k + self.pad, self.n + self.pad, self.n + self.pad, stream)
+
+    def got(self, flat=None):
+        return (host(self.out, np.float16) if flat is None else flat)[:, :self.n]
+
+    def check(self, base=True, got=None):
+        got = self.got() if got is None else got
+        ref, tol = U.lora(self.x, self.a, self.b, self.ranks, self.scales, self.base if base else np.zeros_like(self.base),
+                          self.seqs, self.ids)
+        end = self.seqs[-1][1]
+        U.within(got[:end], ref[:end], tol[:end])
+        assert (got[end:] == np.float16(123.0)).all()  # rows of no sequence
+        if self.pad:
+            assert (host(self.out, np.float16)[:, self.n:] == np.float16(123.0)).all()
+        assert _err() == 0
+
+    def both(self, **kw):
+        self.plan()
+        self.run(**kw)
+        self.check(kw.get("base", True))
+
+
+@pytest.mark.parametrize("counts", [[1], [1] * 9, [1, 0, 3], [2, 5, 1, 8], [63], [64], [65], [200, 1, 0, 130], [7] * 40])
+@pytest.mark.parametrize("rank", [1, 8, 13, 16, 40, 64])
+def test_lora_counts_and_ranks(counts, rank):
+    rng = np.random.default_rng(rank * 100 + len(counts))
+    ids = [i % 3 for i in range(len(counts))]
+    Lora(counts, ids, [rank, max(1, rank // 2), rank], 128, 136, rng, extra=5, pad=8).both()
+
+
+@pytest.mark.parametrize("k", [8, 16, 24, 40, 64, 72, 200, 1024, 2056])
+@pytest.mark.parametrize("n", [8, 24, 64, 264, 1000])
+@pytest.mark.parametrize("counts", [[1, 1, 3], [90, 20]])
+def test_lora_features(k, n, counts):
+    rng = np.random.default_rng(k + n)
+    Lora(counts, [0, 1, 0][:len(counts)], [16, 5], k, n, rng).both()
+
+
+@pytest.mark.parametrize("rank,top", [(128, 128), (256, 256), (200, 256), (72, 72), (3, 256), (250, 256), (104, 104)])
+@pytest.mark.parametrize("counts", [[4], [150]])
+def test_lora_large_ranks(rank, top, counts):
+    rng = np.random.default_rng(rank)
+    Lora(counts, [0], [rank], 264, 200, rng, top=top).both()
+
+
+def test_lora_many_adapters_bare_sequences_and_none_at_all():
+    rng = np.random.default_rng(4)
+    ids = rng.integers(-1, 50, 300).tolist()
+    Lora(rng.integers(0, 4, 300).tolist(), ids, rng.integers(0, 20, 50).tolist(), 72, 96, rng, extra=3).both()
+    Lora([3, 4], [-1, -1], [8], 64, 64, rng, extra=2).both()
+    Lora([5, 80], [0, -1], [0], 64, 64, rng).both()        # an adapter of rank 0
+    call = Lora([5, 80], [-1, -1], [], 64, 64, rng)        # no adapters
+    call.both()
+    Lora([0, 0, 0], [0, 1, 0], [8, 8], 64, 64, rng, tokens=4).both()  # no rows
+    Lora([2] * 1500, (np.arange(1500) % 1200).tolist(), [8] * 1200, 64, 32, rng).both()
+    Lora([3, 70], [0, 1], [4, 8], 64, 64, rng, scales=False).both(base=False)
+
+
+def test_lora_in_place_and_without_ranks():
+    rng = np.random.default_rng(5)
+    for counts in ([1, 2, 1], [100, 3, 64]):
+        call = Lora(counts, [1, -1, 0], [16, 16], 96, 104, rng)
+        call.plan()
+        call.run(out=call.pbase, ranks=False)
+        call.check(got=host(call.dbase, np.float16)[:call.t * call.n].reshape(call.t, call.n))
+
+
+@pytest.mark.parametrize("counts", [[3], [120]])
+def test_lora_middle_product_keeps_its_bits(counts):
+    """Whole numbers whose middle product has 15 bits and more: every step is exact but the last rounding."""
+    rng = np.random.default_rng(6)
+    call = Lora(counts, [0], [24], 512, 80, rng, integers=True, scales=False)
+    call.x[:, ::2], call.a[0, :24, ::2] = 29, 31   # 256 * 899 = 230144 of 18 bits
+    call.b[0, :, 0] = 1 + call.b[0, :, 1]          # large parts that cancel
+    call.b[0, :, 2:24] = 0
+    call.b[0, :, 1] = -call.b[0, :, 0]
+    call.dx, call.px = _padded(call.x, 512, rng)
+    call.da, call.db = dev(call.a), dev(call.b)
+    call.plan()
+    call.run()
+    x, a, b = call.x.astype(np.float64), call.a[0, :24].astype(np.float64), call.b[0, :, :24].astype(np.float64)
+    want = (call.base.astype(np.float64) + (x @ a.T) @ b.T).astype(np.float16)
+    assert np.array_equal(call.got(), want)
+
+
+def test_lora_infinities_and_nan_stay_in_their_rows():
+    rng = np.random.default_rng(7)
+    for counts, ids in (([6, 6], [0, 1]), ([100, 90], [0, 1])):
+        call = Lora(counts, ids, [16, 8], 128, 72, rng)
+        x = call.x.copy()
+        x[2, 5], x[4, 100], x[counts[0] + 1] = np.nan, np.inf, 60000
+        call.x = x
+        call.dx, call.px = _padded(x, 128, rng)
+        call.plan()
+        call.run()
+        got = call.got()
+        rows = np.ones(call.t, bool)
+        rows[[2, 4]] = False
+        ref, tol = U.lora(call.x, call.a, call.b, call.ranks, call.scales, call.base, call.seqs, call.ids)
+        with np.errstate(over="ignore"):
+            over = np.abs(ref) + tol > 65504  # may be infinite
+        ok = np.abs(got[rows].astype(np.float64) - ref[rows]) <= tol[rows]
+        assert (ok | (over[rows] & (np.sign(got[rows]) == np.sign(ref[rows])))).all()
+        assert np.isnan(got[2]).all() and not np.isfinite(got[4]).any()
+
+
+def test_lora_refuses_lists_on_the_device():
+    """Offsets that fall or pass the tokens: no row; ids and ranks that are none: rows as without an adapter."""
+    rng = np.random.default_rng(8)
+    for off in ([0, 5, 3, 9], [0, 4, 8, 500], [-1, 3, 5, 9]):
+        call = Lora([3, 3, 3], [0, 1, 0], [8, 8], 64, 64, rng)
+        call.off = dev(np.array(off, np.int32))
+        call.plan()
+        call.run()
+        assert (call.got() == np.float16(123.0)).all() and _err() == 4
+    call = Lora([3, 3, 3], [0, 1, 2], [8, 8], 64, 64, rng)
+    call.ids = [0, 2, -2]
+    call.did = dev(np.array(call.ids, np.int32))
+    call.plan()
+    call.run()
+    assert _err() == 4
+    call.ids = [0, -1, -1]
+    call.check()
+    for rank in (9, -1):
+        call = Lora([3, 70], [0, 1], [8, 8], 64, 64, rng)
+        call.dr = dev(np.array([8, rank], np.int32))
+        call.plan()
+        call.run()
+        assert _err() == 4
+        call.ids = [0, -1]
+        call.check()
+    call = Lora([3, 3], [0, 1], [8, 8], 64, 64, rng)  # a plan of other numbers
+    call.plan()
+    call.did = dev(np.array([0, 1, 0], np.int32))
+    call.ids = [0, 1, 0]
+    call.pb = batch.lora_plan_bytes(3, call.t, 2)
+    call.dplan = torch().cat([call.dplan, call.dplan])
+    call.run()
+    assert (call.got() == np.float16(123.0)).all() and _err() == 4
+
+
+def test_lora_is_the_same_every_time_and_when_replayed():
+    """Bits of repeated calls, a captured plan and call whose adapters, offsets and inputs change, two streams."""
+    t = torch()
+    rng = np.random.default_rng(10)
+    for counts in ([1] * 20, [150, 1, 90, 3]):
+        ids = rng.integers(-1, 3, len(counts)).tolist()
+        call = Lora(counts, ids, [16, 8, 24], 512, 264, rng)
+        call.both()
+        first = call.got().view(np.uint16).copy()
+        for _ in range(10):
+            call.ws.fill_(255)
+            call.plan()
+            call.run()
+            assert np.array_equal(call.got().view(np.uint16), first)
+        t.cuda.synchronize()
+        graph = t.cuda.CUDAGraph()
+        with t.cuda.graph(graph):
+            stream = t.cuda.current_stream().cuda_stream
+            call.plan(stream)
+            call.run(stream=stream)
+        graph.replay()
+        call.check()
+        call.ids = [2 - max(i, 0) for i in call.ids]
+        call.did.copy_(t.tensor(call.ids, dtype=t.int32))
+        ends = np.cumsum(counts[::-1])
+        call.seqs = list(zip([0] + ends[:-1].tolist(), ends.tolist()))
+        call.off.copy_(t.tensor([0] + ends.tolist(), dtype=t.int32))
+        graph.replay()
+        call.check()
+    one, two = (Lora([40, 1, 9], [0, 1, 0], [16, 8], 256, 128, rng) for _ in range(2))
+    streams = t.cuda.Stream(), t.cuda.Stream()
+    t.cuda.synchronize()
+    for _ in range(20):
+        for call, stream in zip((one, two), streams):
+            call.plan(stream.cuda_stream)
+            call.run(stream=stream.cuda_stream)
+    t.cuda.synchronize()
+    one.check()
+    two.check()
+
+
+def test_lora_split_product_over_a_long_row():
+    rng = np.random.default_rng(11)
+    Lora([1], [0], [16], 16384, 64, rng).both()
+    Lora([1, 1], [0, 1], [64, 64], 8200, 64, rng).both()
+    Lora([130], [0], [64], 8200, 72, rng).both()
+
+
+# ---------------------------------------------------------------------------------------- logits
+class Logits:
+    def __init__(self, rows, vocab, rng, history=None, biases=None, masks=None, penalties=None, prompts=None, pad=0, opad=None,
+                 offset=0, mask_pad=0, x=None):
+        self.rows, self.v, self.pad, self.opad = rows, vocab, pad, pad if opad is None else opad
+        self.x = (rng.standard_normal((rows, vocab)) * 4).astype(np.float16) if x is None else x
+        self.histories = history
+        self.prompts = prompts if prompts is not None else ([0] * rows if history is not None else None)
+        self.penalties = penalties if penalties is not None else np.tile(np.float32([1.3, 0.25, 0.5]), (rows, 1))
+        if history is None:
+            self.penalties = None
+        self.biases, self.masks = biases, masks
+        self.dx, self.px = _padded(self.x, vocab + pad, rng, offset)
+        self.offset = offset
+        flat = np.full(offset + rows * (vocab + self.opad), 123.0, np.float16)
+        self.dout = dev(flat)
+        self.pout = self.dout.data_ptr() + 2 * offset
+        self.kw = {}
+        if history is not None:
+            flat = np.concatenate([np.asarray(h, np.uint32) for h in history] + [np.zeros(1, np.uint32)])
+            self.kw.update(penalties=dev(self.penalties), history=dev(flat),
+                           history_offsets=dev(np.cumsum([0] + [len(h) for h in history]).astype(np.int32)),
+                           num_history=flat.size - 1, prompt_lens=None if prompts is None else dev(np.array(prompts, np.int32)))
+        if biases is not None:
+            ids = np.array([i for b in biases for i, _ in b] + [0], np.uint32)
+            vals = np.array([v for b in biases for _, v in b] + [0], np.float32)
+            self.kw.update(bias_ids=dev(ids), bias_values=dev(vals), num_biases=ids.size - 1,
+                           bias_offsets=dev(np.cumsum([0] + [len(b) for b in biases]).astype(np.int32)))
+        if masks is not None:
+            words = -(-vocab // 32) + mask_pad
+            have = [m for m in masks if m is not None]
+            self.kw.update(masks=dev(np.stack([U.pack_bits(m, words) for m in have] + [np.zeros(words, np.uint32)])),
+                           mask_stride=words, num_masks=len(have))
+            at = iter(range(len(have)))
+            self.kw.update(mask_ids=dev(np.array([-1 if m is None else next(at) for m in masks], np.int32)))
+
+    def run(self, inplace=False, stream=0):
+        batch.logits_process(self.px, self.px if inplace else self.pout, self.rows, self.v, logits_stride=self.v + self.pad,
+                             output_stride=self.v + (self.pad if inplace else self.opad), stream=stream, **self.kw)
+        flat, pad = (self.dx, self.pad) if inplace else (self.dout, self.opad)
+        flat = host(flat, np.float16)[self.offset:self.offset + self.rows * (self.v + pad)].reshape(self.rows, -1)
+        if not inplace:
+            assert (flat[:, self.v:] == np.float16(123.0)).all()
+        return flat[:, :self.v]
+
+    def check(self, inplace=False, err=0):
+        got = self.run(inplace)
+        ref, tol = U.logits(self.x, self.penalties, self.histories, self.prompts, self.biases, self.masks)
+        U.within(got, ref, tol)
+        assert _err() == err
+        return got
+
+
+def _histories(rng, rows, vocab, lengths):
+    return [(rng.random(lengths[b % len(lengths)]) ** 3 * vocab).astype(np.int64) for b in range(rows)]
+
+
+def _biases(rng, rows, vocab, n):
+    return [[(int(i), float(v)) for i, v in zip(rng.integers(0, vocab, n), rng.standard_normal(n) * 3)] for _ in range(rows)]
+
+
+def _masks(rng, rows, vocab, free=0.3):
+    return [None if b % 3 == 1 else rng.random(vocab) < free for b in range(rows)]
+
+
+@pytest.mark.parametrize("vocab", [1, 7, 8, 31, 32, 33, 100, 1000, 4096, 4099, 20011, 32768, 65537, 151936])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_logits_all_together(vocab, rows):
+    rng = np.random.default_rng(vocab + rows)
+    call = Logits(rows, vocab, rng, _histories(rng, rows, vocab, [0, 300, 1, 77]), _biases(rng, rows, vocab, 9),
+                  _masks(rng, rows, vocab), prompts=[0, 100, 1, 20, 5][:rows])
+    call.check()
+
+
+@pytest.mark.parametrize("parts", ["h", "b", "m", "hb", "bm", "hm", ""])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_logits_parts(parts, inplace):
+    rng = np.random.default_rng(len(parts))
+    for vocab in (1001, 5000):
+        call = Logits(4, vocab, rng, _histories(rng, 4, vocab, [50, 200]) if "h" in parts else None,
+                      _biases(rng, 4, vocab, 20) if "b" in parts else None, _masks(rng, 4, vocab) if "m" in parts else None)
+        call.check(inplace)
+
+
+@pytest.mark.parametrize("pad,opad,offset", [(0, 0, 1), (8, 8, 0), (3, 3, 0), (8, 16, 0), (1, 0, 0), (0, 5, 2), (24, 24, 8)])
+def test_logits_strides_and_alignment(pad, opad, offset):
+    rng = np.random.default_rng(pad * 10 + offset)
+    for vocab in (2000, 9001):
+        def make():
+            return Logits(5, vocab, rng, _histories(rng, 5, vocab, [100, 30]), _biases(rng, 5, vocab, 7), _masks(rng, 5, vocab),
+                          pad=pad, opad=opad, offset=offset, mask_pad=3)
+        make().check()
+        make().check(inplace=True)
+
+
+def test_logits_penalties_of_all_kinds():
+    """Counts of one and of many, the prompt alone, negative penalties, logits of either sign, 0 and infinite."""
+    rng = np.random.default_rng(20)
+    vocab = 3000
+    x = (rng.standard_normal((7, vocab)) * 4).astype(np.float16)
+    x[:, 5], x[:, 6], x[:, 7], x[:, 8], x[:, 9] = 0, np.inf, -np.inf, np.nan, 60000
+    hist = [np.r_[np.arange(20), np.full(70000, 11), [vocab - 1]]] * 7
+    pen = np.float32([[1.5, 0.1, 0.2], [0.5, -0.5, -1], [1, 0, 0], [2, 0, 0], [1, 0.5, 0], [1, 0, 3], [1e-3, 100, 1000]])
+    call = Logits(7, vocab, rng, hist, penalties=pen, prompts=[0, 10, 70021, 70021, 15, 3, 21], x=x)
+    got = call.check()
+    assert np.isnan(got[:, 8]).all() and got[6, 9] == 65504 and got[6, 11] == -65504
+
+
+def test_logits_biases_of_one_token_and_of_extreme_values():
+    rng = np.random.default_rng(21)
+    b = [[(3, 1.0), (3, 2.0), (4, -np.inf), (5, np.inf), (6, 1e6), (7, -1e6), (999, 0.5), (3, -7.0)], [], [(0, 0.0)]]
+    got = Logits(3, 1000, rng, biases=b).check()
+    assert got[0, 4] == -np.inf and got[0, 5] == np.inf and got[0, 6] == 65504 and got[0, 7] == -65504
+
+
+def test_logits_masks_that_leave_nothing_or_everything_over_any_value():
+    rng = np.random.default_rng(22)
+    vocab = 5003
+    x = (rng.standard_normal((4, vocab)) * 4).astype(np.float16)
+    x[:, ::7], x[:, 1::7], x[:, 2::7] = np.nan, np.inf, -np.inf
+    one = np.zeros(vocab, bool)
+    one[vocab - 1] = True
+    masks = [np.zeros(vocab, bool), np.ones(vocab, bool), one, None]
+    got = Logits(4, vocab, rng, masks=masks, x=x).check()
+    assert (got[0] == -np.inf).all() and np.array_equal(got[1].view(np.uint16), x[1].view(np.uint16))
+    # without ids row i has mask i
+    call = Logits(3, vocab, rng, masks=masks[:3], x=x[:3].copy())
+    call.kw["mask_ids"] = None
+    call.check()
+    # the greedy choice of a masked row
+    call = Logits(1, vocab, rng, masks=[one])
+    call.run()
+    token = empty((1,), np.uint32)
+    cb.check(cb.lib().cactus_cuda_argmax_f16(call.pout, 1, vocab, token.data_ptr(), None))
+    assert host(token, np.uint32)[0] == vocab - 1
+
+
+def test_logits_refuses_lists_on_the_device():
+    """Ids past the vocabulary, offsets and mask ids that are none, penalties that are no factors: skipped, and said so."""
+    rng = np.random.default_rng(23)
+    call = Logits(2, 500, rng, [[1, 2, 500, 2 ** 32 - 1, 3], [4]], [[(7, 1.0), (500, 2.0)], [(2 ** 31, 1.0)]])
+    call.check(err=4)
+    for name, bad in (("history_offsets", [0, 9, 4]), ("history_offsets", [0, 2, 99]), ("history_offsets", [-3, -1, 0])):
+        call = Logits(2, 500, rng, [[1, 2], [3, 4, 5]])
+        call.kw[name] = dev(np.array(bad, np.int32))
+        call.run()
+        assert _err() == 4
+    call = Logits(2, 500, rng, biases=[[(1, 1.0)], [(2, 2.0)]])
+    call.kw["bias_offsets"] = dev(np.array([0, 1, 7], np.int32))
+    call.biases = [[(1, 1.0)], []]
+    call.check(err=4)
+    call = Logits(3, 500, rng, masks=_masks(rng, 3, 500))
+    call.kw["mask_ids"] = dev(np.array([0, 7, -2], np.int32))
+    call.masks = [call.masks[0], None, None]
+    call.check(err=4)
+    pen = np.float32([[0, 0.5, 0.5], [-1, 0, 0], [np.nan, 0, 1], [np.inf, 1, 0]])
+    Logits(4, 500, rng, [[1, 2, 3]] * 4, penalties=pen).check(err=4)
+
+
+def test_logits_replayed_with_other_lists():
+    t = torch()
+    rng = np.random.default_rng(24)
+    call = Logits(3, 10000, rng, _histories(rng, 3, 10000, [300]), masks=_masks(rng, 3, 10000))
+    call.check()
+    t.cuda.synchronize()
+    graph = t.cuda.CUDAGraph()
+    with t.cuda.graph(graph):
+        batch.logits_process(call.px, call.pout, 3, 10000, stream=t.cuda.current_stream().cuda_stream, **call.kw)
+    call.histories = _histories(rng, 3, 10000, [100, 5, 200])
+    flat = np.concatenate(call.histories).astype(np.int32)
+    call.kw["history"][:flat.size].copy_(t.from_numpy(flat))
+    call.kw["history_offsets"].copy_(t.tensor([0, 100, 105, 305], dtype=t.int32))
+    call.dout.fill_(0)
+    graph.replay()
+    got = host(call.dout, np.float16).reshape(3, -1)
+    U.within(got, *U.logits(call.x, call.penalties, call.histories, call.prompts, call.biases, call.masks))
+    assert _err() == 0
