@@ -1,5 +1,8 @@
 // Low-rank adapters of many requests: a plan that groups a batch's rows by adapter, then two products a
 // row with its adapter's matrices, the low-rank one in fp32 in the workspace between them.
+#include <algorithm>
+#include <atomic>
+
 #include "../common.cuh"
 #include "batch_ops.h"
 
@@ -18,12 +21,11 @@ enum { kHeadSeqs, kHeadTokens, kHeadAdapters, kHeadRows, kHeadTiles, kHeadBare, 
 __host__ __device__ inline long long most_tiles(long long seqs, long long tokens, long long adapters) {
     return tokens / kTileRows + (seqs < adapters ? seqs : adapters);
 }
-struct PlanView {
-    int4* tiles;
-    int *starts, *tile_starts, *cursors, *rows;
-    __host__ __device__ PlanView(int* p, long long seqs, long long tokens, long long adapters) {
-        tiles = reinterpret_cast<int4*>(p + kHeadInts);
-        starts = p + kHeadInts + 4 * most_tiles(seqs, tokens, adapters);
+// where the parts begin, in ints
+struct PlanLayout {
+    long long starts, tile_starts, cursors, rows;
+    __host__ __device__ PlanLayout(long long seqs, long long tokens, long long adapters) {
+        starts = kHeadInts + 4 * most_tiles(seqs, tokens, adapters);
         tile_starts = starts + adapters + 1;
         cursors = tile_starts + adapters + 2;
         rows = cursors + adapters + 1;
@@ -59,7 +61,10 @@ __global__ void __launch_bounds__(kPlanThreads)
     pdl_wait();
     __shared__ int warp_sums[kPlanThreads / 32], s_id[kPlanThreads], s_len[kPlanThreads], s_place[kPlanThreads];
     const int t = threadIdx.x;
-    const PlanView v(plan, num_seqs, num_tokens, num_adapters);
+    const PlanLayout at(num_seqs, num_tokens, num_adapters);
+    int4* tiles = reinterpret_cast<int4*>(plan + kHeadInts);
+    int *starts = plan + at.starts, *tile_starts = plan + at.tile_starts, *cursors = plan + at.cursors;
+    int* rows = plan + at.rows;
     int bad = 0;
     for (int b = t; b < num_seqs; b += kPlanThreads) bad |= offsets[b] < 0 || offsets[b] > offsets[b + 1];
     if (t == 0) bad |= offsets[num_seqs] > num_tokens;
@@ -77,39 +82,39 @@ __global__ void __launch_bounds__(kPlanThreads)
         report_dev_error(kDevBadList);
         return num_adapters;
     };
-    for (int a = t; a <= num_adapters; a += kPlanThreads) v.cursors[a] = 0;
+    for (int a = t; a <= num_adapters; a += kPlanThreads) cursors[a] = 0;
     __syncthreads();
-    for (int b = t; b < num_seqs; b += kPlanThreads) atomicAdd(&v.cursors[adapter_of(b)], offsets[b + 1] - offsets[b]);
+    for (int b = t; b < num_seqs; b += kPlanThreads) atomicAdd(&cursors[adapter_of(b)], offsets[b + 1] - offsets[b]);
     __syncthreads();
     int row0 = 0, tile0 = 0;
     for (int a0 = 0; a0 <= num_adapters; a0 += kPlanThreads) {
-        const int a = a0 + t, n = a <= num_adapters ? v.cursors[a] : 0;
+        const int a = a0 + t, n = a <= num_adapters ? cursors[a] : 0;
         int total = 0;
         const int start = row0 + block_scan(n, warp_sums, &total);
         row0 += total;
         const int tile = tile0 + block_scan(a < num_adapters ? (n + kTileRows - 1) / kTileRows : 0, warp_sums, &total);
         tile0 += total;
         if (a <= num_adapters) {
-            v.starts[a] = start;
-            v.tile_starts[a] = tile;
-            v.cursors[a] = start;
+            starts[a] = start;
+            tile_starts[a] = tile;
+            cursors[a] = start;
         }
     }
-    if (t == 0) v.tile_starts[num_adapters + 1] = tile0;
+    if (t == 0) tile_starts[num_adapters + 1] = tile0;
     __syncthreads();
     if (t < kHeadInts) {
-        const int rows = v.starts[num_adapters];
-        const int head[kHeadInts] = {num_seqs, num_tokens, num_adapters, rows, tile0, row0 - rows};
+        const int some = starts[num_adapters];
+        const int head[kHeadInts] = {num_seqs, num_tokens, num_adapters, some, tile0, row0 - some};
         plan[t] = head[t];
     }
     for (int i = t; i < tile0; i += kPlanThreads) {
         int lo = 0, hi = num_adapters;  // the last adapter whose tiles begin at or before i and that has any
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (v.tile_starts[mid] <= i) lo = mid; else hi = mid;
+            if (tile_starts[mid] <= i) lo = mid; else hi = mid;
         }
-        const int first = v.starts[lo] + (i - v.tile_starts[lo]) * kTileRows;
-        v.tiles[i] = make_int4(lo, first, min(kTileRows, v.starts[lo + 1] - first), 0);
+        const int first = starts[lo] + (i - tile_starts[lo]) * kTileRows;
+        tiles[i] = make_int4(lo, first, min(kTileRows, starts[lo + 1] - first), 0);
     }
     for (int b0 = 0; b0 < num_seqs; b0 += kPlanThreads) {
         const int b = b0 + t, n = min(kPlanThreads, num_seqs - b0);
@@ -122,94 +127,438 @@ __global__ void __launch_bounds__(kPlanThreads)
         s_len[t] = len;
         __syncthreads();
         if (t < n) {
-            place = v.cursors[id];
+            place = cursors[id];
             for (int j = 0; j < t; ++j) place += s_id[j] == id ? s_len[j] : 0;
             s_place[t] = place;
         }
         __syncthreads();
-        if (t < n) atomicAdd(&v.cursors[id], len);
+        if (t < n) atomicAdd(&cursors[id], len);
         for (int j = t >> 5; j < n; j += kPlanThreads / 32)
-            for (int i = t & 31; i < s_len[j]; i += 32) v.rows[s_place[j] + i] = offsets[b0 + j] + i;
+            for (int i = t & 31; i < s_len[j]; i += 32) rows[s_place[j] + i] = offsets[b0 + j] + i;
         __syncthreads();
     }
 }
 
 // ---------------------------------------------------------------- products
-__device__ __forceinline__ bool plan_fits(const LoraCall& c) {
-    return c.plan[kHeadSeqs] == c.num_seqs && c.plan[kHeadTokens] == c.num_tokens &&
-           c.plan[kHeadAdapters] == c.num_adapters;
+// Both products go tile by tile: up to 64 rows of one adapter. The first one's work is (tile, part of K):
+// few tiles are split over K, so that there are about two blocks for each SM, and each part leaves its fp32 sums
+// in the workspace [part][place][max_rank]. The second one adds the parts up in order.
+constexpr int kTargetBlocks = 2 * kNumSMs, kMostParts = 32, kLeastK = 256;
+
+__host__ __device__ inline int parts_of(int tiles, int k) {
+    int p = kTargetBlocks / (tiles > 0 ? tiles : 1);
+    p = p < k / kLeastK ? p : k / kLeastK;
+    p = p < kMostParts ? p : kMostParts;
+    return p > 1 ? p : 1;
+}
+
+struct Plan {
+    int tiles, rows, bare;
+    const int4* tile;
+    const int* row;
+};
+// false (and the error word raised) where the plan is of other numbers
+__device__ __forceinline__ bool open_plan(const LoraCall& c, Plan* p) {
+    const int4 head = __ldg(reinterpret_cast<const int4*>(c.plan)), more = __ldg(reinterpret_cast<const int4*>(c.plan) + 1);
+    if (head.x != c.num_seqs || head.y != c.num_tokens || head.z != c.num_adapters) {
+        report_dev_error(kDevBadList);
+        return false;
+    }
+    p->rows = head.w;
+    p->tiles = more.x;
+    p->bare = more.y;
+    p->tile = reinterpret_cast<const int4*>(c.plan + kHeadInts);
+    p->row = c.plan + PlanLayout(c.num_seqs, c.num_tokens, c.num_adapters).rows;
+    return true;
 }
 __device__ __forceinline__ int rank_of(const LoraCall& c, int adapter) {
-    const int r = c.ranks ? c.ranks[adapter] : c.max_rank;
+    const int r = c.ranks ? __ldg(c.ranks + adapter) : c.max_rank;
     if (r >= 0 && r <= c.max_rank) return r;
     report_dev_error(kDevBadList);
     return 0;
 }
-__device__ __forceinline__ int adapter_at(const LoraCall& c, const PlanView& v, int place) {
-    int lo = 0, hi = c.num_adapters;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (v.starts[mid] <= place) lo = mid; else hi = mid;
-    }
-    return lo;
+
+__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix_x2(uint32_t& r0, uint32_t& r1, uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(addr));
+}
+// 16 bytes global -> shared, zeros where `live` is false (nothing is read then)
+__device__ __forceinline__ void copy16_or_zero(uint32_t to, const void* from, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
 }
 
-// A block a row: each warp the dot products of every eighth row of A.
-__global__ void __launch_bounds__(256) lora_shrink_kernel(LoraCall c) {
+// 16 bytes that are read once
+__device__ __forceinline__ uint4 ldg_nc(const __half* p) {
+    const int4 v = ldg_nc_v4(p);
+    return make_uint4((unsigned)v.x, (unsigned)v.y, (unsigned)v.z, (unsigned)v.w);
+}
+
+// ---- x A^T
+constexpr int kThreads = 256, kWarps = kThreads / 32, kStages = 4, kChunk = 64;  // K elements a stage
+
+// Few rows (8 at most): the adapter's rows are the 16 rows of the product, the batch's its 8 columns. K is
+// free to be dealt out in any order, so a lane takes 8 consecutive elements of its row, one 16-byte load, as
+// its share of two steps; nothing passes through shared memory but the warps' sums.
+__device__ void shrink_few(const LoraCall& c, const Plan& p, const int4& tile, int rank, int k0, int k1, float* out) {
+    __shared__ float s_sum[kWarps][16 * 8];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+    const int blocks = (rank + 15) / 16;  // of 16 rows
+    int split = 1;                        // warps that share one over K
+    while (split * 2 * blocks <= kWarps) split *= 2;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    const __half* x = g < tile.z ? c.x + (long long)__ldg(p.row + tile.y + g) * c.x_stride : nullptr;
+    for (int u0 = 0; u0 < blocks * split; u0 += kWarps) {
+        const int u = u0 + warp, block = u / split, part = u % split;
+        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (u < blocks * split) {
+            const int r = block * 16 + g, steps = (k1 - k0 + 31) / 32;
+            const __half* a = c.a + ((long long)tile.x * c.max_rank + r) * c.k;
+            const int from = k0 + steps * part / split * 32, to = min(k1, k0 + steps * (part + 1) / split * 32);
+#pragma unroll 4
+            for (int k = from; k < to; k += 32) {
+                const int at = k + 8 * t;
+                const bool in = at < to;
+                const uint4 lo = in && r < rank ? ldg_nc(a + at) : zero;
+                const uint4 hi = in && r + 8 < rank ? ldg_nc(a + 8LL * c.k + at) : zero;
+                const uint4 v = in && x ? __ldg(reinterpret_cast<const uint4*>(x + at)) : zero;
+                mma_16816(d, lo.x, hi.x, lo.y, hi.y, v.x, v.y);
+                mma_16816(d, lo.z, hi.z, lo.w, hi.w, v.z, v.w);
+            }
+        }
+        if (split > 1) {
+            __syncthreads();
+            if (u < blocks * split) *reinterpret_cast<float4*>(&s_sum[warp][4 * lane]) = make_float4(d[0], d[1], d[2], d[3]);
+            __syncthreads();
+            if (u >= blocks * split || part) continue;
+            for (int i = 1; i < split; ++i) {
+                const float4 o = *reinterpret_cast<const float4*>(&s_sum[warp + i][4 * lane]);
+                d[0] += o.x, d[1] += o.y, d[2] += o.z, d[3] += o.w;
+            }
+        } else if (u >= blocks) {
+            continue;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = block * 16 + g + 8 * (i >> 1), row = 2 * t + (i & 1);
+            if (row < tile.z && r < c.max_rank) out[(long long)row * c.max_rank + r] = d[i];
+        }
+    }
+}
+
+// Many rows: both operands pass through a ring of shared-memory stages of 64 elements of K (128-byte rows, whose
+// 16-byte pieces are swapped about by the row's low bits); four warps have 16 of the tile's rows each, two such
+// fours half of the adapter's rows each.
+template <int RP>
+__device__ void shrink_many(const LoraCall& c, const Plan& p, const int4& tile, int rank, int k0, int k1, float* out,
+                            uint8_t* smem) {
+    constexpr int kStageBytes = (kTileRows + RP) * 2 * kChunk, kCols = RP / 2, kTilesN = kCols / 8;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m = warp & 3, half = warp >> 2;
+    const uint32_t base = smem_u32(smem);
+    const int piece = threadIdx.x & 7, row = threadIdx.x >> 3;  // a thread copies one piece of every 32nd row
+    const __half* xp[kTileRows / 32];
+#pragma unroll
+    for (int i = 0; i < kTileRows / 32; ++i)
+        xp[i] = row + 32 * i < tile.z ? c.x + (long long)__ldg(p.row + tile.y + row + 32 * i) * c.x_stride : nullptr;
+    const __half* ap = c.a + ((long long)tile.x * c.max_rank + row) * c.k;
+    const uint32_t to = base + row * 128 + ((piece ^ (row & 7)) << 4);
+    auto load = [&](int chunk, int stage) {
+        const int k = k0 + chunk * kChunk + piece * 8;
+        const uint32_t at = to + stage * kStageBytes;
+#pragma unroll
+        for (int i = 0; i < kTileRows / 32; ++i) copy16_or_zero(at + i * 32 * 128, xp[i] ? xp[i] + k : c.x, xp[i] && k < k1);
+#pragma unroll
+        for (int i = 0; i < (RP + 31) / 32; ++i)
+            if (RP >= 32 || row < RP) {
+                const bool live = row + 32 * i < rank && k < k1;
+                copy16_or_zero(at + (kTileRows + i * 32) * 128, live ? ap + (long long)i * 32 * c.k + k : c.a, live);
+            }
+    };
+    float d[kTilesN][4];
+#pragma unroll
+    for (int j = 0; j < kTilesN; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[j][i] = 0.0f;
+    const int chunks = (k1 - k0 + kChunk - 1) / kChunk;
+    __syncthreads();  // the stages of the tile before are read
+#pragma unroll
+    for (int i = 0; i < kStages - 1; ++i) {
+        if (i < chunks) load(i, i);
+        cp_async_commit();
+    }
+    const int xr = m * 16 + (lane & 15), br = kTileRows + half * kCols + (lane & 7) + ((lane >> 4) << 3);
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        cp_async_wait<kStages - 2>();
+        __syncthreads();
+        if (chunk + kStages - 1 < chunks) load(chunk + kStages - 1, (chunk + kStages - 1) % kStages);
+        cp_async_commit();
+        const uint32_t at = base + (chunk % kStages) * kStageBytes;
+#pragma unroll
+        for (int s = 0; s < kChunk / 16; ++s) {
+            uint32_t a[4];
+            ldmatrix_x4(a, at + xr * 128 + (((2 * s + (lane >> 4)) ^ (xr & 7)) << 4));
+            if constexpr (kTilesN == 1) {
+                uint32_t b0, b1;
+                const int r = kTileRows + half * kCols + (lane & 7);
+                ldmatrix_x2(b0, b1, at + r * 128 + (((2 * s + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
+                mma_16816(d[0], a[0], a[1], a[2], a[3], b0, b1);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kTilesN; j += 2) {
+                    uint32_t b[4];  // two blocks of 8 rows, both halves of the step
+                    const int r = br + j * 8;
+                    ldmatrix_x4(b, at + r * 128 + (((2 * s + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
+                    mma_16816(d[j], a[0], a[1], a[2], a[3], b[0], b[1]);
+                    mma_16816(d[j + 1], a[0], a[1], a[2], a[3], b[2], b[3]);
+                }
+            }
+        }
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int j = 0; j < kTilesN; ++j) {
+        const int r = half * kCols + j * 8 + 2 * (lane & 3);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int at = m * 16 + (lane >> 2) + 8 * i;
+            if (at < tile.z && r < c.max_rank)
+                *reinterpret_cast<float2*>(out + (long long)at * c.max_rank + r) = make_float2(d[j][2 * i], d[j][2 * i + 1]);
+        }
+    }
+}
+
+constexpr int kFewRows = 8;
+
+__global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(LoraCall c) {
+    extern __shared__ __align__(128) uint8_t smem[];
     pdl_launch_dependents();
     pdl_wait();
-    if (!plan_fits(c)) {
-        report_dev_error(kDevBadList);
+    Plan p;
+    if (!open_plan(c, &p)) return;
+    const int parts = parts_of(p.tiles, c.k);
+    const int chunks = (c.k + kChunk - 1) / kChunk;
+    for (int item = blockIdx.x; item < p.tiles * parts; item += gridDim.x) {
+        const int part = item % parts;
+        const int4 tile = __ldg(p.tile + item / parts);
+        const int rank = rank_of(c, tile.x);
+        const int k0 = (int)((long long)chunks * part / parts) * kChunk;
+        const int k1 = min(c.k, (int)((long long)chunks * (part + 1) / parts) * kChunk);
+        float* out = c.ws + ((long long)part * p.rows + tile.y) * c.max_rank;
+        if (rank == 0) continue;
+        if (tile.z <= kFewRows) shrink_few(c, p, tile, rank, k0, k1, out);
+        else if (rank <= 16) shrink_many<16>(c, p, tile, rank, k0, k1, out, smem);
+        else if (rank <= 32) shrink_many<32>(c, p, tile, rank, k0, k1, out, smem);
+        else if (rank <= 64) shrink_many<64>(c, p, tile, rank, k0, k1, out, smem);
+        else if (rank <= 128) shrink_many<128>(c, p, tile, rank, k0, k1, out, smem);
+        else shrink_many<256>(c, p, tile, rank, k0, k1, out, smem);
+    }
+}
+
+// ---- base + scale * h B^T
+// A tile's low-rank rows h go to shared memory once, as two fp16 numbers an element (h = 2^e (high + low), e by the
+// row's largest element, so that neither overflows and 22 bits are kept), and the block's warps take 32 outputs of
+// all 64 rows at a time. The columns of the products are dealt out so that a lane's are 8 consecutive outputs (one
+// 16-byte load and store a row), the steps over the rank so that a lane's elements of B are 4 consecutive ones.
+constexpr int kWarpCols = 32, kBlockCols = kWarps * kWarpCols;
+
+__host__ __device__ inline int padded_rank(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : r <= 128 ? 128 : 256; }
+__host__ __device__ inline int h_stride(int rp) { return 2 * rp + 8; }  // fp16 elements: high, low, padding against bank conflicts
+
+// Four threads a row; each has every fourth four of its elements.
+template <int RP>
+__device__ void load_h(const LoraCall& c, const Plan& p, const int4& tile, int rank, int parts, __half* s_h, float* s_scale) {
+    const int row = threadIdx.x >> 2, q = threadIdx.x & 3;
+    float v[RP / 16][4];
+    float top = 0.0f;
+    const float* from = c.ws + (long long)(tile.y + row) * c.max_rank;
+    const long long step = (long long)p.rows * c.max_rank;
+#pragma unroll
+    for (int i = 0; i < RP / 16; ++i) {
+        const int r = 16 * i + 4 * q;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (row < tile.z && r < rank) {
+            const float* at = from + r;
+            for (int part = 0; part < parts; ++part, at += step) {
+                const float4 h = __ldcg(reinterpret_cast<const float4*>(at));
+                sum.x += h.x, sum.y += h.y, sum.z += h.z, sum.w += h.w;
+            }
+        }
+        v[i][0] = sum.x, v[i][1] = sum.y, v[i][2] = sum.z, v[i][3] = sum.w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[i][j]));
+    }
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    // 2^e with the largest element below 2^12 of it; rows with infinities, NaN or nothing but zeros stay as they are
+    const int e = top > 0.0f && top < INFINITY ? max((int)(__float_as_uint(top) >> 23) - 127 - 11, -125) : 0;
+    const float down = __int_as_float((127 - e) << 23);
+    __half* to = s_h + row * h_stride(RP);
+#pragma unroll
+    for (int i = 0; i < RP / 16; ++i) {
+        __half hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float x = v[i][j] * down;
+            hi[j] = __float2half_rn(x);
+            const float rest = x - __half2float(hi[j]);
+            lo[j] = __float2half_rn(fabsf(x) < INFINITY ? rest : 0.0f);
+        }
+        const int r = 16 * i + 4 * q;
+        *reinterpret_cast<uint2*>(to + r) = *reinterpret_cast<const uint2*>(hi);
+        *reinterpret_cast<uint2*>(to + RP + r) = *reinterpret_cast<const uint2*>(lo);
+    }
+    if (q == 0) s_scale[row] = (c.scales ? __ldg(c.scales + tile.x) : 1.0f) * __int_as_float((127 + e) << 23);
+}
+
+// 32 outputs of up to 16 * MT rows, a warp.
+template <int RP, int MT>
+__device__ __forceinline__ void expand_warp(const LoraCall& c, const int4& tile, int rank, int n0, int row0,
+                                            const __half* s_h, const float* s_scale, const int* s_row) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, col = n0 + 8 * t;
+    uint4 y[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = row0 + m * 16 + g + 8 * i;
+            y[m][i] = make_uint4(0, 0, 0, 0);
+            if (c.base && row < tile.z && col < c.n)
+                y[m][i] = *reinterpret_cast<const uint4*>(c.base + (long long)s_row[row] * c.base_stride + col);
+        }
+    float d[MT][4][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[m][j][i] = 0.0f;
+    if (RP) {
+        const int steps = (rank + 15) / 16;
+        const __half* b = c.b + ((long long)tile.x * c.n + n0 + (g >> 1) * 8 + (g & 1)) * c.max_rank + 4 * t;
+        const bool live = n0 + (g >> 1) * 8 < c.n;  // its 8 outputs exist or do not
+#pragma unroll 4
+        for (int s = 0; s < steps; ++s) {
+            uint2 bv[4];
+            const int r = 16 * s + 4 * t, left = rank - r;  // elements that this lane has of the rank
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                bv[j] = make_uint2(0, 0);
+                if (live && left > 0) bv[j] = __ldg(reinterpret_cast<const uint2*>(b + (long long)2 * j * c.max_rank + 16 * s));
+                if (left < 4) {  // what follows the rank may hold anything
+                    bv[j].x = left >= 2 ? bv[j].x : left == 1 ? bv[j].x & 0xffffu : 0u;
+                    bv[j].y = left == 3 ? bv[j].y & 0xffffu : 0u;
+                }
+            }
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                const __half* h = s_h + (row0 + m * 16 + g) * h_stride(RP) + r;
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    const uint2 lo = *reinterpret_cast<const uint2*>(h + part * RP);
+                    const uint2 hi = *reinterpret_cast<const uint2*>(h + part * RP + 8 * h_stride(RP));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma_16816(d[m][j], lo.x, hi.x, lo.y, hi.y, bv[j].x, bv[j].y);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int row = row0 + m * 16 + g + 8 * i;
+            if (row >= tile.z || col >= c.n) continue;
+            uint4 out = y[m][i];
+            if (RP) {
+                const float scale = s_scale[row];
+                __half2* o = reinterpret_cast<__half2*>(&out);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 v = __half22float2(o[j]);
+                    o[j] = __floats2half2_rn(fmaf(scale, d[m][j][2 * i], v.x), fmaf(scale, d[m][j][2 * i + 1], v.y));
+                }
+            }
+            *reinterpret_cast<uint4*>(c.out + (long long)s_row[row] * c.out_stride + col) = out;
+        }
+}
+
+template <int RP>
+__device__ __forceinline__ void expand_rows(const LoraCall& c, const int4& tile, int rank, int n0, const __half* s_h,
+                                            const float* s_scale, const int* s_row) {
+    if (tile.z <= 16) expand_warp<RP, 1>(c, tile, rank, n0, 0, s_h, s_scale, s_row);
+    else
+        for (int row0 = 0; row0 < tile.z; row0 += 32) expand_warp<RP, 2>(c, tile, rank, n0, row0, s_h, s_scale, s_row);
+}
+
+__global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(LoraCall c) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ float s_scale[kTileRows];
+    __shared__ int s_row[kTileRows];
+    pdl_launch_dependents();
+    __half* s_h = reinterpret_cast<__half*>(smem);
+    Plan p;
+    if (!open_plan(c, &p)) {
+        pdl_wait();
         return;
     }
-    const PlanView v(const_cast<int*>(c.plan), c.num_seqs, c.num_tokens, c.num_adapters);
-    const int place = blockIdx.x, lane = threadIdx.x & 31;
-    if (place >= c.plan[kHeadRows]) return;
-    const int adapter = adapter_at(c, v, place), rank = rank_of(c, adapter);
-    const __half* x = c.x + v.rows[place] * c.x_stride;
-    for (int r = threadIdx.x >> 5; r < rank; r += 8) {
-        const __half* a = c.a + ((long long)adapter * c.max_rank + r) * c.k;
-        float sum = 0.0f;
-        for (int k = lane; k < c.k; k += 32) sum = fmaf(h2f(x[k]), h2f(a[k]), sum);
-        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        if (lane == 0) c.ws[(long long)place * c.max_rank + r] = sum;
-    }
-}
-
-// A thread an output of a row.
-__global__ void __launch_bounds__(256) lora_expand_kernel(LoraCall c) {
-    pdl_launch_dependents();
+    const int parts = parts_of(p.tiles, c.k), across = (c.n + kBlockCols - 1) / kBlockCols;
+    // rows without an adapter follow as tiles of rank 0, where they have to be copied
+    const int bare = c.base == c.out ? 0 : (p.bare + kTileRows - 1) / kTileRows;
+    const long long items = (long long)(p.tiles + bare) * across;
+    const long long first = items * blockIdx.x / gridDim.x, end = items * (blockIdx.x + 1) / gridDim.x;
     pdl_wait();
-    if (!plan_fits(c)) return;
-    const PlanView v(const_cast<int*>(c.plan), c.num_seqs, c.num_tokens, c.num_adapters);
-    const int place = blockIdx.x, n = blockIdx.y * 256 + threadIdx.x, rows = c.plan[kHeadRows];
-    if (place >= rows + c.plan[kHeadBare] || n >= c.n) return;
-    const long long row = v.rows[place];
-    float y = c.base ? h2f(c.base[row * c.base_stride + n]) : 0.0f;
-    if (place < rows) {
-        const int adapter = adapter_at(c, v, place), rank = rank_of(c, adapter);
-        const __half* b = c.b + ((long long)adapter * c.n + n) * c.max_rank;
-        const float* h = c.ws + (long long)place * c.max_rank;
-        float sum = 0.0f;
-        for (int r = 0; r < rank; ++r) sum = fmaf(h[r], h2f(b[r]), sum);
-        y = fmaf(c.scales ? c.scales[adapter] : 1.0f, sum, y);
+    int have = -1, rank = 0;
+    int4 tile = make_int4(0, 0, 0, 0);
+    for (long long item = first; item < end; ++item) {
+        const int at = (int)(item / across), n0 = (int)(item % across) * kBlockCols + (threadIdx.x >> 5) * kWarpCols;
+        if (at != have) {
+            have = at;
+            __syncthreads();  // the tile before is done with
+            if (at < p.tiles) {
+                tile = __ldg(p.tile + at);
+                rank = rank_of(c, tile.x);
+            } else {
+                const int i = (at - p.tiles) * kTileRows;
+                tile = make_int4(0, p.rows + i, min(kTileRows, p.bare - i), 0);
+                rank = 0;
+            }
+            if (threadIdx.x < tile.z) s_row[threadIdx.x] = __ldg(p.row + tile.y + threadIdx.x);
+            if (rank > 128) load_h<256>(c, p, tile, rank, parts, s_h, s_scale);
+            else if (rank > 64) load_h<128>(c, p, tile, rank, parts, s_h, s_scale);
+            else if (rank > 32) load_h<64>(c, p, tile, rank, parts, s_h, s_scale);
+            else if (rank > 16) load_h<32>(c, p, tile, rank, parts, s_h, s_scale);
+            else if (rank > 0) load_h<16>(c, p, tile, rank, parts, s_h, s_scale);
+            __syncthreads();
+        }
+        if (n0 >= c.n || (rank == 0 && c.base == c.out)) continue;
+        if (rank > 128) expand_rows<256>(c, tile, rank, n0, s_h, s_scale, s_row);
+        else if (rank > 64) expand_rows<128>(c, tile, rank, n0, s_h, s_scale, s_row);
+        else if (rank > 32) expand_rows<64>(c, tile, rank, n0, s_h, s_scale, s_row);
+        else if (rank > 16) expand_rows<32>(c, tile, rank, n0, s_h, s_scale, s_row);
+        else if (rank > 0) expand_rows<16>(c, tile, rank, n0, s_h, s_scale, s_row);
+        else expand_rows<0>(c, tile, rank, n0, s_h, s_scale, s_row);
     }
-    c.out[row * c.out_stride + n] = f2h(y);
 }
 
 }  // namespace
 
 size_t lora_plan_bytes(long long seqs, long long tokens, long long adapters) {
-    const PlanView v(nullptr, seqs, tokens, adapters);
-    const size_t ints = (size_t)(reinterpret_cast<uintptr_t>(v.rows) / 4) + (size_t)tokens;
+    const size_t ints = (size_t)(PlanLayout(seqs, tokens, adapters).rows + tokens);
     return (ints * 4 + 15) / 16 * 16;
 }
 
-// rows of the low-rank product, times the parts that a product over few tiles has
-constexpr int kTargetBlocks = 2 * kNumSMs, kMostParts = 32;
+// parts * rows is at most kMostParts * tokens, and where there is more than one part at most 64 rows a block
 size_t lora_workspace(long long tokens, int max_rank) {
-    const long long split = tokens * kMostParts < (long long)kTargetBlocks * kTileRows ? tokens * kMostParts
-                                                                                      : (long long)kTargetBlocks * kTileRows;
+    const long long many = tokens * kMostParts, few = (long long)kTargetBlocks * kTileRows, split = many < few ? many : few;
     return ((size_t)(tokens > split ? tokens : split) * (size_t)max_rank * 4 + 15) / 16 * 16 + 16;
 }
 
@@ -222,9 +571,28 @@ int launch_lora_plan(const int* offsets, const int* ids, int num_seqs, int num_t
 }
 
 int launch_lora(const LoraCall& c, cudaStream_t st) {
-    if (launch_k(lora_shrink_kernel, dim3((unsigned)c.num_tokens), dim3(256), 0, st, c) != cudaSuccess) return -1;
-    const dim3 grid((unsigned)c.num_tokens, (unsigned)((c.n + 255) / 256));
-    return launch_k(lora_expand_kernel, grid, dim3(256), 0, st, c) == cudaSuccess ? 0 : -1;
+    const int rp = padded_rank(c.max_rank);
+    const int shrink_smem = kStages * (kTileRows + rp) * 2 * kChunk, expand_smem = kTileRows * h_stride(rp) * 2;
+    static std::atomic<unsigned long long> set{0};  // a bit a device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!(set.load() >> (dev & 63) & 1)) {
+        if (cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kStages * (kTileRows + kLoraMaxRank) * 2 * kChunk) != cudaSuccess ||
+            cudaFuncSetAttribute(lora_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kTileRows * h_stride(kLoraMaxRank) * 2) != cudaSuccess)
+            return -1;
+        set.fetch_or(1ull << (dev & 63));
+    }
+    // as many blocks as the most tiles that there can be need, two for each SM at most
+    const long long tiles = most_tiles(c.num_seqs, c.num_tokens, c.num_adapters);
+    const long long shrink = std::min<long long>(kTargetBlocks, tiles * parts_of(1, c.k));
+    if (shrink > 0 && launch_k(lora_shrink_kernel, dim3((unsigned)shrink), dim3(kThreads), shrink_smem, st, c) != cudaSuccess)
+        return -1;
+    const long long across = (c.n + kBlockCols - 1) / kBlockCols;
+    const long long expand = std::min<long long>(kTargetBlocks, (tiles + (c.num_tokens + kTileRows - 1) / kTileRows) * across);
+    pdl_scope beside(shrink > 0);  // the second kernel starts while the first one ends, and waits for it
+    return launch_k(lora_expand_kernel, dim3((unsigned)expand), dim3(kThreads), expand_smem, st, c) == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace batch
