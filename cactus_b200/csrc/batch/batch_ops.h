@@ -37,6 +37,9 @@ struct LoraCall {
     float* ws;
 };
 int launch_lora(const LoraCall& c, cudaStream_t st);
+// lora_tc.cu: the second product for batches of many rows, ranks up to kLoraWideRank
+constexpr int kLoraWideRank = 128;
+int launch_lora_expand_wide(const LoraCall& c, cudaStream_t st);
 
 // logits.cu
 struct LogitsCall {

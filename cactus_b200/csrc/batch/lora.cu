@@ -5,6 +5,7 @@
 
 #include "../common.cuh"
 #include "batch_ops.h"
+#include "lora_plan.cuh"
 
 namespace cb {
 namespace batch {
@@ -12,26 +13,6 @@ namespace batch {
 namespace {
 
 // ---------------------------------------------------------------- plan
-// ints: header [16] | tiles [max_tiles][4] (adapter, first place, rows, 0) | starts [A + 1] | tile starts [A + 2]
-// | cursors [A + 1] | rows [num_tokens]: the batch's rows in order of their adapters, the batch's order
-// kept among those of one; rows without an adapter stand last.
-constexpr int kTileRows = 64;
-enum { kHeadSeqs, kHeadTokens, kHeadAdapters, kHeadRows, kHeadTiles, kHeadBare, kHeadInts = 16 };
-
-__host__ __device__ inline long long most_tiles(long long seqs, long long tokens, long long adapters) {
-    return tokens / kTileRows + (seqs < adapters ? seqs : adapters);
-}
-// where the parts begin, in ints
-struct PlanLayout {
-    long long starts, tile_starts, cursors, rows;
-    __host__ __device__ PlanLayout(long long seqs, long long tokens, long long adapters) {
-        starts = kHeadInts + 4 * most_tiles(seqs, tokens, adapters);
-        tile_starts = starts + adapters + 1;
-        cursors = tile_starts + adapters + 2;
-        rows = cursors + adapters + 1;
-    }
-};
-
 constexpr int kPlanThreads = 1024;
 
 // exclusive sum over the block, and the total
@@ -62,8 +43,8 @@ __global__ void __launch_bounds__(kPlanThreads)
     __shared__ int warp_sums[kPlanThreads / 32], s_id[kPlanThreads], s_len[kPlanThreads], s_place[kPlanThreads];
     const int t = threadIdx.x;
     const PlanLayout at(num_seqs, num_tokens, num_adapters);
-    int4* tiles = reinterpret_cast<int4*>(plan + kHeadInts);
-    int *starts = plan + at.starts, *tile_starts = plan + at.tile_starts, *cursors = plan + at.cursors;
+    int *starts = plan + at.starts, *tile_starts = plan + at.tile_starts, *wide_starts = plan + at.wide_starts;
+    int* cursors = plan + at.cursors;
     int* rows = plan + at.rows;
     int bad = 0;
     for (int b = t; b < num_seqs; b += kPlanThreads) bad |= offsets[b] < 0 || offsets[b] > offsets[b + 1];
@@ -86,7 +67,7 @@ __global__ void __launch_bounds__(kPlanThreads)
     __syncthreads();
     for (int b = t; b < num_seqs; b += kPlanThreads) atomicAdd(&cursors[adapter_of(b)], offsets[b + 1] - offsets[b]);
     __syncthreads();
-    int row0 = 0, tile0 = 0;
+    int row0 = 0, tile0 = 0, wide0 = 0;
     for (int a0 = 0; a0 <= num_adapters; a0 += kPlanThreads) {
         const int a = a0 + t, n = a <= num_adapters ? cursors[a] : 0;
         int total = 0;
@@ -94,28 +75,34 @@ __global__ void __launch_bounds__(kPlanThreads)
         row0 += total;
         const int tile = tile0 + block_scan(a < num_adapters ? (n + kTileRows - 1) / kTileRows : 0, warp_sums, &total);
         tile0 += total;
+        const int wide = wide0 + block_scan(a < num_adapters ? (n + kWideRows - 1) / kWideRows : 0, warp_sums, &total);
+        wide0 += total;
         if (a <= num_adapters) {
             starts[a] = start;
             tile_starts[a] = tile;
+            wide_starts[a] = wide;
             cursors[a] = start;
         }
     }
-    if (t == 0) tile_starts[num_adapters + 1] = tile0;
     __syncthreads();
     if (t < kHeadInts) {
         const int some = starts[num_adapters];
-        const int head[kHeadInts] = {num_seqs, num_tokens, num_adapters, some, tile0, row0 - some};
+        const int head[kHeadInts] = {num_seqs, num_tokens, num_adapters, some, tile0, row0 - some, wide0};
         plan[t] = head[t];
     }
-    for (int i = t; i < tile0; i += kPlanThreads) {
-        int lo = 0, hi = num_adapters;  // the last adapter whose tiles begin at or before i and that has any
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (tile_starts[mid] <= i) lo = mid; else hi = mid;
+    auto list = [&](int4* tiles, const int* first_of, int n, int height) {
+        for (int i = t; i < n; i += kPlanThreads) {
+            int lo = 0, hi = num_adapters;  // the last adapter whose tiles begin at or before i and that has any
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (first_of[mid] <= i) lo = mid; else hi = mid;
+            }
+            const int first = starts[lo] + (i - first_of[lo]) * height;
+            tiles[i] = make_int4(lo, first, min(height, starts[lo + 1] - first), 0);
         }
-        const int first = starts[lo] + (i - tile_starts[lo]) * kTileRows;
-        tiles[i] = make_int4(lo, first, min(kTileRows, starts[lo + 1] - first), 0);
-    }
+    };
+    list(reinterpret_cast<int4*>(plan + at.tiles), tile_starts, tile0, kTileRows);
+    list(reinterpret_cast<int4*>(plan + at.wide), wide_starts, wide0, kWideRows);
     for (int b0 = 0; b0 < num_seqs; b0 += kPlanThreads) {
         const int b = b0 + t, n = min(kPlanThreads, num_seqs - b0);
         int id = -1, len = 0, place = 0;
@@ -140,36 +127,11 @@ __global__ void __launch_bounds__(kPlanThreads)
 }
 
 // ---------------------------------------------------------------- products
-// Both products go tile by tile: up to 64 rows of one adapter. The first one's work is (tile, part of K):
-// few tiles are split over K, so that there are about two blocks for each SM, and each part leaves its fp32 sums
-// in the workspace [part][place][max_rank]. The second one adds the parts up in order.
-constexpr int kTargetBlocks = 2 * kNumSMs, kMostParts = 32, kLeastK = 256;
-
-__host__ __device__ inline int parts_of(int tiles, int k) {
-    int p = kTargetBlocks / (tiles > 0 ? tiles : 1);
-    p = p < k / kLeastK ? p : k / kLeastK;
-    p = p < kMostParts ? p : kMostParts;
-    return p > 1 ? p : 1;
-}
-
-struct Plan {
-    int tiles, rows, bare;
-    const int4* tile;
-    const int* row;
-};
-// false (and the error word raised) where the plan is of other numbers
+// Both products go tile by tile: up to 64 rows of one adapter. The first one's work is (tile, part of K).
 __device__ __forceinline__ bool open_plan(const LoraCall& c, Plan* p) {
-    const int4 head = __ldg(reinterpret_cast<const int4*>(c.plan)), more = __ldg(reinterpret_cast<const int4*>(c.plan) + 1);
-    if (head.x != c.num_seqs || head.y != c.num_tokens || head.z != c.num_adapters) {
-        report_dev_error(kDevBadList);
-        return false;
-    }
-    p->rows = head.w;
-    p->tiles = more.x;
-    p->bare = more.y;
-    p->tile = reinterpret_cast<const int4*>(c.plan + kHeadInts);
-    p->row = c.plan + PlanLayout(c.num_seqs, c.num_tokens, c.num_adapters).rows;
-    return true;
+    if (read_plan(c, p)) return true;
+    report_dev_error(kDevBadList);
+    return false;
 }
 __device__ __forceinline__ int rank_of(const LoraCall& c, int adapter) {
     const int r = c.ranks ? __ldg(c.ranks + adapter) : c.max_rank;
@@ -192,11 +154,9 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
 __device__ __forceinline__ void ldmatrix_x2(uint32_t& r0, uint32_t& r1, uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(addr));
 }
-// 16 bytes global -> shared, zeros where `live` is false (nothing is read then)
 __device__ __forceinline__ void copy16_or_zero(uint32_t to, const void* from, bool live) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+    copy_or_zero(to, from, live ? 16 : 0);
 }
-
 // 16 bytes that are read once
 __device__ __forceinline__ uint4 ldg_nc(const __half* p) {
     const int4 v = ldg_nc_v4(p);
@@ -398,25 +358,19 @@ __device__ void load_h(const LoraCall& c, const Plan& p, const int4& tile, int r
     }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // 2^e with the largest element below 2^12 of it; rows with infinities, NaN or nothing but zeros stay as they are
-    const int e = top > 0.0f && top < INFINITY ? max((int)(__float_as_uint(top) >> 23) - 127 - 11, -125) : 0;
-    const float down = __int_as_float((127 - e) << 23);
+    const int e = exponent_of(top);
+    const float down = two_to(-e);
     __half* to = s_h + row * h_stride(RP);
 #pragma unroll
     for (int i = 0; i < RP / 16; ++i) {
         __half hi[4], lo[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float x = v[i][j] * down;
-            hi[j] = __float2half_rn(x);
-            const float rest = x - __half2float(hi[j]);
-            lo[j] = __float2half_rn(fabsf(x) < INFINITY ? rest : 0.0f);
-        }
+        for (int j = 0; j < 4; ++j) two_halves(v[i][j] * down, &hi[j], &lo[j]);
         const int r = 16 * i + 4 * q;
         *reinterpret_cast<uint2*>(to + r) = *reinterpret_cast<const uint2*>(hi);
         *reinterpret_cast<uint2*>(to + RP + r) = *reinterpret_cast<const uint2*>(lo);
     }
-    if (q == 0) s_scale[row] = (c.scales ? __ldg(c.scales + tile.x) : 1.0f) * __int_as_float((127 + e) << 23);
+    if (q == 0) s_scale[row] = (c.scales ? __ldg(c.scales + tile.x) : 1.0f) * two_to(e);
 }
 
 // 32 outputs of up to 16 * MT rows, a warp.
@@ -500,7 +454,7 @@ __device__ __forceinline__ void expand_rows(const LoraCall& c, const int4& tile,
 }
 
 __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(LoraCall c) {
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float s_scale[kTileRows];
     __shared__ int s_row[kTileRows];
     pdl_launch_dependents();
@@ -570,6 +524,9 @@ int launch_lora_plan(const int* offsets, const int* ids, int num_seqs, int num_t
                : -1;
 }
 
+// From how many tokens on the second product is the wide tiles' kernel's.
+constexpr int kManyTokens = 512;
+
 int launch_lora(const LoraCall& c, cudaStream_t st) {
     const int rp = padded_rank(c.max_rank);
     const int shrink_smem = kStages * (kTileRows + rp) * 2 * kChunk, expand_smem = kTileRows * h_stride(rp) * 2;
@@ -592,6 +549,7 @@ int launch_lora(const LoraCall& c, cudaStream_t st) {
     const long long across = (c.n + kBlockCols - 1) / kBlockCols;
     const long long expand = std::min<long long>(kTargetBlocks, (tiles + (c.num_tokens + kTileRows - 1) / kTileRows) * across);
     pdl_scope beside(shrink > 0);  // the second kernel starts while the first one ends, and waits for it
+    if (c.num_tokens >= kManyTokens && c.max_rank <= kLoraWideRank) return launch_lora_expand_wide(c, st);
     return launch_k(lora_expand_kernel, dim3((unsigned)expand), dim3(kThreads), expand_smem, st, c) == cudaSuccess ? 0 : -1;
 }
 

@@ -1,0 +1,82 @@
+// The adapters' plan, as its kernel writes it and the products' kernels read it.
+#pragma once
+#include "../common.cuh"
+#include "batch_ops.h"
+
+namespace cb {
+namespace batch {
+
+// ints: header [16] | tiles [most_tiles(64)][4] (adapter, first place, rows, 0) | wide tiles, of up to 128 rows, the same
+// | starts [A + 1] | tile starts, wide ones [A + 2 each] | cursors [A + 1] | rows [num_tokens]: the batch's rows in order
+// of their adapters, the batch's order kept among those of one; rows without an adapter stand last.
+constexpr int kTileRows = 64, kWideRows = 128;
+enum { kHeadSeqs, kHeadTokens, kHeadAdapters, kHeadRows, kHeadTiles, kHeadBare, kHeadWide, kHeadInts = 16 };
+
+// every adapter that has rows can have one tile that is not full
+__host__ __device__ inline long long most_tiles(long long seqs, long long tokens, long long adapters, int rows = kTileRows) {
+    return tokens / rows + (seqs < adapters ? seqs : adapters);
+}
+// where the parts begin, in ints
+struct PlanLayout {
+    long long tiles, wide, starts, tile_starts, wide_starts, cursors, rows;
+    __host__ __device__ PlanLayout(long long seqs, long long tokens, long long adapters) {
+        tiles = kHeadInts;
+        wide = tiles + 4 * most_tiles(seqs, tokens, adapters);
+        starts = wide + 4 * most_tiles(seqs, tokens, adapters, kWideRows);
+        tile_starts = starts + adapters + 1;
+        wide_starts = tile_starts + adapters + 2;
+        cursors = wide_starts + adapters + 2;
+        rows = cursors + adapters + 1;
+    }
+};
+
+// Few tiles' first products are split over K, so that there are about two blocks for each SM; each part leaves its
+// fp32 sums in the workspace [part][place][max_rank], and the second product's kernel adds them up in order.
+constexpr int kTargetBlocks = 2 * kNumSMs, kMostParts = 32, kLeastK = 256;
+
+__host__ __device__ inline int parts_of(int tiles, int k) {
+    int p = kTargetBlocks / (tiles > 0 ? tiles : 1);
+    p = p < k / kLeastK ? p : k / kLeastK;
+    p = p < kMostParts ? p : kMostParts;
+    return p > 1 ? p : 1;
+}
+
+struct Plan {
+    int tiles, rows, bare, wide_tiles;
+    const int4 *tile, *wide;
+    const int* row;
+};
+// false where the plan is of other numbers
+__device__ __forceinline__ bool read_plan(const LoraCall& c, Plan* p) {
+    const int4 head = __ldg(reinterpret_cast<const int4*>(c.plan)), more = __ldg(reinterpret_cast<const int4*>(c.plan) + 1);
+    if (head.x != c.num_seqs || head.y != c.num_tokens || head.z != c.num_adapters) return false;
+    const PlanLayout at(c.num_seqs, c.num_tokens, c.num_adapters);
+    p->rows = head.w;
+    p->tiles = more.x;
+    p->bare = more.y;
+    p->wide_tiles = more.z;
+    p->tile = reinterpret_cast<const int4*>(c.plan + at.tiles);
+    p->wide = reinterpret_cast<const int4*>(c.plan + at.wide);
+    p->row = c.plan + at.rows;
+    return true;
+}
+
+// 2^e with a row's largest element below 2^12 of it; rows with infinities, NaN or nothing but zeros stay as they are
+__device__ __forceinline__ int exponent_of(float top) {
+    return top > 0.0f && top < INFINITY ? max((int)(__float_as_uint(top) >> 23) - 127 - 11, -125) : 0;
+}
+__device__ __forceinline__ float two_to(int e) { return __int_as_float((127 + e) << 23); }
+// x as two fp16 numbers; an infinity or a NaN is the first one
+__device__ __forceinline__ void two_halves(float x, __half* high, __half* low) {
+    *high = __float2half_rn(x);
+    const float rest = x - __half2float(*high);
+    *low = __float2half_rn(fabsf(x) < INFINITY ? rest : 0.0f);
+}
+
+// the first `bytes` of 16 bytes global -> shared, and zeros behind them (nothing is read where there are none)
+__device__ __forceinline__ void copy_or_zero(uint32_t to, const void* from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+
+}  // namespace batch
+}  // namespace cb

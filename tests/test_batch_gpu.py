@@ -371,6 +371,102 @@ def test_lora_split_product_over_a_long_row():
     Lora([130], [0], [64], 8200, 72, rng).both()
 
 
+# batches of many rows: tiles of 128, items ahead of one another
+@pytest.mark.parametrize("counts", [[512], [600], [511, 1], [128] * 4, [129, 0, 127, 300], [70] * 12, [1] * 700, [37] * 40,
+                                    [1500]])
+@pytest.mark.parametrize("rank", [1, 16, 40, 64, 100, 128])
+def test_lora_many_rows(counts, rank):
+    rng = np.random.default_rng(rank * 100 + len(counts))
+    ids = [(i * 5) % 4 - 1 for i in range(len(counts))] if len(counts) > 1 else [1]
+    Lora(counts, ids, [rank, max(1, rank // 2), rank], 128, 136, rng, extra=5, pad=8).both()
+
+
+@pytest.mark.parametrize("n", [8, 64, 120, 128, 136, 264, 2000])
+@pytest.mark.parametrize("k", [8, 200])
+@pytest.mark.parametrize("rank", [13, 72])
+def test_lora_many_rows_features(n, k, rank):
+    rng = np.random.default_rng(n + k + rank)
+    Lora([300, 40, 260, 5], [0, 1, -1, 0], [rank, 5], k, n, rng).both()
+    call = Lora([300, 40, 260, 5], [0, 1, -1, 0], [rank, 5], k, n, rng)
+    call.both(base=False)
+
+
+def test_lora_many_rows_of_many_adapters_and_of_few():
+    rng = np.random.default_rng(14)
+    ids = rng.integers(-1, 60, 400).tolist()
+    Lora(rng.integers(0, 9, 400).tolist(), ids, rng.integers(0, 65, 60).tolist(), 72, 96, rng, extra=3).both()
+    Lora(rng.integers(0, 9, 400).tolist(), ids, rng.integers(0, 129, 60).tolist(), 72, 200, rng, extra=3).both()
+    Lora([300, 400], [-1, -1], [8], 64, 64, rng, extra=2).both()
+    Lora([500, 80], [0, -1], [0], 64, 64, rng).both()
+    Lora([500, 80], [-1, -1], [], 64, 64, rng).both()
+    Lora([700, 3], [0, 1], [4, 200], 64, 320, rng).both()  # a rank past the wide tiles' kernel
+    for top in (64, 128):
+        call = Lora([100, 350, 164, 30], [1, -1, 0, 1], [top, 16], 96, 424, rng, top=top)
+        call.plan()
+        call.run(out=call.pbase)  # in place
+        call.check(got=host(call.dbase, np.float16)[:call.t * call.n].reshape(call.t, call.n))
+
+
+def test_lora_many_rows_keep_their_bits():
+    """As test_lora_middle_product_keeps_its_bits; and calls repeated, and replayed with other lists."""
+    rng = np.random.default_rng(15)
+    call = Lora([600], [0], [24], 512, 80, rng, integers=True, scales=False)
+    call.x[:, ::2], call.a[0, :24, ::2] = 29, 31
+    call.b[0, :, 0] = 1 + call.b[0, :, 1]
+    call.b[0, :, 2:24] = 0
+    call.b[0, :, 1] = -call.b[0, :, 0]
+    call.dx, call.px = _padded(call.x, 512, rng)
+    call.da, call.db = dev(call.a), dev(call.b)
+    call.plan()
+    call.run()
+    x, a, b = call.x.astype(np.float64), call.a[0, :24].astype(np.float64), call.b[0, :, :24].astype(np.float64)
+    assert np.array_equal(call.got(), (call.base.astype(np.float64) + (x @ a.T) @ b.T).astype(np.float16))
+    t = torch()
+    counts = [150, 1, 290, 3, 300, 65]
+    call = Lora(counts, [2, 1, 0, -1, 2, 0], [64, 8, 24], 512, 776, rng)
+    call.both()
+    first = call.got().view(np.uint16).copy()
+    for _ in range(20):
+        call.ws.fill_(255)
+        call.out.fill_(0)
+        call.run()
+        assert np.array_equal(call.got().view(np.uint16), first)
+    t.cuda.synchronize()
+    graph = t.cuda.CUDAGraph()
+    with t.cuda.graph(graph):
+        stream = t.cuda.current_stream().cuda_stream
+        call.plan(stream)
+        call.run(stream=stream)
+    for ids, order in (([0, 0, 1, 2, -1, 1], counts[::-1]), ([-1] * 6, counts), ([1] * 6, [0, 800, 0, 0, 9, 0])):
+        call.ids = ids
+        call.did.copy_(t.tensor(ids, dtype=t.int32))
+        ends = np.cumsum(order)
+        call.seqs = list(zip([0] + ends[:-1].tolist(), ends.tolist()))
+        call.off.copy_(t.tensor([0] + ends.tolist(), dtype=t.int32))
+        call.out.fill_(np.float16(123.0).view(np.int16).item())
+        for _ in range(3):
+            graph.replay()
+        call.check()
+
+
+def test_lora_many_rows_infinities_and_nan_stay_in_their_rows():
+    rng = np.random.default_rng(16)
+    call = Lora([300, 290], [0, 1], [64, 40], 128, 264, rng)
+    call.x[2, 5], call.x[290, 100], call.x[301] = np.nan, np.inf, 60000
+    call.dx, call.px = _padded(call.x, 128, rng)
+    call.plan()
+    call.run()
+    got = call.got()
+    rows = np.ones(call.t, bool)
+    rows[[2, 290]] = False
+    ref, tol = U.lora(call.x, call.a, call.b, call.ranks, call.scales, call.base, call.seqs, call.ids)
+    with np.errstate(over="ignore"):
+        over = np.abs(ref) + tol > 65504  # may be infinite
+    ok = np.abs(got[rows].astype(np.float64) - ref[rows]) <= tol[rows]
+    assert (ok | (over[rows] & (np.sign(got[rows]) == np.sign(ref[rows])))).all()
+    assert np.isnan(got[2]).all() and not np.isfinite(got[290]).any()
+
+
 # ---------------------------------------------------------------------------------------- logits
 class Logits:
     def __init__(self, rows, vocab, rng, history=None, biases=None, masks=None, penalties=None, prompts=None, pad=0, opad=None,
