@@ -164,7 +164,10 @@ __device__ __forceinline__ uint4 ldg_nc(const __half* p) {
 }
 
 // ---- x A^T
-constexpr int kThreads = 256, kWarps = kThreads / 32, kStages = 4, kChunk = 64;  // K elements a stage
+constexpr int kThreads = 256, kWarps = kThreads / 32, kChunk = 64;  // K elements a stage
+// stages of the ring for a padded rank: about 100 KB, so that an SM holds two blocks
+__host__ __device__ constexpr int stages_of(int rp) { return rp <= 64 ? 6 : rp <= 128 ? 4 : 3; }
+__host__ __device__ constexpr int ring_bytes(int rp) { return stages_of(rp) * (kTileRows + rp) * 2 * kChunk; }
 
 // Few rows (8 at most): the adapter's rows are the 16 rows of the product, the batch's its 8 columns. K is
 // free to be dealt out in any order, so a lane takes 8 consecutive elements of its row, one 16-byte load, as
@@ -221,7 +224,7 @@ __device__ void shrink_few(const LoraCall& c, const Plan& p, const int4& tile, i
 template <int RP>
 __device__ void shrink_many(const LoraCall& c, const Plan& p, const int4& tile, int rank, int k0, int k1, float* out,
                             uint8_t* smem) {
-    constexpr int kStageBytes = (kTileRows + RP) * 2 * kChunk, kCols = RP / 2, kTilesN = kCols / 8;
+    constexpr int kStages = stages_of(RP), kStageBytes = (kTileRows + RP) * 2 * kChunk, kCols = RP / 2, kTilesN = kCols / 8;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m = warp & 3, half = warp >> 2;
     const uint32_t base = smem_u32(smem);
     const int piece = threadIdx.x & 7, row = threadIdx.x >> 3;  // a thread copies one piece of every 32nd row
@@ -337,25 +340,12 @@ __host__ __device__ inline int h_stride(int rp) { return 2 * rp + 8; }  // fp16 
 template <int RP>
 __device__ void load_h(const LoraCall& c, const Plan& p, const int4& tile, int rank, int parts, __half* s_h, float* s_scale) {
     const int row = threadIdx.x >> 2, q = threadIdx.x & 3;
-    float v[RP / 16][4];
+    float4 v[RP / 16];
+    sum_parts<RP / 16>(c.ws + (long long)(tile.y + row) * c.max_rank + 4 * q, (long long)p.rows * c.max_rank, parts,
+                       row < tile.z ? rank - 4 * q : 0, v);
     float top = 0.0f;
-    const float* from = c.ws + (long long)(tile.y + row) * c.max_rank;
-    const long long step = (long long)p.rows * c.max_rank;
 #pragma unroll
-    for (int i = 0; i < RP / 16; ++i) {
-        const int r = 16 * i + 4 * q;
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (row < tile.z && r < rank) {
-            const float* at = from + r;
-            for (int part = 0; part < parts; ++part, at += step) {
-                const float4 h = __ldcg(reinterpret_cast<const float4*>(at));
-                sum.x += h.x, sum.y += h.y, sum.z += h.z, sum.w += h.w;
-            }
-        }
-        v[i][0] = sum.x, v[i][1] = sum.y, v[i][2] = sum.z, v[i][3] = sum.w;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[i][j]));
-    }
+    for (int i = 0; i < RP / 16; ++i) top = fmaxf(top, largest_of(v[i]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int e = exponent_of(top);
@@ -365,7 +355,7 @@ __device__ void load_h(const LoraCall& c, const Plan& p, const int4& tile, int r
     for (int i = 0; i < RP / 16; ++i) {
         __half hi[4], lo[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) two_halves(v[i][j] * down, &hi[j], &lo[j]);
+        for (int j = 0; j < 4; ++j) two_halves((&v[i].x)[j] * down, &hi[j], &lo[j]);
         const int r = 16 * i + 4 * q;
         *reinterpret_cast<uint2*>(to + r) = *reinterpret_cast<const uint2*>(hi);
         *reinterpret_cast<uint2*>(to + RP + r) = *reinterpret_cast<const uint2*>(lo);
@@ -529,19 +519,19 @@ constexpr int kManyTokens = 512;
 
 int launch_lora(const LoraCall& c, cudaStream_t st) {
     const int rp = padded_rank(c.max_rank);
-    const int shrink_smem = kStages * (kTileRows + rp) * 2 * kChunk, expand_smem = kTileRows * h_stride(rp) * 2;
+    const int shrink_smem = ring_bytes(rp), expand_smem = kTileRows * h_stride(rp) * 2;
     static std::atomic<unsigned long long> set{0};  // a bit a device
     int dev = 0;
     cudaGetDevice(&dev);
     if (!(set.load() >> (dev & 63) & 1)) {
         if (cudaFuncSetAttribute(lora_shrink_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 kStages * (kTileRows + kLoraMaxRank) * 2 * kChunk) != cudaSuccess ||
+                                 ring_bytes(kLoraMaxRank)) != cudaSuccess ||
             cudaFuncSetAttribute(lora_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  kTileRows * h_stride(kLoraMaxRank) * 2) != cudaSuccess)
             return -1;
         set.fetch_or(1ull << (dev & 63));
     }
-    // as many blocks as the most tiles that there can be need, two for each SM at most
+    // as many blocks as the most tiles that there can be need, one or two for each SM at most
     const long long tiles = most_tiles(c.num_seqs, c.num_tokens, c.num_adapters);
     const long long shrink = std::min<long long>(kTargetBlocks, tiles * parts_of(1, c.k));
     if (shrink > 0 && launch_k(lora_shrink_kernel, dim3((unsigned)shrink), dim3(kThreads), shrink_smem, st, c) != cudaSuccess)

@@ -30,9 +30,9 @@ struct PlanLayout {
     }
 };
 
-// Few tiles' first products are split over K, so that there are about two blocks for each SM; each part leaves its
+// Few tiles' first products are split over K, so that there is about a block for each SM; each part leaves its
 // fp32 sums in the workspace [part][place][max_rank], and the second product's kernel adds them up in order.
-constexpr int kTargetBlocks = 2 * kNumSMs, kMostParts = 32, kLeastK = 256;
+constexpr int kTargetBlocks = kNumSMs, kMostParts = 32, kLeastK = 256;
 
 __host__ __device__ inline int parts_of(int tiles, int k) {
     int p = kTargetBlocks / (tiles > 0 ? tiles : 1);
@@ -71,6 +71,28 @@ __device__ __forceinline__ void two_halves(float x, __half* high, __half* low) {
     *high = __float2half_rn(x);
     const float rest = x - __half2float(*high);
     *low = __float2half_rn(fabsf(x) < INFINITY ? rest : 0.0f);
+}
+
+// N fours of a row of the first product, 16 elements apart, as far as `left` goes: the sums of the parts, which lie
+// `step` apart. The loads of a part do not wait for one another.
+template <int N>
+__device__ __forceinline__ void sum_parts(const float* from, long long step, int parts, int left, float4 (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        v[i] = left > 16 * i ? __ldcg(reinterpret_cast<const float4*>(from + 16 * i)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 2
+    for (int part = 1; part < parts; ++part) {
+        from += step;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (left > 16 * i) {
+                const float4 h = __ldcg(reinterpret_cast<const float4*>(from + 16 * i));
+                v[i].x += h.x, v[i].y += h.y, v[i].z += h.z, v[i].w += h.w;
+            }
+    }
+}
+__device__ __forceinline__ float largest_of(const float4& v) {
+    return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
 }
 
 // the first `bytes` of 16 bytes global -> shared, and zeros behind them (nothing is read where there are none)

@@ -1,7 +1,7 @@
 // Low-rank adapters, many rows: base + scale * h B^T on tcgen05, h the low-rank product that lora.cu left in the
 // workspace. What an output costs is the base's element in and its own out, 4 bytes for 2 * rank operations, so all is
 // built to keep those moving: a persistent block for each SM goes over items of 128 rows of one adapter and 128 outputs.
-//   loaders   (4 warps) B's rows and the base's rows into a ring of stages, 16 bytes a copy, items ahead; for each new
+//   loaders   (8 warps) B's rows and the base's rows into a ring of stages, 16 bytes a copy, items ahead; for each new
 //             tile h as two fp16 numbers an element (h = 2^e (high + low), e by the row's largest element, so that
 //             neither overflows and 22 bits are kept), in the operands' swizzled layout;
 //   epilogue  (8 warps) sums from TMEM, a thread a row's 64 outputs; the results replace the base's elements in
@@ -19,7 +19,7 @@ namespace batch {
 namespace {
 
 constexpr int kCols = 128;
-constexpr int kLoaders = 4, kEpilogue = 8, kIssuer = kLoaders + kEpilogue, kThreads = (kIssuer + 1) * 32;
+constexpr int kLoaders = 8, kEpilogue = 8, kIssuer = kLoaders + kEpilogue, kThreads = (kIssuer + 1) * 32;
 constexpr int kLoadThreads = 32 * kLoaders;
 constexpr int kRowLists = 4;  // tiles whose rows' places are kept: more than the ring has items
 
@@ -199,9 +199,11 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_wide_kernel(const __g
                 ok = __all_sync(0xffffffffu, wait_or_abort(&empty[stage], (item / C::kStages - 1) & 1, abort));
             if (w.fresh) {
                 list = (list + 1) % kRowLists;
-                const long long row = tid < w.tile.z ? __ldg(p.row + w.tile.y + tid) : 0;
-                s_from[list][tid] = row * c.base_stride;
-                s_to[list][tid] = row * c.out_stride;
+                if (tid < kWideRows) {
+                    const long long row = tid < w.tile.z ? __ldg(p.row + w.tile.y + tid) : 0;
+                    s_from[list][tid] = row * c.base_stride;
+                    s_to[list][tid] = row * c.out_stride;
+                }
                 named_barrier<2, kLoadThreads>();
             }
             if (!ok) continue;
@@ -210,8 +212,9 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_wide_kernel(const __g
                 const __half* base = c.base + n0 + col;
                 uint32_t to = at_smem + C::kY + stage * C::kBytesY + row0 * C::kPitch + col * 2;
                 if (n0 + col < c.n)
-#pragma unroll 8
-                    for (int row = row0; row < w.tile.z; row += 8, to += 8 * C::kPitch) copy_or_zero(to, base + s_from[list][row], 16);
+#pragma unroll
+                    for (int row = 0; row < kWideRows; row += kLoadThreads / 16)
+                        if (row + row0 < w.tile.z) copy_or_zero(to + row * C::kPitch, base + s_from[list][row + row0], 16);
             }
             if (rank) {  // a thread copies one piece of every kStep-th row; what follows the rank is zeros
                 constexpr int kPieces = RP / 8, kStep = kLoadThreads / kPieces;
@@ -237,24 +240,14 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_wide_kernel(const __g
                 uint8_t* h0 = smem + slot * C::kBytesH;
                 const long long step = (long long)p.rows * c.max_rank;
 #pragma unroll 1
-                for (int pass = 0; pass < 4; ++pass) {
-                    const int row = pass * 32 + (tid >> 2), q = tid & 3;
-                    float v[RP / 16][4];
+                for (int pass = 0; pass < kWideRows * 4 / kLoadThreads; ++pass) {
+                    const int row = pass * (kLoadThreads / 4) + (tid >> 2), q = tid & 3;
+                    float4 v[RP / 16];
+                    sum_parts<RP / 16>(c.ws + (long long)(w.tile.y + row) * c.max_rank + 4 * q, step, parts,
+                                       row < w.tile.z ? rank - 4 * q : 0, v);
                     float top = 0.0f;
-                    const float* from = c.ws + (long long)(w.tile.y + row) * c.max_rank;
 #pragma unroll
-                    for (int i = 0; i < RP / 16; ++i) {
-                        const int r = 16 * i + 4 * q;
-                        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                        if (row < w.tile.z && r < rank)
-                            for (int part = 0; part < parts; ++part) {
-                                const float4 h = __ldcg(reinterpret_cast<const float4*>(from + part * step + r));
-                                sum.x += h.x, sum.y += h.y, sum.z += h.z, sum.w += h.w;
-                            }
-                        v[i][0] = sum.x, v[i][1] = sum.y, v[i][2] = sum.z, v[i][3] = sum.w;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(v[i][j]));
-                    }
+                    for (int i = 0; i < RP / 16; ++i) top = fmaxf(top, largest_of(v[i]));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     const int e = exponent_of(top);
@@ -263,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_wide_kernel(const __g
                     for (int i = 0; i < RP / 16; ++i) {
                         __half hi[4], lo[4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) two_halves(v[i][j] * down, &hi[j], &lo[j]);
+                        for (int j = 0; j < 4; ++j) two_halves((&v[i].x)[j] * down, &hi[j], &lo[j]);
                         const int piece = 2 * i + (q >> 1);
                         uint8_t* to = h0 + (piece >> 3) * (kWideRows * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4) + 8 * (q & 1);
                         *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(hi);
