@@ -142,7 +142,7 @@ __device__ __forceinline__ int rank_of(const LoraCall& c, int adapter) {
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                           uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -150,9 +150,6 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                  : "r"(addr));
-}
-__device__ __forceinline__ void ldmatrix_x2(uint32_t& r0, uint32_t& r1, uint32_t addr) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0,%1}, [%2];" : "=r"(r0), "=r"(r1) : "r"(addr));
 }
 __device__ __forceinline__ void copy16_or_zero(uint32_t to, const void* from, bool live) {
     copy_or_zero(to, from, live ? 16 : 0);
@@ -164,9 +161,9 @@ __device__ __forceinline__ uint4 ldg_nc(const __half* p) {
 }
 
 // ---- x A^T
-constexpr int kThreads = 256, kWarps = kThreads / 32, kChunk = 64;  // K elements a stage
-// stages of the ring for a padded rank: about 100 KB, so that an SM holds two blocks
-__host__ __device__ constexpr int stages_of(int rp) { return rp <= 64 ? 6 : rp <= 128 ? 4 : 3; }
+constexpr int kThreads = 256, kWarps = kThreads / 32, kChunk = 128;  // K elements a stage
+// stages of the ring for a padded rank: 60 to 160 KB
+__host__ __device__ constexpr int stages_of(int rp) { return rp <= 64 ? 4 : rp <= 128 ? 3 : 2; }
 __host__ __device__ constexpr int ring_bytes(int rp) { return stages_of(rp) * (kTileRows + rp) * 2 * kChunk; }
 
 // Few rows (8 at most): the adapter's rows are the 16 rows of the product, the batch's its 8 columns. K is
@@ -218,14 +215,18 @@ __device__ void shrink_few(const LoraCall& c, const Plan& p, const int4& tile, i
     }
 }
 
-// Many rows: both operands pass through a ring of shared-memory stages of 64 elements of K (128-byte rows, whose
-// 16-byte pieces are swapped about by the row's low bits); four warps have 16 of the tile's rows each, two such
-// fours half of the adapter's rows each.
+// Many rows: both operands pass through a ring of shared-memory stages of 128 elements of K (two blocks of 128-byte rows, whose
+// 16-byte pieces are swapped about by the row's low bits). What the matrix loads move bounds it, so a warp has 32 of
+// the tile's rows and up to 64 of the adapter's, and warps share the steps of a stage before they share those: 16 x 32
+// a warp read twice as much, and 9000 rows of 2048 took 19 us where this takes ____.
 template <int RP>
 __device__ void shrink_many(const LoraCall& c, const Plan& p, const int4& tile, int rank, int k0, int k1, float* out,
                             uint8_t* smem) {
-    constexpr int kStages = stages_of(RP), kStageBytes = (kTileRows + RP) * 2 * kChunk, kCols = RP / 2, kTilesN = kCols / 8;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m = warp & 3, half = warp >> 2;
+    constexpr int kStages = stages_of(RP), kBlockBytes = (kTileRows + RP) * 128, kBlocks = kChunk / 64, kStageBytes = kBlocks * kBlockBytes;
+    constexpr int kSplitK = RP <= 64 ? 4 : RP <= 128 ? 2 : 1, kSplitN = kWarps / 2 / kSplitK;
+    constexpr int kCols = RP / kSplitN, kTilesN = kCols / 8, kSteps = kChunk / 16 / kSplitK;  // of a warp
+    static_assert(kWarps * 2 * kTilesN * 512 <= kStages * kStageBytes, "the warps' sums fit into the ring");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, m = warp & 1, n = warp >> 1 & (kSplitN - 1), part = warp / (2 * kSplitN);
     const uint32_t base = smem_u32(smem);
     const int piece = threadIdx.x & 7, row = threadIdx.x >> 3;  // a thread copies one piece of every 32nd row
     const __half* xp[kTileRows / 32];
@@ -235,22 +236,27 @@ __device__ void shrink_many(const LoraCall& c, const Plan& p, const int4& tile, 
     const __half* ap = c.a + ((long long)tile.x * c.max_rank + row) * c.k;
     const uint32_t to = base + row * 128 + ((piece ^ (row & 7)) << 4);
     auto load = [&](int chunk, int stage) {
-        const int k = k0 + chunk * kChunk + piece * 8;
-        const uint32_t at = to + stage * kStageBytes;
 #pragma unroll
-        for (int i = 0; i < kTileRows / 32; ++i) copy16_or_zero(at + i * 32 * 128, xp[i] ? xp[i] + k : c.x, xp[i] && k < k1);
+        for (int block = 0; block < kBlocks; ++block) {
+            const int k = k0 + chunk * kChunk + block * 64 + piece * 8;
+            const uint32_t at = to + stage * kStageBytes + block * kBlockBytes;
 #pragma unroll
-        for (int i = 0; i < (RP + 31) / 32; ++i)
-            if (RP >= 32 || row < RP) {
-                const bool live = row + 32 * i < rank && k < k1;
-                copy16_or_zero(at + (kTileRows + i * 32) * 128, live ? ap + (long long)i * 32 * c.k + k : c.a, live);
-            }
+            for (int i = 0; i < kTileRows / 32; ++i) copy16_or_zero(at + i * 32 * 128, xp[i] ? xp[i] + k : c.x, xp[i] && k < k1);
+#pragma unroll
+            for (int i = 0; i < (RP + 31) / 32; ++i)
+                if (RP >= 32 || row < RP) {
+                    const bool live = row + 32 * i < rank && k < k1;
+                    copy16_or_zero(at + (kTileRows + i * 32) * 128, live ? ap + (long long)i * 32 * c.k + k : c.a, live);
+                }
+        }
     };
-    float d[kTilesN][4];
+    float d[2][kTilesN][4];
 #pragma unroll
-    for (int j = 0; j < kTilesN; ++j)
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[j][i] = 0.0f;
+        for (int j = 0; j < kTilesN; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[u][j][i] = 0.0f;
     const int chunks = (k1 - k0 + kChunk - 1) / kChunk;
     __syncthreads();  // the stages of the tile before are read
 #pragma unroll
@@ -258,50 +264,71 @@ __device__ void shrink_many(const LoraCall& c, const Plan& p, const int4& tile, 
         if (i < chunks) load(i, i);
         cp_async_commit();
     }
-    const int xr = m * 16 + (lane & 15), br = kTileRows + half * kCols + (lane & 7) + ((lane >> 4) << 3);
+    const int xr = m * 32 + (lane & 15), br = kTileRows + n * kCols + (lane & 7) + ((lane >> 4) << 3);
     for (int chunk = 0; chunk < chunks; ++chunk) {
         cp_async_wait<kStages - 2>();
         __syncthreads();
         if (chunk + kStages - 1 < chunks) load(chunk + kStages - 1, (chunk + kStages - 1) % kStages);
         cp_async_commit();
-        const uint32_t at = base + (chunk % kStages) * kStageBytes;
+        const uint32_t stage = base + (chunk % kStages) * kStageBytes;
 #pragma unroll
-        for (int s = 0; s < kChunk / 16; ++s) {
-            uint32_t a[4];
-            ldmatrix_x4(a, at + xr * 128 + (((2 * s + (lane >> 4)) ^ (xr & 7)) << 4));
-            if constexpr (kTilesN == 1) {
-                uint32_t b0, b1;
-                const int r = kTileRows + half * kCols + (lane & 7);
-                ldmatrix_x2(b0, b1, at + r * 128 + (((2 * s + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
-                mma_16816(d[0], a[0], a[1], a[2], a[3], b0, b1);
-            } else {
+        for (int i = 0; i < kSteps; ++i) {
+            const int step = part * kSteps + i, s = step & 3;
+            const uint32_t at = stage + (step >> 2) * kBlockBytes;
+            uint32_t a[2][4];
 #pragma unroll
-                for (int j = 0; j < kTilesN; j += 2) {
-                    uint32_t b[4];  // two blocks of 8 rows, both halves of the step
-                    const int r = br + j * 8;
-                    ldmatrix_x4(b, at + r * 128 + (((2 * s + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
-                    mma_16816(d[j], a[0], a[1], a[2], a[3], b[0], b[1]);
-                    mma_16816(d[j + 1], a[0], a[1], a[2], a[3], b[2], b[3]);
+            for (int u = 0; u < 2; ++u) ldmatrix_x4(a[u], at + (xr + u * 16) * 128 + (((2 * s + (lane >> 4)) ^ (xr & 7)) << 4));
+#pragma unroll
+            for (int j = 0; j < kTilesN; j += 2) {
+                uint32_t b[4];  // two blocks of 8 rows, both halves of the step
+                const int r = br + j * 8;
+                ldmatrix_x4(b, at + r * 128 + (((2 * s + ((lane >> 3) & 1)) ^ (r & 7)) << 4));
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    mma_16816(d[u][j], a[u][0], a[u][1], a[u][2], a[u][3], b[0], b[1]);
+                    mma_16816(d[u][j + 1], a[u][0], a[u][1], a[u][2], a[u][3], b[2], b[3]);
                 }
             }
         }
     }
     cp_async_wait<0>();
+    if (kSplitK > 1) {  // the sums of the warps that had the first steps, and after them those of the others
+        __syncthreads();  // all stages are read
+        float4* sums = reinterpret_cast<float4*>(smem) + lane;
+        if (part)
 #pragma unroll
-    for (int j = 0; j < kTilesN; ++j) {
-        const int r = half * kCols + j * 8 + 2 * (lane & 3);
+            for (int j = 0; j < 2 * kTilesN; ++j) {
+                const float* v = d[j / kTilesN][j % kTilesN];
+                sums[(warp * 2 * kTilesN + j) * 32] = make_float4(v[0], v[1], v[2], v[3]);
+            }
+        __syncthreads();
+        if (part) return;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int at = m * 16 + (lane >> 2) + 8 * i;
-            if (at < tile.z && r < c.max_rank)
-                *reinterpret_cast<float2*>(out + (long long)at * c.max_rank + r) = make_float2(d[j][2 * i], d[j][2 * i + 1]);
-        }
+        for (int other = 1; other < kSplitK; ++other)
+#pragma unroll
+            for (int j = 0; j < 2 * kTilesN; ++j) {
+                const float4 o = sums[((warp + other * 2 * kSplitN) * 2 * kTilesN + j) * 32];
+                float* v = d[j / kTilesN][j % kTilesN];
+                v[0] += o.x, v[1] += o.y, v[2] += o.z, v[3] += o.w;
+            }
     }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < kTilesN; ++j) {
+            const int r = n * kCols + j * 8 + 2 * (lane & 3);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int at = m * 32 + u * 16 + (lane >> 2) + 8 * i;
+                if (at < tile.z && r < c.max_rank)
+                    *reinterpret_cast<float2*>(out + (long long)at * c.max_rank + r) = make_float2(d[u][j][2 * i], d[u][j][2 * i + 1]);
+            }
+        }
 }
 
 constexpr int kFewRows = 8;
 
-__global__ void __launch_bounds__(kThreads, 2) lora_shrink_kernel(LoraCall c) {
+__global__ void __launch_bounds__(kThreads, 1) lora_shrink_kernel(LoraCall c) {
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_launch_dependents();
     pdl_wait();
