@@ -39,7 +39,7 @@ struct LoraCall {
 int launch_lora(const LoraCall& c, cudaStream_t st);
 // lora_tc.cu: the second product for batches of many rows, ranks up to kLoraWideRank
 constexpr int kLoraWideRank = 128;
-int launch_lora_expand_wide(const LoraCall& c, cudaStream_t st);
+int launch_lora_expand_wide(const LoraCall& c, unsigned* error_word, cudaStream_t st);
 
 // logits.cu
 struct LogitsCall {

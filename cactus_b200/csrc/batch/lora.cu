@@ -541,6 +541,15 @@ int launch_lora_plan(const int* offsets, const int* ids, int num_seqs, int num_t
                : -1;
 }
 
+// The device error word's address on the current device, for the kernel that is compiled by itself.
+unsigned* error_word(int dev) {
+    static std::atomic<unsigned*> known[64];
+    unsigned* p = known[dev & 63].load();
+    void* at = nullptr;
+    if (!p && cudaGetSymbolAddress(&at, g_dev_error) == cudaSuccess) known[dev & 63].store(p = static_cast<unsigned*>(at));
+    return p;
+}
+
 // From how many tokens on the second product is the wide tiles' kernel's.
 constexpr int kManyTokens = 512;
 
@@ -566,7 +575,7 @@ int launch_lora(const LoraCall& c, cudaStream_t st) {
     const long long across = (c.n + kBlockCols - 1) / kBlockCols;
     const long long expand = std::min<long long>(kTargetBlocks, (tiles + (c.num_tokens + kTileRows - 1) / kTileRows) * across);
     pdl_scope beside(shrink > 0);  // the second kernel starts while the first one ends, and waits for it
-    if (c.num_tokens >= kManyTokens && c.max_rank <= kLoraWideRank) return launch_lora_expand_wide(c, st);
+    if (c.num_tokens >= kManyTokens && c.max_rank <= kLoraWideRank) return launch_lora_expand_wide(c, error_word(dev), st);
     return launch_k(lora_expand_kernel, dim3((unsigned)expand), dim3(kThreads), expand_smem, st, c) == cudaSuccess ? 0 : -1;
 }
 

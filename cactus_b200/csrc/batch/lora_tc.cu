@@ -388,7 +388,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_wide_kernel(const __g
 }
 
 template <int RP>
-int launch(const LoraCall& c, cudaStream_t st) {
+int launch(const LoraCall& c, unsigned* error_word, cudaStream_t st) {
     using C = Cfg<RP>;
     static std::atomic<unsigned long long> set{0};  // a bit a device
     int dev = 0;
@@ -398,7 +398,7 @@ int launch(const LoraCall& c, cudaStream_t st) {
             return -1;
         set.fetch_or(1ull << (dev & 63));
     }
-    Args a = {c, dev_error_ptr()};
+    Args a = {c, error_word};
     if (!a.err) return -1;
     const long long tiles = most_tiles(c.num_seqs, c.num_tokens, c.num_adapters, kWideRows) + (c.num_tokens + kWideRows - 1) / kWideRows;
     const long long items = tiles * ((c.n + kCols - 1) / kCols);
@@ -410,7 +410,9 @@ int launch(const LoraCall& c, cudaStream_t st) {
 
 }  // namespace
 
-int launch_lora_expand_wide(const LoraCall& c, cudaStream_t st) { return c.max_rank <= 64 ? launch<64>(c, st) : launch<128>(c, st); }
+int launch_lora_expand_wide(const LoraCall& c, unsigned* error_word, cudaStream_t st) {
+    return c.max_rank <= 64 ? launch<64>(c, error_word, st) : launch<128>(c, error_word, st);
+}
 
 }  // namespace batch
 }  // namespace cb

@@ -7,9 +7,10 @@
  *
  * Conventions are those of cactus_b200.h: DEVICE pointers, fp16 as uint16_t bits, asynchronous calls on
  * `stream`, 0 or a negative code with a message in cactus_cuda_last_error(). Nothing here allocates, and
- * every call can be captured in a CUDA graph. Strides are in elements. Lists, lengths and ids are read on
+ * every call can be captured in a CUDA graph (after a first call of the same kind outside of it on that
+ * device, which sets kernel attributes). Strides are in elements. Lists, lengths and ids are read on
  * the device; what they name outside the arguments is skipped and raises the device error word
- * (cactus_cuda_device_error() == 4). Calls of any sizes of zero do nothing.
+ * (cactus_cuda_device_error() == 4). Calls with a size of zero do nothing.
  */
 #ifndef CACTUS_B200_BATCH_H
 #define CACTUS_B200_BATCH_H

@@ -604,6 +604,18 @@ def test_logits_masks_that_leave_nothing_or_everything_over_any_value():
     assert host(token, np.uint32)[0] == vocab - 1
 
 
+@pytest.mark.parametrize("rows,vocab", [(1, 6000), (2, 40000), (300, 20000)])
+def test_logits_of_many_named_tokens(rows, vocab):
+    """More tokens of one slice in the lists than are counted at a time; every token, named by history or biases."""
+    rng = np.random.default_rng(25)
+    every = rng.permutation(vocab)
+    hist = [np.r_[every[:vocab * 4 // 5], every[:50]] if b % 3 == 0 else every[:b + 1] for b in range(rows)]
+    bias = [[(int(i), float(i % 7) - 3.0) for i in (every[::2] if b % 3 == 0 else every[:5])] for b in range(rows)]
+    call = Logits(rows, vocab, rng, hist, bias, _masks(rng, rows, vocab, 0.7), prompts=[(b * 37) % 4000 for b in range(rows)])
+    call.check()
+    call.check(inplace=True)
+
+
 def test_logits_refuses_lists_on_the_device():
     """Ids past the vocabulary, offsets and mask ids that are none, penalties that are no factors: skipped, and said so."""
     rng = np.random.default_rng(23)
