@@ -44,25 +44,19 @@ __device__ __forceinline__ unsigned mask8(const uint32_t* mask, int v, int words
     return bits & 0xffu;
 }
 
-// A row's list as two passes go through it: a thread's first ids stay in registers in between.
-template <int T>
-struct Ids {
-    static constexpr int kHeld = 3;
-    const uint32_t* ids;
-    int count;
-    unsigned held[kHeld];
-    __device__ __forceinline__ void load() {
+// Each id of a list, with its place there.
+template <int T, typename F>
+__device__ __forceinline__ void each(const uint32_t* ids, int count, F f) {
+    constexpr int kAhead = 4;  // loads in flight
+    for (int i0 = threadIdx.x; i0 < count; i0 += T * kAhead) {
+        unsigned id[kAhead];
 #pragma unroll
-        for (int k = 0; k < kHeld; ++k) held[k] = (int)threadIdx.x + k * T < count ? __ldg(ids + threadIdx.x + k * T) : 0u;
-    }
-    template <typename F>
-    __device__ __forceinline__ void each(F f) const {  // f(id, its place)
+        for (int k = 0; k < kAhead; ++k) id[k] = i0 + k * T < count ? __ldg(ids + i0 + k * T) : 0xffffffffu;
 #pragma unroll
-        for (int k = 0; k < kHeld; ++k)
-            if ((int)threadIdx.x + k * T < count) f(held[k], (int)threadIdx.x + k * T);
-        for (int i = threadIdx.x + kHeld * T; i < count; i += T) f(__ldg(ids + i), i);
+        for (int k = 0; k < kAhead; ++k)
+            if (i0 + k * T < count) f(id[k], i0 + k * T);
     }
-};
+}
 
 // Pieces begin where the input's 16-byte units do: piece i of a row has its tokens 8 i - skew to 8 i - skew + 7, as
 // far as there are such.
@@ -117,9 +111,7 @@ __global__ void __launch_bounds__(T, T == 512 ? 3 : 1) logits_kernel(LogitsCall 
     List history = {0, 0}, biases = {0, 0};
     if (c.penalties) history = list_of(c.history_offsets, row, c.num_history);
     if (c.bias_ids) biases = list_of(c.bias_offsets, row, c.num_biases);
-    Ids<T> ids = {c.history + history.first, history.count}, bias_ids = {c.bias_ids + biases.first, biases.count};
-    ids.load();
-    bias_ids.load();
+    const uint32_t *ids = c.history + history.first, *bias_ids = c.bias_ids + biases.first;
     const bool lists = history.count + biases.count > 0;
     // the slice's tokens among the ids; one before the slice wraps around
     auto inside = [&](unsigned id) { return id - (unsigned)v0 < (unsigned)S::kTokens && id < (unsigned)c.vocab; };
@@ -131,17 +123,13 @@ __global__ void __launch_bounds__(T, T == 512 ? 3 : 1) logits_kernel(LogitsCall 
         auto note = [&](unsigned id, int) {
             const unsigned at = id - (unsigned)v0;
             if (inside(id)) {
-                if (!(atomicOr(&s_bits[at >> 5], 1u << (at & 31)) >> (at & 31) & 1u)) {
-                    const int n = atomicAdd(&s_noted, 1);
-                    s_number[at] = (uint16_t)n;
-                    if (n < kRound) s_list[n] = (uint16_t)at;
-                }
+                if (!(atomicOr(&s_bits[at >> 5], 1u << (at & 31)) >> (at & 31) & 1u)) s_number[at] = (uint16_t)atomicAdd(&s_noted, 1);
             } else if (id >= (unsigned)c.vocab) {
                 report_dev_error(kDevBadList);
             }
         };
-        ids.each(note);
-        bias_ids.each(note);
+        each<T>(ids, history.count, note);
+        each<T>(bias_ids, biases.count, note);
     }
     // the pass over the slice
     const __half none = __ushort_as_half(0xFC00);
@@ -181,40 +169,28 @@ __global__ void __launch_bounds__(T, T == 512 ? 3 : 1) logits_kernel(LogitsCall 
         __syncthreads();  // the pass has written what the results replace; numbers and zeros are there
         const int noted = min(s_noted - first, kRound);
         if (noted <= 0) break;
-        constexpr int kEach = kRound / T;  // noted tokens of a thread
-        __half logit[kEach];
-        auto fetch = [&] {
-#pragma unroll
-            for (int k = 0; k < kEach; ++k)
-                if ((int)threadIdx.x + k * T < noted) logit[k] = in[v0 + s_list[threadIdx.x + k * T]];
-        };
-        if (first == 0) fetch();  // on their way while the tokens are counted; later rounds' lists are made below
         auto number = [&](unsigned id) { return inside(id) ? (unsigned)s_number[id - (unsigned)v0] - (unsigned)first : 0xffffffffu; };
-        ids.each([&](unsigned id, int i) {
+        each<T>(ids, history.count, [&](unsigned id, int i) {
             const unsigned n = number(id);
             if (n >= (unsigned)kRound) return;
-            if (first) s_list[n] = (uint16_t)(id - (unsigned)v0);
+            s_list[n] = (uint16_t)(id - (unsigned)v0);
             if (i >= prompt) atomicAdd(&s_count[n], 1u);
             atomicOr(&s_count[n], kSeen);
         });
-        bias_ids.each([&](unsigned id, int i) {
+        each<T>(bias_ids, biases.count, [&](unsigned id, int i) {
             const unsigned n = number(id);
             if (n >= (unsigned)kRound) return;
-            if (first) s_list[n] = (uint16_t)(id - (unsigned)v0);
+            s_list[n] = (uint16_t)(id - (unsigned)v0);
             atomicMax(&s_bias[n], i + 1);
         });
         __syncthreads();
-        if (first) fetch();
-#pragma unroll
-        for (int k = 0; k < kEach; ++k) {
-            const int i = threadIdx.x + k * T;
-            if (i >= noted) break;
+        for (int i = threadIdx.x; i < noted; i += T) {
             const int v = v0 + s_list[i];
             const unsigned n = s_count[i];
             const int bias = s_bias[i];
             s_count[i] = 0, s_bias[i] = 0;  // for the next round
             if (mask && !(__ldg(mask + (v >> 5)) >> (v & 31) & 1u)) continue;
-            float l = h2f(logit[k]);
+            float l = h2f(in[v]);
             if (n) {
                 l = l > 0.0f ? __fdiv_rn(l, repetition) : __fmul_rn(l, repetition);
                 const unsigned made = n & ~kSeen;
