@@ -120,30 +120,26 @@ __device__ __forceinline__ uint4 norm_and_turn(const uint4& in, const uint4& wei
     return out;
 }
 
-// Eight elements of a row into its block: codes, and the parameters of their group. All lanes take part; `codes` and
-// `pair` are where the lane's go, null where nothing does.
-__device__ __forceinline__ void quantise_eight(const uint4& x, uint8_t* codes, uint8_t* pair, int per_group) {
-    const unsigned full = 0xffffffffu;
+// Eight elements' codes, and step and low of their group (G / 8 lanes share one; all lanes take part): the
+// parameters as they are stored.
+template <int G>
+__device__ __forceinline__ uint32_t quantise_eight(const uint4& x, __half2* pair) {
     const __half2* h = reinterpret_cast<const __half2*>(&x);
     // (largest, -smallest): exact in fp16, and a NaN stays one
     const __half2 hi2 = __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3]));
     const __half2 lo2 = __hmin2_nan(__hmin2_nan(h[0], h[1]), __hmin2_nan(h[2], h[3]));
     __half2 ends = __hmax2_nan(__lows2half2(hi2, __hneg2(lo2)), __highs2half2(hi2, __hneg2(lo2)));
-    ends = __hmax2_nan(ends, __shfl_xor_sync(full, ends, 1));
-    ends = __hmax2_nan(ends, __shfl_xor_sync(full, ends, 2));
-    if (per_group > 4) ends = __hmax2_nan(ends, __shfl_xor_sync(full, ends, 4));
-    if (per_group > 8) ends = __hmax2_nan(ends, __shfl_xor_sync(full, ends, 8));
+#pragma unroll
+    for (int o = 1; o < G / 8; o <<= 1) ends = __hmax2_nan(ends, __shfl_xor_sync(0xffffffffu, ends, o));
     const float hi = __low2float(ends), lo = -__high2float(ends);
     const __half step = step_of(hi, lo);
     const float fs = __half2float(step);
     const bool bad = !(__fsub_rn(hi, lo) < INFINITY);  // an infinity or a NaN in the group
     uint32_t w = 0;
     if (!bad && fs > 0.0f) w = quant_codes(h, lo, fs);
-    if (codes) *reinterpret_cast<uint32_t*>(codes) = w;
-    if (pair) {
-        const __half nan = __ushort_as_half(0x7FFF);
-        *reinterpret_cast<__half2*>(pair) = bad ? __halves2half2(nan, nan) : __halves2half2(step, __float2half_rn(lo));
-    }
+    const __half nan = __ushort_as_half(0x7FFF);
+    *pair = bad ? __halves2half2(nan, nan) : __halves2half2(step, __float2half_rn(lo));
+    return w;
 }
 
 // Block (x, y): tokens kWarps x .., one a warp, and the y-th share of its heads. Units of work, each with kBatch
@@ -152,7 +148,7 @@ constexpr int kWarps = kRopeThreads / 32, kBatch = 4;
 
 __host__ __device__ inline int units_of(int heads, int a_group, int groups) { return (heads + a_group * groups - 1) / (a_group * groups); }
 
-template <int D, bool ALL>
+template <int D, int G, bool ALL>
 __global__ void __launch_bounds__(kRopeThreads, 3) kv4_rope_append_kernel(RopeCall c, Pages pg, Geom ge) {
     pdl_launch_dependents();
     pdl_wait();
@@ -162,94 +158,125 @@ __global__ void __launch_bounds__(kRopeThreads, 3) kv4_rope_append_kernel(RopeCa
     if (t >= c.num_tokens) return;
     const int q_units = units_of(c.hq, kHeads, kBatch), units = q_units + units_of(ge.hkv, kHeads, kBatch / 2);
     const int first = units * blockIdx.y / gridDim.y, end = units * (blockIdx.y + 1) / gridDim.y;
-    const __half* q = c.q + t * c.q_stride + sub * D + lane * 8;
-    const __half* k = c.k + t * c.row_stride + sub * D + lane * 8;
-    const __half* v = c.v + t * c.row_stride + sub * D + lane * 8;
+    const int in_row = sub * D + lane * 8;
+    const __half* q = c.q + t * c.q_stride + in_row;
+    const __half* k = c.k + t * c.row_stride + in_row;
+    const long long to_v = c.v - c.k;
     uint4 x[kBatch];
-    auto load = [&](int unit) {
-        if (unit < q_units) {
-            const int head = unit * kBatch * kHeads;
+    auto load_q = [&](int unit) {
+        const int head = unit * kBatch * kHeads;
 #pragma unroll
-            for (int i = 0; i < kBatch; ++i) {
-                x[i] = make_uint4(0, 0, 0, 0);
-                if (head + i * kHeads + sub < c.hq) x[i] = *reinterpret_cast<const uint4*>(q + (head + i * kHeads) * D);
-            }
-        } else {
-            const int head = (unit - q_units) * (kBatch / 2) * kHeads;
-#pragma unroll
-            for (int i = 0; i < kBatch / 2; ++i) {
-                x[2 * i] = x[2 * i + 1] = make_uint4(0, 0, 0, 0);
-                if (head + i * kHeads + sub < ge.hkv) {
-                    x[2 * i] = *reinterpret_cast<const uint4*>(k + (head + i * kHeads) * D);
-                    x[2 * i + 1] = *reinterpret_cast<const uint4*>(v + (head + i * kHeads) * D);
-                }
-            }
-        }
+        for (int i = 0; i < kBatch; ++i)
+            if (head + i * kHeads + sub < c.hq) x[i] = *reinterpret_cast<const uint4*>(q + (head + i * kHeads) * D);
     };
-    load(first);  // in flight while the token's place is looked up
+    auto load_kv = [&](int unit) {
+        const int head = (unit - q_units) * (kBatch / 2) * kHeads;
+#pragma unroll
+        for (int i = 0; i < kBatch / 2; ++i)
+            if (head + i * kHeads + sub < ge.hkv) {
+                const __half* at = k + (head + i * kHeads) * D;
+                x[2 * i] = *reinterpret_cast<const uint4*>(at);
+                x[2 * i + 1] = *reinterpret_cast<const uint4*>(at + to_v);
+            }
+    };
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) x[i] = make_uint4(0, 0, 0, 0);  // heads that are none are computed all the same
+    if (first < q_units) load_q(first); else load_kv(first);  // in flight while the token's place is looked up
     const int b = find_seq_warp(c.offsets, c.num_seqs, t);
     if (b < 0) return;
     const long long pos = (long long)__ldg(c.lens + b) - __ldg(c.offsets + b + 1) + t;
-    const bool past = c.rotary && pos >= c.num_positions, placed = pos >= 0 && !past;
-    if (past && threadIdx.x % 32 == 0) report_dev_error(kDevBadPage);
+    __half* out = c.out + t * c.out_stride + in_row;
+    if (pos < 0 || (c.rotary && pos >= c.num_positions)) {  // no place to turn to
+        if (pos >= 0 && threadIdx.x % 32 == 0) report_dev_error(kDevBadPage);
+        for (int head = first * kBatch * kHeads; head < min(end, q_units) * kBatch * kHeads; head += kHeads)
+            if (head + sub < c.hq) *reinterpret_cast<uint4*>(out + head * D) = make_uint4(0, 0, 0, 0);
+        return;
+    }
     const int part = c.rotary >> 4;
     float2 turn[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) turn[j] = make_float2(0.0f, 0.0f);
-    if (part && placed && (ALL || lane < 2 * part)) {
+    if (ALL || lane < 2 * part) {
         const bool upper = lane >= part;
         const float4* at = reinterpret_cast<const float4*>(c.turns + pos * (c.rotary / 2)) + (upper ? lane - part : lane) * 4;
+        const float sign = upper ? 1.0f : -1.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            *reinterpret_cast<float4*>(&turn[2 * j]) = __ldg(at + j);
-            if (!upper) turn[2 * j].y = -turn[2 * j].y, turn[2 * j + 1].y = -turn[2 * j + 1].y;
+            const float4 two = __ldg(at + j);
+            turn[2 * j] = make_float2(two.x, sign * two.y);
+            turn[2 * j + 1] = make_float2(two.z, sign * two.w);
         }
     }
-    const uint4 none = make_uint4(0, 0, 0, 0);
     int unit = first;
-    if (unit < q_units) {
-        const bool norm = c.q_weight != nullptr;
-        const uint4 weight = norm ? __ldg(reinterpret_cast<const uint4*>(c.q_weight) + lane) : none;
-        __half* out = c.out + t * c.out_stride + sub * D + lane * 8;
+    auto queries = [&](auto norm, const uint4& weight) {
         for (; unit < min(end, q_units); ++unit) {
-            if (unit != first) load(unit);
+            if (unit != first) load_q(unit);
             const int head = unit * kBatch * kHeads;
 #pragma unroll
             for (int i = 0; i < kBatch; ++i) {
-                if (head + i * kHeads >= c.hq) break;
-                uint4 y = norm ? norm_and_turn<D, ALL, true>(x[i], weight, c.eps, turn, part, lane)
-                               : norm_and_turn<D, ALL, false>(x[i], weight, c.eps, turn, part, lane);
-                if (!placed) y = none;
+                const uint4 y = norm_and_turn<D, ALL, decltype(norm)::value>(x[i], weight, c.eps, turn, part, lane);
                 if (head + i * kHeads + sub < c.hq) *reinterpret_cast<uint4*>(out + (head + i * kHeads) * D) = y;
             }
         }
+    };
+    if (unit < q_units) {
+        if (c.q_weight) queries(std::true_type{}, __ldg(reinterpret_cast<const uint4*>(c.q_weight) + lane));
+        else queries(std::false_type{}, make_uint4(0, 0, 0, 0));
     }
     if (unit >= end) return;
-    const long long page = placed ? page_offset(pg, b, pos, ge.page_shift) : -1;
+    const long long page = page_offset(pg, b, pos, ge.page_shift);
     if (page < 0) return;
-    const bool norm = c.k_weight != nullptr;
-    const uint4 weight = norm ? __ldg(reinterpret_cast<const uint4*>(c.k_weight) + lane) : none;
-    const int row = (int)(pos & (ge.page() - 1)), per_group = ge.g >> 3;
-    const bool leads = (lane & (per_group - 1)) == 0;
+    constexpr int kPerGroup = G / 8, kGroups = D / G;
+    const int row = (int)(pos & (ge.page() - 1));
     // of the warp's first head: the lane's codes and, where it leads its group, its parameters
-    uint8_t* codes = pg.pool + page + (long long)sub * ge.block_bytes() + row * (D / 2) + lane * 4;
-    uint8_t* pair = pg.pool + page + (long long)sub * ge.block_bytes() + ge.k_params() +
-                    (row * ge.ng() + (lane >> (__ffs(per_group) - 1))) * 4;
-    for (; unit < end; ++unit) {
-        if (unit != first) load(unit);
+    uint8_t* block = pg.pool + page + (long long)sub * ge.block_bytes();
+    uint8_t* codes = block + row * (D / 2) + lane * 4;
+    uint8_t* pair = block + ge.k_params() + (row * kGroups + lane / kPerGroup) * 4;
+    const bool leads = lane % kPerGroup == 0;
+    auto keys = [&](auto norm, const uint4& weight) {
+        for (; unit < end; ++unit) {
+            if (unit != first) load_kv(unit);
 #pragma unroll
-        for (int i = 0; i < kBatch / 2; ++i) {
-            const int head = ((unit - q_units) * (kBatch / 2) + i) * kHeads;
-            if (head >= ge.hkv) break;
-            const bool live = head + sub < ge.hkv;
-            const long long at = (long long)head * ge.block_bytes();
-            const uint4 y = norm ? norm_and_turn<D, ALL, true>(x[2 * i], weight, c.eps, turn, part, lane)
-                                 : norm_and_turn<D, ALL, false>(x[2 * i], weight, c.eps, turn, part, lane);
-            quantise_eight(y, live ? codes + at : nullptr, live && leads ? pair + at : nullptr, per_group);
-            quantise_eight(x[2 * i + 1], live ? codes + at + ge.v_codes() : nullptr,
-                           live && leads ? pair + at + ge.v_codes() : nullptr, per_group);
+            for (int i = 0; i < kBatch / 2; ++i) {
+                const int head = ((unit - q_units) * (kBatch / 2) + i) * kHeads;
+                if (head >= ge.hkv) break;
+                const bool live = head + sub < ge.hkv;
+                const int at = head * ge.block_bytes();
+                const uint4 y = norm_and_turn<D, ALL, decltype(norm)::value>(x[2 * i], weight, c.eps, turn, part, lane);
+                __half2 kp, vp;
+                const uint32_t kw = quantise_eight<G>(y, &kp), vw = quantise_eight<G>(x[2 * i + 1], &vp);
+                if (live) {
+                    *reinterpret_cast<uint32_t*>(codes + at) = kw;
+                    *reinterpret_cast<uint32_t*>(codes + at + ge.v_codes()) = vw;
+                    if (leads) {
+                        *reinterpret_cast<__half2*>(pair + at) = kp;
+                        *reinterpret_cast<__half2*>(pair + at + ge.v_codes()) = vp;
+                    }
+                }
+            }
         }
-    }
+    };
+    if (c.k_weight) keys(std::true_type{}, __ldg(reinterpret_cast<const uint4*>(c.k_weight) + lane));
+    else keys(std::false_type{}, make_uint4(0, 0, 0, 0));
+}
+
+template <int D, int G>
+cudaError_t launch_group(const RopeCall& c, const Pages& pg, const Geom& ge, dim3 grid, cudaStream_t st) {
+    auto kernel = c.rotary == D ? kv4_rope_append_kernel<D, G, true> : kv4_rope_append_kernel<D, G, false>;
+    return launch_k(kernel, grid, dim3(kRopeThreads), 0, st, c, pg, ge);
+}
+template <int D>
+cudaError_t launch_dim(const RopeCall& c, const Pages& pg, const Geom& ge, cudaStream_t st) {
+    // many tokens: a warp takes all heads of one; few: its units are dealt out to several, until there are about two
+    // blocks for each SM
+    constexpr int kHeads = 256 / D;
+    const int units = units_of(c.hq, kHeads, kBatch) + units_of(ge.hkv, kHeads, kBatch / 2);
+    const long long blocks = ((long long)c.num_tokens + kWarps - 1) / kWarps;
+    const dim3 grid((unsigned)blocks, (unsigned)std::min<long long>(units, std::max<long long>(1, 2 * kNumSMs / blocks)));
+    if (ge.g == 32) return launch_group<D, 32>(c, pg, ge, grid, st);
+    if (ge.g == 64) return launch_group<D, 64>(c, pg, ge, grid, st);
+    if constexpr (D >= 128) return launch_group<D, 128>(c, pg, ge, grid, st);
+    return cudaErrorInvalidValue;
 }
 
 }  // namespace
@@ -263,16 +290,10 @@ int launch_rope_table(float theta, int half, long long positions, float* table, 
 }
 
 int launch_rope_append(const RopeCall& c, const Pages& pg, const Geom& ge, cudaStream_t st) {
-    // many tokens: a warp takes all heads of one; few: its units are dealt out to several, until there are about two
-    // blocks for each SM
-    const int heads = 256 / ge.d, units = units_of(c.hq, heads, kBatch) + units_of(ge.hkv, heads, kBatch / 2);
-    const long long blocks = ((long long)c.num_tokens + kWarps - 1) / kWarps;
-    const long long shares = std::min<long long>(units, std::max<long long>(1, 2 * kNumSMs / blocks));
-    const bool all = c.rotary == ge.d;
-    auto kernel = ge.d == 64    ? (all ? kv4_rope_append_kernel<64, true> : kv4_rope_append_kernel<64, false>)
-                  : ge.d == 128 ? (all ? kv4_rope_append_kernel<128, true> : kv4_rope_append_kernel<128, false>)
-                                : (all ? kv4_rope_append_kernel<256, true> : kv4_rope_append_kernel<256, false>);
-    return launch_k(kernel, dim3((unsigned)blocks, (unsigned)shares), dim3(kRopeThreads), 0, st, c, pg, ge) == cudaSuccess ? 0 : -1;
+    const cudaError_t e = ge.d == 64    ? launch_dim<64>(c, pg, ge, st)
+                          : ge.d == 128 ? launch_dim<128>(c, pg, ge, st)
+                                        : launch_dim<256>(c, pg, ge, st);
+    return e == cudaSuccess ? 0 : -1;
 }
 
 }  // namespace kv4
