@@ -218,7 +218,7 @@ __device__ void shrink_few(const LoraCall& c, const Plan& p, const int4& tile, i
 // Many rows: both operands pass through a ring of shared-memory stages of 128 elements of K (two blocks of 128-byte rows, whose
 // 16-byte pieces are swapped about by the row's low bits). What the matrix loads move bounds it, so a warp has 32 of
 // the tile's rows and up to 64 of the adapter's, and warps share the steps of a stage before they share those: 16 x 32
-// a warp read twice as much, and 9000 rows of 2048 took 19 us where this takes ____.
+// a warp read twice as much, and 9000 rows of 2048 took 19 us where this takes 16.5 (its bytes 6).
 template <int RP>
 __device__ void shrink_many(const LoraCall& c, const Plan& p, const int4& tile, int rank, int k0, int k1, float* out,
                             uint8_t* smem) {
@@ -550,8 +550,13 @@ unsigned* error_word(int dev) {
     return p;
 }
 
-// From how many tokens on the second product is the wide tiles' kernel's.
-constexpr int kManyTokens = 512;
+// Which kernel has the second product: the wide tiles' from this much work (tokens * outputs * rank) and 64 tokens on.
+// Whole calls at K = 2048, lora_expand_kernel / lora_expand_wide_kernel: rank 64, 2048 outputs, one sequence of 512
+// tokens 18.5 / 20.6 us, of 1024 18.6 / 20.6, of 2048 28.7 / 22.7, 1024 tokens of 40 adapters 27.6 / 24.3; 8192 outputs, 256
+// tokens 18.5 / 18.5, 512 25.3 / 22.6, 1024 40.3 / 30.4; rank 16, 8192 outputs, 512 tokens 15.0 / 16.8, 1024 22.6 / 22.6;
+// rank 128, 2048 outputs, 256 tokens 19.7 / 20.7, 512 26.7 / 24.6.
+constexpr long long kWideWork = 1LL << 27;
+constexpr int kWideTokens = 64;
 
 int launch_lora(const LoraCall& c, cudaStream_t st) {
     const int rp = padded_rank(c.max_rank);
@@ -575,7 +580,8 @@ int launch_lora(const LoraCall& c, cudaStream_t st) {
     const long long across = (c.n + kBlockCols - 1) / kBlockCols;
     const long long expand = std::min<long long>(kTargetBlocks, (tiles + (c.num_tokens + kTileRows - 1) / kTileRows) * across);
     pdl_scope beside(shrink > 0);  // the second kernel starts while the first one ends, and waits for it
-    if (c.num_tokens >= kManyTokens && c.max_rank <= kLoraWideRank) return launch_lora_expand_wide(c, error_word(dev), st);
+    if (c.num_tokens >= kWideTokens && c.max_rank <= kLoraWideRank && (long long)c.num_tokens * c.n * c.max_rank >= kWideWork)
+        return launch_lora_expand_wide(c, error_word(dev), st);
     return launch_k(lora_expand_kernel, dim3((unsigned)expand), dim3(kThreads), expand_smem, st, c) == cudaSuccess ? 0 : -1;
 }
 

@@ -15,7 +15,7 @@ namespace kv4 {
 
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 128;
 
 // (cos, sin) of position p's angles: p * theta^(-2 i / R), in 64 bits up to the last rounding.
 __global__ void rope_table_kernel(double theta, int half, long long n, float2* __restrict__ table) {
@@ -149,7 +149,7 @@ constexpr int kWarps = kRopeThreads / 32, kBatch = 4;
 __host__ __device__ inline int units_of(int heads, int a_group, int groups) { return (heads + a_group * groups - 1) / (a_group * groups); }
 
 template <int D, int G, bool ALL>
-__global__ void __launch_bounds__(kRopeThreads, 3) kv4_rope_append_kernel(RopeCall c, Pages pg, Geom ge) {
+__global__ void __launch_bounds__(kRopeThreads, 6) kv4_rope_append_kernel(RopeCall c, Pages pg, Geom ge) {
     pdl_launch_dependents();
     pdl_wait();
     constexpr int kLanes = D / 8, kHeads = 32 / kLanes;
@@ -267,12 +267,12 @@ cudaError_t launch_group(const RopeCall& c, const Pages& pg, const Geom& ge, dim
 }
 template <int D>
 cudaError_t launch_dim(const RopeCall& c, const Pages& pg, const Geom& ge, cudaStream_t st) {
-    // many tokens: a warp takes all heads of one; few: its units are dealt out to several, until there are about two
+    // many tokens: a warp takes all heads of one; few: its units are dealt out to several, until there are about four
     // blocks for each SM
     constexpr int kHeads = 256 / D;
     const int units = units_of(c.hq, kHeads, kBatch) + units_of(ge.hkv, kHeads, kBatch / 2);
     const long long blocks = ((long long)c.num_tokens + kWarps - 1) / kWarps;
-    const dim3 grid((unsigned)blocks, (unsigned)std::min<long long>(units, std::max<long long>(1, 2 * kNumSMs / blocks)));
+    const dim3 grid((unsigned)blocks, (unsigned)std::min<long long>(units, std::max<long long>(1, 4 * kNumSMs / blocks)));
     if (ge.g == 32) return launch_group<D, 32>(c, pg, ge, grid, st);
     if (ge.g == 64) return launch_group<D, 64>(c, pg, ge, grid, st);
     if constexpr (D >= 128) return launch_group<D, 128>(c, pg, ge, grid, st);

@@ -371,46 +371,61 @@ def test_lora_split_product_over_a_long_row():
     Lora([130], [0], [64], 8200, 72, rng).both()
 
 
-# batches of many rows: tiles of 128, items ahead of one another
-@pytest.mark.parametrize("counts", [[512], [600], [511, 1], [128] * 4, [129, 0, 127, 300], [70] * 12, [1] * 700, [37] * 40,
-                                    [1500]])
+# Batches of so much work (tokens * outputs * rank) that the second product has tiles of 128 rows and goes over items
+# ahead of one another.
+WIDE = 1 << 27
+
+
+def _wide(n, top, pattern):
+    """Token counts in the pattern's proportions that make enough work."""
+    t = WIDE // (n * top) + 1
+    counts = [max(p > 0, p * t // sum(pattern)) for p in pattern]
+    counts[0] += max(0, t - sum(counts))
+    return counts
+
+
+@pytest.mark.parametrize("pattern", [[1], [511, 1], [1] * 4, [129, 0, 127, 300], [70] * 12, [37] * 40, [1] * 900])
 @pytest.mark.parametrize("rank", [1, 16, 40, 64, 100, 128])
-def test_lora_many_rows(counts, rank):
-    rng = np.random.default_rng(rank * 100 + len(counts))
+def test_lora_many_rows(pattern, rank):
+    rng = np.random.default_rng(rank * 100 + len(pattern))
+    n = 1544
+    counts = _wide(n, -(-rank // 8) * 8, pattern)
     ids = [(i * 5) % 4 - 1 for i in range(len(counts))] if len(counts) > 1 else [1]
-    Lora(counts, ids, [rank, max(1, rank // 2), rank], 128, 136, rng, extra=5, pad=8).both()
+    Lora(counts, ids, [rank, max(1, rank // 2), rank], 72, n, rng, extra=5, pad=8).both()
 
 
 @pytest.mark.parametrize("n", [8, 64, 120, 128, 136, 264, 2000])
 @pytest.mark.parametrize("k", [8, 200])
-@pytest.mark.parametrize("rank", [13, 72])
-def test_lora_many_rows_features(n, k, rank):
-    rng = np.random.default_rng(n + k + rank)
-    Lora([300, 40, 260, 5], [0, 1, -1, 0], [rank, 5], k, n, rng).both()
-    call = Lora([300, 40, 260, 5], [0, 1, -1, 0], [rank, 5], k, n, rng)
-    call.both(base=False)
+@pytest.mark.parametrize("top", [64, 128])
+def test_lora_many_rows_features(n, k, top):
+    if n * k == 1600:
+        k = 40
+    rng = np.random.default_rng(n + k + top)
+    counts = _wide(n, top, [300, 40, 260, 5])
+    for base in (True, False):
+        Lora(counts, [0, 1, -1, 0], [top - 11, 5], k, n, rng, top=top).both(base=base)
 
 
 def test_lora_many_rows_of_many_adapters_and_of_few():
     rng = np.random.default_rng(14)
     ids = rng.integers(-1, 60, 400).tolist()
-    Lora(rng.integers(0, 9, 400).tolist(), ids, rng.integers(0, 65, 60).tolist(), 72, 96, rng, extra=3).both()
-    Lora(rng.integers(0, 9, 400).tolist(), ids, rng.integers(0, 129, 60).tolist(), 72, 200, rng, extra=3).both()
-    Lora([300, 400], [-1, -1], [8], 64, 64, rng, extra=2).both()
-    Lora([500, 80], [0, -1], [0], 64, 64, rng).both()
-    Lora([500, 80], [-1, -1], [], 64, 64, rng).both()
-    Lora([700, 3], [0, 1], [4, 200], 64, 320, rng).both()  # a rank past the wide tiles' kernel
     for top in (64, 128):
-        call = Lora([100, 350, 164, 30], [1, -1, 0, 1], [top, 16], 96, 424, rng, top=top)
+        counts = rng.integers(0, 9, 400) * (WIDE // (1032 * top * 1600) + 1)
+        Lora(counts.tolist(), ids, rng.integers(0, top + 1, 60).tolist(), 72, 1032, rng, extra=WIDE // (1032 * top), top=top).both()
+        counts = _wide(776, top, [300, 400])
+        Lora(counts, [-1, -1], [8], 64, 776, rng, extra=2, top=top).both()
+        Lora(counts, [0, -1], [0], 64, 776, rng, top=top).both()
+        call = Lora(_wide(776, top, [100, 350, 164, 30]), [1, -1, 0, 1], [top, 16], 96, 776, rng, top=top)
         call.plan()
         call.run(out=call.pbase)  # in place
         call.check(got=host(call.dbase, np.float16)[:call.t * call.n].reshape(call.t, call.n))
+    Lora([1300, 3], [0, 1], [4, 200], 64, 1320, rng).both()  # a rank past that kernel's
 
 
 def test_lora_many_rows_keep_their_bits():
     """As test_lora_middle_product_keeps_its_bits; and calls repeated, and replayed with other lists."""
     rng = np.random.default_rng(15)
-    call = Lora([600], [0], [24], 512, 80, rng, integers=True, scales=False)
+    call = Lora(_wide(1040, 24, [1]), [0], [24], 512, 1040, rng, integers=True, scales=False)
     call.x[:, ::2], call.a[0, :24, ::2] = 29, 31
     call.b[0, :, 0] = 1 + call.b[0, :, 1]
     call.b[0, :, 2:24] = 0
@@ -422,8 +437,8 @@ def test_lora_many_rows_keep_their_bits():
     x, a, b = call.x.astype(np.float64), call.a[0, :24].astype(np.float64), call.b[0, :, :24].astype(np.float64)
     assert np.array_equal(call.got(), (call.base.astype(np.float64) + (x @ a.T) @ b.T).astype(np.float16))
     t = torch()
-    counts = [150, 1, 290, 3, 300, 65]
-    call = Lora(counts, [2, 1, 0, -1, 2, 0], [64, 8, 24], 512, 776, rng)
+    counts = _wide(1608, 64, [150, 1, 290, 3, 300, 65])
+    call = Lora(counts, [2, 1, 0, -1, 2, 0], [64, 8, 24], 512, 1608, rng)
     call.both()
     first = call.got().view(np.uint16).copy()
     for _ in range(20):
@@ -437,7 +452,7 @@ def test_lora_many_rows_keep_their_bits():
         stream = t.cuda.current_stream().cuda_stream
         call.plan(stream)
         call.run(stream=stream)
-    for ids, order in (([0, 0, 1, 2, -1, 1], counts[::-1]), ([-1] * 6, counts), ([1] * 6, [0, 800, 0, 0, 9, 0])):
+    for ids, order in (([0, 0, 1, 2, -1, 1], counts[::-1]), ([-1] * 6, counts), ([1] * 6, [0, call.t - 9, 0, 0, 9, 0])):
         call.ids = ids
         call.did.copy_(t.tensor(ids, dtype=t.int32))
         ends = np.cumsum(order)
@@ -451,20 +466,36 @@ def test_lora_many_rows_keep_their_bits():
 
 def test_lora_many_rows_infinities_and_nan_stay_in_their_rows():
     rng = np.random.default_rng(16)
-    call = Lora([300, 290], [0, 1], [64, 40], 128, 264, rng)
-    call.x[2, 5], call.x[290, 100], call.x[301] = np.nan, np.inf, 60000
+    call = Lora(_wide(1608, 64, [300, 290]), [0, 1], [64, 40], 128, 1608, rng)
+    odd = call.seqs[0][1]
+    call.x[2, 5], call.x[odd - 10, 100], call.x[odd + 1] = np.nan, np.inf, 60000
     call.dx, call.px = _padded(call.x, 128, rng)
     call.plan()
     call.run()
     got = call.got()
     rows = np.ones(call.t, bool)
-    rows[[2, 290]] = False
+    rows[[2, odd - 10]] = False
     ref, tol = U.lora(call.x, call.a, call.b, call.ranks, call.scales, call.base, call.seqs, call.ids)
     with np.errstate(over="ignore"):
         over = np.abs(ref) + tol > 65504  # may be infinite
     ok = np.abs(got[rows].astype(np.float64) - ref[rows]) <= tol[rows]
     assert (ok | (over[rows] & (np.sign(got[rows]) == np.sign(ref[rows])))).all()
-    assert np.isnan(got[2]).all() and not np.isfinite(got[290]).any()
+    assert np.isnan(got[2]).all() and not np.isfinite(got[odd - 10]).any()
+
+
+def test_lora_many_rows_on_two_streams():
+    t = torch()
+    rng = np.random.default_rng(17)
+    one, two = (Lora(_wide(1544, top, [40, 1, 9]), [0, 1, 0], [top, 8], 256, 1544, rng) for top in (64, 128))
+    streams = t.cuda.Stream(), t.cuda.Stream()
+    t.cuda.synchronize()
+    for _ in range(10):
+        for call, stream in zip((one, two), streams):
+            call.plan(stream.cuda_stream)
+            call.run(stream=stream.cuda_stream)
+    t.cuda.synchronize()
+    one.check()
+    two.check()
 
 
 # ---------------------------------------------------------------------------------------- logits
