@@ -1,5 +1,7 @@
 // The residual's addition, RMSNorm and 8-bit rows in one pass: a row's elements are loaded once, wait in
-// registers for the sum of squares and the largest result, and leave as codes (and fp16).
+// registers for the sum of squares and the largest result, and leave as codes (and fp16). HBM bounds it, and close
+// behind its instructions: 16384 rows of 4096 take 85 us, 5.5 TB/s, with 80 % of the issue slots used. Two passes
+// over elements kept as scalars took 664 us.
 #include "../common.cuh"
 #include "batch_ops.h"
 
@@ -151,16 +153,18 @@ __global__ void __launch_bounds__(WARP ? 32 * kWarpRows : kMostThreads) norm_q8_
 template <bool VEC>
 cudaError_t launch(const NormCall& c, cudaStream_t st) {
     const int pieces = (c.dims + 7) / 8;
-    const bool many = c.rows >= 4 * kNumSMs;
-    if (many && pieces <= (VEC ? 128 : 32)) {  // short rows: a warp each, no barriers
+    // Many rows: four pieces a thread, so that a block's loads are in flight together and its reductions are short.
+    // Few: one piece a thread, for the fewest steps. Few / many, us: 64 rows of 2048 3.1 / 3.7, 256 rows of 2048 3.6 / 4.2,
+    // of 4096 4.7 / 4.6, 592 rows of 1024 3.6 / 3.7, of 4096 8.3 / 5.8, 64 rows of 8192 5.7 / 4.7; 1200 rows of 128
+    // 3.1 / 3.1, 4000 rows of 128 5.7 / 3.7.
+    const bool many = c.rows >= 2048 || (long long)c.rows * c.dims >= 1 << 20 || c.dims > 4096;
+    if (many && pieces <= (VEC ? 128 : 32)) {  // short rows: a warp each, no barriers (4000 rows of 512 4.7 us, a block each 6.7)
         const dim3 grid((unsigned)((c.rows + kWarpRows - 1) / kWarpRows)), block(32, kWarpRows);
         auto kernel = norm_q8_kernel<1, VEC, true>;
         if constexpr (VEC)
             if (pieces > 32) kernel = pieces <= 64 ? norm_q8_kernel<2, VEC, true> : norm_q8_kernel<4, VEC, true>;
         return launch_k(kernel, grid, block, 0, st, c);
     }
-    // Many rows: four pieces a thread, so that a block's loads are in flight together and its reductions are
-    // short. Few, or elements one by one: one piece a thread, where a row's threads allow it.
     const int v = (many && VEC) || pieces > 2 * kMostThreads ? 4 : pieces > kMostThreads ? 2 : 1;
     const unsigned threads = (unsigned)(((pieces + v - 1) / v + 31) / 32 * 32);
     auto kernel = v == 4 ? norm_q8_kernel<4, VEC, false> : v == 2 ? norm_q8_kernel<2, VEC, false> : norm_q8_kernel<1, VEC, false>;
