@@ -1,5 +1,8 @@
-// Low-rank adapters of many requests: a plan that groups a batch's rows by adapter, then two products a
-// row with its adapter's matrices, the low-rank one in fp32 in the workspace between them.
+// Low-rank adapters of many requests: a plan that groups a batch's rows by adapter, then two products with each
+// tile's adapter, the low-rank one in fp32 between them. Three ways, by the measurements at the end of this file:
+// one kernel, a cluster of blocks a tile (lora_few_kernel); two kernels with the sums in the workspace (lora_shrink_kernel,
+// lora_expand_kernel); and for much work the second product by lora_tc.cu. What a call has to move is x, the base and
+// the result once and the adapters it uses, 2 bytes each; of that 9288 rows of 2048 into 8192 reach 4.0 TB/s (85 us).
 #include <algorithm>
 #include <atomic>
 
@@ -159,6 +162,8 @@ __device__ __forceinline__ uint4 ldg_nc(const __half* p) {
     const int4 v = ldg_nc_v4(p);
     return make_uint4((unsigned)v.x, (unsigned)v.y, (unsigned)v.z, (unsigned)v.w);
 }
+
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 
 // ---- x A^T
 constexpr int kThreads = 256, kWarps = kThreads / 32, kChunk = 128;  // K elements a stage
@@ -361,15 +366,12 @@ __global__ void __launch_bounds__(kThreads, 1) lora_shrink_kernel(LoraCall c) {
 constexpr int kWarpCols = 32, kBlockCols = kWarps * kWarpCols;
 
 __host__ __device__ inline int padded_rank(int r) { return r <= 16 ? 16 : r <= 32 ? 32 : r <= 64 ? 64 : r <= 128 ? 128 : 256; }
-__host__ __device__ inline int h_stride(int rp) { return 2 * rp + 8; }  // fp16 elements: high, low, padding against bank conflicts
+__host__ __device__ inline int h_stride(int rp) { return 2 * rp + 16; }  // fp16 elements: high, low, padding against bank conflicts
 
-// Four threads a row; each has every fourth four of its elements.
+// A tile's h into shared memory: four threads a row, each with every fourth four of its elements.
 template <int RP>
-__device__ void load_h(const LoraCall& c, const Plan& p, const int4& tile, int rank, int parts, __half* s_h, float* s_scale) {
+__device__ __forceinline__ void store_h(const LoraCall& c, const int4& tile, const float4 (&v)[RP / 16], __half* s_h, float* s_scale) {
     const int row = threadIdx.x >> 2, q = threadIdx.x & 3;
-    float4 v[RP / 16];
-    sum_parts<RP / 16>(c.ws + (long long)(tile.y + row) * c.max_rank + 4 * q, (long long)p.rows * c.max_rank, parts,
-                       row < tile.z ? rank - 4 * q : 0, v);
     float top = 0.0f;
 #pragma unroll
     for (int i = 0; i < RP / 16; ++i) top = fmaxf(top, largest_of(v[i]));
@@ -388,6 +390,14 @@ __device__ void load_h(const LoraCall& c, const Plan& p, const int4& tile, int r
         *reinterpret_cast<uint2*>(to + RP + r) = *reinterpret_cast<const uint2*>(lo);
     }
     if (q == 0) s_scale[row] = (c.scales ? __ldg(c.scales + tile.x) : 1.0f) * two_to(e);
+}
+template <int RP>
+__device__ void load_h(const LoraCall& c, const Plan& p, const int4& tile, int rank, int parts, __half* s_h, float* s_scale) {
+    const int row = threadIdx.x >> 2, q = threadIdx.x & 3;
+    float4 v[RP / 16];
+    sum_parts<RP / 16>(c.ws + (long long)(tile.y + row) * c.max_rank + 4 * q, (long long)p.rows * c.max_rank, parts,
+                       row < tile.z ? rank - 4 * q : 0, v);
+    store_h<RP>(c, tile, v, s_h, s_scale);
 }
 
 // 32 outputs of up to 16 * MT rows, a warp.
@@ -520,6 +530,124 @@ __global__ void __launch_bounds__(kThreads, 2) lora_expand_kernel(LoraCall c) {
     }
 }
 
+// ---- both products of few rows in one kernel
+// A cluster of blocks has a tile: each block the low-rank product of its share of K, in its shared memory, then, with
+// the sums of all of them, its share of the outputs. One launch, and h never leaves the SMs; but a tile's rows have one
+// cluster alone.
+constexpr int kClusterRank = 64;
+
+// Where it is the faster one: up to 8 rows for each group that there can be (a block's warps take 8 at a time), and no
+// more of B for a cluster than 2^18 elements unless clusters are many. Whole calls, two kernels / this one, us: K and outputs
+// 2048, rank 16, one sequence of 8 tokens 8.3 / 6.3, of 32 9.4 / 10.4, 64 sequences of 8 adapters 9.6 / 8.3, 64 of 64 adapters
+// 12.3 / 8.3; rank 64, 64 of 64 16.5 / 12.4, 256 of 256 49 / 37; 8192 outputs, rank 64, 4 of 4 10.4 / 14.4, 16 of 16 15.7 / 14.4.
+inline bool cluster_pays(const LoraCall& c, long long tiles) {
+    const long long groups = c.num_seqs < c.num_adapters ? c.num_seqs : c.num_adapters;
+    return c.max_rank <= kClusterRank && c.num_tokens <= kFewRows * groups && ((long long)c.n * c.max_rank <= 1 << 18 || tiles >= 16);
+}
+// Blocks of a cluster: 8 while two blocks a SM are enough for them, else 4 (64 sequences of 64 adapters, rank 64, K and
+// outputs 2048: 17.6 and 12.4 us).
+inline int cluster_blocks(long long tiles) { return tiles * 8 <= 2 * kNumSMs ? 8 : 4; }
+
+__device__ __forceinline__ unsigned cluster_size() {
+    unsigned n;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+    return n;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// 16 bytes of another block's shared memory at the place that `at` is in this one's
+__device__ __forceinline__ float4 load_of_block(const float* at, unsigned block) {
+    uint32_t there;
+    float4 v;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_u32(at)), "r"(block));
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
+    return v;
+}
+
+template <int RP>
+__device__ void gather_h(const LoraCall& c, const int4& tile, int rank, const float* s_sum, __half* s_h, float* s_scale) {
+    const int row = threadIdx.x >> 2, q = threadIdx.x & 3;
+    const unsigned blocks = cluster_size();
+    float4 v[RP / 16];
+#pragma unroll
+    for (int i = 0; i < RP / 16; ++i) {
+        v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (row < tile.z && 16 * i + 4 * q < rank)
+#pragma unroll 4
+            for (unsigned block = 0; block < blocks; ++block) {
+                const float4 h = load_of_block(s_sum + row * c.max_rank + 16 * i + 4 * q, block);
+                v[i].x += h.x, v[i].y += h.y, v[i].z += h.z, v[i].w += h.w;
+            }
+    }
+    store_h<RP>(c, tile, v, s_h, s_scale);
+}
+
+__global__ void __launch_bounds__(kThreads, 2) lora_few_kernel(LoraCall c) {
+    extern __shared__ __align__(128) uint8_t smem[];  // the block's sums [64][max_rank], then h
+    __shared__ float s_scale[kTileRows];
+    __shared__ int s_row[kTileRows];
+    pdl_launch_dependents();
+    pdl_wait();
+    Plan p;
+    if (!open_plan(c, &p)) return;
+    const int blocks = (int)cluster_size(), tile_no = blockIdx.x / blocks, me = blockIdx.x % blocks;
+    const int bare = c.base == c.out ? 0 : (p.bare + kTileRows - 1) / kTileRows;
+    if (tile_no >= p.tiles + bare) return;  // and so do the cluster's others
+    float* s_sum = reinterpret_cast<float*>(smem);
+    __half* s_h = reinterpret_cast<__half*>(smem + kTileRows * c.max_rank * 4);
+    const int i0 = (tile_no - p.tiles) * kTileRows;
+    const int4 tile = tile_no < p.tiles ? __ldg(p.tile + tile_no) : make_int4(-1, p.rows + i0, min(kTileRows, p.bare - i0), 0);
+    const int rank = tile.x < 0 ? 0 : rank_of(c, tile.x);
+    const int columns = (c.n + 31) / 32, from = columns * me / blocks, to = columns * (me + 1) / blocks;  // blocks of 32 outputs
+    if (threadIdx.x < tile.z) s_row[threadIdx.x] = __ldg(p.row + tile.y + threadIdx.x);
+    if (rank) {
+        // the block's rows of B on their way to L2 meanwhile
+        const char* b = reinterpret_cast<const char*>(c.b + ((long long)tile.x * c.n + from * 32) * c.max_rank);
+        const long long bytes = (long long)(min(to * 32, c.n) - from * 32) * c.max_rank * 2;
+        for (long long at = threadIdx.x * 128LL; at < bytes; at += kThreads * 128LL) prefetch_l2(b + at);
+        const int steps = (c.k + 31) / 32, k0 = min(c.k, steps * me / blocks * 32), k1 = min(c.k, steps * (me + 1) / blocks * 32);
+        for (int r0 = 0; r0 < tile.z; r0 += kFewRows) {
+            const int4 some = make_int4(tile.x, tile.y + r0, min(kFewRows, tile.z - r0), 0);
+            shrink_few(c, p, some, rank, k0, k1, s_sum + r0 * c.max_rank);
+        }
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();  // all sums are there
+        if (rank > 32) gather_h<64>(c, tile, rank, s_sum, s_h, s_scale);
+        else if (rank > 16) gather_h<32>(c, tile, rank, s_sum, s_h, s_scale);
+        else gather_h<16>(c, tile, rank, s_sum, s_h, s_scale);
+        __syncwarp();
+        cluster_arrive();  // this block has read the others' sums
+    }
+    __syncthreads();
+    if (rank || c.base != c.out)
+        for (int column = from + (threadIdx.x >> 5); column < to; column += kWarps) {
+            if (rank > 32) expand_rows<64>(c, tile, rank, column * 32, s_h, s_scale, s_row);
+            else if (rank > 16) expand_rows<32>(c, tile, rank, column * 32, s_h, s_scale, s_row);
+            else if (rank > 0) expand_rows<16>(c, tile, rank, column * 32, s_h, s_scale, s_row);
+            else expand_rows<0>(c, tile, rank, column * 32, s_h, s_scale, s_row);
+        }
+    if (rank) {
+        __syncwarp();
+        cluster_wait();  // no block leaves while its sums are read
+    }
+}
+
+int launch_few(const LoraCall& c, long long tiles, int blocks, cudaStream_t st) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * blocks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = kTileRows * c.max_rank * 4 + kTileRows * h_stride(padded_rank(c.max_rank)) * 2;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)blocks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, lora_few_kernel, c) == cudaSuccess ? 0 : -1;
+}
+
 }  // namespace
 
 size_t lora_plan_bytes(long long seqs, long long tokens, long long adapters) {
@@ -572,6 +700,8 @@ int launch_lora(const LoraCall& c, cudaStream_t st) {
             return -1;
         set.fetch_or(1ull << (dev & 63));
     }
+    const long long all_tiles = most_tiles(c.num_seqs, c.num_tokens, c.num_adapters) + (c.num_tokens + kTileRows - 1) / kTileRows;
+    if (cluster_pays(c, all_tiles)) return launch_few(c, all_tiles, cluster_blocks(all_tiles), st);
     // as many blocks as the most tiles that there can be need, one or two for each SM at most
     const long long tiles = most_tiles(c.num_seqs, c.num_tokens, c.num_adapters);
     const long long shrink = std::min<long long>(kTargetBlocks, tiles * parts_of(1, c.k));

@@ -7,6 +7,9 @@
 //   epilogue  (8 warps) sums from TMEM, a thread a row's 64 outputs; the results replace the base's elements in
 //             shared memory and leave from there in whole rows;
 //   issuer    (1 warp) the products: steps of 16 over the rank, first with the high parts, then with the low ones.
+// 9288 rows of 8192 outputs, ranks 16 to 64: 70 us behind the first product, 4.2 TB/s (copying the base alone takes 60); by
+// mma.sync with operands through shared memory 100, straight from and to memory 140. What is left over the copy: a tile's
+// first h, which nothing hides at a block's start, and the copies of B (16 KB an item).
 // This file is compiled as whole-program device code (build.py WHOLE_PROGRAM).
 #include <algorithm>
 #include <atomic>

@@ -371,6 +371,66 @@ def test_lora_split_product_over_a_long_row():
     Lora([130], [0], [64], 8200, 72, rng).both()
 
 
+# Few tokens for as many adapters as there may be: both products by a cluster of blocks a tile, of 8 or of 4.
+@pytest.mark.parametrize("seqs", [1, 6, 30, 60])
+@pytest.mark.parametrize("k,n", [(8, 8), (40, 24), (264, 1000), (2048, 72), (1000, 2056)])
+@pytest.mark.parametrize("rank", [3, 16, 29, 64])
+def test_lora_tokens_by_clusters(seqs, k, n, rank):
+    rng = np.random.default_rng(seqs + k + rank)
+    ids = rng.integers(-1, seqs, seqs).tolist()
+    ranks = rng.integers(0, rank + 1, seqs).tolist()
+    ranks[0] = rank
+    Lora(rng.integers(0, 4, seqs).tolist() if seqs > 1 else [8], ids, ranks, k, n, rng, extra=3, pad=8).both()
+
+
+def test_lora_tokens_by_clusters_skewed_in_place_and_replayed():
+    t = torch()
+    rng = np.random.default_rng(31)
+    # all rows of one adapter: tiles of 64 rows, 8 at a time; none of any; one of each
+    for ids in ([3] * 50, [-1] * 50, list(range(50)), [7] * 49 + [-1]):
+        call = Lora([8] * 50, ids, [16] * 50, 136, 264, rng)
+        call.both()
+        call.both(base=False)
+        call = Lora([8] * 50, ids, [16] * 50, 136, 264, rng)
+        call.plan()
+        call.run(out=call.pbase)
+        call.check(got=host(call.dbase, np.float16)[:call.t * call.n].reshape(call.t, call.n))
+    call = Lora([1] * 64, rng.integers(-1, 64, 64).tolist(), [24] * 64, 512, 392, rng)
+    call.both()
+    first = call.got().view(np.uint16).copy()
+    for _ in range(20):
+        call.ws.fill_(255)
+        call.out.fill_(0)
+        call.run()
+        assert np.array_equal(call.got().view(np.uint16), first)
+    t.cuda.synchronize()
+    graph = t.cuda.CUDAGraph()
+    with t.cuda.graph(graph):
+        stream = t.cuda.current_stream().cuda_stream
+        call.plan(stream)
+        call.run(stream=stream)
+    for ids in ([5] * 64, [-1] * 63 + [0], rng.integers(-1, 64, 64).tolist()):
+        call.ids = ids
+        call.did.copy_(t.tensor(ids, dtype=t.int32))
+        call.out.fill_(np.float16(123.0).view(np.int16).item())
+        for _ in range(3):
+            graph.replay()
+        call.check()
+    x = call.x.copy()
+    x[2, 5], x[40, 100] = np.nan, np.inf
+    call.x = x
+    call.ids = list(range(64))
+    call.did.copy_(t.arange(64, dtype=t.int32))
+    call.dx, call.px = _padded(x, 512, rng)
+    call.plan()
+    call.run()
+    got, rows = call.got(), np.ones(64, bool)
+    rows[[2, 40]] = False
+    ref, tol = U.lora(call.x, call.a, call.b, call.ranks, call.scales, call.base, call.seqs, call.ids)
+    U.within(got[rows], ref[rows], tol[rows])
+    assert np.isnan(got[2]).all() and not np.isfinite(got[40]).any()
+
+
 # Batches of so much work (tokens * outputs * rank) that the second product has tiles of 128 rows and goes over items
 # ahead of one another.
 WIDE = 1 << 27
