@@ -215,7 +215,8 @@ __device__ void shrink_few(const LoraCall& c, const Plan& p, const int4& tile, i
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = block * 16 + g + 8 * (i >> 1), row = 2 * t + (i & 1);
-            if (row < tile.z && r < c.max_rank) out[(long long)row * c.max_rank + r] = d[i];
+            // an infinity of x makes a NaN of the zeros that stand for rows past the rank
+            if (row < tile.z && r < c.max_rank) out[(long long)row * c.max_rank + r] = r < rank ? d[i] : 0.0f;
         }
     }
 }
@@ -326,7 +327,8 @@ __device__ void shrink_many(const LoraCall& c, const Plan& p, const int4& tile, 
             for (int i = 0; i < 2; ++i) {
                 const int at = m * 32 + u * 16 + (lane >> 2) + 8 * i;
                 if (at < tile.z && r < c.max_rank)
-                    *reinterpret_cast<float2*>(out + (long long)at * c.max_rank + r) = make_float2(d[u][j][2 * i], d[u][j][2 * i + 1]);
+                    *reinterpret_cast<float2*>(out + (long long)at * c.max_rank + r) =
+                        make_float2(r < rank ? d[u][j][2 * i] : 0.0f, r + 1 < rank ? d[u][j][2 * i + 1] : 0.0f);  // as shrink_few
             }
         }
 }

@@ -45,7 +45,8 @@ CB_API int cactus_cuda_lora_plan(const int32_t* token_offsets, const int32_t* ad
  * base[t] for rows of sequences without one; base NULL stands for zeros. Rows of no sequence stay as they are.
  * a [num_adapters][max_rank][in_features], b [num_adapters][out_features][max_rank]: adapter i has the first
  * ranks[i] rows of its a and columns of its b (ranks NULL: all; 0: none), and what the others hold does not
- * reach a result. scales NULL: 1. output may be base (with the same stride) and otherwise overlaps nothing.
+ * reach a result. Infinities of x and a go through as the formula has them; one in b may come out as a NaN.
+ * scales NULL: 1. output may be base (with the same stride) and otherwise overlaps nothing.
  * in_features, out_features, max_rank (8 to 256) and the strides are multiples of 8, all pointers 16-byte
  * aligned. The middle product is fp32, and enters the second one as two fp16 numbers of a row's own power of
  * two (22 bits of the row's largest). plan: of cactus_cuda_lora_plan with the same num_seqs, num_tokens and

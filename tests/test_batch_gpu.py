@@ -288,6 +288,27 @@ def test_lora_infinities_and_nan_stay_in_their_rows():
         assert np.isnan(got[2]).all() and not np.isfinite(got[4]).any()
 
 
+@pytest.mark.parametrize("rank", [1, 3, 8, 21])
+@pytest.mark.parametrize("counts,ids,n", [([6], [0], 72), ([40], [0], 72), ([100], [0], 72), (None, [0, 0], 1608)])
+def test_lora_an_infinity_keeps_its_sign(counts, ids, n, rank):
+    """Factors of one sign: the row's results are infinities, whatever the rank is padded with."""
+    rng = np.random.default_rng(rank)
+    top = 24 if counts else 64
+    call = Lora(counts or _wide(n, top, [70, 60]), ids, [rank], 128, n, rng, top=top)
+    call.a, call.b, call.x = np.abs(call.a), np.abs(call.b) + np.float16(0.01), np.abs(call.x) + np.float16(0.01)
+    call.a[0, :rank] += np.float16(0.01)
+    call.x[2, 5], call.x[4, 127] = np.inf, -np.inf
+    call.da, call.db = dev(call.a), dev(call.b)
+    call.dx, call.px = _padded(call.x, 128, rng)
+    call.plan()
+    call.run()
+    got, rows = call.got(), np.ones(call.t, bool)
+    rows[[2, 4]] = False
+    ref, tol = U.lora(call.x, call.a, call.b, call.ranks, call.scales, call.base, call.seqs, call.ids)
+    U.within(got[rows], ref[rows], tol[rows])
+    assert (got[2] == np.inf).all() and (got[4] == -np.inf).all()
+
+
 def test_lora_refuses_lists_on_the_device():
     """Offsets that fall or pass the tokens: no row; ids and ranks that are none: rows as without an adapter."""
     rng = np.random.default_rng(8)
