@@ -37,9 +37,10 @@ struct LoraCall {
     float* ws;
 };
 int launch_lora(const LoraCall& c, cudaStream_t st);
-// lora_tc.cu: the second product for batches of many rows, ranks up to kLoraWideRank
+// lora_tc.cu: the products for batches of many rows, ranks up to kLoraWideRank; split: the first one was that file's
 constexpr int kLoraWideRank = 128;
-int launch_lora_expand_wide(const LoraCall& c, unsigned* error_word, cudaStream_t st);
+int launch_lora_shrink_wide(const LoraCall& c, unsigned* error_word, cudaStream_t st);
+int launch_lora_expand_wide(const LoraCall& c, bool split, unsigned* error_word, cudaStream_t st);
 
 // logits.cu
 struct LogitsCall {

@@ -1,7 +1,7 @@
 // Low-rank adapters of many requests: a plan that groups a batch's rows by adapter, then two products with each
 // tile's adapter, the low-rank one in fp32 between them. Three ways, by the measurements at the end of this file:
 // one kernel, a cluster of blocks a tile (lora_few_kernel); two kernels with the sums in the workspace (lora_shrink_kernel,
-// lora_expand_kernel); and for much work the second product by lora_tc.cu. What a call has to move is x, the base and
+// lora_expand_kernel); and for much work the second product, or both, by lora_tc.cu. What a call has to move is x, the base and
 // the result once and the adapters it uses, 2 bytes each; of that 9288 rows of 2048 into 8192 reach 4.0 TB/s (85 us).
 #include <algorithm>
 #include <atomic>
@@ -657,9 +657,9 @@ size_t lora_plan_bytes(long long seqs, long long tokens, long long adapters) {
     return (ints * 4 + 15) / 16 * 16;
 }
 
-// parts * rows is at most kMostParts * tokens, and where there is more than one part at most 64 rows a block
+// parts * rows is at most kMostParts * tokens, and where there is more than one part at most a wide tile's rows a block
 size_t lora_workspace(long long tokens, int max_rank) {
-    const long long many = tokens * kMostParts, few = (long long)kTargetBlocks * kTileRows, split = many < few ? many : few;
+    const long long many = tokens * kMostParts, few = (long long)kTargetBlocks * kWideRows, split = many < few ? many : few;
     return ((size_t)(tokens > split ? tokens : split) * (size_t)max_rank * 4 + 15) / 16 * 16 + 16;
 }
 
@@ -680,13 +680,15 @@ unsigned* error_word(int dev) {
     return p;
 }
 
-// Which kernel has the second product: the wide tiles' from this much work (tokens * outputs * rank) and 64 tokens on.
-// Whole calls at K = 2048, lora_expand_kernel / lora_expand_wide_kernel: rank 64, 2048 outputs, one sequence of 512
-// tokens 18.5 / 20.6 us, of 1024 18.6 / 20.6, of 2048 28.7 / 22.7, 1024 tokens of 40 adapters 27.6 / 24.3; 8192 outputs, 256
-// tokens 18.5 / 18.5, 512 25.3 / 22.6, 1024 40.3 / 30.4; rank 16, 8192 outputs, 512 tokens 15.0 / 16.8, 1024 22.6 / 22.6;
-// rank 128, 2048 outputs, 256 tokens 19.7 / 20.7, 512 26.7 / 24.6.
-constexpr long long kWideWork = 1LL << 27;
-constexpr int kWideTokens = 64;
+// Which products lora_tc.cu's kernels have, from 64 tokens on, by the work (tokens * outputs * rank). Whole calls, us.
+// Both from 2^25 on where the rank is above 32; both by mma.sync / tcgen05: rank 64, K and outputs 2048, 128 tokens 14.4 / 14.5, 256 14.4 /
+// 14.4, 512 18.5 / 16.5, 1024 20.6 / 16.5; K 2048, 8192 outputs 64 tokens 14.5 / 14.4, 128 of 8 adapters 16.5 / 18.6, 512 22.6 / 18.5;
+// rank 128, K 14336, 4096 outputs 64 tokens 26.8 / 23.1, 256 47.7 / 28.7. With a rank up to 32 mma.sync keeps up, and starts
+// sooner: both from 2^27 on and 2^25 elements of x (rank 16, 1024 / 4096 tokens of 8 adapters, mma.sync first / tcgen05 both: K
+// 2048, 8192 outputs 26.7 / 28.7 and 42.2 / 44.1, 16384 of them 125 / 121; K 14336 28.7 / 32.9 and 52.9 / 54.9, 8192 90 / 85), only the
+// second below that (K 2048, 8192 outputs, both by mma.sync / it alone: 1024 tokens 22.4 / 20.6, 2048 34.2 / 27.5).
+constexpr int kWideTokens = 64, kSmallRank = 32;
+constexpr long long kWideWork = 1LL << 25, kWideWorkSmallRank = 1LL << 27, kWideElements = 1LL << 25;
 
 int launch_lora(const LoraCall& c, cudaStream_t st) {
     const int rp = padded_rank(c.max_rank);
@@ -704,6 +706,14 @@ int launch_lora(const LoraCall& c, cudaStream_t st) {
     }
     const long long all_tiles = most_tiles(c.num_seqs, c.num_tokens, c.num_adapters) + (c.num_tokens + kTileRows - 1) / kTileRows;
     if (cluster_pays(c, all_tiles)) return launch_few(c, all_tiles, cluster_blocks(all_tiles), st);
+    const long long work = (long long)c.num_tokens * c.n * c.max_rank;
+    const bool wide = c.num_tokens >= kWideTokens && c.max_rank <= kLoraWideRank && c.num_adapters > 0 &&
+                      work >= (c.max_rank > kSmallRank ? kWideWork : kWideWorkSmallRank);
+    if (wide && (c.max_rank > kSmallRank || (long long)c.num_tokens * c.k >= kWideElements)) {
+        if (launch_lora_shrink_wide(c, error_word(dev), st)) return -1;
+        pdl_scope beside(true);  // as below
+        return launch_lora_expand_wide(c, true, error_word(dev), st);
+    }
     // as many blocks as the most tiles that there can be need, one or two for each SM at most
     const long long tiles = most_tiles(c.num_seqs, c.num_tokens, c.num_adapters);
     const long long shrink = std::min<long long>(kTargetBlocks, tiles * parts_of(1, c.k));
@@ -712,8 +722,7 @@ int launch_lora(const LoraCall& c, cudaStream_t st) {
     const long long across = (c.n + kBlockCols - 1) / kBlockCols;
     const long long expand = std::min<long long>(kTargetBlocks, (tiles + (c.num_tokens + kTileRows - 1) / kTileRows) * across);
     pdl_scope beside(shrink > 0);  // the second kernel starts while the first one ends, and waits for it
-    if (c.num_tokens >= kWideTokens && c.max_rank <= kLoraWideRank && (long long)c.num_tokens * c.n * c.max_rank >= kWideWork)
-        return launch_lora_expand_wide(c, error_word(dev), st);
+    if (wide) return launch_lora_expand_wide(c, false, error_word(dev), st);
     return launch_k(lora_expand_kernel, dim3((unsigned)expand), dim3(kThreads), expand_smem, st, c) == cudaSuccess ? 0 : -1;
 }
 

@@ -1,6 +1,10 @@
-// Low-rank adapters, many rows: base + scale * h B^T on tcgen05, h the low-rank product that lora.cu left in the
-// workspace. What an output costs is the base's element in and its own out, 4 bytes for 2 * rank operations, so all is
-// built to keep those moving: a persistent block for each SM goes over items of 128 rows of one adapter and 128 outputs.
+// Low-rank adapters, many rows, on tcgen05. First x A^T (lora_shrink_wide_kernel): tiles of rows of one adapter, cut over
+// K; 8 warps copy both operands into a ring of stages, one issues the products, and the 8 store the sums from TMEM.
+// Against mma.sync (lora.cu), whose few warps wait for their matrix loads, whole calls with the same second product, us:
+// rank 64, 9288 rows of 2048, 8192 outputs 86 / 85; 16384 rows of 14336, rank 128, 4096 outputs 296 / 169.
+// Then base + scale * h B^T, h being those sums. What an output costs is the base's element in and its own out, 4 bytes for 2 *
+// rank operations, so all is built to keep those moving: a persistent block for each SM goes over items of 128 rows of one
+// adapter and 128 outputs.
 //   loaders   (8 warps) B's rows and the base's rows into a ring of stages, 16 bytes a copy, items ahead; for each new
 //             tile h as two fp16 numbers an element (h = 2^e (high + low), e by the row's largest element, so that
 //             neither overflows and 22 bits are kept), in the operands' swizzled layout;
@@ -39,6 +43,7 @@ struct Cfg {
 struct Args {
     LoraCall c;
     unsigned* err;
+    bool split;  // the first product is lora_shrink_wide_kernel's, cut as split_of() says
 };
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -56,10 +61,10 @@ __device__ __forceinline__ uint32_t elect_one() {
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
     return r;
 }
-__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t acc) {
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d, uint64_t a, uint64_t b, uint32_t acc, uint32_t idesc) {
     asm volatile(
         "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(kIdesc), "r"(acc),
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc),
         "r"(leader));
 }
 __device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
@@ -94,6 +99,210 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, unsigned parity, vo
     return false;
 }
 
+// ---- x A^T
+// Which tiles this kernel goes over, and how many parts of K: what takes less, counted in elements of a row of either
+// operand that a block goes through, one wave after another, and kPartCost of them for each part, which the second product's
+// kernel has to add up. Whole calls with as many parts as there are SMs for / as many as here, us: rank 64, K 2048, 8192
+// outputs, 1024 tokens 30.8 / 22.6; K 14336, 4096 outputs, 512 tokens 34.9 / 25.5. Tiles of 64 / 128 rows: rank 64, K 8192, 2048
+// outputs, 16384 tokens 106 / 96; 18000 tokens of 40 adapters 115 / 129.
+constexpr float kPartCost = 65536.0f;
+struct Split {
+    int rows, tiles, parts;
+};
+__device__ __forceinline__ Split split_of(const LoraCall& c, const Plan& p) {
+    auto cut = [&](int rows, int tiles) {
+        const int best = (int)(sqrtf((float)c.k * (float)(rows + c.max_rank) / kPartCost) + 0.5f);
+        return Split{rows, tiles, max(1, min(parts_of(tiles, c.k), best))};
+    };
+    auto cost = [&](const Split& s) {
+        const float waves = (float)((s.tiles * s.parts + kTargetBlocks - 1) / kTargetBlocks);
+        return waves * (float)c.k * (float)(s.rows + c.max_rank) / (float)s.parts + kPartCost * (float)s.parts;
+    };
+    const Split wide = cut(kWideRows, p.wide_tiles), narrow = cut(kTileRows, p.tiles);
+    return cost(wide) < cost(narrow) ? wide : narrow;
+}
+
+__host__ __device__ constexpr int shrink_stages(int rp) { return rp == 64 ? 4 : 3; }
+template <int RP, int ROWS>
+struct ShrinkCfg {
+    static constexpr int kStages = shrink_stages(RP), kLag = kStages - 2;
+    static constexpr int kBlockX = ROWS * 128, kBlockA = RP * 128, kBlocks = 2, kChunk = 64 * kBlocks;  // rows of 64 elements of K
+    static constexpr int kA = kBlocks * kBlockX, kStage = kA + kBlocks * kBlockA;
+    static constexpr int smem = kStages * kStage + 1024;
+};
+
+template <int STAGES>
+struct ShrinkBars {
+    uint64_t full[STAGES], empty[STAGES], acc_full, acc_empty, drain;
+};
+
+template <int RP, int ROWS>
+__device__ __forceinline__ void shrink_items(const Args& a, const Plan& p, int tiles, int parts, uint8_t* smem,
+                                             ShrinkBars<shrink_stages(RP)>& b, uint32_t tmem, volatile int* abort) {
+    using C = ShrinkCfg<RP, ROWS>;
+    const int4* const list = ROWS == kWideRows ? p.wide : p.tile;
+    const LoraCall& c = a.c;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int chunks = (c.k + C::kChunk - 1) / C::kChunk;
+    int n = 0, product = 0;  // chunks and items with a product so far
+    bool ok = true;
+    for (int item = blockIdx.x; item < tiles * parts && ok; item += gridDim.x) {
+        const int part = item % parts;
+        const int4 tile = __ldg(list + item / parts);
+        int rank = c.ranks ? __ldg(c.ranks + tile.x) : c.max_rank;
+        if (rank < 0 || rank > c.max_rank) {
+            if (tid == 0) atomicCAS(a.err, 0u, (unsigned)kDevBadList);
+            rank = 0;
+        }
+        if (rank == 0) continue;
+        const int from = (int)((long long)chunks * part / parts), count = (int)((long long)chunks * (part + 1) / parts) - from;
+        const int padded = (rank + 15) / 16 * 16, live_cols = count ? rank : 0;  // without a K nothing is multiplied
+        if (warp < kLoaders) {
+            const int piece = tid & 7, row = tid >> 3;  // a thread copies one piece of every 32nd row
+            const int k1 = min(c.k, (from + count) * C::kChunk);
+            const __half* xp[ROWS / 32];
+#pragma unroll
+            for (int i = 0; i < ROWS / 32; ++i)
+                xp[i] = row + 32 * i < tile.z ? c.x + (long long)__ldg(p.row + tile.y + row + 32 * i) * c.x_stride : nullptr;
+            const __half* ap = c.a + ((long long)tile.x * c.max_rank + row) * c.k;
+            const uint32_t to = smem_u32(smem) + row * 128 + ((piece ^ (row & 7)) << 4);
+            auto hand_on = [&](int i) {  // chunk i's copies of this thread are there
+                fence_proxy_async_shared();
+                mbar_arrive(&b.full[(n + i) % C::kStages]);
+            };
+            for (int i = 0; i < count; ++i) {
+                const int stage = (n + i) % C::kStages;
+                if (n + i >= C::kStages) {
+                    ok = __all_sync(0xffffffffu, wait_or_abort(&b.empty[stage], ((n + i) / C::kStages - 1) & 1, abort));
+                    if (!ok) break;
+                }
+#pragma unroll
+                for (int block = 0; block < C::kBlocks; ++block) {
+                    const int k = (from + i) * C::kChunk + block * 64 + piece * 8;
+                    const uint32_t at = to + stage * C::kStage;
+#pragma unroll
+                    for (int j = 0; j < ROWS / 32; ++j) {
+                        const bool live = xp[j] && k < k1;
+                        copy_or_zero(at + block * C::kBlockX + j * 32 * 128, live ? xp[j] + k : c.x, live ? 16 : 0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < RP / 32; ++j)
+                        if (row + 32 * j < padded) {
+                            const bool live = row + 32 * j < rank && k < k1;
+                            copy_or_zero(at + C::kA + block * C::kBlockA + j * 32 * 128, live ? ap + (long long)j * 32 * c.k + k : c.a,
+                                         live ? 16 : 0);
+                        }
+                }
+                cp_async_commit();
+                if (i >= C::kLag) {
+                    cp_async_wait<C::kLag>();
+                    hand_on(i - C::kLag);
+                }
+            }
+            if (!ok) break;
+            cp_async_wait<0>();
+            for (int i = max(0, count - C::kLag); i < count; ++i) hand_on(i);
+            ok = __all_sync(0xffffffffu, wait_or_abort(&b.acc_full, product & 1, abort));
+            if (!ok) break;
+            tc_fence_after();
+            const int quarter = warp & 3, half = warp >> 2, at = quarter * 32 + lane;
+            float* out = c.ws + ((long long)part * p.rows + tile.y + at) * c.max_rank;
+#pragma unroll
+            for (int j = 0; j < RP / 64; ++j) {
+                const int col = half * (RP / 2) + j * 32;
+                float d[32];
+                tmem_ld32(tmem + ((uint32_t)(quarter * 32) << 16) + col, d);
+#pragma unroll
+                for (int i = 0; i < 32; i += 4)
+                    if (at < tile.z && col + i < c.max_rank)
+                        *reinterpret_cast<float4*>(out + col + i) =
+                            make_float4(col + i < live_cols ? d[i] : 0.0f, col + i + 1 < live_cols ? d[i + 1] : 0.0f,
+                                        col + i + 2 < live_cols ? d[i + 2] : 0.0f, col + i + 3 < live_cols ? d[i + 3] : 0.0f);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b.acc_empty);
+        } else {
+            const uint32_t leader = elect_one(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+            const uint32_t idesc = (1u << 4) | ((uint32_t)(padded >> 3) << 17) | ((128u >> 4) << 24);
+            if (product) ok = __all_sync(0xffffffffu, wait_or_abort(&b.acc_empty, (product - 1) & 1, abort));
+            for (int i = 0; i < count && ok; ++i) {
+                const int stage = (n + i) % C::kStages;
+                ok = __all_sync(0xffffffffu, wait_or_abort(&b.full[stage], ((n + i) / C::kStages) & 1, abort));
+                if (!ok) break;
+                tc_fence_after();
+                const uint64_t xd = desc(smem_u32(smem + stage * C::kStage)), ad = desc(smem_u32(smem + stage * C::kStage + C::kA));
+#pragma unroll
+                for (int k = 0; k < C::kChunk / 16; ++k)
+                    mma_ss(leader, tm, xd + ((k >> 2) * C::kBlockX + (k & 3) * 32) / 16, ad + ((k >> 2) * C::kBlockA + (k & 3) * 32) / 16,
+                           i > 0 || k > 0, idesc);
+                commit(leader, &b.empty[stage]);
+            }
+            if (!ok) break;
+            commit(leader, &b.acc_full);
+        }
+        n += count;
+        ++product;
+    }
+}
+
+// An item is a part of a tile. RP: rows of A that a stage has room for (the products have the rank, rounded up to 16). Rows
+// 64 to 127 of the products of a tile of 64 are of what follows in shared memory, and not stored.
+template <int RP>
+__global__ void __launch_bounds__(kLoadThreads + 32, 1) lora_shrink_wide_kernel(const __grid_constant__ Args a) {
+    constexpr int kStages = shrink_stages(RP);
+    extern __shared__ uint8_t raw_smem[];
+    __shared__ __align__(8) ShrinkBars<kStages> b;
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_abort;
+    const LoraCall& c = a.c;
+    uint8_t* smem = raw_smem + (1024 - (smem_u32(raw_smem) & 1023) & 1023);
+    const int tid = threadIdx.x, warp = tid >> 5;
+    pdl_launch_dependents();
+    pdl_wait();
+    Plan p;
+    if (!read_plan(c, &p)) {
+        if (tid == 0) atomicCAS(a.err, 0u, (unsigned)kDevBadList);
+        return;
+    }
+    if (warp == kLoaders) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)), "r"(128)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            mbar_init(&b.full[i], kLoadThreads);
+            mbar_init(&b.empty[i], 1);
+        }
+        mbar_init(&b.acc_full, 1);
+        mbar_init(&b.acc_empty, kLoaders);
+        mbar_init(&b.drain, 1);
+        fence_mbar_init();
+        s_abort = 0;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const Split split = split_of(c, p);
+    if (split.rows == kWideRows) shrink_items<RP, kWideRows>(a, p, split.tiles, split.parts, smem, b, s_tmem, &s_abort);
+    else shrink_items<RP, kTileRows>(a, p, split.tiles, split.parts, smem, b, s_tmem, &s_abort);
+    if (warp == kLoaders) {
+        commit(elect_one(), &b.drain);  // no product may run on when the block leaves
+        mbar_wait_bounded(&b.drain, 0);
+    }
+    cp_async_wait<0>();
+    tc_fence_before();
+    __syncwarp();
+    __syncthreads();
+    if (tid == 0 && s_abort) atomicCAS(a.err, 0u, (unsigned)kDevTmaTimeout);
+    if (warp == kLoaders) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s_tmem), "r"(128) : "memory");
+    }
+}
+
+// ---- base + scale * h B^T
 // The block's items in order: tiles, and for each its blocks of outputs. Rows without an adapter follow as tiles of
 // rank 0, where they have to be copied.
 struct Walk {
@@ -189,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_wide_kernel(const __g
 
     if (warp < kLoaders) {
         const uint32_t at_smem = smem_u32(smem);
-        const int parts = parts_of(p.tiles, c.k);
+        const int parts = a.split ? split_of(c, p).parts : parts_of(p.tiles, c.k);
         int list = -1, tiles_h = 0, item = 0;
         bool waited = false, ok = true;  // once a wait has given up, only the barriers that warps share are met
         auto hand_on = [&](int i) {  // item i's copies of this thread are there
@@ -305,7 +514,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_wide_kernel(const __g
                 for (int k = 0; k < RP / 16; ++k) {
                     if (k >= steps) break;
                     const uint64_t in = ((k >> 2) * (128 * 128) + (k & 3) * 32) / 16;  // both operands have 128 rows
-                    mma_ss(leader, tm + acc * kCols, hd + part * (C::kBytesH / 32) + in, bd + in, part > 0 || k > 0);
+                    mma_ss(leader, tm + acc * kCols, hd + part * (C::kBytesH / 32) + in, bd + in, part > 0 || k > 0, kIdesc);
                 }
             commit(leader, &acc_full[acc]);
             commit(leader, &empty[stage]);
@@ -391,7 +600,25 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_wide_kernel(const __g
 }
 
 template <int RP>
-int launch(const LoraCall& c, unsigned* error_word, cudaStream_t st) {
+int launch_shrink(const LoraCall& c, unsigned* error_word, cudaStream_t st) {
+    constexpr int smem = ShrinkCfg<RP, kWideRows>::smem;
+    static std::atomic<unsigned long long> set{0};  // a bit a device
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (!(set.load() >> (dev & 63) & 1)) {
+        if (cudaFuncSetAttribute(lora_shrink_wide_kernel<RP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+            return -1;
+        set.fetch_or(1ull << (dev & 63));
+    }
+    Args a = {c, error_word, true};
+    if (!a.err) return -1;
+    const long long tiles = most_tiles(c.num_seqs, c.num_tokens, c.num_adapters);
+    const long long items = std::min<long long>(kNumSMs, tiles * parts_of(1, c.k));
+    return launch_k(lora_shrink_wide_kernel<RP>, dim3((unsigned)items), dim3(kLoadThreads + 32), smem, st, a) == cudaSuccess ? 0 : -1;
+}
+
+template <int RP>
+int launch(const LoraCall& c, bool split, unsigned* error_word, cudaStream_t st) {
     using C = Cfg<RP>;
     static std::atomic<unsigned long long> set{0};  // a bit a device
     int dev = 0;
@@ -401,7 +628,7 @@ int launch(const LoraCall& c, unsigned* error_word, cudaStream_t st) {
             return -1;
         set.fetch_or(1ull << (dev & 63));
     }
-    Args a = {c, error_word};
+    Args a = {c, error_word, split};
     if (!a.err) return -1;
     const long long tiles = most_tiles(c.num_seqs, c.num_tokens, c.num_adapters, kWideRows) + (c.num_tokens + kWideRows - 1) / kWideRows;
     const long long items = tiles * ((c.n + kCols - 1) / kCols);
@@ -413,8 +640,11 @@ int launch(const LoraCall& c, unsigned* error_word, cudaStream_t st) {
 
 }  // namespace
 
-int launch_lora_expand_wide(const LoraCall& c, unsigned* error_word, cudaStream_t st) {
-    return c.max_rank <= 64 ? launch<64>(c, error_word, st) : launch<128>(c, error_word, st);
+int launch_lora_shrink_wide(const LoraCall& c, unsigned* error_word, cudaStream_t st) {
+    return c.max_rank <= 64 ? launch_shrink<64>(c, error_word, st) : launch_shrink<128>(c, error_word, st);
+}
+int launch_lora_expand_wide(const LoraCall& c, bool split, unsigned* error_word, cudaStream_t st) {
+    return c.max_rank <= 64 ? launch<64>(c, split, error_word, st) : launch<128>(c, split, error_word, st);
 }
 
 }  // namespace batch

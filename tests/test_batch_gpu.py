@@ -158,7 +158,7 @@ class Lora:
         ad = max(self.ad, 1)
         self.a, self.b = make(ad, self.top, k), make(ad, n, self.top)
         if not integers:
-            self.a = (self.a * (k ** -0.5 * spread)).astype(np.float16)
+            self.a = (self.a * (max(k, 1) ** -0.5 * spread)).astype(np.float16)
         for i, r in enumerate(self.ranks):
             self.a[i, r:], self.b[i, :, r:] = np.nan, np.nan
         self.scales = (rng.random(ad) + 0.5).astype(np.float32) if scales else np.ones(ad, np.float32)
@@ -289,11 +289,11 @@ def test_lora_infinities_and_nan_stay_in_their_rows():
 
 
 @pytest.mark.parametrize("rank", [1, 3, 8, 21])
-@pytest.mark.parametrize("counts,ids,n", [([6], [0], 72), ([40], [0], 72), ([100], [0], 72), (None, [0, 0], 1608)])
+@pytest.mark.parametrize("counts,ids,n", [([6], [0], 72), ([40], [0], 72), ([100], [0], 72), (None, [0, 0], 1608), ([300], [0], 2800)])
 def test_lora_an_infinity_keeps_its_sign(counts, ids, n, rank):
     """Factors of one sign: the row's results are infinities, whatever the rank is padded with."""
     rng = np.random.default_rng(rank)
-    top = 24 if counts else 64
+    top = 40 if n == 2800 else 24 if counts else 64  # 40, 64: both products by the kernels of much work
     call = Lora(counts or _wide(n, top, [70, 60]), ids, [rank], 128, n, rng, top=top)
     call.a, call.b, call.x = np.abs(call.a), np.abs(call.b) + np.float16(0.01), np.abs(call.x) + np.float16(0.01)
     call.a[0, :rank] += np.float16(0.01)
@@ -539,6 +539,55 @@ def test_lora_many_rows_keep_their_bits():
         ends = np.cumsum(order)
         call.seqs = list(zip([0] + ends[:-1].tolist(), ends.tolist()))
         call.off.copy_(t.tensor([0] + ends.tolist(), dtype=t.int32))
+        call.out.fill_(np.float16(123.0).view(np.int16).item())
+        for _ in range(3):
+            graph.replay()
+        call.check()
+
+
+# Ranks above 32 and 2^25 of work: the first product on the same tensor cores, its tiles of 64 or 128 rows, whole or in
+# parts of K.
+@pytest.mark.parametrize("k", [0, 8, 72, 136, 264, 1000, 2056])
+@pytest.mark.parametrize("ranks", [[33], [64, 3, 17], [100, 0, 128]])
+def test_lora_first_product_of_many_rows(k, ranks):
+    rng = np.random.default_rng(k + len(ranks))
+    counts = [150, 64, 0, 65, 1, 130]
+    ids = [0, 1, 2, 2, -1, 0] if len(ranks) > 1 else [0, 0, 0, 0, -1, 0]
+    top = max(40, -(-max(ranks) // 8) * 8)
+    n = -(-2 ** 25 // (sum(counts) * top) // 8) * 8 + 8
+    Lora(counts, ids, ranks, k, n, rng, top=top, extra=7, pad=8).both()
+
+
+@pytest.mark.parametrize("t,k,ranks", [(64, 4096, [48]), (300, 14344, [40, 33]), (9600, 136, [64]), (30000, 136, [64, 20]),
+                                       (20000, 136, [40]), (16400, 2056, [16]), (8200, 4104, [8, 32])])
+def test_lora_first_product_by_tiles_and_parts(t, k, ranks):
+    """Few tiles in many parts; more tiles than there are blocks, of either height; ranks up to 32 of much work."""
+    rng = np.random.default_rng(t)
+    top = -(-max(ranks) // 8) * 8
+    work = 2 ** 25 if top > 32 else 2 ** 27
+    n = max(24, -(-work // (t * top) // 8) * 8 + 8)
+    counts = [t // 2 + 3, t - t // 2 - 3]
+    Lora(counts, [0, len(ranks) - 1], ranks, k, n, rng, top=top, extra=3).both()
+
+
+def test_lora_first_product_of_many_rows_replayed():
+    """Other tokens, adapters and rows by the same graph, its second kernel launched while the first one ends."""
+    t = torch()
+    rng = np.random.default_rng(91)
+    call = Lora([200, 100, 90], [0, 1, 1], [64, 40], 1032, 2048, rng)
+    stream = t.cuda.Stream()
+    stream.wait_stream(t.cuda.current_stream())
+    with t.cuda.stream(stream):
+        call.plan(stream.cuda_stream)
+        call.run(stream=stream.cuda_stream)
+    stream.synchronize()
+    graph = t.cuda.CUDAGraph()
+    with t.cuda.graph(graph, stream=stream):
+        call.plan(t.cuda.current_stream().cuda_stream)
+        call.run(stream=t.cuda.current_stream().cuda_stream)
+    for ids in ([1, 0, 0], [-1, -1, 0], [0, 0, 0]):
+        call.ids = ids
+        call.did.copy_(t.tensor(ids, dtype=t.int32))
         call.out.fill_(np.float16(123.0).view(np.int16).item())
         for _ in range(3):
             graph.replay()
