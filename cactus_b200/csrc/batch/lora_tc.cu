@@ -122,10 +122,12 @@ __device__ __forceinline__ Split split_of(const LoraCall& c, const Plan& p) {
     return cost(wide) < cost(narrow) ? wide : narrow;
 }
 
-__host__ __device__ constexpr int shrink_stages(int rp) { return rp == 64 ? 4 : 3; }
+// stages of the ring, in 192 KB (tiles of 64 rows, four stages instead of six: 18000 rows of 14336 of 40 adapters, rank 128, 246
+// us for 234)
+__host__ __device__ constexpr int shrink_stages(int rp, int rows) { return 192 * 1024 / (256 * (rp + rows)); }
 template <int RP, int ROWS>
 struct ShrinkCfg {
-    static constexpr int kStages = shrink_stages(RP), kLag = kStages - 2;
+    static constexpr int kStages = shrink_stages(RP, ROWS), kLag = kStages - 2;
     static constexpr int kBlockX = ROWS * 128, kBlockA = RP * 128, kBlocks = 2, kChunk = 64 * kBlocks;  // rows of 64 elements of K
     static constexpr int kA = kBlocks * kBlockX, kStage = kA + kBlocks * kBlockA;
     static constexpr int smem = kStages * kStage + 1024;
@@ -138,7 +140,7 @@ struct ShrinkBars {
 
 template <int RP, int ROWS>
 __device__ __forceinline__ void shrink_items(const Args& a, const Plan& p, int tiles, int parts, uint8_t* smem,
-                                             ShrinkBars<shrink_stages(RP)>& b, uint32_t tmem, volatile int* abort) {
+                                             ShrinkBars<shrink_stages(RP, kTileRows)>& b, uint32_t tmem, volatile int* abort) {
     using C = ShrinkCfg<RP, ROWS>;
     const int4* const list = ROWS == kWideRows ? p.wide : p.tile;
     const LoraCall& c = a.c;
@@ -250,7 +252,7 @@ __device__ __forceinline__ void shrink_items(const Args& a, const Plan& p, int t
 // 64 to 127 of the products of a tile of 64 are of what follows in shared memory, and not stored.
 template <int RP>
 __global__ void __launch_bounds__(kLoadThreads + 32, 1) lora_shrink_wide_kernel(const __grid_constant__ Args a) {
-    constexpr int kStages = shrink_stages(RP);
+    constexpr int kStages = shrink_stages(RP, kTileRows);  // at the most
     extern __shared__ uint8_t raw_smem[];
     __shared__ __align__(8) ShrinkBars<kStages> b;
     __shared__ uint32_t s_tmem;
