@@ -594,6 +594,32 @@ def test_lora_first_product_of_many_rows_replayed():
         call.check()
 
 
+def test_lora_first_product_of_many_rows_refuses_lists_on_the_device():
+    """As test_lora_refuses_lists_on_the_device."""
+    rng = np.random.default_rng(92)
+    for rank in (65, -1):
+        call = Lora([200, 100], [0, 1], [64, 40], 136, 2048, rng)
+        call.dr = dev(np.array([64, rank], np.int32))
+        call.plan()
+        call.run()
+        assert _err() == 4
+        call.ids = [0, -1]
+        call.check()
+    call = Lora([200, 100], [0, 1], [64, 40], 136, 2048, rng)  # a plan of other numbers
+    call.plan()
+    call.did = dev(np.array([0, 1, 0], np.int32))
+    call.ids = [0, 1, 0]
+    call.pb = batch.lora_plan_bytes(3, call.t, 2)
+    call.dplan = torch().cat([call.dplan, call.dplan])
+    call.run()
+    assert (call.got() == np.float16(123.0)).all() and _err() == 4
+    call = Lora([200, 100], [0, 1], [64, 40], 136, 2048, rng)  # lists that fall: a plan without rows
+    call.off = dev(np.array([0, 200, 100], np.int32))
+    call.plan()
+    call.run()
+    assert (call.got() == np.float16(123.0)).all() and _err() == 4
+
+
 def test_lora_many_rows_infinities_and_nan_stay_in_their_rows():
     rng = np.random.default_rng(16)
     call = Lora(_wide(1608, 64, [300, 290]), [0, 1], [64, 40], 128, 1608, rng)
