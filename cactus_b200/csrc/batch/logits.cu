@@ -1,11 +1,10 @@
 // Penalties, biases and masks on a batch's logits. A block takes a slice of a row's vocabulary: it notes which of the
-// slice's tokens the row's history or biases name, passes over the slice in 16-byte pieces for the mask, and then
+// slice's tokens the row's history or biases name, and where, passes over the slice in 16-byte pieces for the mask, and then
 // counts and computes the noted tokens. Each logit is read and written once, what a mask hides only written, and in
-// place what stays is not touched. 256 rows of 128256 with histories of 750 to 1500 ids take 38 us, 3.5 TB/s of what that
+// place what stays is not touched. 256 rows of 128256 with histories of 750 to 1500 ids take 37 us, 3.6 TB/s of what that
 // moves; the barriers between noting, passing and counting bound it (with counters for every token of a slice, which
-// left room for two blocks a SM, it took 92). Masks alone, in place: 48 rows of 262144 9.0 us.
-#include <atomic>
-
+// left room for two blocks a SM, it took 92; with the lists read once more for the count 39). Masks alone, in place: 48
+// rows of 262144 9.0 us.
 #include "../common.cuh"
 #include "batch_ops.h"
 
@@ -15,15 +14,17 @@ namespace batch {
 namespace {
 
 constexpr unsigned kSeen = 0x80000000u;  // the history has it; the other bits: how often behind the prompt
+constexpr int kKept = 512;               // entries of the lists in a slice that are kept for the count
 constexpr int kRound = 1024;             // noted tokens that are counted at a time
 
 // T threads, V pieces of 8 tokens a thread. Shared memory: bits of the noted tokens, their numbers (in the order of
-// their noting), and of one round the counts, last biases and tokens.
+// their noting), of one round the counts, last biases and tokens, and the entries that are kept: place in the list and token.
 template <int T, int V>
 struct Slice {
     static constexpr int kTokens = T * 8 * V;
     static constexpr int kNumbers = kTokens / 8, kCounts = kNumbers + 2 * kTokens, kBiases = kCounts + 4 * kRound;
-    static constexpr int kList = kBiases + 4 * kRound, smem = kList + 2 * kRound;
+    static constexpr int kList = kBiases + 4 * kRound, kPlaces = kList + 2 * kRound, kAts = kPlaces + 4 * kKept;
+    static constexpr int smem = kAts + 2 * kKept;
     static_assert(kTokens <= 65536, "16-bit numbers");
 };
 
@@ -72,7 +73,9 @@ __global__ void __launch_bounds__(T, T == 512 ? 3 : 1) logits_kernel(LogitsCall 
     unsigned* s_count = reinterpret_cast<unsigned*>(smem + S::kCounts);
     int* s_bias = reinterpret_cast<int*>(smem + S::kBiases);  // place of a token's last bias + 1
     uint16_t* s_list = reinterpret_cast<uint16_t*>(smem + S::kList);
-    __shared__ int s_noted;
+    int* s_place = reinterpret_cast<int*>(smem + S::kPlaces);
+    uint16_t* s_at = reinterpret_cast<uint16_t*>(smem + S::kAts);
+    __shared__ int s_noted, s_kept;
     pdl_launch_dependents();
     pdl_wait();
     const int row = blockIdx.x;
@@ -82,11 +85,36 @@ __global__ void __launch_bounds__(T, T == 512 ? 3 : 1) logits_kernel(LogitsCall 
     const bool in_place = in == out, same_skew = (int)(reinterpret_cast<uintptr_t>(out) >> 1 & 7) == skew;
     const int v0 = blockIdx.y * S::kTokens - skew;
     if (v0 >= c.vocab) return;
+    List history = {0, 0}, biases = {0, 0};
+    if (c.penalties) history = list_of(c.history_offsets, row, c.num_history);
+    if (c.bias_ids) biases = list_of(c.bias_offsets, row, c.num_biases);
+    const uint32_t *ids = c.history + history.first, *bias_ids = c.bias_ids + biases.first;
+    const bool lists = history.count + biases.count > 0;
     const uint32_t* mask = nullptr;
     if (c.masks) {
         const int m = c.mask_ids ? __ldg(c.mask_ids + row) : row;
         if (m >= 0 && m < c.num_masks) mask = c.masks + m * c.mask_stride;
         else if (m != -1 && threadIdx.x == 0) report_dev_error(kDevBadList);
+    }
+    // the slice's tokens among the ids; one before the slice wraps around
+    auto inside = [&](unsigned id) { return id - (unsigned)v0 < (unsigned)S::kTokens && id < (unsigned)c.vocab; };
+    if (lists) {  // the tokens that they name get numbers
+        for (int i = threadIdx.x; i < S::kTokens / 32; i += T) s_bits[i] = 0;
+        for (int i = threadIdx.x; i < kRound; i += T) s_count[i] = 0, s_bias[i] = 0;
+        if (threadIdx.x == 0) s_noted = s_kept = 0;
+        __syncthreads();
+        auto note = [&](unsigned id, int i) {
+            const unsigned at = id - (unsigned)v0;
+            if (inside(id)) {
+                const int kept = atomicAdd(&s_kept, 1);
+                if (kept < kKept) s_place[kept] = i, s_at[kept] = (uint16_t)at;
+                if (!(atomicOr(&s_bits[at >> 5], 1u << (at & 31)) >> (at & 31) & 1u)) s_number[at] = (uint16_t)atomicAdd(&s_noted, 1);
+            } else if (id >= (unsigned)c.vocab) {
+                report_dev_error(kDevBadList);
+            }
+        };
+        each<T>(ids, history.count, note);
+        each<T>(bias_ids, biases.count, [&](unsigned id, int i) { note(id, i - biases.count); });
     }
     // the pieces: what a mask leaves nothing of is not read, and in place neither is what stays whole
     unsigned bits[V];
@@ -109,30 +137,6 @@ __global__ void __launch_bounds__(T, T == 512 ? 3 : 1) logits_kernel(LogitsCall 
             for (int j = 0; j < 8; ++j)
                 if (v + j >= 0 && v + j < c.vocab) reinterpret_cast<__half*>(&x[i])[j] = in[v + j];
         }
-    }
-    // the tokens that the lists name get numbers
-    List history = {0, 0}, biases = {0, 0};
-    if (c.penalties) history = list_of(c.history_offsets, row, c.num_history);
-    if (c.bias_ids) biases = list_of(c.bias_offsets, row, c.num_biases);
-    const uint32_t *ids = c.history + history.first, *bias_ids = c.bias_ids + biases.first;
-    const bool lists = history.count + biases.count > 0;
-    // the slice's tokens among the ids; one before the slice wraps around
-    auto inside = [&](unsigned id) { return id - (unsigned)v0 < (unsigned)S::kTokens && id < (unsigned)c.vocab; };
-    if (lists) {
-        for (int i = threadIdx.x; i < S::kTokens / 32; i += T) s_bits[i] = 0;
-        for (int i = threadIdx.x; i < kRound; i += T) s_count[i] = 0, s_bias[i] = 0;
-        if (threadIdx.x == 0) s_noted = 0;
-        __syncthreads();
-        auto note = [&](unsigned id, int) {
-            const unsigned at = id - (unsigned)v0;
-            if (inside(id)) {
-                if (!(atomicOr(&s_bits[at >> 5], 1u << (at & 31)) >> (at & 31) & 1u)) s_number[at] = (uint16_t)atomicAdd(&s_noted, 1);
-            } else if (id >= (unsigned)c.vocab) {
-                report_dev_error(kDevBadList);
-            }
-        };
-        each<T>(ids, history.count, note);
-        each<T>(bias_ids, biases.count, note);
     }
     // the pass over the slice
     const __half none = __ushort_as_half(0xFC00);
@@ -172,20 +176,25 @@ __global__ void __launch_bounds__(T, T == 512 ? 3 : 1) logits_kernel(LogitsCall 
         __syncthreads();  // the pass has written what the results replace; numbers and zeros are there
         const int noted = min(s_noted - first, kRound);
         if (noted <= 0) break;
-        auto number = [&](unsigned id) { return inside(id) ? (unsigned)s_number[id - (unsigned)v0] - (unsigned)first : 0xffffffffu; };
-        each<T>(ids, history.count, [&](unsigned id, int i) {
-            const unsigned n = number(id);
+        // of the token at a place of the slice: place i of the history, or, with i below 0, i + their count of the biases
+        auto count = [&](unsigned at, int i) {
+            const unsigned n = (unsigned)s_number[at] - (unsigned)first;
             if (n >= (unsigned)kRound) return;
-            s_list[n] = (uint16_t)(id - (unsigned)v0);
-            if (i >= prompt) atomicAdd(&s_count[n], 1u);
-            atomicOr(&s_count[n], kSeen);
-        });
-        each<T>(bias_ids, biases.count, [&](unsigned id, int i) {
-            const unsigned n = number(id);
-            if (n >= (unsigned)kRound) return;
-            s_list[n] = (uint16_t)(id - (unsigned)v0);
-            atomicMax(&s_bias[n], i + 1);
-        });
+            s_list[n] = (uint16_t)at;
+            if (i < 0) atomicMax(&s_bias[n], i + biases.count + 1);
+            else if (i >= prompt) atomicAdd(&s_count[n], 1u);
+            else atomicOr(&s_count[n], kSeen);
+        };
+        if (s_kept <= kKept) {  // else the lists once more
+            for (int i = threadIdx.x; i < s_kept; i += T) count(s_at[i], s_place[i]);
+        } else {
+            each<T>(ids, history.count, [&](unsigned id, int i) {
+                if (inside(id)) count(id - (unsigned)v0, i);
+            });
+            each<T>(bias_ids, biases.count, [&](unsigned id, int i) {
+                if (inside(id)) count(id - (unsigned)v0, i - biases.count);
+            });
+        }
         __syncthreads();
         for (int i = threadIdx.x; i < noted; i += T) {
             const int v = v0 + s_list[i];
