@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_shrink_kernel(LoraCall c) {
 
 // ---- base + scale * h B^T
 // A tile's low-rank rows h go to shared memory once, as two fp16 numbers an element (h = 2^e (high + low), e by the
-// row's largest element, so that neither overflows and 22 bits are kept), and the block's warps take 32 outputs of
+// row's largest finite element, so that neither overflows and 22 bits are kept), and the block's warps take 32 outputs of
 // all 64 rows at a time. The columns of the products are dealt out so that a lane's are 8 consecutive outputs (one
 // 16-byte load and store a row), the steps over the rank so that a lane's elements of B are 4 consecutive ones.
 constexpr int kWarpCols = 32, kBlockCols = kWarps * kWarpCols;
@@ -376,7 +376,7 @@ __device__ __forceinline__ void store_h(const LoraCall& c, const int4& tile, con
     const int row = threadIdx.x >> 2, q = threadIdx.x & 3;
     float top = 0.0f;
 #pragma unroll
-    for (int i = 0; i < RP / 16; ++i) top = fmaxf(top, largest_of(v[i]));
+    for (int i = 0; i < RP / 16; ++i) top = fmaxf(top, largest_finite(v[i]));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     const int e = exponent_of(top);

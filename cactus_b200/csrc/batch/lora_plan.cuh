@@ -61,9 +61,10 @@ __device__ __forceinline__ bool read_plan(const LoraCall& c, Plan* p) {
     return true;
 }
 
-// 2^e with a row's largest element below 2^12 of it; rows with infinities, NaN or nothing but zeros stay as they are
+// 2^e with a row's largest finite element, `top`, below 2^12 of it (an infinity or a NaN beside it is one at any power,
+// but what is finite must not become one); rows without such an element or with nothing but zeros stay as they are
 __device__ __forceinline__ int exponent_of(float top) {
-    return top > 0.0f && top < INFINITY ? max((int)(__float_as_uint(top) >> 23) - 127 - 11, -125) : 0;
+    return top > 0.0f ? max((int)(__float_as_uint(top) >> 23) - 127 - 11, -125) : 0;
 }
 __device__ __forceinline__ float two_to(int e) { return __int_as_float((127 + e) << 23); }
 // x as two fp16 numbers; an infinity or a NaN is the first one
@@ -91,8 +92,9 @@ __device__ __forceinline__ void sum_parts(const float* from, long long step, int
             }
     }
 }
-__device__ __forceinline__ float largest_of(const float4& v) {
-    return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w)));
+__device__ __forceinline__ float size_if_finite(float v) { return fabsf(v) < INFINITY ? fabsf(v) : 0.0f; }
+__device__ __forceinline__ float largest_finite(const float4& v) {
+    return fmaxf(fmaxf(size_if_finite(v.x), size_if_finite(v.y)), fmaxf(size_if_finite(v.z), size_if_finite(v.w)));
 }
 
 // the first `bytes` of 16 bytes global -> shared, and zeros behind them (nothing is read where there are none)

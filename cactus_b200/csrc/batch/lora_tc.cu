@@ -6,7 +6,7 @@
 // rank operations, so all is built to keep those moving: a persistent block for each SM goes over items of 128 rows of one
 // adapter and 128 outputs.
 //   loaders   (8 warps) B's rows and the base's rows into a ring of stages, 16 bytes a copy, items ahead; for each new
-//             tile h as two fp16 numbers an element (h = 2^e (high + low), e by the row's largest element, so that
+//             tile h as two fp16 numbers an element (h = 2^e (high + low), e by the row's largest finite element, so that
 //             neither overflows and 22 bits are kept), in the operands' swizzled layout;
 //   epilogue  (8 warps) sums from TMEM, a thread a row's 64 outputs; the results replace the base's elements in
 //             shared memory and leave from there in whole rows;
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) lora_expand_wide_kernel(const __g
                                        row < w.tile.z ? rank - 4 * q : 0, v);
                     float top = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < RP / 16; ++i) top = fmaxf(top, largest_of(v[i]));
+                    for (int i = 0; i < RP / 16; ++i) top = fmaxf(top, largest_finite(v[i]));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                     const int e = exponent_of(top);

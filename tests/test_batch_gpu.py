@@ -309,6 +309,38 @@ def test_lora_an_infinity_keeps_its_sign(counts, ids, n, rank):
     assert (got[2] == np.inf).all() and (got[4] == -np.inf).all()
 
 
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("rank", [2, 7, 21])
+@pytest.mark.parametrize("counts,n,top", [
+    ([6, 2], 72, 24),        # one kernel, a cluster of blocks a tile
+    ([40, 20], 72, 24), ([40, 20], 72, 256), ([130], 264, 24), ([5, 90], 264, 200),  # both products by lora.cu's two kernels
+    ([520, 3], 8192, 32),    # the second product by tcgen05
+    ([300, 20], 2800, 40), ([300, 20], 2800, 104),  # both of them
+])
+def test_lora_an_infinity_of_an_adapter_beside_large_sums(counts, n, top, rank, sign):
+    """One infinity in a's first row, sums past fp16's end in its others: their products are finite, of either sign, so that
+    the results are the infinity's, rows of the other adapter what they are without it."""
+    rng = np.random.default_rng(1000 * rank + top)
+    call = Lora(counts, range(len(counts)), [rank, 8][:len(counts)], 128, n, rng, top=top)
+    call.x[:counts[0]] = rng.uniform(50, 100, (counts[0], 128))
+    call.x[:counts[0], 77] *= np.where(np.arange(counts[0]) % 3 == 1, -1, 1).astype(np.float16)
+    call.a[0, 1:rank] = rng.uniform(20, 40, (rank - 1, 128))  # sums from 126 * 50 * 20 on: above 65504
+    call.a[0, 0, 77] = np.inf
+    call.b[0, :, :rank] = np.abs(call.b[0, :, :rank]) + np.float16(0.01)
+    call.b[0, :, 1:rank] *= np.float16(sign)
+    call.da, call.db = dev(call.a), dev(call.b)
+    call.dx, call.px = _padded(call.x, 128, rng)
+    call.plan()
+    call.run()
+    got = call.got()
+    want = np.where(call.x[:counts[0], 77] > 0, np.inf, -np.inf)[:, None]
+    assert (got[:counts[0]] == want).all()
+    call.ids[0] = -1  # the others' rows
+    ref, tol = U.lora(call.x, call.a, call.b, call.ranks, call.scales, call.base, call.seqs, call.ids)
+    U.within(got[counts[0]:], ref[counts[0]:], tol[counts[0]:])
+    assert _err() == 0
+
+
 def test_lora_refuses_lists_on_the_device():
     """Offsets that fall or pass the tokens: no row; ids and ranks that are none: rows as without an adapter."""
     rng = np.random.default_rng(8)
