@@ -706,6 +706,9 @@ int launch_lora(const LoraCall& c, cudaStream_t st) {
     }
     const long long all_tiles = most_tiles(c.num_seqs, c.num_tokens, c.num_adapters) + (c.num_tokens + kTileRows - 1) / kTileRows;
     if (cluster_pays(c, all_tiles)) return launch_few(c, all_tiles, cluster_blocks(all_tiles), st);
+    // The second kernel reads the plan and the base before it waits for the first one, so that one starts behind all
+    // that wrote them, whatever the caller's thread has switched on.
+    pdl_scope behind(false);
     const long long work = (long long)c.num_tokens * c.n * c.max_rank;
     const bool wide = c.num_tokens >= kWideTokens && c.max_rank <= kLoraWideRank && c.num_adapters > 0 &&
                       work >= (c.max_rank > kSmallRank ? kWideWork : kWideWorkSmallRank);

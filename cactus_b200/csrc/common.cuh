@@ -252,7 +252,8 @@ __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepc
 // attribute while pdl_scope is active on the calling thread (the engine enables it for its
 // decode/prefill sequences; standalone C-ABI calls run without it, where griddepcontrol.wait
 // is a no-op). Every kernel calls pdl_launch_dependents()/pdl_wait() before touching data
-// produced by earlier launches.
+// produced by earlier launches; batch/lora.cu's second kernels touch such data sooner, but none of the
+// kernel right before them, which is launched without the attribute.
 bool& pdl_flag();
 struct pdl_scope {
     bool prev;

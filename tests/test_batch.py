@@ -127,3 +127,16 @@ def test_a_failed_launch_is_an_error(tmp_path):
                     os.path.join(ROOT, "tests", "native", "batch_abi_launch_test.cpp"), "-o", exe], check=True)
     r = subprocess.run([exe], capture_output=True, text=True)
     assert r.returncode == 0 and r.stdout == "ok\n", r.stdout + r.stderr
+
+
+def test_the_first_product_waits_for_what_was_launched_before(tmp_path):
+    """lora.cu and lora_tc.cu over a runtime that records their launches, in a thread with programmatic launches on and off."""
+    exe, src = str(tmp_path / "lora_launch_test"), os.path.join(ROOT, "cactus_b200", "csrc")
+    calls = ("cudaLaunchKernelExC", "cudaGetDevice", "cudaFuncSetAttribute", "cudaGetSymbolAddress")
+    subprocess.run([build.nvcc(), build.ARCH, "-std=c++17", "-rdc=true", "--fmad=false", "--expt-relaxed-constexpr",
+                    "-diag-suppress=177", "-I", os.path.join(ROOT, "include"), "-I", src,
+                    *(o for call in calls for o in ("-Xlinker", "--wrap=" + call)), os.path.join(src, "batch", "lora.cu"),
+                    os.path.join(src, "batch", "lora_tc.cu"), os.path.join(ROOT, "tests", "native", "lora_launch_test.cu"),
+                    "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True)
+    assert r.returncode == 0 and r.stdout == "ok\n", r.stdout + r.stderr
