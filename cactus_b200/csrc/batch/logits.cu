@@ -157,19 +157,19 @@ __global__ void __launch_bounds__(T, T == 512 ? 3 : 1) logits_kernel(LogitsCall 
                 if (v + j >= 0 && v + j < c.vocab) out[v + j] = h[j];
         }
     }
-    if (!lists) return;
     float repetition = 1.0f, frequency = 0.0f, presence = 0.0f;
     int prompt = 0;
-    if (c.penalties) {
+    // what is no factor or no length is said of a row without lists too, by one of its slices
+    if (c.penalties && (lists || (blockIdx.y == 0 && threadIdx.x == 0))) {
         repetition = __ldg(c.penalties + 3LL * row);
         frequency = __ldg(c.penalties + 3LL * row + 1);
         presence = __ldg(c.penalties + 3LL * row + 2);
-        if (!(repetition > 0.0f && repetition < INFINITY)) {
-            if (threadIdx.x == 0) report_dev_error(kDevBadList);
-            repetition = 1.0f;
-        }
         prompt = c.prompt_lens ? __ldg(c.prompt_lens + row) : 0;
+        const bool factor = repetition > 0.0f && repetition < INFINITY;
+        if ((!factor || prompt < 0) && threadIdx.x == 0) report_dev_error(kDevBadList);
+        if (!factor) repetition = 1.0f;
     }
+    if (!lists) return;
     // The noted tokens, kRound numbers at a time (nearly always all of them). In place their logits are still there:
     // the pass wrote them as they were, but for hidden ones, which are left out here.
     for (int first = 0;; first += kRound) {

@@ -64,10 +64,10 @@ CB_API int cactus_cuda_lora_f16(const uint16_t* x, size_t x_stride, const uint16
 /* Logits [rows][vocab] before sampling (output may be logits, with the same stride). For each row, in this order:
  *  - penalties [rows][3] (repetition, frequency, presence; NULL: none) for the tokens of its history,
  *    history[history_offsets[row]] .. history[history_offsets[row + 1] - 1], of which the first
- *    prompt_lens[row] (NULL: 0) are the prompt: l / repetition where l > 0, else l * repetition, for a token
- *    that occurs; minus frequency * count and, where count is not 0, minus presence, with its count behind
- *    the prompt. A repetition penalty that is not positive and finite raises the device error word and
- *    counts as 1.
+ *    prompt_lens[row] (NULL: 0; all, where there are fewer) are the prompt: l / repetition where l > 0, else
+ *    l * repetition, for a token that occurs; minus frequency * count and, where count is not 0, minus
+ *    presence, with its count behind the prompt. A repetition penalty that is not positive and finite raises the device error word and
+ *    counts as 1, a prompt's length below 0 raises it and counts as 0.
  *  - biases: bias_values[j] is added to token bias_ids[j], j from bias_offsets[row] to bias_offsets[row + 1] - 1.
  *    Of a token's several entries the last one counts. -inf bans a token.
  *  - a mask: -inf for tokens whose bit is 0 in masks[mask_ids[row]] (bit t % 32 of word t / 32; masks

@@ -857,6 +857,25 @@ def test_logits_refuses_lists_on_the_device():
     Logits(4, 500, rng, [[1, 2, 3]] * 4, penalties=pen).check(err=4)
 
 
+@pytest.mark.parametrize("vocab,rows", [(500, 3), (40000, 3), (40000, 300)])
+def test_logits_refuses_lengths_and_penalties_of_every_row(vocab, rows):
+    """A prompt of less than no tokens counts as none, a repetition penalty that is no factor as 1, and both are said of
+    rows without a history too; a prompt of more than the history is all of it."""
+    rng = np.random.default_rng(26)
+    hist = [[1, 2, 1], [], [vocab - 1]] * (rows // 3)
+    for at, value in ((0, -1), (1, -7), (rows - 1, -2 ** 31), (rows - 2, -1)):
+        prompts = [b % 3 for b in range(rows)]
+        prompts[at] = value
+        call = Logits(rows, vocab, rng, hist, prompts=prompts)
+        call.prompts = [max(p, 0) for p in prompts]
+        call.check(err=4)
+    for at, value in ((1, 0.0), (rows - 2, np.nan), (2, -1.0), (0, np.inf)):
+        pen = np.tile(np.float32([1.3, 0.25, 0.5]), (rows, 1))
+        pen[at, 0] = value
+        Logits(rows, vocab, rng, hist, penalties=pen).check(err=4)
+    Logits(rows, vocab, rng, hist, prompts=[2 ** 31 - 1] * rows).check()
+
+
 def test_logits_replayed_with_other_lists():
     t = torch()
     rng = np.random.default_rng(24)
