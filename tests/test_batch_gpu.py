@@ -876,6 +876,21 @@ def test_logits_refuses_lengths_and_penalties_of_every_row(vocab, rows):
     Logits(rows, vocab, rng, hist, prompts=[2 ** 31 - 1] * rows).check()
 
 
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("offsets,rest", [([0, 9, 4], [[], []]), ([0, 2, 99], [[1, 2], []]), ([-3, -1, 0], [[], []]),
+                                          ([5, 3, 5], [[], [4, 5]]), ([-1, 2, 5], [[], [3, 4, 5]])])
+def test_logits_rows_with_refused_lists_stay_as_they_are(offsets, rest, inplace):
+    rng = np.random.default_rng(27)
+    for vocab in (500, 40000):
+        call = Logits(2, vocab, rng, [[1, 2], [3, 4, 5]])
+        call.kw["history_offsets"] = dev(np.array(offsets, np.int32))
+        call.histories = rest
+        got = call.check(inplace, err=4)
+        for row in range(2):
+            if not rest[row]:
+                assert np.array_equal(got[row].view(np.uint16), call.x[row].view(np.uint16))
+
+
 def test_logits_replayed_with_other_lists():
     t = torch()
     rng = np.random.default_rng(24)
