@@ -226,9 +226,10 @@ cudaError_t launch(const LogitsCall& c, cudaStream_t st) {
 }  // namespace
 
 int launch_logits(const LogitsCall& c, cudaStream_t st) {
-    // Large slices, since each block goes through the row's lists twice; small ones, for the shortest time, where those
-    // are no more than four blocks for each SM. Slices of 2048 / 16384, us: 4 rows of 128256 5.7 / 6.7, of 262144
-    // 6.2 / 6.7, 16 rows of 32000 6.2 / 6.7, of 128256 10.3 / 6.7, 64 rows of 32000 11.3 / 7.2.
+    // Large slices, since each block goes through the row's lists (and once more where it has more than kKept of their
+    // entries); small ones, for the shortest time, where those are no more than four blocks for each SM. Slices of 2048 /
+    // 16384, histories of 750 to 1500, a graph's replay, us: 4 rows of 128256 6.3 / 8.3, of 262144 6.3 / 8.3, 16 rows of
+    // 32000 7.5 / 8.3, 32 of 32000 8.3 / 8.3, 16 rows of 128256 10.4 / 8.3, 64 rows of 32000 12.4 / 8.3.
     const long long small = (long long)c.rows * ((c.vocab + 7) / 2048 + 1);
     const cudaError_t e = small <= 4 * kNumSMs ? launch<256, 1>(c, st) : launch<512, 4>(c, st);
     return e == cudaSuccess ? 0 : -1;

@@ -105,6 +105,8 @@ __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, unsigned parity, vo
 // kernel has to add up. Whole calls with as many parts as there are SMs for / as many as here, us: rank 64, K 2048, 8192
 // outputs, 1024 tokens 30.8 / 22.6; K 14336, 4096 outputs, 512 tokens 34.9 / 25.5. Tiles of 64 / 128 rows: rank 64, K 8192, 2048
 // outputs, 16384 tokens 106 / 96; 18000 tokens of 40 adapters 115 / 129.
+// Both products' kernels evaluate it and have to find the same: the same IEEE steps on the same numbers, none of which the
+// compiler may join into another (kPartCost is a power of two, so that its products are exact besides).
 constexpr float kPartCost = 65536.0f;
 struct Split {
     int rows, tiles, parts;

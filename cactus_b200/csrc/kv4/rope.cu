@@ -2,9 +2,9 @@
 // that it reads. A warp takes a token's heads one group after another, 32 * 8 / D heads at a time: D / 8 lanes
 // share a head's row (8 elements, one 16-byte load each), and the token's turns stay in registers for all of
 // them. Shuffles add up the squares of the norm, fetch the other element of each rotated pair and reduce a
-// group's ends for the quantisation. Each element is read and written once; the instructions of the exact
-// quantisation bound it: 65 thousand prompt rows of 24 query heads, 8 key heads and 8 of values, of 64, take 126 us, 4.5 TB/s
-// and 69 % of the issue slots (a block a head and 32 rows took 300).
+// group's ends for the quantisation. Each element is read and written once. 65 thousand prompt rows of 24 query heads, 8 key
+// heads and 8 of values, of 64, take 126 us, 4.5 TB/s (a block a head and 32 rows took 300). Neither HBM nor the issue slots
+// (68 %) are full then: 24 warps a SM, of 80 registers and some words spilled, wait for their loads first.
 #include <type_traits>
 
 #include "kv4.cuh"
@@ -42,9 +42,12 @@ __device__ __forceinline__ int find_seq_warp(const int* offsets, int n, int t) {
     return lo;
 }
 
-// The sum of a row's squares, eight of them a lane. The halves of the row are added to one another, element by
-// element, then the halves of that (down to 32 sums of four neighbours for D >= 128): a fixed order of few steps,
-// of which every lane has its share, as each exchange passes on the part that the lane does not keep.
+// The sum of a row's squares, eight of them a lane: the halves of the row are added to one another, element by
+// element, then the halves of that; at D = 128 after four neighbours each, at D = 256 after the first halves and four
+// neighbours each. Any fixed order would be as close to the 64-bit sum. This one, another for each D, is that of the plain form's row means (PyTorch in fp32 on this GPU,
+// found by trying orders out), and with rsqrtf as its root a normalised key has the plain form's bits: a code next to the
+// border of two does not differ between the two. That equality is no evidence of exactness; the bound is against 64 bits.
+// Every lane has its share, as each exchange passes on the part that the lane does not keep.
 template <int D>
 __device__ __forceinline__ float sum_of_squares(const float (&v)[8], int lane) {
     const unsigned full = 0xffffffffu;
