@@ -72,6 +72,8 @@ CB_API int cactus_cuda_lora_f16(const uint16_t* x, size_t x_stride, const uint16
  *    Of a token's several entries the last one counts. -inf bans a token.
  *  - a mask: -inf for tokens whose bit is 0 in masks[mask_ids[row]] (bit t % 32 of word t / 32; masks
  *    [num_masks][mask_stride]); mask_ids[row] == -1: none; mask_ids NULL: row i has mask i.
+ * What is left of a row goes to cactus_cuda_argmax_f16 or cactus_cuda_sample_f16 (whose `uniform` has to be above
+ * 0 then: with 0 it answers index 0, masked or not).
  * history, bias_ids and masks are NULL where there are none. Offsets rise from 0 and end at num_history and
  * num_biases at most; ids are below vocab. Arithmetic is fp32, each step rounded; a finite result past fp16's
  * range becomes its largest number of that sign. */

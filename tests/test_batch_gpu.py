@@ -823,6 +823,30 @@ def test_logits_masks_that_leave_nothing_or_everything_over_any_value():
     assert host(token, np.uint32)[0] == vocab - 1
 
 
+@pytest.mark.parametrize("vocab", [5003, 40000])
+def test_logits_then_a_sample_is_what_the_mask_leaves(vocab):
+    """Penalties, bans and masks, then a token of each row by temperature, top-k and top-p: one that is left."""
+    rng = np.random.default_rng(28)
+    left = [1, 2, 40, 3000]
+    masks = [np.zeros(vocab, bool) for _ in left]
+    for mask, n in zip(masks, left):
+        mask[rng.permutation(vocab)[:n]] = True
+    ban = [int(np.flatnonzero(m)[-1]) for m in masks]
+    bias = [[(ban[b], -np.inf)] if left[b] > 1 else [] for b in range(4)]
+    call = Logits(4, vocab, rng, _histories(rng, 4, vocab, [50]), bias, masks)
+    got = call.check(inplace=True)
+    token, work = empty((1,), np.uint32), empty((vocab,), np.float16)
+    for b in range(4):
+        if left[b] > 1:
+            masks[b][ban[b]] = False
+        assert np.array_equal(np.isfinite(got[b]), masks[b])
+        for top_k, top_p in ((0, 0.9), (0, 1.0), (20, 0.9), (5, 1.0)):
+            for uniform in (1e-7, 0.5, 1 - 2.0 ** -24):
+                cb.check(cb.lib().cactus_cuda_sample_f16(call.px + 2 * b * vocab, 1, vocab, 0.8, top_p, top_k, uniform, None, 0,
+                                                         work.data_ptr(), token.data_ptr(), None))
+                assert masks[b][host(token, np.uint32)[0]]
+
+
 @pytest.mark.parametrize("rows,vocab", [(1, 6000), (2, 40000), (300, 20000)])
 def test_logits_of_many_named_tokens(rows, vocab):
     """More tokens of one slice in the lists than are counted at a time; every token, named by history or biases."""
